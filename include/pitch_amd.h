@@ -340,6 +340,130 @@ int pitch_enqueue_attention_decode_channel_keys(
     uint64_t output_offset, void* lse, uint64_t lse_bytes, uint64_t lse_offset, void* workspace,
     uint64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Paged caches. The reference keeps one sequence's cache in contiguous buffers (README.md:65-76); a program that serves
+ * many sequences keeps their keys and values in the pages of one pool and a table of pages per sequence. The pages hold
+ * per-vector codes and scales as pitch_enqueue_encode_io writes them. A pool has `pages` pages of page_size token slots
+ * for each of kv_heads KV heads. The vector of (page p, head h, slot s), for codes (code_stride bytes each) and scales
+ * (4 bytes each) alike, is p * page_stride + h * page_size + s (PITCH_PAGES_HEAD_MAJOR) or p * page_stride +
+ * s * kv_heads + h (PITCH_PAGES_TOKEN_MAJOR). The three operators below are captured into graphs like the others: they
+ * launch kernels only. What lies in device memory (slots, positions, page tables, lengths) cannot be checked before the
+ * launch; the kernels check every value against the pool and the tables and take none on trust. */
+#define PITCH_PAGES_HEAD_MAJOR 0u
+#define PITCH_PAGES_TOKEN_MAJOR 1u
+
+typedef struct pitch_paged_cache {
+  pitch_config_t key_config, value_config; /* one dimension, 64 or 128; methods, bit widths and seeds may differ */
+  void* key_codes;
+  uint64_t key_codes_bytes;
+  void* key_scales;
+  uint64_t key_scales_bytes;
+  void* value_codes;
+  uint64_t value_codes_bytes;
+  void* value_scales;
+  uint64_t value_scales_bytes;
+  uint64_t pages;       /* pages * page_size < 2^32 */
+  uint64_t page_stride; /* vectors from page to page, at least kv_heads * page_size */
+  uint32_t page_size;   /* token slots of a page: a multiple of 16, at most 65536 */
+  uint32_t kv_heads;    /* 1..65535 */
+  uint32_t layout;      /* PITCH_PAGES_* */
+  uint32_t reserved;    /* 0 */
+} pitch_paged_cache_t;
+
+/* The vectors of a paged call: coordinate i of (token t, head h) is element t * token_stride + h * head_stride + i of
+ * data, of the call's io_type. For 16-bit types data and both strides are multiples of 4 bytes. bytes is what the buffer
+ * holds from data on. */
+typedef struct pitch_paged_vectors {
+  void* data;
+  uint64_t bytes;
+  uint64_t token_stride, head_stride; /* elements */
+} pitch_paged_vectors_t;
+
+/* Writes tokens to the cache. Token t's keys and values [kv_heads][dim] are encoded into slot slots[t] = page * page_size
+ * + slot; a token whose slot lies outside the pool (-1 for the padding of a batch) is not written. Two tokens of a call
+ * must not have the same slot (what such a slot holds afterwards is undefined).
+ * With key_norm, a key is x / sqrt(mean(x^2) + eps) times the weights (dim elements of io_type); with positions, its first
+ * rotary_dim coordinates are then rotated: x * cos[p] + rotate_half(x) * sin[p], rotate_half over these coordinates
+ * (-x[rotary_dim / 2:], x[:rotary_dim / 2]), p = positions[t], cos and sin [rows][rotary_dim] fp32. A key is not rounded
+ * between these steps and its codes. Queries (q_heads per token, 0 for none) are normed with query_norm and rotated alike,
+ * in float32, and written to queries_out in io_type; they may be written in place. A token whose position lies outside the
+ * tables is not written, nor are its queries. Without norm and positions the codes and scales are those of
+ * pitch_enqueue_encode_io, up to values within 1e-11 of an edge between two codes (relative to the vector's norm).
+ * For a decode step's or a prompt's write (README.md:65-71 appends with one PITCH.enqueueEncode per cache). */
+typedef struct pitch_paged_append {
+  uint32_t io_type; /* PITCH_IO_*: keys, values, queries, norm weights */
+  uint32_t q_heads;
+  uint64_t tokens;  /* at least 1; tokens * heads < 2^31 */
+  pitch_paged_vectors_t keys, values, queries, queries_out;
+  const void* slots;     /* int64 [tokens] */
+  uint64_t slots_bytes;
+  const void* positions; /* int64 [tokens], or null: no rotation */
+  uint64_t positions_bytes;
+  const void* cos;
+  const void* sin;
+  uint64_t table_bytes;  /* bytes of cos and of sin each */
+  const void* query_norm; /* or null */
+  uint64_t query_norm_bytes;
+  const void* key_norm;   /* or null */
+  uint64_t key_norm_bytes;
+  uint32_t rotary_dim;    /* a multiple of 16, at most dim; 0 without positions */
+  float eps;              /* at least 0 */
+} pitch_paged_append_t;
+int pitch_enqueue_paged_append(const pitch_paged_cache_t* cache, const pitch_paged_append_t* call, void* stream);
+
+/* Reads tokens back. Row r of the outputs, row_starts[b] <= r < row_starts[b + 1], is token first_tokens[b] + r -
+ * row_starts[b] of sequence b, found in page block_tables[b][token / page_size]; it is decoded as pitch_enqueue_decode_io
+ * decodes it. row_starts does not decrease. Rows outside the sequences' ranges, and rows whose page lies outside the pool or
+ * the table, are left as they were. keys or values may have null data (not read back). */
+typedef struct pitch_paged_decode {
+  uint32_t io_type;   /* PITCH_IO_* of the outputs */
+  uint32_t sequences; /* at least 1 */
+  uint64_t rows;      /* rows of the outputs, 1 .. 2^31 - 1 */
+  const void* block_tables; /* int32 [sequences][table_width] */
+  uint64_t block_tables_bytes;
+  uint64_t table_width; /* at least 1 */
+  const void* row_starts; /* int32 [sequences + 1] */
+  uint64_t row_starts_bytes;
+  const void* first_tokens; /* int32 [sequences], or null: 0 */
+  uint64_t first_tokens_bytes;
+  pitch_paged_vectors_t keys, values;
+} pitch_paged_decode_t;
+int pitch_enqueue_paged_decode(const pitch_paged_cache_t* cache, const pitch_paged_decode_t* call, void* stream);
+
+/* Attention of one new token of every sequence over its pages. Sequence b has lengths[b] = L cached tokens, the new one
+ * among them; query head h of its q_per_kv * kv_heads heads reads KV head h / q_per_kv:
+ *   out = softmax(z) V,  lse = log sum exp(z),  z_t = cap(scale * q . k_t) + slopes[h] * (t - (L - 1))
+ * over the tokens t of [0, L), of [L - window, L) with a window; cap(x) = softcap * tanh(x / softcap), x itself with
+ * softcap 0. Queries and outputs are float16 or bfloat16: the products run on the 16-bit matrix cores. A length of 0 or
+ * less gives zeros and an lse of minus infinity; lengths are cut to table_width * page_size tokens; tokens of pages
+ * outside the pool (-1) take no part. Page tables need be right only up to the sequences' lengths. Extends
+ * pitch_enqueue_attention_decode, which the reference does not have (README.md:96). */
+typedef struct pitch_paged_attention {
+  uint32_t io_type;   /* PITCH_IO_F16 or PITCH_IO_BF16 */
+  uint32_t sequences; /* at least 1 */
+  uint32_t q_per_kv;  /* 1..8 */
+  uint32_t window;    /* tokens; 0: all */
+  pitch_paged_vectors_t queries, output; /* token = sequence, head = query head */
+  const void* block_tables; /* int32 [sequences][table_width] */
+  uint64_t block_tables_bytes;
+  uint64_t table_width;
+  const void* lengths; /* int32 [sequences] */
+  uint64_t lengths_bytes;
+  const void* slopes; /* fp32 [q_per_kv * kv_heads], or null */
+  uint64_t slopes_bytes;
+  void* lse; /* fp32 [sequences][q_per_kv * kv_heads], or null */
+  uint64_t lse_bytes;
+  float scale;
+  float softcap; /* 0: none */
+  void* workspace; /* pitch_paged_attention_workspace_size bytes; not used by another call until this one has completed */
+  uint64_t workspace_bytes;
+} pitch_paged_attention_t;
+/* Bytes of device workspace pitch_enqueue_paged_attention needs on the current device for these arguments (call needs
+ * sequences and q_per_kv only). */
+int pitch_paged_attention_workspace_size(const pitch_paged_cache_t* cache, const pitch_paged_attention_t* call,
+                                         uint64_t* bytes);
+int pitch_enqueue_paged_attention(const pitch_paged_cache_t* cache, const pitch_paged_attention_t* call, void* stream);
+
 /* Packs count rows of dim unpacked codes (one uint8 per code, each < 2^bits) into count * code_stride
  * bytes, code i at bits [i * bits, i * bits + bits) of the row's little-endian 32-bit words.
  * Replaces pack_codes (reference/pitch_reference.py:68-78). */

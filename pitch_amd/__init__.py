@@ -6,7 +6,8 @@ enqueueDecode and the per-channel forms), ``QuantConfig``, ``ChannelQuantConfig`
 reference/pitch_reference.py (``turbo_encode``, ``polar_decode``, ``channel_encode``, ``pack_codes``, ...)
 that run on device tensors. ``PITCH.enqueueEncodeBatch`` / ``EncodeBatch`` encode many caches' segments (a
 token's append to every layer) in one call, and ``PITCH.enqueueDecodeBatch`` / ``DecodeBatch`` decode them. ``attention_decode`` / ``PITCH.enqueueAttentionDecode`` compute decode-step
-attention directly over the compressed caches.
+attention directly over the compressed caches. ``PagedCache`` keeps many sequences' keys and values as codes in the pages of
+one pool, written by ``PagedAppend``, read back by ``PagedDecode`` and attended over by ``PagedAttention``.
 """
 from .api import (  # noqa: F401
     CHANNEL_DEFAULT_GROUP, DECODERS, DEFAULT_SEED, ENCODERS, FP16_MAX, PITCH, SUPPORTED_BITS, SUPPORTED_DIMS,
@@ -16,5 +17,6 @@ from .api import (  # noqa: F401
     channel_group_count, code_stride_bytes, half_to_float, pack_codes, polar_decode, polar_encode, rand_signs,
     turbo_decode, turbo_encode, unpack_codes,
 )
+from .paged import PagedAppend, PagedAttention, PagedCache, PagedDecode  # noqa: F401
 
 __version__ = "0.1.0"

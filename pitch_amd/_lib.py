@@ -38,6 +38,44 @@ class PitchAttentionDescC(ctypes.Structure):
                 ("reserved", ctypes.c_uint32)]
 
 
+class PitchPagedCacheC(ctypes.Structure):
+    _fields_ = ([("key_config", PitchConfigC), ("value_config", PitchConfigC)]
+                + [f for n in ("key_codes", "key_scales", "value_codes", "value_scales")
+                   for f in ((n, ctypes.c_void_p), (n + "_bytes", ctypes.c_uint64))]
+                + [("pages", ctypes.c_uint64), ("page_stride", ctypes.c_uint64), ("page_size", ctypes.c_uint32),
+                   ("kv_heads", ctypes.c_uint32), ("layout", ctypes.c_uint32), ("reserved", ctypes.c_uint32)])
+
+
+class PitchPagedVectorsC(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("bytes", ctypes.c_uint64), ("token_stride", ctypes.c_uint64),
+                ("head_stride", ctypes.c_uint64)]
+
+
+def _with_bytes(*names):
+    return [f for n in names for f in ((n, ctypes.c_void_p), (n + "_bytes", ctypes.c_uint64))]
+
+
+class PitchPagedAppendC(ctypes.Structure):
+    _fields_ = ([("io_type", ctypes.c_uint32), ("q_heads", ctypes.c_uint32), ("tokens", ctypes.c_uint64)]
+                + [(n, PitchPagedVectorsC) for n in ("keys", "values", "queries", "queries_out")]
+                + _with_bytes("slots", "positions")
+                + [("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p), ("table_bytes", ctypes.c_uint64)]
+                + _with_bytes("query_norm", "key_norm") + [("rotary_dim", ctypes.c_uint32), ("eps", ctypes.c_float)])
+
+
+class PitchPagedDecodeC(ctypes.Structure):
+    _fields_ = ([("io_type", ctypes.c_uint32), ("sequences", ctypes.c_uint32), ("rows", ctypes.c_uint64)]
+                + _with_bytes("block_tables") + [("table_width", ctypes.c_uint64)]
+                + _with_bytes("row_starts", "first_tokens") + [("keys", PitchPagedVectorsC), ("values", PitchPagedVectorsC)])
+
+
+class PitchPagedAttentionC(ctypes.Structure):
+    _fields_ = ([("io_type", ctypes.c_uint32), ("sequences", ctypes.c_uint32), ("q_per_kv", ctypes.c_uint32),
+                 ("window", ctypes.c_uint32), ("queries", PitchPagedVectorsC), ("output", PitchPagedVectorsC)]
+                + _with_bytes("block_tables") + [("table_width", ctypes.c_uint64)] + _with_bytes("lengths", "slopes", "lse")
+                + [("scale", ctypes.c_float), ("softcap", ctypes.c_float)] + _with_bytes("workspace"))
+
+
 class PitchKeyBiasC(ctypes.Structure):
     _fields_ = [("bias", ctypes.c_void_p), ("bias_bytes", ctypes.c_uint64), ("cos", ctypes.c_void_p),
                 ("sin", ctypes.c_void_p), ("table_bytes", ctypes.c_uint64), ("first_position", ctypes.c_uint64),
@@ -119,6 +157,11 @@ SIGNATURES = {
                                                            ctypes.POINTER(PitchConfigC),
                                                            ctypes.POINTER(PitchAttentionDescC)] + [_vp, _u64, _u64] * 7
                                                     + [_vp, _u64, _vp]),
+    "pitch_enqueue_paged_append": (_int, [ctypes.POINTER(PitchPagedCacheC), ctypes.POINTER(PitchPagedAppendC), _vp]),
+    "pitch_enqueue_paged_decode": (_int, [ctypes.POINTER(PitchPagedCacheC), ctypes.POINTER(PitchPagedDecodeC), _vp]),
+    "pitch_paged_attention_workspace_size": (_int, [ctypes.POINTER(PitchPagedCacheC),
+                                                    ctypes.POINTER(PitchPagedAttentionC), ctypes.POINTER(_u64)]),
+    "pitch_enqueue_paged_attention": (_int, [ctypes.POINTER(PitchPagedCacheC), ctypes.POINTER(PitchPagedAttentionC), _vp]),
     "pitch_enqueue_pack_codes": (_int, [_u32, _u32, _vp, _u64, _u64, _vp, _u64, _u64, _u64, _vp]),
     "pitch_enqueue_unpack_codes": (_int, [_u32, _u32, _vp, _u64, _u64, _vp, _u64, _u64, _u64, _vp]),
     "pitch_selftest_reciprocal": (_int, [ctypes.POINTER(_u64)]),

@@ -5,7 +5,9 @@
 Steps: generate csrc/pitch_tables.inc from data/codebooks.json, compile csrc/pitch_vector.hip once per
 dimension and element type of the uncompressed vectors (-DPITCH_DIM=2..1024, -DPITCH_IO=0/1/2 for
 float32/float16/bfloat16), csrc/pitch_channel.hip once per element type, csrc/pitch_attention.hip once per
-attention dimension (64, 128), csrc/pitch_attn_codes.hip once per attention dimension and kind of caches, and csrc/pitch_abi.cpp, and link the shared library next to this file. Object files go to <repo>/_build/.
+attention dimension (64, 128), csrc/pitch_attn_codes.hip once per attention dimension and kind of caches, csrc/pitch_paged.hip once per
+attention dimension and element type, csrc/pitch_paged_attn.hip once per attention dimension, and csrc/pitch_abi.cpp, and link the
+shared library next to this file. Object files go to <repo>/_build/.
 Also builds libpitch_calib.so from csrc/pitch_calib.hip: the measurement kernels bench.py times beside the
 codec (not part of the codec's C ABI).
 """
@@ -56,12 +58,8 @@ def _run(cmd: list[str]) -> None:
         raise RuntimeError(f"command failed ({r.returncode}): {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
 
 
-def build(jobs: int | None = None, verbose: bool = False) -> Path:
-    """Compiles every source and links LIB. Always rebuilds."""
-    hipcc = _hipcc()
-    BUILD.mkdir(exist_ok=True)
-    _run([sys.executable, str(CSRC / "gen_tables.py"), str(PKG / "data" / "codebooks.json"),
-          str(CSRC / "pitch_tables.inc")])
+def units() -> list[tuple[Path, Path, list[str], int]]:
+    """(source, object, macros, weight) of every translation unit; heavier ones take longer to compile."""
     units = [(CSRC / "pitch_vector.hip", BUILD / f"vector_d{d}_io{io}.o", [f"-DPITCH_DIM={d}", f"-DPITCH_IO={io}"], d)
              for d in DIMS for io in IO_TYPES]
     units += [(CSRC / "pitch_channel.hip", BUILD / f"channel_io{io}.o", [f"-DPITCH_IO={io}"], 512) for io in IO_TYPES]
@@ -70,8 +68,20 @@ def build(jobs: int | None = None, verbose: bool = False) -> Path:
     units += [(CSRC / "pitch_attn_codes.hip", BUILD / f"attn_codes_d{d}_k{k}.o",
                [f"-DPITCH_DIM={d}", f"-DPITCH_KIND={k}"], 1024 + d) for d in ATTENTION_DIMS for k in ATTENTION_KINDS]
     units += [(CSRC / "pitch_abi.cpp", BUILD / "abi.o", [], 0)]
+    units += [(CSRC / "pitch_paged.hip", BUILD / f"paged_d{d}_io{io}.o", [f"-DPITCH_DIM={d}", f"-DPITCH_IO={io}"], 256 + d)
+              for d in ATTENTION_DIMS for io in IO_TYPES]
+    units += [(CSRC / "pitch_paged_attn.hip", BUILD / f"paged_attn_d{d}.o", [f"-DPITCH_DIM={d}"], 1024 + d)
+              for d in ATTENTION_DIMS]
     # largest dims first: they take longest to compile
-    units.sort(key=lambda u: -u[3])
+    return sorted(units, key=lambda u: -u[3])
+
+
+def build(jobs: int | None = None, verbose: bool = False) -> Path:
+    """Compiles every source and links LIB. Always rebuilds."""
+    hipcc = _hipcc()
+    BUILD.mkdir(exist_ok=True)
+    _run([sys.executable, str(CSRC / "gen_tables.py"), str(PKG / "data" / "codebooks.json"),
+          str(CSRC / "pitch_tables.inc")])
     jobs = jobs or min(8, os.cpu_count() or 4)
 
     def compile_one(u):
@@ -83,7 +93,7 @@ def build(jobs: int | None = None, verbose: bool = False) -> Path:
         return obj
 
     with ThreadPoolExecutor(max_workers=jobs) as ex:
-        objs = list(ex.map(compile_one, units))
+        objs = list(ex.map(compile_one, units()))
     tmp = LIB.with_suffix(".so.tmp")
     _run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)])
     os.replace(tmp, LIB)

@@ -19,6 +19,7 @@
 
 #include "../../include/pitch_amd.h"
 #include "pitch_launch.h"
+#include "pitch_paged.h"
 
 namespace {
 
@@ -44,6 +45,13 @@ int ok() {
     const int rc_ = (expr);   \
     if (rc_ != PITCH_OK) return rc_; \
   } while (0)
+
+// The rotation sign of a coordinate (sign_is_negative of pitch_device.h, which host code does not include).
+bool pitch_sign_is_negative(uint32_t seed, uint32_t i) {
+  const uint32_t state = (seed + i) * 747796405u + 2891336453u;
+  const uint32_t word = ((state >> ((state >> 28u) + 4u)) ^ state) * 277803737u;
+  return (((word >> 22u) ^ word) & 1u) == 0u;
+}
 
 bool is_pow2(uint32_t x) { return x != 0 && (x & (x - 1)) == 0; }
 
@@ -557,6 +565,8 @@ int device_cu_count() {
   cache[dev] = n;
   return n;
 }
+
+uint64_t paged_attention_workspace_floats(uint32_t, uint32_t, uint32_t) { return 0; }
 
 uint32_t attention_chunk_tokens(uint64_t tokens, uint32_t kv_heads) {
   // The largest chunk that still gives at least PITCH_ATTN_MIN_WG workgroups (512: two per compute unit; 1024 and
@@ -1254,6 +1264,305 @@ int pitch_selftest_attention_route(uint32_t dim, uint64_t tokens, uint32_t kv_he
     return fail(PITCH_ERR_INVALID_INPUT, "tokens, KV heads and queries must be at least 1");
   *codes = pitch::attention_codes_pays(dim, tokens, kv_heads, padded_queries(q_per_kv), key_bits, value_bits,
                                        head_major != 0, compute_units);
+  return ok();
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------------------------------- paged caches
+namespace {
+
+// Checks a paged cache without device access and fills the kernels' view of it.
+int paged_cache(const pitch_paged_cache_t* c, pitch::PagedPool* k, pitch::PagedPool* v, pitch::PagedLayout* l) {
+  if (!c) return fail(PITCH_ERR_INVALID_INPUT, "cache is null");
+  PITCH_TRY(validate_config(&c->key_config));
+  PITCH_TRY(validate_config(&c->value_config));
+  const uint32_t dim = c->key_config.dim;
+  if (dim != c->value_config.dim)
+    return fail(PITCH_ERR_CONFIGURATION_MISMATCH, "key dimension %u and value dimension %u differ", dim, c->value_config.dim);
+  if (dim != 64 && dim != 128)
+    return fail(PITCH_ERR_INVALID_DIMENSION, "Invalid dimension %u. A paged cache holds vectors of 64 or 128.", dim);
+  if (c->page_size < 16 || c->page_size > 65536 || c->page_size % 16 != 0)
+    return fail(PITCH_ERR_INVALID_INPUT, "page size %u must be a multiple of 16 in 16...65536", c->page_size);
+  if (c->kv_heads < 1 || c->kv_heads > 65535)
+    return fail(PITCH_ERR_INVALID_INPUT, "KV heads %u must be in 1...65535", c->kv_heads);
+  if (c->layout > PITCH_PAGES_TOKEN_MAJOR) return fail(PITCH_ERR_INVALID_INPUT, "unknown page layout %u", c->layout);
+  if (c->pages < 1 || c->pages > 0x7FFFFFFFull || c->pages * c->page_size > 0xFFFFFFFFull)
+    return fail(PITCH_ERR_INVALID_INPUT, "a pool holds 1 page or more and fewer than 2^32 token slots, got %llu pages of %u",
+                (unsigned long long)c->pages, c->page_size);
+  const uint64_t page = (uint64_t)c->kv_heads * c->page_size;
+  if (c->page_stride < page)
+    return fail(PITCH_ERR_INVALID_INPUT, "page stride %llu does not hold the page's %llu vectors",
+                (unsigned long long)c->page_stride, (unsigned long long)page);
+  if (c->page_stride > (1ull << 40)) return fail(PITCH_ERR_INVALID_INPUT, "page stride is too large");
+  // pages < 2^31 and page_stride <= 2^40: divide instead of multiplying past 2^64
+  if (c->pages > 1 && c->page_stride > (UINT64_MAX / 256u - page) / (c->pages - 1))
+    return fail(PITCH_ERR_INVALID_INPUT, "page stride is too large");
+  const uint64_t vectors = (c->pages - 1) * c->page_stride + page;
+  const pitch_config_t* cfg[2] = {&c->key_config, &c->value_config};
+  void* const codes[2] = {c->key_codes, c->value_codes};
+  void* const scales[2] = {c->key_scales, c->value_scales};
+  const uint64_t codes_bytes[2] = {c->key_codes_bytes, c->value_codes_bytes};
+  const uint64_t scales_bytes[2] = {c->key_scales_bytes, c->value_scales_bytes};
+  pitch::PagedPool* const pool[2] = {k, v};
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t cs = code_stride_of(dim, cfg[i]->bits);
+    PITCH_TRY(check_buffer(codes[i], codes_bytes[i], 0, vectors * cs, i ? "value codes" : "key codes"));
+    PITCH_TRY(check_buffer(scales[i], scales_bytes[i], 0, vectors * 4u, i ? "value scales" : "key scales"));
+    if ((uintptr_t)codes[i] % 4 || (uintptr_t)scales[i] % 4)
+      return fail(PITCH_ERR_INVALID_INPUT, "cache buffers must be aligned to 4 bytes");
+    pitch::PagedPool& p = *pool[i];
+    p = pitch::PagedPool{};
+    p.codes = (uint8_t*)codes[i];
+    p.scales = (float*)scales[i];
+    p.polar = cfg[i]->method == PITCH_METHOD_POLAR;
+    p.bits = cfg[i]->bits;
+    p.row_bytes = cs;
+    for (uint32_t j = 0; j < dim; ++j)
+      if (pitch_sign_is_negative(cfg[i]->seed, j)) p.signs[j >> 5] |= 1u << (j & 31);
+  }
+  l->page_stride = c->page_stride;
+  l->pages = (uint32_t)c->pages;
+  l->page_size = c->page_size;
+  l->kv_heads = c->kv_heads;
+  l->head_step = c->layout == PITCH_PAGES_HEAD_MAJOR ? c->page_size : 1u;
+  l->slot_step = c->layout == PITCH_PAGES_HEAD_MAJOR ? 1u : c->kv_heads;
+  return PITCH_OK;
+}
+
+int paged_cache_device(const pitch_paged_cache_t* c, BatchDeviceCheck& check) {
+  PITCH_TRY(check(c->key_codes, "key codes"));
+  PITCH_TRY(check(c->key_scales, "key scales"));
+  PITCH_TRY(check(c->value_codes, "value codes"));
+  return check(c->value_scales, "value scales");
+}
+
+// Strided vectors of tokens x heads: extent, alignment. With write, no two vectors may share memory.
+int paged_vectors(const pitch_paged_vectors_t& v, uint64_t tokens, uint64_t heads, uint32_t dim, uint32_t esize, bool write,
+                  const char* name, pitch::PagedVectors* out) {
+  if (!v.data) return fail(PITCH_ERR_INVALID_INPUT, "%s buffer is null", name);
+  if ((uintptr_t)v.data % 4 || (v.token_stride * esize) % 4 || (v.head_stride * esize) % 4)
+    return fail(PITCH_ERR_INVALID_INPUT, "%s: the buffer and its strides must be multiples of 4 bytes", name);
+  if (v.token_stride > (1ull << 40) || v.head_stride > (1ull << 40))
+    return fail(PITCH_ERR_INVALID_INPUT, "%s: strides are too large", name);
+  if (mul_overflows(tokens - 1, v.token_stride * 8u) || mul_overflows(heads - 1, v.head_stride * 8u))
+    return fail(PITCH_ERR_INVALID_INPUT, "%s: strides are too large", name);
+  const uint64_t t = (tokens - 1) * v.token_stride, h = (heads - 1) * v.head_stride;
+  if (t + h > UINT64_MAX / 16) return fail(PITCH_ERR_INVALID_INPUT, "%s: strides are too large", name);
+  PITCH_TRY(check_buffer(v.data, v.bytes, 0, (t + h + dim) * esize, name));
+  if (write) {
+    auto apart = [&](uint64_t s1, uint64_t n1, uint64_t s2, uint64_t n2) {   // runs of n1 vectors, n2 runs
+      return (n1 == 1 || s1 >= dim) && (n2 == 1 || s2 >= (n1 - 1) * s1 + dim);
+    };
+    if (!apart(v.head_stride, heads, v.token_stride, tokens) && !apart(v.token_stride, tokens, v.head_stride, heads))
+      return fail(PITCH_ERR_INVALID_INPUT, "%s: vectors of the output overlap", name);
+  }
+  out->data = v.data;
+  out->token_stride = v.token_stride;
+  out->head_stride = v.head_stride;
+  return PITCH_OK;
+}
+
+int check_aligned(const void* ptr, uint64_t bytes, uint64_t need, uint32_t align, const char* name) {
+  PITCH_TRY(check_buffer(ptr, bytes, 0, need, name));
+  if ((uintptr_t)ptr % align) return fail(PITCH_ERR_INVALID_INPUT, "%s buffer must be aligned to %u bytes", name, align);
+  return PITCH_OK;
+}
+
+int check_tables(const void* tables, uint64_t bytes, uint64_t width, uint32_t sequences) {
+  if (sequences < 1 || sequences > 0x7FFFFFFFu)
+    return fail(PITCH_ERR_INVALID_INPUT, "sequences must be in 1...2^31 - 1");
+  if (width < 1 || width > 0x7FFFFFFFull) return fail(PITCH_ERR_INVALID_INPUT, "page table width must be in 1...2^31 - 1");
+  return check_aligned(tables, bytes, width * sequences * 4u, 4, "page tables");
+}
+
+int validate_paged_attention(const pitch_paged_cache_t* cache, const pitch_paged_attention_t* call) {
+  if (!call) return fail(PITCH_ERR_INVALID_INPUT, "call is null");
+  if (call->sequences < 1 || call->sequences > 0x7FFFFFFFu)
+    return fail(PITCH_ERR_INVALID_INPUT, "sequences must be in 1...2^31 - 1");
+  if (call->q_per_kv < 1 || call->q_per_kv > 8)
+    return fail(PITCH_ERR_INVALID_INPUT, "query heads per KV head %u must be in 1...8", call->q_per_kv);
+  if ((uint64_t)call->sequences * cache->kv_heads > 0x7FFFFFFFull)
+    return fail(PITCH_ERR_INVALID_INPUT, "sequences times KV heads must be below 2^31");
+  return PITCH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pitch_enqueue_paged_append(const pitch_paged_cache_t* cache, const pitch_paged_append_t* call, void* stream) {
+  pitch::PagedAppendArgs a{};
+  PITCH_TRY(paged_cache(cache, &a.pool[0], &a.pool[1], &a.layout));
+  if (!call) return fail(PITCH_ERR_INVALID_INPUT, "call is null");
+  PITCH_TRY(check_io(call->io_type));
+  const uint32_t dim = cache->key_config.dim, esize = io_bytes(call->io_type);
+  const uint64_t n = call->tokens;
+  const uint32_t most_heads = std::max(cache->kv_heads, call->q_heads);
+  if (n < 1) return fail(PITCH_ERR_INVALID_INPUT, "tokens must be at least 1");
+  if (n > 0x7FFFFFFFull / most_heads) return fail(PITCH_ERR_INVALID_INPUT, "tokens times heads must be below 2^31");
+  PITCH_TRY(paged_vectors(call->keys, n, cache->kv_heads, dim, esize, false, "keys", &a.in[0]));
+  PITCH_TRY(paged_vectors(call->values, n, cache->kv_heads, dim, esize, false, "values", &a.in[1]));
+  if (call->q_heads) {
+    PITCH_TRY(paged_vectors(call->queries, n, call->q_heads, dim, esize, false, "queries", &a.q));
+    PITCH_TRY(paged_vectors(call->queries_out, n, call->q_heads, dim, esize, true, "queries' output", &a.q_out));
+    if (call->query_norm) PITCH_TRY(check_aligned(call->query_norm, call->query_norm_bytes, dim * esize, 4, "query norm"));
+  } else if (call->query_norm) {
+    return fail(PITCH_ERR_INVALID_INPUT, "a query norm needs queries");
+  }
+  if (call->key_norm) PITCH_TRY(check_aligned(call->key_norm, call->key_norm_bytes, dim * esize, 4, "key norm"));
+  if ((call->key_norm || call->query_norm) && !(call->eps >= 0.f && call->eps <= 3.0e38f))
+    return fail(PITCH_ERR_INVALID_INPUT, "eps must be finite and not negative");
+  PITCH_TRY(check_aligned(call->slots, call->slots_bytes, n * 8u, 8, "slots"));
+  if (call->positions) {
+    PITCH_TRY(check_aligned(call->positions, call->positions_bytes, n * 8u, 8, "positions"));
+    if (call->rotary_dim < 16 || call->rotary_dim > dim || call->rotary_dim % 16 != 0)
+      return fail(PITCH_ERR_INVALID_INPUT, "rotary dimension %u must be a multiple of 16 in 16...%u", call->rotary_dim, dim);
+    const uint64_t row = 4ull * call->rotary_dim;
+    PITCH_TRY(check_aligned(call->cos, call->table_bytes, row, 4, "RoPE cos"));
+    PITCH_TRY(check_aligned(call->sin, call->table_bytes, row, 4, "RoPE sin"));
+    a.table_rows = call->table_bytes / row;
+  } else if (call->cos || call->sin || call->rotary_dim) {
+    return fail(PITCH_ERR_INVALID_INPUT, "RoPE tables need positions");
+  }
+  int dev = 0;
+  PITCH_TRY(current_device(&dev));
+  BatchDeviceCheck check(dev);
+  PITCH_TRY(paged_cache_device(cache, check));
+  PITCH_TRY(check(call->keys.data, "keys"));
+  PITCH_TRY(check(call->values.data, "values"));
+  PITCH_TRY(check(call->slots, "slots"));
+  if (call->q_heads) {
+    PITCH_TRY(check(call->queries.data, "queries"));
+    PITCH_TRY(check(call->queries_out.data, "queries' output"));
+    if (call->query_norm) PITCH_TRY(check(call->query_norm, "query norm"));
+  }
+  if (call->key_norm) PITCH_TRY(check(call->key_norm, "key norm"));
+  if (call->positions) {
+    PITCH_TRY(check(call->positions, "positions"));
+    PITCH_TRY(check(call->cos, "RoPE cos"));
+    PITCH_TRY(check(call->sin, "RoPE sin"));
+  }
+  a.slots = (const int64_t*)call->slots;
+  a.positions = (const int64_t*)call->positions;
+  a.cos = (const float*)call->cos;
+  a.sin = (const float*)call->sin;
+  a.q_norm = call->query_norm;
+  a.k_norm = call->key_norm;
+  a.tokens = (uint32_t)n;
+  a.q_heads = call->q_heads;
+  a.rotary = call->positions ? call->rotary_dim : 0;
+  a.eps = call->eps;
+  static constexpr hipError_t (*kLaunch[2][3])(const pitch::PagedAppendArgs&, hipStream_t) = {
+      {pitch::launch_paged_append_d64_io0, pitch::launch_paged_append_d64_io1, pitch::launch_paged_append_d64_io2},
+      {pitch::launch_paged_append_d128_io0, pitch::launch_paged_append_d128_io1, pitch::launch_paged_append_d128_io2}};
+  const hipError_t e = kLaunch[dim == 128][call->io_type](a, (hipStream_t)stream);
+  if (e != hipSuccess) return fail(PITCH_ERR_ENCODING_FAILED, "Encoding failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+int pitch_enqueue_paged_decode(const pitch_paged_cache_t* cache, const pitch_paged_decode_t* call, void* stream) {
+  pitch::PagedDecodeArgs a{};
+  PITCH_TRY(paged_cache(cache, &a.pool[0], &a.pool[1], &a.layout));
+  if (!call) return fail(PITCH_ERR_INVALID_INPUT, "call is null");
+  PITCH_TRY(check_io(call->io_type));
+  const uint32_t dim = cache->key_config.dim, esize = io_bytes(call->io_type);
+  if (call->rows < 1 || call->rows > 0x7FFFFFFFull) return fail(PITCH_ERR_INVALID_INPUT, "rows must be in 1...2^31 - 1");
+  PITCH_TRY(check_tables(call->block_tables, call->block_tables_bytes, call->table_width, call->sequences));
+  PITCH_TRY(check_aligned(call->row_starts, call->row_starts_bytes, (call->sequences + 1ull) * 4u, 4, "row starts"));
+  if (call->first_tokens)
+    PITCH_TRY(check_aligned(call->first_tokens, call->first_tokens_bytes, call->sequences * 4ull, 4, "first tokens"));
+  if (!call->keys.data && !call->values.data) return fail(PITCH_ERR_INVALID_INPUT, "keys and values are both null");
+  if (call->keys.data) PITCH_TRY(paged_vectors(call->keys, call->rows, cache->kv_heads, dim, esize, true, "keys", &a.out[0]));
+  if (call->values.data)
+    PITCH_TRY(paged_vectors(call->values, call->rows, cache->kv_heads, dim, esize, true, "values", &a.out[1]));
+  int dev = 0;
+  PITCH_TRY(current_device(&dev));
+  BatchDeviceCheck check(dev);
+  PITCH_TRY(paged_cache_device(cache, check));
+  PITCH_TRY(check(call->block_tables, "page tables"));
+  PITCH_TRY(check(call->row_starts, "row starts"));
+  if (call->first_tokens) PITCH_TRY(check(call->first_tokens, "first tokens"));
+  if (call->keys.data) PITCH_TRY(check(call->keys.data, "keys"));
+  if (call->values.data) PITCH_TRY(check(call->values.data, "values"));
+  a.tables = (const int32_t*)call->block_tables;
+  a.row_starts = (const int32_t*)call->row_starts;
+  a.first_tokens = (const int32_t*)call->first_tokens;
+  a.table_width = (uint32_t)call->table_width;
+  a.sequences = call->sequences;
+  a.rows = (uint32_t)call->rows;
+  static constexpr hipError_t (*kLaunch[2][3])(const pitch::PagedDecodeArgs&, hipStream_t) = {
+      {pitch::launch_paged_decode_d64_io0, pitch::launch_paged_decode_d64_io1, pitch::launch_paged_decode_d64_io2},
+      {pitch::launch_paged_decode_d128_io0, pitch::launch_paged_decode_d128_io1, pitch::launch_paged_decode_d128_io2}};
+  const hipError_t e = kLaunch[dim == 128][call->io_type](a, (hipStream_t)stream);
+  if (e != hipSuccess) return fail(PITCH_ERR_DECODING_FAILED, "Decoding failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+int pitch_paged_attention_workspace_size(const pitch_paged_cache_t* cache, const pitch_paged_attention_t* call, uint64_t* bytes) {
+  pitch::PagedAttnArgs a{};
+  PITCH_TRY(paged_cache(cache, &a.k, &a.v, &a.layout));
+  PITCH_TRY(validate_paged_attention(cache, call));
+  if (!bytes) return fail(PITCH_ERR_INVALID_INPUT, "bytes is null");
+  int dev = 0;
+  PITCH_TRY(current_device(&dev));
+  *bytes = 4u * pitch::paged_attention_workspace_floats(cache->key_config.dim, call->q_per_kv, (uint32_t)pitch::device_cu_count());
+  return ok();
+}
+
+int pitch_enqueue_paged_attention(const pitch_paged_cache_t* cache, const pitch_paged_attention_t* call, void* stream) {
+  pitch::PagedAttnArgs a{};
+  PITCH_TRY(paged_cache(cache, &a.k, &a.v, &a.layout));
+  PITCH_TRY(validate_paged_attention(cache, call));
+  PITCH_TRY(check_io(call->io_type));
+  if (call->io_type == PITCH_IO_F32)
+    return fail(PITCH_ERR_INVALID_INPUT, "paged attention takes float16 or bfloat16 queries");
+  const uint32_t dim = cache->key_config.dim, heads = cache->kv_heads * call->q_per_kv;
+  PITCH_TRY(paged_vectors(call->queries, call->sequences, heads, dim, 2, false, "query", &a.q));
+  PITCH_TRY(paged_vectors(call->output, call->sequences, heads, dim, 2, true, "output", &a.out));
+  PITCH_TRY(check_tables(call->block_tables, call->block_tables_bytes, call->table_width, call->sequences));
+  PITCH_TRY(check_aligned(call->lengths, call->lengths_bytes, call->sequences * 4ull, 4, "lengths"));
+  if (call->slopes) PITCH_TRY(check_aligned(call->slopes, call->slopes_bytes, heads * 4ull, 4, "slopes"));
+  if (call->lse) PITCH_TRY(check_aligned(call->lse, call->lse_bytes, (uint64_t)call->sequences * heads * 4u, 4, "lse"));
+  if (!(call->scale >= -3.0e38f && call->scale <= 3.0e38f)) return fail(PITCH_ERR_INVALID_INPUT, "scale must be finite");
+  if (!(call->softcap >= 0.f && call->softcap <= 3.0e38f))
+    return fail(PITCH_ERR_INVALID_INPUT, "softcap must be finite and not negative");
+  if (call->window > 0x7FFFFFFFu) return fail(PITCH_ERR_INVALID_INPUT, "window must be below 2^31");
+  int dev = 0;
+  PITCH_TRY(current_device(&dev));
+  const uint32_t cus = (uint32_t)pitch::device_cu_count();
+  const uint64_t ws = 4u * pitch::paged_attention_workspace_floats(dim, call->q_per_kv, cus);
+  if (ws) PITCH_TRY(check_aligned(call->workspace, call->workspace_bytes, ws, 16, "workspace"));
+  BatchDeviceCheck check(dev);
+  PITCH_TRY(paged_cache_device(cache, check));
+  PITCH_TRY(check(call->queries.data, "query"));
+  PITCH_TRY(check(call->output.data, "output"));
+  PITCH_TRY(check(call->block_tables, "page tables"));
+  PITCH_TRY(check(call->lengths, "lengths"));
+  if (call->slopes) PITCH_TRY(check(call->slopes, "slopes"));
+  if (call->lse) PITCH_TRY(check(call->lse, "lse"));
+  if (ws) PITCH_TRY(check(call->workspace, "workspace"));
+  a.tables = (const int32_t*)call->block_tables;
+  a.lengths = (const int32_t*)call->lengths;
+  a.slopes = (const float*)call->slopes;
+  a.lse = (float*)call->lse;
+  a.ws = (float*)call->workspace;
+  a.table_width = (uint32_t)call->table_width;
+  a.sequences = call->sequences;
+  a.nq = call->q_per_kv;
+  a.window = call->window;
+  a.groups = cus;
+  // the softmax scale, the key decode's 1 / sqrt(d) and log2(e) (scores in log2 units) are folded into the queries; with a
+  // cap the queries give 2 log2(e) x instead, so that exp2 of a product is exp(2 x) of tanh(x) = 1 - 2 / (1 + exp(2 x))
+  constexpr double kLog2E = 1.4426950408889634;
+  const double s = (double)call->scale / __builtin_sqrt((double)dim);
+  a.qscale = (float)(call->softcap > 0.f ? s / call->softcap * 2.0 * kLog2E : s * kLog2E);
+  a.cap = (float)(call->softcap * kLog2E);
+  a.slope_scale = (float)kLog2E;
+  a.oscale = (float)(1.0 / __builtin_sqrt((double)dim));
+  const hipError_t e = dim == 64 ? pitch::launch_paged_attention_d64(a, call->io_type, (hipStream_t)stream)
+                                 : pitch::launch_paged_attention_d128(a, call->io_type, (hipStream_t)stream);
+  if (e != hipSuccess) return fail(PITCH_ERR_DECODING_FAILED, "Attention failed: %s", hipGetErrorString(e));
   return ok();
 }
 

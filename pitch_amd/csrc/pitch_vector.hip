@@ -79,36 +79,6 @@ __device__ __forceinline__ BatchSlot batch_slot(const VecBatchArgs& pb) {
                    (uint64_t)(blockIdx.x - pb.block_start[i]), (uint64_t)(pb.block_start[i + 1] - pb.block_start[i])};
 }
 
-constexpr double kTwoPi = 0x1.921fb54442d18p+2;  // 2 * np.pi
-
-// Fast PolarQuant quantisation. A radius or angle code is floor(t) with t = value * levels + 0.5
-// (pitch_reference.py:116-117). The encoder first evaluates t in float32; when t is at least kPolarGuard
-// from an integer, floor(t) is certain and used. Otherwise (and for a pair at the origin) the float64 path
-// that follows the reference's operation order decides. kPolarGuard is about four times the worst float32
-// error of t at b = 8 (radius: under 7e-5; angle: under 1e-4), so only pairs within 3e-4 of a rounding
-// point take the float64 path.
-constexpr float kPolarGuard = 3e-4f;
-
-// theta / (2 pi) in [0, 1] of the direction (a, c) = atan2(c, a) mod 2 pi, in float32: octant reduction and
-// atan(z) = z * P(z^2) on [0, 1] with the least-squares polynomial gen_tables.py fits for bit width B, whose
-// error keeps t = turns * 2^B + 0.5 within 1e-4 of its exact value.
-template <int B>
-__device__ __forceinline__ float angle_turns(float c, float a) {
-  constexpr int DEG = pitch_atan_degree(B);
-  const float ax = __builtin_fabsf(a), ay = __builtin_fabsf(c);
-  const float mx = __builtin_fmaxf(ax, ay), mn = __builtin_fminf(ax, ay);
-  const float z = mn * __builtin_amdgcn_rcpf(mx);
-  const float s = z * z;
-  float poly = pitch_atan_coef[DEG][DEG];
-#pragma unroll
-  for (int i = DEG - 1; i >= 0; --i) poly = __builtin_fmaf(poly, s, pitch_atan_coef[DEG][i]);
-  float at = poly * z;                                   // atan(mn / mx) in [0, pi / 4]
-  if (ay > ax) at = 0x1.921fb6p+0f - at;                 // pi / 2 - at
-  if (a < 0.f) at = 0x1.921fb6p+1f - at;                 // pi - at
-  const float turns = at * 0x1.45f306p-3f;               // / (2 pi), in [0, 0.5]
-  return c < 0.f ? 1.f - turns : turns;
-}
-
 // Radius and angle codes of the pair (a, c) with r2 = a^2 + c^2 in float64, in the reference's order
 // (pitch_reference.py:111-117): floor(r / rmax * (2^B - 1) + 0.5) clipped, floor(theta / 2 pi * 2^B + 0.5)
 // mod 2^B with theta = atan2(c, a) mod 2 pi. Out of line: only pairs near a rounding point come here.
@@ -122,14 +92,6 @@ __device__ __attribute__((noinline)) uint2 polar_codes_exact(double a, double c,
   if (th < 0.0) th += kTwoPi;  // np.mod(theta, 2 pi) for theta in [-pi, 0)
   const double tq = __builtin_floor(th / kTwoPi * N + 0.5);
   return make_uint2((uint32_t)rq, (uint32_t)tq & (uint32_t)(L - 1));
-}
-
-// floor(t) when t is at least kPolarGuard from an integer (then ok is left alone), else ok = false.
-__device__ __forceinline__ float guarded_floor(float t, bool& ok) {
-  const float k = __builtin_floorf(t);
-  const float f = t - k;
-  ok = ok && f > kPolarGuard && f < 1.f - kPolarGuard;
-  return k;
 }
 
 // The staged-stage PolarQuant encoder's angle in sector units, w = (atan2(c, a) mod 2 pi) * 2^B / (2 pi) in
