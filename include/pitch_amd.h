@@ -363,7 +363,7 @@ typedef struct pitch_paged_cache {
   void* value_scales;
   uint64_t value_scales_bytes;
   uint64_t pages;       /* pages * page_size < 2^32 */
-  uint64_t page_stride; /* vectors from page to page, at least kv_heads * page_size */
+  uint64_t page_stride; /* vectors from page to page, at least kv_heads * page_size, below 2^25 */
   uint32_t page_size;   /* token slots of a page: a multiple of 16, at most 65536 */
   uint32_t kv_heads;    /* 1..65535 */
   uint32_t layout;      /* PITCH_PAGES_* */

@@ -12,6 +12,8 @@
   encoder's fast angle path (atan_poly), each checked here against the exact answer.
 * For the PolarQuant encoder's angle codes at b <= 5: the tangents of the sector boundaries inside the first
   octant, RN(tan((k - 1/2) 2 pi / 2^b)) for k = 1 .. ceil(2^b / 8) (sector_tans).
+* For paged attention: factors at which table values lose least as float16 (f16_factor), and the values of every code pair of
+  two to four bits times that factor as float16, with the float16 values of what that leaves.
 
 Usage: python gen_tables.py <codebooks.json> <out.inc>
 """
@@ -127,6 +129,20 @@ def sector_tans(b: int) -> np.ndarray:
     return t
 
 
+def f16_factor(values: np.ndarray) -> tuple[float, float]:
+    """The factor in [2^12, 2^13), of 2^16 tried, at which rounding factor * values to float16 is off least, and how much (2-norm
+    over 2-norm). A codebook of eight magnitudes (four bits) has a factor with 4e-5, five times less than a power of two."""
+    m = np.unique(np.abs(values.astype(np.float64)))
+    f = (4096.0 * (1 + np.arange(1 << 16) / (1 << 16))).astype(np.float32).astype(np.float64)
+    off = np.zeros(len(f))
+    for v in m:
+        x = f * v
+        off += ((x.astype(np.float32).astype(np.float16).astype(np.float64) - x) / f) ** 2
+    i = int(off.argmin())
+    assert f[i] * m.max() < 60000
+    return float(f[i]), float(np.sqrt(off[i] / (m * m).sum()))
+
+
 def main(src: str, dst: str) -> None:
     books = json.loads(open(src).read())
     cb_all, edge_all = [], []
@@ -208,6 +224,51 @@ def main(src: str, dst: str) -> None:
     # sector-boundary tangents: row b - 2 holds the ceil(2^b / 8) tangents of bit width b (zero-padded)
     rows = ["{" + _floats(list(sector_tans(b)) + [0.0] * (4 - len(sector_tans(b)))) + "}" for b in SECTOR_BITS]
     lines.append(f"static constexpr float pitch_sector_tan[{len(rows)}][4] = {{{','.join(rows)}}};")
+    # float16 factors: rows TurboQuant d = 64, 128, PolarQuant (pair tables up to four bits, radii above), columns b = 2 .. 8
+    rows = []
+    for d in (64, 128, 0):
+        row = []
+        for b in BITS:
+            if d:
+                v = np.array(books[f"{d}_{b}"], dtype=np.float32)
+            else:
+                k = np.arange(2 ** b) / 2 ** b * 2 * np.pi
+                v = np.arange(2 ** b) / (2 ** b - 1)
+                v = np.outer(v, np.cos(k)).ravel() if b <= 4 else v
+            row.append(f16_factor(v)[0])
+        rows.append("{" + _floats(row) + "}")
+    lines.append(f"static constexpr float pitch_f16_factor_tab[3][7] = {{{','.join(rows)}}};")
+    lines.append("static constexpr float pitch_f16_factor(int log2d, bool polar, int bits) "
+                 "{ return pitch_f16_factor_tab[polar ? 2 : log2d - 6][bits - 2]; }")
+    # code pairs: (hi, lo) words, each the pair's two float16 values; rows TurboQuant d = 64, 128, PolarQuant of 336 pairs each:
+    # 16 of two bits, 64 of three, 256 of four
+    words = []
+    f32 = np.float32
+    for row, d in enumerate((64, 128, 0)):
+        for b in (2, 3, 4):
+            L = 2 ** b
+            c0, c1 = np.arange(L * L) & (L - 1), np.arange(L * L) >> b
+            if d:
+                cb = np.array(books[f"{d}_{b}"], dtype=f32)
+                x, y = cb[c0], cb[c1]
+            else:
+                o = poffs[b]
+                r, c, sn = (np.array(t[o:o + L], dtype=f32) for t in (rad, cos_, sin_))
+                x, y = (r[c0] * c[c1]).astype(f32), (r[c0] * sn[c1]).astype(f32)
+            if d:
+                v = np.array(books[f"{d}_{b}"], dtype=f32)
+            else:
+                k = np.arange(L) / L * 2 * np.pi
+                v = np.outer(np.arange(L) / (L - 1), np.cos(k)).ravel()
+            fac = f32(f16_factor(v)[0])
+            x, y = (x * fac).astype(f32), (y * fac).astype(f32)
+            hx, hy = x.astype(np.float16), y.astype(np.float16)
+            lx, ly = (x - hx.astype(f32)).astype(np.float16), (y - hy.astype(f32)).astype(np.float16)
+            bits16 = [t.view(np.uint16).astype(np.uint32) for t in (hx, hy, lx, ly)]
+            words.extend(np.stack([bits16[0] | bits16[1] << 16, bits16[2] | bits16[3] << 16], 1).ravel().tolist())
+    lines.append(f"static __device__ const uint32_t pitch_pair16_tab[{len(words)}] = {{{','.join(str(int(w)) for w in words)}}};")
+    lines.append("static constexpr int pitch_pair16_offset(int log2d, bool polar, int bits) "
+                 "{ return (polar ? 2 : log2d - 6) * 336 + (bits == 2 ? 0 : bits == 3 ? 16 : 80); }")
     for b in BITS:
         assert poffs[b] == (1 << b) - 4
     open(dst, "w").write("\n".join(lines) + "\n")

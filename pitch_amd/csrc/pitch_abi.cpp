@@ -566,8 +566,6 @@ int device_cu_count() {
   return n;
 }
 
-uint64_t paged_attention_workspace_floats(uint32_t, uint32_t, uint32_t) { return 0; }
-
 uint32_t attention_chunk_tokens(uint64_t tokens, uint32_t kv_heads) {
   // The largest chunk that still gives at least PITCH_ATTN_MIN_WG workgroups (512: two per compute unit; 1024 and
   // 2048 measured 0-51 % slower), between 128 and 1024 tokens; PITCH_ATTN_CHUNK (a compile-time tuning macro:
@@ -1294,10 +1292,8 @@ int paged_cache(const pitch_paged_cache_t* c, pitch::PagedPool* k, pitch::PagedP
   if (c->page_stride < page)
     return fail(PITCH_ERR_INVALID_INPUT, "page stride %llu does not hold the page's %llu vectors",
                 (unsigned long long)c->page_stride, (unsigned long long)page);
-  if (c->page_stride > (1ull << 40)) return fail(PITCH_ERR_INVALID_INPUT, "page stride is too large");
-  // pages < 2^31 and page_stride <= 2^40: divide instead of multiplying past 2^64
-  if (c->pages > 1 && c->page_stride > (UINT64_MAX / 256u - page) / (c->pages - 1))
-    return fail(PITCH_ERR_INVALID_INPUT, "page stride is too large");
+  // (a page's codes, at most 128 bytes a vector, are addressed with 32 bits)
+  if (c->page_stride >= (1ull << 25)) return fail(PITCH_ERR_INVALID_INPUT, "page stride must be below 2^25 vectors");
   const uint64_t vectors = (c->pages - 1) * c->page_stride + page;
   const pitch_config_t* cfg[2] = {&c->key_config, &c->value_config};
   void* const codes[2] = {c->key_codes, c->value_codes};
@@ -1378,12 +1374,10 @@ int check_tables(const void* tables, uint64_t bytes, uint64_t width, uint32_t se
 
 int validate_paged_attention(const pitch_paged_cache_t* cache, const pitch_paged_attention_t* call) {
   if (!call) return fail(PITCH_ERR_INVALID_INPUT, "call is null");
-  if (call->sequences < 1 || call->sequences > 0x7FFFFFFFu)
-    return fail(PITCH_ERR_INVALID_INPUT, "sequences must be in 1...2^31 - 1");
+  if (call->sequences < 1 || call->sequences > pitch::kPagedMostSequences)
+    return fail(PITCH_ERR_INVALID_INPUT, "sequences must be in 1...%u", pitch::kPagedMostSequences);
   if (call->q_per_kv < 1 || call->q_per_kv > 8)
     return fail(PITCH_ERR_INVALID_INPUT, "query heads per KV head %u must be in 1...8", call->q_per_kv);
-  if ((uint64_t)call->sequences * cache->kv_heads > 0x7FFFFFFFull)
-    return fail(PITCH_ERR_INVALID_INPUT, "sequences times KV heads must be below 2^31");
   return PITCH_OK;
 }
 
@@ -1506,7 +1500,8 @@ int pitch_paged_attention_workspace_size(const pitch_paged_cache_t* cache, const
   if (!bytes) return fail(PITCH_ERR_INVALID_INPUT, "bytes is null");
   int dev = 0;
   PITCH_TRY(current_device(&dev));
-  *bytes = 4u * pitch::paged_attention_workspace_floats(cache->key_config.dim, call->q_per_kv, (uint32_t)pitch::device_cu_count());
+  *bytes = 4u * pitch::paged_attention_workspace_floats(cache->key_config.dim, call->q_per_kv, call->sequences,
+                                                        (uint32_t)pitch::device_cu_count());
   return ok();
 }
 
@@ -1527,12 +1522,17 @@ int pitch_enqueue_paged_attention(const pitch_paged_cache_t* cache, const pitch_
   if (!(call->scale >= -3.0e38f && call->scale <= 3.0e38f)) return fail(PITCH_ERR_INVALID_INPUT, "scale must be finite");
   if (!(call->softcap >= 0.f && call->softcap <= 3.0e38f))
     return fail(PITCH_ERR_INVALID_INPUT, "softcap must be finite and not negative");
+  // tokens of a sequence and tiles of the call are counted in 32 bits
+  const uint64_t most = call->table_width * cache->page_size;
+  if (most > 0x7FFFFFFFull || ((most >> 6) + 2) * call->sequences * cache->kv_heads > 0x7FFFFFFFull)
+    return fail(PITCH_ERR_INVALID_INPUT, "page tables of %u x %llu pages hold too many tokens", call->sequences,
+                (unsigned long long)call->table_width);
   if (call->window > 0x7FFFFFFFu) return fail(PITCH_ERR_INVALID_INPUT, "window must be below 2^31");
   int dev = 0;
   PITCH_TRY(current_device(&dev));
   const uint32_t cus = (uint32_t)pitch::device_cu_count();
-  const uint64_t ws = 4u * pitch::paged_attention_workspace_floats(dim, call->q_per_kv, cus);
-  if (ws) PITCH_TRY(check_aligned(call->workspace, call->workspace_bytes, ws, 16, "workspace"));
+  const uint64_t ws = 4u * pitch::paged_attention_workspace_floats(dim, call->q_per_kv, call->sequences, cus);
+  PITCH_TRY(check_aligned(call->workspace, call->workspace_bytes, ws, 16, "workspace"));
   BatchDeviceCheck check(dev);
   PITCH_TRY(paged_cache_device(cache, check));
   PITCH_TRY(check(call->queries.data, "query"));
@@ -1541,7 +1541,7 @@ int pitch_enqueue_paged_attention(const pitch_paged_cache_t* cache, const pitch_
   PITCH_TRY(check(call->lengths, "lengths"));
   if (call->slopes) PITCH_TRY(check(call->slopes, "slopes"));
   if (call->lse) PITCH_TRY(check(call->lse, "lse"));
-  if (ws) PITCH_TRY(check(call->workspace, "workspace"));
+  PITCH_TRY(check(call->workspace, "workspace"));
   a.tables = (const int32_t*)call->block_tables;
   a.lengths = (const int32_t*)call->lengths;
   a.slopes = (const float*)call->slopes;
@@ -1551,6 +1551,7 @@ int pitch_enqueue_paged_attention(const pitch_paged_cache_t* cache, const pitch_
   a.sequences = call->sequences;
   a.nq = call->q_per_kv;
   a.window = call->window;
+  a.most_tokens = (uint32_t)most;
   a.groups = cus;
   // the softmax scale, the key decode's 1 / sqrt(d) and log2(e) (scores in log2 units) are folded into the queries; with a
   // cap the queries give 2 log2(e) x instead, so that exp2 of a product is exp(2 x) of tanh(x) = 1 - 2 / (1 + exp(2 x))
@@ -1560,8 +1561,12 @@ int pitch_enqueue_paged_attention(const pitch_paged_cache_t* cache, const pitch_
   a.cap = (float)(call->softcap * kLog2E);
   a.slope_scale = (float)kLog2E;
   a.oscale = (float)(1.0 / __builtin_sqrt((double)dim));
-  const hipError_t e = dim == 64 ? pitch::launch_paged_attention_d64(a, call->io_type, (hipStream_t)stream)
-                                 : pitch::launch_paged_attention_d128(a, call->io_type, (hipStream_t)stream);
+  static constexpr hipError_t (*kLaunch[2][4])(const pitch::PagedAttnArgs&, uint32_t, hipStream_t) = {
+      {pitch::launch_paged_attention_d64_k2, pitch::launch_paged_attention_d64_k3, pitch::launch_paged_attention_d64_k4,
+       pitch::launch_paged_attention_d64_k0},
+      {pitch::launch_paged_attention_d128_k2, pitch::launch_paged_attention_d128_k3, pitch::launch_paged_attention_d128_k4,
+       pitch::launch_paged_attention_d128_k0}};
+  const hipError_t e = kLaunch[dim == 128][std::min(a.k.bits, 5u) - 2](a, call->io_type, (hipStream_t)stream);
   if (e != hipSuccess) return fail(PITCH_ERR_DECODING_FAILED, "Attention failed: %s", hipGetErrorString(e));
   return ok();
 }

@@ -66,11 +66,17 @@ struct PagedAttnArgs {
   float* lse;                // [sequences][query heads] or null
   float* ws;
   uint32_t table_width, sequences, nq, window;
+  uint32_t most_tokens;      // table_width * page_size
   float qscale;              // what the rotated queries are multiplied by
   float cap;                 // scores are cap * tanh(x) when positive (log2 units), else x
   float slope_scale;         // log2(e): slopes to log2 units
   float oscale;              // 1 / sqrt(dim) of the value decode
+  float kfactor, vfactor;    // the tables' factors and their reciprocals (set by the launcher)
+  float kinv, vinv;
   uint32_t groups;           // workgroups
+  uint32_t groups_r, page_r; // floor((2^32 - 1) / d) of groups and of page_size / 16 (set by the launcher, as the next two)
+  uint32_t tile_cols, tile_rest;  // 64 tokens as pages and the rest
+  uint32_t kpage, vpage, khead, vhead, kslot, vslot;  // bytes of codes from page to page, head to head, slot to slot
 };
 
 #define PITCH_DECLARE_PAGED(D, IO)                                                     \
@@ -84,9 +90,21 @@ PITCH_DECLARE_PAGED(128, 1)
 PITCH_DECLARE_PAGED(128, 2)
 #undef PITCH_DECLARE_PAGED
 
-// Floats of workspace of a call with nq query heads per KV head on a device of cus compute units.
-uint64_t paged_attention_workspace_floats(uint32_t dim, uint32_t nq, uint32_t cus);
-hipError_t launch_paged_attention_d64(const PagedAttnArgs& a, uint32_t io, hipStream_t s);
-hipError_t launch_paged_attention_d128(const PagedAttnArgs& a, uint32_t io, hipStream_t s);
+// Attention: most sequences of a call (their tiles' prefix sum lies in LDS), most waves of a workgroup, floats of a partial
+// result (maxima and sums of eight heads, accumulators of nh heads), floats of workspace of a call.
+constexpr uint32_t kPagedMostSequences = 2048;
+constexpr uint32_t kPagedAttnWaves = 8;
+constexpr uint32_t paged_slot_floats(uint32_t dim, uint32_t nh) { return 16 + dim * nh; }
+constexpr uint64_t paged_attention_workspace_floats(uint32_t dim, uint32_t nq, uint32_t sequences, uint32_t groups) {
+  return ((sequences + 4ull) & ~3ull) + 2ull * groups * kPagedAttnWaves * paged_slot_floats(dim, nq <= 4 ? 4 : 8);
+}
+#define PITCH_DECLARE_PAGED_ATTN(K)                                                             \
+  hipError_t launch_paged_attention_d64_k##K(const PagedAttnArgs& a, uint32_t io, hipStream_t s); \
+  hipError_t launch_paged_attention_d128_k##K(const PagedAttnArgs& a, uint32_t io, hipStream_t s);
+PITCH_DECLARE_PAGED_ATTN(0)
+PITCH_DECLARE_PAGED_ATTN(2)
+PITCH_DECLARE_PAGED_ATTN(3)
+PITCH_DECLARE_PAGED_ATTN(4)
+#undef PITCH_DECLARE_PAGED_ATTN
 
 }  // namespace pitch

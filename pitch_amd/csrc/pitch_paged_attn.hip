@@ -1,183 +1,1099 @@
-// Attention of one new token of every sequence over a paged cache, for one dimension (PITCH_DIM = 64 or 128).
+// Attention of one new token of every sequence over a paged cache, for one dimension (PITCH_DIM = 64 or 128) and one width of
+// the key codes (PITCH_KB = 2, 3, 4; 0 for the widths 5 to 8).
 //
-// out = softmax(z) V with z_t = cap tanh(scale q . k_t / cap) + slope (t - (L - 1)) over the tokens t of [L - window, L).
-// No token is decoded: k_t = s H c(code_t) n_t / sqrt(d), so a query is rotated once (H s q), scores are its products
-// with the table values of the codes times the token's scale, and the weighted table values are rotated back once.
-#include "pitch_device.h"
+//   out = softmax(z) V,  z_t = cap tanh(scale q . k_t / cap) + slope (t - (L - 1)),  t in [L - window, L)
+//
+// No token is decoded: k_t = s H c(code_t) n_t / sqrt(d), so a query is rotated once (H s q), scores are its products with the
+// table values of the codes times the token's scale, and the weighted table values are rotated back once.
+//
+// Work split. The sequences' tiles of 64 tokens, sequence by sequence and KV head by KV head, form one line that is cut into
+// equal runs, one per workgroup (one per compute unit), and each run into equal runs of its waves: a batch of any lengths loads
+// every wave alike, and only the host-known number of workgroups is launched. A wave goes through its run by itself (scores,
+// online softmax, weighted values; no barrier), pair of sequence and KV head by pair. A pair that lies in one wave is written by
+// it; the others leave partial results: the last one of each wave is merged with its neighbours' of the same pair through LDS,
+// and paged_join merges what remains through the workspace, in an order fixed by the lengths alone.
+//
+// Contractions on the 16-bit matrix cores (v_mfma_f32_16x16x32_f16), 16 rows of one operand for a KV head's query heads. A code
+// pair is looked up in LDS as two float16 values, which are operand words as they are: for the scores two neighbouring
+// coordinates of a token on the contraction axis; for the values a pair's two coordinates of one token side by side on it, with
+// the weight at the one or the other: rows 0 - 7 weigh the first coordinate, rows 8 - 15 the second. What rows remain hold the
+// operands' rest after rounding to float16: up to four heads, queries and weights both in two parts (22 bits); five to eight
+// heads, the queries in two, the weights in one (11 bits). TurboQuant's table values are stored times a factor at which they
+// nearly are float16 values (gen_tables.py: 4e-5 of a codebook's size for four bits, instead of 2e-4). With float16 queries the
+// keys' table values have two parts as well, whose products are added by a second instruction: a rounding of 2e-4 in the keys
+// moves a score of size 5 by 1e-3, several times what float16 outputs resolve (bfloat16: a quarter).
+//
+// The table's entry of a pair (four codes for two bits) is 256 bytes long, copies for the keys in its first half and for the
+// values in its second (float16 queries: a table each): lanes read copies in different banks, and where the index is a byte of
+// the row, one v_perm makes the address.
+#include "pitch_attn_shared.h"
 #include "pitch_paged.h"
 
 #ifndef PITCH_DIM
 #error "compile with -DPITCH_DIM=<dim>"
+#endif
+#ifndef PITCH_KB
+#error "compile with -DPITCH_KB=<key bits>"
 #endif
 
 namespace pitch {
 namespace {
 
 constexpr int D = PITCH_DIM;
-constexpr int kChunk = 256;
-constexpr float kLn2 = 0x1.62e430p-1f;
+constexpr int NC = D / 32;       // groups of 16 pairs: accumulators of a wave
+constexpr int KS = D / 32;       // score instructions per 16 tokens
+constexpr int kPRow = 68;        // dwords of a row of staged weights
+constexpr float kLoScale = 2048.f;
+constexpr float kTop = 32768.f;  // largest weight in an operand
 
-typedef uint32_t u32_any __attribute__((aligned(1)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint64_t u64_any __attribute__((aligned(1)));
+typedef __attribute__((address_space(3))) const uint32_t lds_cu32;
+typedef __attribute__((address_space(3))) const u2 lds_cu2;
+typedef __attribute__((address_space(3))) const w4 lds_cw4;
 
-__device__ void load_tab(const PagedPool& p, float* tab) {
-  const int levels = 1 << p.bits;
-  for (int i = threadIdx.x; i < levels; i += kChunk) {
-    if (p.polar) {
-      const int off = pitch_polar_offset(p.bits);
-      tab[i] = pitch_polar_radius_tab[off + i];
-      tab[256 + i] = pitch_polar_cos_tab[off + i];
-      tab[512 + i] = pitch_polar_sin_tab[off + i];
-    } else {
-      tab[i] = pitch_codebook_tab[pitch_codebook_offset(ilog2(D), p.bits) + i];
+constexpr int W = 8;   // waves of a workgroup: two per SIMD (256 registers each)
+static_assert(W <= (int)kPagedAttnWaves, "waves of a workgroup");
+
+__device__ __forceinline__ uint32_t f16_pair(float a, float b) { return narrow2<1>(a, b); }
+
+// ---------------------------------------------------------------------------------------------------- tables
+// Bytes of LDS of a table: 256 bytes per entry.
+constexpr uint32_t table_bytes(int b) { return b == 3 ? 64u * 256u : 65536u; }
+// With two parts of the keys the tables follow each other, else they share their entries. A table of 64 KB begins at a multiple
+// of its size: its lane bytes hold the base in their third byte, which v_perm passes on.
+constexpr uint32_t key_base(int kb, int vb, bool two) { return two && kb == 3 && vb != 3 ? 65536u : 0u; }
+constexpr uint32_t value_base(int kb, int vb, bool two) { return !two ? 128u : kb != 3 ? 65536u : vb != 3 ? 0u : 16384u; }
+constexpr uint32_t tables_bytes(int kb, int vb, bool two) {
+  return two ? table_bytes(kb) + table_bytes(vb) : table_bytes(kb) > table_bytes(vb) ? table_bytes(kb) : table_bytes(vb);
+}
+
+// What float16 rounding leaves of a pair of values: (the values as float16, the rests as float16).
+__device__ __forceinline__ u2 split_pair(float x, float y) {
+  const uint32_t hi = f16_pair(x, y);
+  float a, b;
+  widen2<1>(hi, a, b);
+  return u2{hi, f16_pair(x - a, y - b)};
+}
+
+// A table for codes of B bits (0: p.bits), of the values (TWO false) or of keys in two parts (TWO), in two steps: a thread's
+// source values are loaded when the kernel begins, and written to LDS when other loads are on their way.
+//   B = 3, 4, two codes: 32 copies of the pair, or of its two parts
+//   B = 2, four codes: 16 copies of two pairs, or of their two parts
+//   B = 0, one code: 16 copies of (value at an even coordinate, 1), then of (1, value at an odd one), PolarQuant (radius, radius)
+//     and (cosine, sine): a pair's values are the products. TWO: 32 copies of the value's two parts; PolarQuant 16 copies of the
+//     radius, then of (cosine, sine), as float32.
+template <int B, bool TWO>
+struct Table {
+  static constexpr int kEntries = B == 2 || B == 0 ? 256 : 1 << (2 * B);
+  static constexpr int R = (kEntries * 4 + 64 * W - 1) / (64 * W);   // quarters of entries per thread
+  uint32_t x[R][B == 0 ? 3 : B == 2 ? 4 : 2];
+
+  __device__ __forceinline__ void load(const PagedPool& p, int tid) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const uint32_t e = min((uint32_t)(tid + r * 64 * W) >> 2, (uint32_t)kEntries - 1u);
+      if constexpr (B == 0) {
+        const uint32_t c = min(e, (1u << p.bits) - 1u);
+        if (p.polar) {
+          const int off = pitch_polar_offset(p.bits) + c;
+          x[r][0] = __float_as_uint(pitch_polar_radius_tab[off]);
+          x[r][1] = __float_as_uint(pitch_polar_cos_tab[off]);
+          x[r][2] = __float_as_uint(pitch_polar_sin_tab[off]);
+        } else {
+          x[r][0] = __float_as_uint(pitch_codebook_tab[pitch_codebook_offset(ilog2(D), p.bits) + c]);
+          x[r][1] = x[r][2] = 0u;
+        }
+      } else {
+        const u2* const tab = (const u2*)pitch_pair16_tab + pitch_pair16_offset(ilog2(D), p.polar != 0, B);
+        const u2 v = tab[B == 2 ? e & 15u : e];
+        x[r][0] = v.x;
+        x[r][1] = v.y;
+        if constexpr (B == 2) {
+          const u2 w = tab[e >> 4];
+          x[r][2] = w.x;
+          x[r][3] = w.y;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void write(uint32_t* tab, const PagedPool& p, float factor, int tid) const {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = tid + r * 64 * W;
+      if (i >= kEntries * 4) break;
+      const uint32_t e = (uint32_t)i >> 2;
+      w4* const at = (w4*)(tab + 64 * e) + (TWO ? 4 : 2) * (i & 3);
+      w4* const one = (w4*)(tab + 64 * e) + (i & 3);
+      if constexpr (B == 2) {
+        const w4 w = TWO ? w4{x[r][0], x[r][2], x[r][1], x[r][3]} : w4{x[r][0], x[r][2], x[r][0], x[r][2]};
+#pragma unroll
+        for (int k = 0; k < (TWO ? 4 : 2); ++k) at[k] = w;
+      } else if constexpr (B != 0) {
+        const w4 w = TWO ? w4{x[r][0], x[r][1], x[r][0], x[r][1]} : w4{x[r][0], x[r][0], x[r][0], x[r][0]};
+#pragma unroll
+        for (int k = 0; k < (TWO ? 4 : 2); ++k) at[k] = w;
+      } else {
+        const float v = __uint_as_float(x[r][0]) * factor, c = __uint_as_float(x[r][1]), n = __uint_as_float(x[r][2]);
+        if constexpr (TWO) {
+          if (p.polar) {
+            const uint32_t u = __float_as_uint(v);
+            one[0] = w4{u, u, u, u};
+            one[4] = one[8] = w4{x[r][1], x[r][2], x[r][1], x[r][2]};
+          } else {
+            const u2 s = split_pair(v, 0.f);
+            const uint32_t u = (s.x & 0xFFFFu) | s.y << 16;
+            one[0] = one[4] = w4{u, u, u, u};
+          }
+        } else {
+          const uint32_t even = f16_pair(v, p.polar ? v : 1.f), odd = p.polar ? f16_pair(c, n) : f16_pair(1.f, v);
+          one[0] = w4{even, even, even, even};
+          one[4] = w4{odd, odd, odd, odd};
+        }
+      }
+    }
+  }
+};
+
+// A lane's byte of an entry.
+template <int B, bool TWO>
+__device__ __forceinline__ uint32_t lane_byte(int lane) {
+  if constexpr (B == 2) return (uint32_t)(lane & 15) * (TWO ? 16u : 8u);
+  if constexpr (B == 0) return TWO ? (uint32_t)(lane & 31) * 4u : (uint32_t)(lane & 15) * 4u;
+  return (uint32_t)(lane & 31) * (TWO ? 8u : 4u);
+}
+
+__device__ __forceinline__ uint32_t product(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, a) * __builtin_bit_cast(f16x2, b));
+}
+
+// The COUNT pairs of 2 COUNT codes: the N words w hold the codes from bit `at` on (constants); the widths above four bits have
+// them in w[0], w[1], `bits` bits each. hi: the pairs' float16 values, lo (TWO): their rests.
+template <int B, bool TWO, int COUNT, int N>
+__device__ __forceinline__ void look_pairs(const uint32_t (&w)[N], int at, uint32_t lb, uint32_t bits, bool polar, uint32_t (&hi)[COUNT],
+                                           uint32_t (&lo)[COUNT]) {
+  constexpr uint32_t kSel = 0x0C060004u;   // bytes: the lane's, a byte of the codes, the table's base above 64 KB, 0
+  if constexpr (B == 2) {
+#pragma unroll
+    for (int i = 0; i < COUNT / 2; ++i) {
+      const int p = at + 8 * i;
+      const uint32_t a = __builtin_amdgcn_perm(lb, w[p >> 5], kSel | (uint32_t)((p & 31) >> 3) << 8);
+      if constexpr (TWO) {
+        const w4 v = *(lds_cw4*)(uintptr_t)a;
+        hi[2 * i] = v.x; hi[2 * i + 1] = v.y; lo[2 * i] = v.z; lo[2 * i + 1] = v.w;
+      } else {
+        const u2 v = *(lds_cu2*)(uintptr_t)a;
+        hi[2 * i] = v.x; hi[2 * i + 1] = v.y;
+      }
+    }
+  } else if constexpr (B != 0) {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+      const int p = at + 2 * B * i;
+      uint32_t a;
+      if constexpr (B == 4) a = __builtin_amdgcn_perm(lb, w[p >> 5], kSel | (uint32_t)((p & 31) >> 3) << 8);
+      else a = and_or(bits_at(w, p, 6, 8), 0x3F00u, lb);
+      if constexpr (TWO) {
+        const u2 v = *(lds_cu2*)(uintptr_t)a;
+        hi[i] = v.x; lo[i] = v.y;
+      } else {
+        hi[i] = *(lds_cu32*)(uintptr_t)a;
+      }
+    }
+  } else {
+    uint64_t x = w[0];
+    if constexpr (N > 1) x |= (uint64_t)w[1] << 32;
+    const uint32_t mask8 = ((1u << bits) - 1u) << 8;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+      const uint32_t a0 = ((uint32_t)(x >> (bits * (2 * i))) << 8 & mask8) | lb, a1 = ((uint32_t)(x >> (bits * (2 * i + 1))) << 8 & mask8) | lb;
+      if constexpr (!TWO) {
+        hi[i] = product(*(lds_cu32*)(uintptr_t)a0, *(lds_cu32*)(uintptr_t)(a1 + 64u));
+      } else if (polar) {   // the copies' bytes: 16 of four, then 16 of eight
+        const uint32_t c = lb & 63u;
+        const float r = __uint_as_float(*(lds_cu32*)(uintptr_t)((a0 & ~127u) | c));
+        const u2 v = *(lds_cu2*)(uintptr_t)((a1 & ~127u) + 64u + 2u * c);
+        const u2 t = split_pair(r * __uint_as_float(v.x), r * __uint_as_float(v.y));
+        hi[i] = t.x; lo[i] = t.y;
+      } else {
+        const uint32_t u = *(lds_cu32*)(uintptr_t)a0, v = *(lds_cu32*)(uintptr_t)a1;
+        hi[i] = __builtin_amdgcn_perm(v, u, 0x05040100u);
+        lo[i] = __builtin_amdgcn_perm(v, u, 0x07060302u);
+      }
     }
   }
 }
 
-template <int IO>
-__global__ __launch_bounds__(kChunk) void paged_attn(PagedAttnArgs a) {
-  __shared__ float s_kt[768], s_vt[768], s_q[8][D], s_p[8][kChunk], s_o[8][D], s_red[8], s_m[8], s_l[8], s_al[8];
-  __shared__ uint64_t s_row[kChunk];
-  const int tid = threadIdx.x;
-  const uint32_t b = blockIdx.x / a.layout.kv_heads, kv = blockIdx.x % a.layout.kv_heads, nq = a.nq;
-  load_tab(a.k, s_kt);
-  load_tab(a.v, s_vt);
-  for (int i = tid; i < 8 * D; i += kChunk) {
-    const uint32_t h = i / D, j = i % D;
-    float x = 0.f;
-    if (h < nq) {
-      float f[1];
-      load_elems<IO, 1>(a.q.data, b * a.q.token_stride + (kv * nq + h) * a.q.head_stride + j, f);
-      x = (a.k.signs[j >> 5] >> (j & 31)) & 1 ? -f[0] : f[0];
-    }
-    s_q[h][j] = x;
-    s_o[h][j] = 0.f;
+// ---------------------------------------------------------------------------------------------------- the line of tiles
+struct Span {            // what a sequence's new token sees
+  uint32_t begin, end;   // tokens
+  uint32_t base, tiles;  // the tiles' first token (a multiple of 16), tiles of 64 tokens
+};
+// len: cached tokens, cut to the table.
+__device__ __forceinline__ Span span_of(const PagedAttnArgs& a, uint32_t len) {
+  Span s;
+  s.end = len;
+  s.begin = a.window && s.end > a.window ? s.end - a.window : 0u;
+  s.base = s.begin & ~15u;
+  s.tiles = s.end > s.base ? (s.end - s.base + 63u) >> 6 : 0u;
+  return s;
+}
+__device__ __forceinline__ uint32_t length_of(const PagedAttnArgs& a, uint32_t b) {
+  const int32_t len = a.lengths[b];
+  return len < 0 ? 0u : min((uint32_t)len, a.most_tokens);
+}
+
+// pref[i] = tiles of the sequences before i (one KV head), i = 0 .. sequences; lens[i] = their lengths. `part`: a word per wave.
+// The line's tiles, and its tiles times KV heads, are below 2^31 (checked by the caller).
+__device__ __forceinline__ void scan_tiles(const PagedAttnArgs& a, uint32_t* pref, uint32_t* lens, uint32_t* part, int tid) {
+  const uint32_t n = a.sequences, per = (n + 64 * W - 1) / (64 * W), first = min((uint32_t)tid * per, n), last = min(first + per, n);
+  uint32_t len = first < last ? length_of(a, first) : 0u;
+  uint32_t sum = 0;
+  for (uint32_t i = first; i < last; ++i) {
+    const uint32_t t = span_of(a, len).tiles;
+    lens[i] = len;
+    pref[i] = t;
+    sum += t;
+    if (i + 1 < last) len = length_of(a, i + 1);
   }
-  if (tid < 8) {
-    s_m[tid] = -__FLT_MAX__;
-    s_l[tid] = 0.f;
+  uint32_t inc = sum;
+  const int lane = tid & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint32_t o = (uint32_t)__builtin_amdgcn_ds_bpermute((lane - d) << 2, (int)inc);
+    inc += lane >= d ? o : 0u;
+  }
+  if (lane == 63) part[tid >> 6] = inc;
+  __syncthreads();
+  uint32_t before = inc - sum;
+  for (int w = 0; w < tid >> 6; ++w) before += part[w];
+  for (uint32_t i = first; i < last; ++i) {
+    const uint32_t t = pref[i];
+    pref[i] = before;
+    before += t;
+  }
+  if (last == n && first < n) pref[n] = before;   // one thread has the last sequence
+  __syncthreads();
+}
+
+// How the line of n tiles is cut: tiles per workgroup, and of a workgroup's tiles per wave.
+// x / d for x < 2^31, with r = floor((2^32 - 1) / d): one too small at most before the correction.
+__device__ __forceinline__ uint32_t quotient(uint32_t x, uint32_t d, uint32_t r) {
+  const uint32_t q = __umulhi(x, r);
+  return x - q * d >= d ? q + 1u : q;
+}
+__device__ __forceinline__ uint32_t group_tiles(uint32_t n, const PagedAttnArgs& a) {
+  return quotient(n + a.groups - 1, a.groups, a.groups_r);
+}
+__device__ __forceinline__ uint32_t wave_tiles(uint32_t n, uint32_t per_group, uint32_t g) {
+  return (min(n - g * per_group, per_group) + W - 1) / W;
+}
+
+// The workspace: the prefix (sequences + 1 words, rounded up to 4), then two slots per wave of partial results: maxima and sums of
+// eight heads, and the accumulators as the lanes hold them. The last partial result of a wave (merged with its neighbours': of the
+// first of them) has its first slot, that of a pair which ends inside the wave's run its second.
+constexpr uint32_t slot_floats(int nh) { return 16 + NC * 4 * (nh == 4 ? 32 : 64); }
+
+// ---------------------------------------------------------------------------------------------------- output
+// acc: a lane (n, g) has coordinates 2 (NC n + c) + (g >> 1) of head v (NH = 4) or v + 4 (g & 1); the transform back runs over its
+// registers and across lanes.
+template <int NH, int IO>
+__device__ __forceinline__ void write_output(const PagedAttnArgs& a, uint32_t b, uint32_t kv, v4f (&acc)[NC], const float (&m)[NH],
+                                             const float (&l)[NH], int lane) {
+  const int n = lane & 15, g = lane >> 4;
+  const bool odd = g & 1;
+  const uint32_t upper = odd ? ~0u : 0u;   // this lane has heads 4 - 7 of eight
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    const float total = NH == 8 ? pick(upper, l[v], l[NH - 4 + v]) : l[v];
+    const float f = total > 0.f ? a.oscale / total : 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[c][v]), __float_as_uint(acc[c][v]), false, false);
+      const float x = __uint_as_float(r[0]), y = __uint_as_float(r[1]);
+      acc[c][v] = total > 0.f ? (g >= 2 ? x - y : x + y) * f : 0.f;
+    }
+  }
+#pragma unroll
+  for (int s = 1; s < NC; s *= 2)
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      if (!(c & s)) {
+        const v4f x = acc[c], y = acc[c | s];
+        acc[c] = x + y;
+        acc[c | s] = x - y;
+      }
+  static_for<0, 4>([&](auto bit_c) {
+    constexpr int lm = 1 << decltype(bit_c)::value;
+    const float sg = (n & lm) ? -1.f : 1.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) acc[c][v] = __builtin_fmaf(acc[c][v], sg, xchg<lm>(acc[c][v]));
+  });
+  // pairs of coordinates: lanes g < 2 take heads 0 and 1 (of their four), the others 2 and 3
+  const uint32_t signs = a.v.signs[(2 * NC * n) >> 5] >> ((2 * NC * n) & 31);
+#pragma unroll
+  for (int v = 0; v < 2; ++v) {
+    uint32_t word[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[c][v]), __float_as_uint(acc[c][v + 2]), false, false);
+      word[c] = narrow2<IO>(__uint_as_float(r[0] ^ (signs >> (2 * c) & 1u) << 31), __uint_as_float(r[1] ^ (signs >> (2 * c + 1) & 1u) << 31));
+    }
+    const uint32_t h = (g >= 2 ? v + 2 : v) + (NH == 8 && odd ? 4 : 0);
+    if (h < a.nq && (NH == 8 || !odd)) {
+      uint32_t* dst = (uint32_t*)((uint16_t*)a.out.data + b * a.out.token_stride + (kv * a.nq + h) * a.out.head_stride + 2 * NC * n);
+      store_words<NC>(dst, word);
+    }
+  }
+  if (a.lse && lane == 0) {
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+      if (h < (int)a.nq)
+        a.lse[((uint64_t)b * a.layout.kv_heads + kv) * a.nq + h] = l[h] > 0.f ? (m[h] + log2f(l[h])) * kLn2 : -__builtin_inff();
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------- the kernel
+template <int KB, int VB, int NH, bool TWO>
+struct Lds {  // dwords
+  static constexpr uint32_t kTab = tables_bytes(KB, VB, TWO) / 4;
+  static constexpr uint32_t kMerge = W * (2 * NH + NC * 4 * (NH == 4 ? 32 : 64));
+  static constexpr uint32_t kHead = kTab > kMerge ? kTab : kMerge;
+  static constexpr uint32_t words(uint32_t sequences) { return kHead + W * 4 * kPRow + 2 * W + 2 * sequences + 1; }
+};
+
+template <int KB, int VB, int NH, int IO>
+__global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
+  constexpr bool TWO = IO == 1;
+  using L = Lds<KB, VB, NH, TWO>;
+  constexpr int GC = D / 4;                                  // codes of a key row that one lane group holds
+  constexpr int KW = KB ? (GC * (KB ? KB : 1) + 31) / 32 : GC / 4;   // words a lane holds of them
+  constexpr int RC = D / 16;                                 // codes of a value row that one lane holds
+  constexpr int VW = VB == 0 && D == 128 ? 2 : 1;
+  extern __shared__ __attribute__((aligned(16))) uint32_t s_mem[];   // at LDS address 0
+  uint32_t* const s_stage = s_mem + L::kHead;
+  uint32_t* const s_part = s_stage + W * 4 * kPRow;
+  uint32_t* const s_key = s_part + W;
+  uint32_t* const s_pref = s_key + W;
+  uint32_t* const s_len = s_pref + a.sequences + 1;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const uint32_t wid = __builtin_amdgcn_readfirstlane(tid >> 6), upper = g & 1 ? ~0u : 0u;
+  const uint32_t heads = a.layout.kv_heads;
+
+  Table<KB, TWO> ktab;
+  Table<VB, false> vtab;
+  ktab.load(a.k, tid);
+  vtab.load(a.v, tid);
+  scan_tiles(a, s_pref, s_len, s_part, tid);
+  auto before = [&](uint32_t i) { return __builtin_amdgcn_readfirstlane(s_pref[i]) * heads; };
+  const uint32_t total = before(a.sequences);
+  if (blockIdx.x == 0)
+    for (uint32_t i = tid; i <= a.sequences; i += 64 * W) ((uint32_t*)a.ws)[i] = s_pref[i];
+  const uint32_t per_group = group_tiles(total, a), g0 = blockIdx.x * per_group;
+  if (g0 >= total) return;
+  const uint32_t per_wave = wave_tiles(total, per_group, blockIdx.x), g1 = min(g0 + per_group, total);
+
+  uint32_t x0 = g0 + wid * per_wave;
+  const uint32_t x1 = min(x0 + per_wave, g1);
+  float* const ws = a.ws + ((a.sequences + 4u) & ~3u);
+  const uint32_t slot = blockIdx.x * W + wid;
+  const uint32_t klb = lane_byte<KB, TWO>(lane) + key_base(KB, VB, TWO), vlb = lane_byte<VB, false>(lane) + value_base(KB, VB, TWO);
+  uint32_t* const s_w = s_stage + wid * 4 * kPRow;
+
+  // A part of a pair of sequence and KV head: tiles [.., end) of the line belong to it and to this wave's run.
+  struct Part {
+    uint32_t seq, kv, pair_begin, pair_end, end;
+    bool whole;
+  };
+  // ---- offsets of this lane inside a row of codes
+  const uint32_t kstep = a.kslot;
+  uint32_t koff[KB ? 1 : KW / 2], ksh[KB ? 1 : KW / 2];
+  if constexpr (KB != 0) {
+    koff[0] = (uint32_t)n * kstep + (uint32_t)((GC * KB * g) >> 5) * 4u;
+    ksh[0] = (uint32_t)((GC * KB * g) & 31);
+  } else {  // groups of eight codes, `bits` bytes each, read as eight bytes that stay inside the row
+#pragma unroll
+    for (int i = 0; i < KW / 2; ++i) {
+      const uint32_t at = ((uint32_t)g * (GC / 8) + i) * a.k.bits, lo = min(at, a.k.row_bytes - 8u);
+      koff[i] = (uint32_t)n * kstep + lo;
+      ksh[i] = 8u * (at - lo);
+    }
+  }
+  const uint32_t vbit = (uint32_t)(RC * n) * a.v.bits, vlo = min(vbit >> 3, a.v.row_bytes - 4u * VW), vsh = vbit - 8u * vlo;
+  constexpr bool kShiftV = !(VB == 4 && D == 128);
+
+  // ---- the loads run a tile ahead of the computation: the part of the next tile to load, this lane's page and offset (of its 16
+  // tokens) in it
+  uint32_t xl = x0, seq = 0, tok = 0, col = 0, off = 0, run_end = 0, page = ~0u, span_begin = 0, span_end = 0;
+  Part part{};
+  const int32_t* table = a.tables;
+  if (x0 < x1) {  // the sequence of the first tile
+    uint32_t lo = 0, hi = a.sequences;
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (before(mid) <= x0) lo = mid;
+      else hi = mid;
+    }
+    seq = lo;
+  }
+  auto begin_part = [&]() __attribute__((always_inline)) {
+    Span sp;
+    for (;; ++seq) {   // (empty sequences have no tiles)
+      sp = span_of(a, __builtin_amdgcn_readfirstlane(s_len[seq]));
+      if (xl < before(seq + 1)) break;
+    }
+    const uint32_t into = xl - before(seq);
+    part.seq = seq;
+    part.kv = into / sp.tiles;
+    const uint32_t tile = into - part.kv * sp.tiles;
+    part.pair_begin = xl - tile;
+    part.pair_end = part.pair_begin + sp.tiles;
+    part.end = min(part.pair_end, x1);
+    part.whole = tile == 0 && part.end == part.pair_end;
+    tok = sp.base + tile * 64u + 16u * g;
+    col = quotient(tok >> 4, a.layout.page_size >> 4, a.page_r);
+    off = tok - col * a.layout.page_size;
+    run_end = min(sp.end, sp.base + (tile + part.end - xl) * 64u);
+    span_begin = sp.begin;
+    span_end = sp.end;
+    table = a.tables + (uint64_t)seq * a.table_width;
+  };
+  auto page_of = [&]() __attribute__((always_inline)) { return tok < run_end ? (uint32_t)table[col] : ~0u; };   // no page beyond the part is looked up
+  // A tile's loads run ahead of its computation: the keys' are issued when the tile before has its scores, the values' and the
+  // scales' when it is done. A page outside the pool, or past the run, is read as page 0 (in bounds, weight zero); there is no
+  // branch around a load, so that the compiler knows how many are in flight.
+  uint32_t kw[4][KW], vw[16][VW], safe = 0, offs = 0;
+  float nk = 0.f, nv = 0.f, dist = 0.f;
+  bool in = false;
+  Part loaded{};
+  auto load_keys = [&]() __attribute__((always_inline)) {
+    loaded = part;
+    safe = page < a.layout.pages ? page : 0u;
+    offs = off;
+    in = page < a.layout.pages && tok + n < span_end && tok + n >= span_begin;
+    dist = (float)(int32_t)(tok + n - (span_end - 1u));
+    // the first row of this lane's 16 tokens; of all four groups of 16 in scalar registers
+    const uint64_t row = (uint64_t)(a.k.codes + (uint64_t)part.kv * a.khead) + (uint64_t)safe * a.kpage + (uint64_t)(offs * a.kslot);
+    uint32_t k0[KB ? 1 : KW / 2];
+#pragma unroll
+    for (int i = 0; i < (KB ? 1 : KW / 2); ++i) {
+      k0[i] = koff[i];
+      asm volatile("" : "+v"(k0[i]));   // a 32-bit lane offset to a scalar base, not a 64-bit sum kept in registers
+    }
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const uint8_t* const base = (const uint8_t*)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)row, 16 * m) |
+                                                   (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(row >> 32), 16 * m) << 32);
+      if constexpr (KB != 0) {
+        const uint32_t* const q = (const uint32_t*)(base + k0[0]);
+        if constexpr (KW == 4) {
+          const u32x4 v = *(const u32x4*)q;
+          kw[m][0] = v.x; kw[m][1] = v.y; kw[m][2] = v.z; kw[m][3] = v.w;
+        } else if constexpr (KW == 3) {
+          const u32x3 v = *(const u32x3*)q;
+          kw[m][0] = v.x; kw[m][1] = v.y; kw[m][2] = v.z;
+        } else if constexpr (KW == 2) {
+          const u32x2 v = *(const u32x2*)q;
+          kw[m][0] = v.x; kw[m][1] = v.y;
+        } else {
+          kw[m][0] = *q;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < KW / 2; ++i) {
+          const uint64_t v = *(const u64_any*)(base + k0[i]);
+          kw[m][2 * i] = (uint32_t)v;
+          kw[m][2 * i + 1] = (uint32_t)(v >> 32);
+        }
+      }
+    }
+    ++xl;
+    tok += 64u;
+    col += a.tile_cols;
+    off += a.tile_rest;
+    if (off >= a.layout.page_size) {
+      off -= a.layout.page_size;
+      ++col;
+    }
+    if (xl < x1 && xl == part.end) begin_part();
+    page = page_of();
+  };
+  // values: a lane group takes the 16 tokens of its own page, so that a lane's rows follow each other
+  auto load_values = [&]() __attribute__((always_inline)) {
+    const uint8_t* base = a.v.codes + (uint64_t)loaded.kv * a.vhead + (uint64_t)safe * a.vpage + (uint64_t)(offs * a.vslot + vlo);
+    auto load_row = [&](int j, const uint8_t* q) __attribute__((always_inline)) {
+      if constexpr (VW == 2) {
+        const uint64_t v = *(const u64_any*)q;
+        vw[j][0] = (uint32_t)v;
+        vw[j][1] = (uint32_t)(v >> 32);
+      } else {
+        vw[j][0] = *(const u32_any*)q;
+      }
+    };
+    if (VB != 0 && a.layout.slot_step == 1) {   // head-major pages: constant distances
+#pragma unroll
+      for (int j = 0; j < 16; ++j) load_row(j, base + j * (D * VB / 8));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j, base += a.vslot) load_row(j, base);
+    }
+    const uint64_t row = (uint64_t)loaded.kv * a.layout.head_step + (uint64_t)safe * (uint32_t)a.layout.page_stride +
+                         (uint64_t)((offs + n) * a.layout.slot_step);
+    nk = a.k.scales[row];
+    nv = a.v.scales[row];
+  };
+
+  // Queries: a lane (head, group) loads eight coordinates from 32 t + 8 g of its head for every t, the other operand of the rotation.
+  uint32_t yraw[KS][4];
+  auto load_queries = [&](const Part& p) __attribute__((always_inline)) {
+    const uint32_t h = NH == 4 ? n & 3 : n & 7;
+    const uint16_t* const q = (const uint16_t*)a.q.data + p.seq * a.q.token_stride + (p.kv * a.nq + min(h, a.nq - 1u)) * a.q.head_stride + 8 * g;
+#pragma unroll
+    for (int t = 0; t < KS; ++t) {
+      const u32x4 v = *(const u32x4*)(q + 32 * t);
+      yraw[t][0] = v.x; yraw[t][1] = v.y; yraw[t][2] = v.z; yraw[t][3] = v.w;
+    }
+  };
+
+  uint32_t qa[KS][4];
+  float qs[NH], slope[NH], M[NH], l[NH], S[NH];
+  v4f acc[NC];
+  bool tail = false;
+  Part cur{};
+  // ---- a part begins: the score operand of its queries, which are in yraw
+  auto prepare = [&]() __attribute__((always_inline)) {
+    {
+      const uint32_t h = NH == 4 ? n & 3 : n & 7, part = NH == 4 ? n >> 2 : n >> 3;
+      // H (s q) on the matrix cores, exactly: rows of +1 and -1 times the raw queries with their signs flipped. Instruction b
+      // gives this lane (head n, group g) coordinates GC g + 4 b .. + 3: its row r is coordinate i = GC (r / 4) + 4 b + r % 4, and
+      // the entry at coordinate j = 32 t + 8 g + e is the parity of i & j.
+#pragma unroll
+      for (int t = 0; t < KS; ++t) {
+        const uint32_t sg = a.k.signs[t] >> (8 * g);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) yraw[t][k] ^= (sg >> (2 * k) & 1u) << 15 | (sg >> (2 * k + 1) & 1u) << 31;
+      }
+      constexpr uint32_t kOne = IO == 1 ? 0x3C003C00u : 0x3F803F80u;
+      uint32_t row = n, grp = g;   // (opaque: the matrix's rows are formed here, not kept in registers for all parts)
+      asm volatile("" : "+v"(row), "+v"(grp));
+      uint32_t one[2][4];   // b even, odd: parity of (4 b + r % 4) & e for e = 2 k, 2 k + 1
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t r = row & 3, lo = (uint32_t)__builtin_popcount(r & (2 * k)) & 1u, hi = (uint32_t)__builtin_popcount(r & (2 * k + 1)) & 1u;
+        one[0][k] = kOne ^ (lo << 15 | hi << 31);
+        one[1][k] = one[0][k] ^ (k >= 2 ? 0x80008000u : 0u);
+      }
+      const uint32_t rt = row >> 2;
+      float y[GC];
+#pragma unroll
+      for (int b = 0; b < GC / 4; ++b) {
+        // i's bits 3 and up within a quarter go with g, its quarter with t
+        const uint32_t sb = (uint32_t)__builtin_popcount((b >> 1) & grp) & 1u;
+        v4f c{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < KS; ++t) {
+          const uint32_t flip = (D == 128 ? sb ^ ((uint32_t)__builtin_popcount(rt & t) & 1u)
+                                          : (uint32_t)__builtin_popcount((((rt & 1) << 1) | (b >> 1)) & grp) + (rt >> 1 & (uint32_t)t) & 1u) ? 0x80008000u : 0u;
+          const w4 hrow{one[b & 1][0] ^ flip, one[b & 1][1] ^ flip, one[b & 1][2] ^ flip, one[b & 1][3] ^ flip};
+          const w4 q{yraw[t][0], yraw[t][1], yraw[t][2], yraw[t][3]};
+          c = IO == 1 ? mfma_f16(hrow, q, c) : mfma_bf16(hrow, q, c);
+        }
+#pragma unroll
+        for (int v = 0; v < 4; ++v) y[4 * b + v] = c[v];
+      }
+      float mx = 0.f;
+#pragma unroll
+      for (int e = 0; e < GC; ++e) mx = fmax_hw(mx, __builtin_fabsf(y[e]));
+      mx = max16(mx, mx);
+      mx = max32(mx, mx);
+      const int ex = min(max(exponent_of(mx), -100), 126);
+      // heads that the call has not, and the rows of further parts, are zero
+      const float sc = h < a.nq && part < 2 ? pow2i(14 - ex > 127 ? 127 : 14 - ex) : 0.f;
+#pragma unroll
+      for (int h2 = 0; h2 < NH; ++h2) qs[h2] = lane_value(pow2i(ex - 14) * a.kinv * a.qscale, h2);
+#pragma unroll
+      for (int e = 0; e < GC; e += 2) {
+        const float p = y[e] * sc, r = y[e + 1] * sc;
+        const uint32_t hi = f16_pair(p, r);
+        float hp, hr;
+        widen2<1>(hi, hp, hr);
+        const uint32_t low = f16_pair(p - hp, r - hr);
+        qa[e / 8][(e % 8) / 2] = part == 0 ? hi : low;
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      slope[h] = a.slopes && h < (int)a.nq ? a.slopes[cur.kv * a.nq + h] * a.slope_scale : 0.f;
+      M[h] = -__FLT_MAX__;   // the lowest finite value: a score of minus infinity weighs nothing, also before any other
+      l[h] = 0.f;
+      S[h] = 1.f;
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[c] = v4f{0.f, 0.f, 0.f, 0.f};
+  };
+
+  auto compute = [&]() __attribute__((always_inline)) {
+    // ---- scores: rows 4 g .. 4 g + 3 (parts, heads) of token 16 m + n
+    v4f cs[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      cs[m] = v4f{0.f, 0.f, 0.f, 0.f};
+      if constexpr (KB == 0) {
+#pragma unroll
+        for (int j = 0; j < KW / 2; ++j) {
+          const uint64_t v = ((uint64_t)kw[m][2 * j + 1] << 32 | kw[m][2 * j]) >> ksh[j];
+          kw[m][2 * j] = (uint32_t)v;
+          kw[m][2 * j + 1] = (uint32_t)(v >> 32);
+        }
+      } else if constexpr (GC * KB % 32 != 0) {
+#pragma unroll
+        for (int k = 0; k < KW; ++k) kw[m][k] = __builtin_amdgcn_alignbit(k + 1 < KW ? kw[m][k + 1] : 0u, kw[m][k], ksh[0]);
+      }
+    }
+    {
+      // the table reads of three instructions' operands ahead (12 or so are what the LDS counter tells apart)
+      uint32_t hi[4][4], lo[4][4];
+      auto look = [&](int k) {
+        const int s = k >> 2, m = k & 3;
+        if constexpr (KB == 0) {
+          const uint32_t w[2] = {kw[m][2 * s], kw[m][2 * s + 1]};
+          look_pairs<KB, TWO, 4>(w, 0, klb, a.k.bits, a.k.polar != 0, hi[k & 3], lo[k & 3]);
+        } else {
+          look_pairs<KB, TWO, 4>(kw[m], 8 * KB * s, klb, 0u, false, hi[k & 3], lo[k & 3]);
+        }
+      };
+      constexpr int kAhead = KB == 0 ? 1 : 2;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) look(k);
+#pragma unroll
+      for (int k = 0; k < 4 * KS; ++k) {
+        if (k + kAhead < 4 * KS) look(k + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
+        const int s = k >> 2, m = k & 3;
+        const w4 q{qa[s][0], qa[s][1], qa[s][2], qa[s][3]};
+        cs[m] = mfma_f16(q, w4{hi[k & 3][0], hi[k & 3][1], hi[k & 3][2], hi[k & 3][3]}, cs[m]);
+        if constexpr (TWO) cs[m] = mfma_f16(q, w4{lo[k & 3][0], lo[k & 3][1], lo[k & 3][2], lo[k & 3][3]}, cs[m]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    // sum of the parts; lane l gets the scores of token l of the tile
+    float z[NH];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const float p = fold32(cs[0][v], cs[2][v]), r = fold32(cs[1][v], cs[3][v]);
+      if constexpr (NH == 8) {
+        const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(p), __float_as_uint(r), false, false);
+        z[v] = __uint_as_float(x[0]);
+        z[4 + v] = __uint_as_float(x[1]);
+      } else {
+        z[v] = fold16(p, r);
+      }
+    }
+
+    const bool now_in = in;
+    const float now_dist = dist, now_nk = nk, now_nv = nv;
+    load_keys();
+    __builtin_amdgcn_sched_barrier(0);
+    // ---- online softmax. The maximum and the weights' factor S are kept until a score or a weight leaves their range.
+    const float n_t = now_in ? now_nv : 0.f;
+#pragma unroll
+    for (int h = 0; h < NH; ++h) z[h] *= qs[h] * now_nk;
+    if (a.cap > 0.f) {
+      asm volatile("");   // a branch: the exponentials are not computed where no score is capped
+#pragma unroll
+      for (int h = 0; h < NH; ++h) z[h] = a.cap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z[h])));
+    }
+#pragma unroll
+    for (int h = 0; h < NH; ++h) z[h] = now_in ? __builtin_fmaf(slope[h], now_dist, z[h]) : -__builtin_inff();
+    float p[NH], y[NH], top = -__FLT_MAX__, most = 0.f;
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      const float x = z[h] - M[h];
+      p[h] = __builtin_amdgcn_exp2f(x);
+      y[h] = p[h] * n_t * S[h];
+      top = fmax_hw(top, x);
+      most = fmax_hw(most, __builtin_fabsf(y[h]));
+    }
+    const bool over = top > 6.f || most > kTop;
+    if (__any(over)) {
+      float f[NH], mx[NH];
+      wave_max_heads(z, mx);
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const float m = fmax_hw(M[h], mx[h]), al = __builtin_amdgcn_exp2f(M[h] - m);
+        M[h] = m;
+        l[h] *= al;
+        f[h] = al;
+        p[h] = __builtin_amdgcn_exp2f(z[h] - m);
+        y[h] = __builtin_fabsf(p[h] * n_t);
+      }
+      wave_max_heads(y, mx);
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        // the accumulators are relative to M and times S: a new maximum leaves them as they are with S / al
+        const float keep = S[h] * __builtin_amdgcn_rcpf(f[h]);
+        float s_new = keep, fac = 1.f;
+        if (!(keep <= 0x1p60f && mx[h] * keep <= kTop)) {
+          s_new = mx[h] > 0.f ? pow2i(min(13 - max(exponent_of(mx[h]), -100), 60)) : 1.f;
+          fac = f[h] * s_new * __builtin_amdgcn_rcpf(S[h]);
+        }
+        S[h] = s_new;
+        f[h] = fac;
+        y[h] = p[h] * n_t * S[h];
+      }
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float fv = NH == 8 ? pick(upper, f[v], f[NH - 4 + v]) : f[v];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) acc[c][v] *= fv;
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < NH; ++h) l[h] += p[h];
+    // row r of the staged weights: four heads, head r's two parts; eight, the weights of heads r and r + 4
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if constexpr (NH == 4) {
+        const float hi = (float)(_Float16)y[r];
+        s_w[r * kPRow + lane] = f16_pair(hi, (y[r] - hi) * kLoScale);
+      } else {
+        s_w[r * kPRow + lane] = f16_pair(y[r], y[r + 4]);
+      }
+    }
+    wave_lds_fence();
+
+    // ---- weighted values: the accumulators' rows 0 - 7 weigh a pair's first coordinate, 8 - 15 its second
+    if constexpr (kShiftV) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if constexpr (VW == 2) {
+          const uint64_t v = ((uint64_t)vw[j][1] << 32 | vw[j][0]) >> vsh;
+          vw[j][0] = (uint32_t)v;
+          vw[j][1] = (uint32_t)(v >> 32);
+        } else {
+          vw[j][0] >>= vsh;
+        }
+      }
+    }
+    const uint32_t* const s_row = s_w + (n & 3) * kPRow + 16 * g;   // tokens 16 g + 4 m + j
+    const uint32_t sel = n < 8 ? (n & 4 ? 0x0C0C0302u : 0x0C0C0100u) : (n & 4 ? 0x03020C0Cu : 0x01000C0Cu);
+    // a step: the pairs c (two bits: c and c + 1, which one table read gives) of four tokens
+    constexpr int PC = VB == 2 ? 2 : 1, NS = 4 * NC / PC, kAhead = VB == 0 ? 1 : 2;
+    uint32_t v[4][4][PC], none[PC];
+    w4 d[4], wa{};
+    auto look = [&](int k) __attribute__((always_inline)) {
+      const int m = k / (NC / PC), c = k % (NC / PC) * PC;
+      if (c == 0) d[m] = *(const w4*)(s_row + 4 * m);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (VB != 0) {
+          look_pairs<VB, false, PC>(vw[4 * m + j], 2 * VB * c, vlb, 0u, false, v[k & 3][j], none);
+        } else {
+          uint64_t x = vw[4 * m + j][0];
+          if constexpr (VW == 2) x |= (uint64_t)vw[4 * m + j][VW - 1] << 32;
+          x >>= a.v.bits * (2 * c);
+          const uint32_t w[2] = {(uint32_t)x, (uint32_t)(x >> 32)};
+          look_pairs<VB, false, PC>(w, 0, vlb, a.v.bits, false, v[k & 3][j], none);
+        }
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) look(k);
+#pragma unroll
+    for (int k = 0; k < NS; ++k) {
+      if (k + kAhead < NS) look(k + kAhead);
+      __builtin_amdgcn_sched_barrier(0);
+      const int m = k / (NC / PC), c = k % (NC / PC) * PC;
+      if (c == 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) wa[j] = __builtin_amdgcn_perm(0u, d[m][j], sel);
+      }
+#pragma unroll
+      for (int i = 0; i < PC; ++i) acc[c + i] = mfma_f16(wa, w4{v[k & 3][0][i], v[k & 3][1][i], v[k & 3][2][i], v[k & 3][3][i]}, acc[c + i]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    wave_lds_fence();
+  };
+
+  // ---- a part is done: sums over the lanes, parts added, factors taken out
+  auto finish = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < NH; ++h) l[h] = wave_sum(l[h]);
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const float f = a.vinv * __builtin_amdgcn_rcpf(NH == 8 ? pick(upper, S[v], S[NH - 4 + v]) : S[v]);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        if constexpr (NH == 4) {
+          const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[c][v]), __float_as_uint(acc[c][v]), false, false);
+          acc[c][v] = __builtin_fmaf(__uint_as_float(r[1]), 1.f / kLoScale, __uint_as_float(r[0]));
+        }
+        acc[c][v] *= f;
+      }
+    }
+    if (cur.whole) {
+      write_output<NH, IO>(a, cur.seq, cur.kv, acc, M, l, lane);
+    } else if (cur.end == x1) {
+      tail = true;
+    } else {
+      float* const out = ws + (uint64_t)(2 * slot + 1) * slot_floats(NH);
+      if (lane == 0) {
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          out[h] = M[h];
+          out[8 + h] = l[h];
+        }
+      }
+      if (NH == 8 || !(g & 1)) {
+        const int at = NH == 8 ? lane : n + 16 * (g >> 1);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) *(v4f*)(out + 16 + (c * (NH == 4 ? 32 : 64) + at) * 4) = acc[c];
+      }
+    }
+  };
+  if (x0 < x1) {
+    begin_part();
+    page = page_of();
+    cur = part;
+    load_queries(cur);
+    load_keys();
+    load_values();
+  }
+  ktab.write(s_mem + key_base(KB, VB, TWO) / 4, a.k, a.kfactor, tid);
+  vtab.write(s_mem + value_base(KB, VB, TWO) / 4, a.v, a.vfactor, tid);
+  // (orders LDS only: the loads of the first tile stay on their way)
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+  if (x0 < x1) {
+    prepare();
+    for (uint32_t xc = x0;;) {
+      compute();
+      load_values();
+      __builtin_amdgcn_sched_barrier(0);
+      if (++xc == cur.end) {
+        const bool more = xc < x1;
+        const Part next = loaded;
+        if (more) load_queries(next);
+        finish();
+        if (!more) break;
+        cur = next;
+        prepare();
+      }
+    }
+  }
+  const uint32_t key = tail ? cur.seq * heads + cur.kv : ~0u;   // (pairs with tiles: below 2^31)
+
+  // ---- the last parts of neighbouring waves, where they are of one pair, merge through LDS (the tables' space)
+  __syncthreads();
+  constexpr int kMl = 2 * NH, kLanes = NH == 4 ? 32 : 64;
+  float* const s_ml = (float*)s_mem;
+  v4f* const s_acc = (v4f*)(s_mem + W * kMl);
+  const int at = NH == 8 ? lane : n + 16 * (g >> 1);
+  if (lane == 0) s_key[wid] = key;
+  if (tail) {
+    if (lane == 0) {
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        s_ml[wid * kMl + h] = M[h];
+        s_ml[wid * kMl + NH + h] = l[h];
+      }
+    }
+    if (NH == 8 || !(g & 1)) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) s_acc[(wid * NC + c) * kLanes + at] = acc[c];
+    }
   }
   __syncthreads();
-  for (int m = 1; m < D; m *= 2) {
-    float x[8 * D / 2 / kChunk][2];
-    for (int i = tid, k = 0; i < 8 * D / 2; i += kChunk, ++k) {
-      const int h = i / (D / 2), r = i % (D / 2), j = (r / m) * 2 * m + r % m;
-      x[k][0] = s_q[h][j];
-      x[k][1] = s_q[h][j + m];
-      s_q[h][j] = x[k][0] + x[k][1];
-      s_q[h][j + m] = x[k][0] - x[k][1];
+  auto key_of = [&](uint32_t w) { return (uint32_t)__builtin_amdgcn_readfirstlane(s_key[w]); };
+  if (!tail || (wid > 0 && key_of(wid - 1) == key)) return;   // (uniform per wave; no barrier follows)
+  uint32_t last = wid + 1;
+  while (last < W && key_of(last) == key) ++last;
+  float mm[NH], lm[NH];
+#pragma unroll
+  for (int h = 0; h < NH; ++h) mm[h] = M[h];
+  for (uint32_t w = wid + 1; w < last; ++w)
+#pragma unroll
+    for (int h = 0; h < NH; ++h) mm[h] = fmax_hw(mm[h], s_ml[w * kMl + h]);
+#pragma unroll
+  for (int h = 0; h < NH; ++h) lm[h] = 0.f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) acc[c] = v4f{0.f, 0.f, 0.f, 0.f};
+  for (uint32_t w = wid; w < last; ++w) {
+    float e[NH];
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      e[h] = __builtin_amdgcn_exp2f(s_ml[w * kMl + h] - mm[h]);
+      lm[h] = __builtin_fmaf(s_ml[w * kMl + NH + h], e[h], lm[h]);
     }
-    __syncthreads();
-  }
-  const uint64_t most = (uint64_t)a.table_width * a.layout.page_size;
-  const int64_t len0 = a.lengths[b];
-  const uint64_t len = len0 < 0 ? 0 : min((uint64_t)len0, most);
-  const uint64_t begin = a.window && len > a.window ? len - a.window : 0;
-  for (uint64_t t0 = begin; t0 < len; t0 += kChunk) {
-    const uint64_t t = t0 + tid;
-    bool in = t < len;
-    uint64_t row = 0;
-    if (in) {
-      const uint64_t col = t / a.layout.page_size;
-      const int32_t page = a.tables[(uint64_t)b * a.table_width + col];
-      in = (uint32_t)page < a.layout.pages;
-      if (in)
-        row = (uint64_t)page * a.layout.page_stride + (uint64_t)kv * a.layout.head_step + (t - col * a.layout.page_size) * a.layout.slot_step;
-    }
-    s_row[tid] = in ? row : ~0ull;
-    float s[8] = {};
-    const uint8_t* kr = a.k.codes + row * a.k.row_bytes;
-    const uint32_t mask = (1u << a.k.bits) - 1;
-    for (int g = 0; g < D / 8; ++g) {
-      const uint32_t at = g * a.k.bits, lo = min(at, a.k.row_bytes - 8u);
-      const uint64_t w = *(const u64_any*)(kr + lo) >> (8u * (at - lo));
-      float y[8];
-      for (int e = 0; e < 8; e += 2) {
-        const uint32_t c0 = (uint32_t)(w >> (a.k.bits * e)) & mask, c1 = (uint32_t)(w >> (a.k.bits * (e + 1))) & mask;
-        y[e] = a.k.polar ? s_kt[c0] * s_kt[256 + c1] : s_kt[c0];
-        y[e + 1] = a.k.polar ? s_kt[c0] * s_kt[512 + c1] : s_kt[c1];
-      }
-      for (int h = 0; h < 8; ++h)
-        for (int e = 0; e < 8; ++e) s[h] = __builtin_fmaf(s_q[h][8 * g + e], y[e], s[h]);
-    }
-    const float nk = in ? a.k.scales[row] * a.qscale : 0.f;
-    for (int h = 0; h < 8; ++h) {
-      float z = s[h] * nk;
-      if (a.cap > 0.f) z = a.cap * (1.f - 2.f / (1.f + __builtin_amdgcn_exp2f(z)));
-      if (a.slopes && h < (int)nq) z += a.slopes[kv * nq + h] * a.slope_scale * ((float)t - (float)(len - 1));
-      s_p[h][tid] = in ? z : -__builtin_inff();
-    }
-    __syncthreads();
-    // the chunk's maximum, the weights and their sum: two heads per wave
-    for (int h = (tid >> 6) * 2; h < (tid >> 6) * 2 + 2; ++h) {
-      float m = s_m[h], l = 0.f;
-      for (int i = tid & 63; i < kChunk; i += 64) m = fmaxf(m, s_p[h][i]);
-      for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
-      for (int i = tid & 63; i < kChunk; i += 64) {
-        const float p = __builtin_amdgcn_exp2f(s_p[h][i] - m);
-        l += p;
-        s_p[h][i] = s_row[i] == ~0ull ? 0.f : p * a.v.scales[s_row[i]];
-      }
-      for (int d = 1; d < 64; d *= 2) l += __shfl_xor(l, d);
-      if ((tid & 63) == 0) {
-        s_al[h] = __builtin_amdgcn_exp2f(s_m[h] - m);
-        s_l[h] = s_l[h] * s_al[h] + l;
-        s_m[h] = m;
-      }
-    }
-    __syncthreads();
-    // values: thread = pair of coordinates x part of the chunk's tokens, four or two heads at a time
-    constexpr int P = kChunk / (D / 2);
-    const int j = 2 * (tid % (D / 2)), part = tid / (D / 2);
-    float o[8][2] = {};
-    const uint32_t vmask = (1u << a.v.bits) - 1, vat = (j * a.v.bits) / 8, vlo = min(vat, a.v.row_bytes - 4u);
-    const uint32_t vsh = j * a.v.bits - 8 * vlo;
-    for (int i = part; i < kChunk; i += P) {
-      const uint64_t r = s_row[i];
-      if (r == ~0ull) continue;
-      const uint32_t w = *(const u32_any*)(a.v.codes + r * a.v.row_bytes + vlo) >> vsh;
-      const uint32_t c0 = w & vmask, c1 = (w >> a.v.bits) & vmask;
-      const float y0 = a.v.polar ? s_vt[c0] * s_vt[256 + c1] : s_vt[c0], y1 = a.v.polar ? s_vt[c0] * s_vt[512 + c1] : s_vt[c1];
-      for (int h = 0; h < 8; ++h) {
-        o[h][0] = __builtin_fmaf(s_p[h][i], y0, o[h][0]);
-        o[h][1] = __builtin_fmaf(s_p[h][i], y1, o[h][1]);
-      }
-    }
-    for (int k = 0; k < P; ++k) {
-      if (part == k)
-        for (int h = 0; h < 8; ++h)
-          for (int e = 0; e < 2; ++e) s_o[h][j + e] = (k == 0 ? s_o[h][j + e] * s_al[h] : s_o[h][j + e]) + o[h][e];
-      __syncthreads();
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const v4f x = s_acc[(w * NC + c) * kLanes + at];
+#pragma unroll
+      for (int v = 0; v < 4; ++v) acc[c][v] = __builtin_fmaf(x[v], NH == 8 ? pick(upper, e[v], e[NH - 4 + v]) : e[v], acc[c][v]);
     }
   }
-  for (int m = 1; m < D; m *= 2) {
-    for (int i = tid; i < 8 * D / 2; i += kChunk) {
-      const int h = i / (D / 2), r = i % (D / 2), j = (r / m) * 2 * m + r % m;
-      const float x = s_o[h][j], y = s_o[h][j + m];
-      s_o[h][j] = x + y;
-      s_o[h][j + m] = x - y;
+  const uint32_t begin = g0 + wid * per_wave, end = min(g0 + last * per_wave, g1);
+  if (begin <= cur.pair_begin && end >= cur.pair_end) {
+    write_output<NH, IO>(a, cur.seq, cur.kv, acc, mm, lm, lane);
+    return;
+  }
+  float* const out = ws + (uint64_t)(2 * slot) * slot_floats(NH);
+  if (lane == 0) {
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      out[h] = mm[h];
+      out[8 + h] = lm[h];
     }
-    __syncthreads();
   }
-  for (int i = tid; i < (int)nq * D; i += kChunk) {
-    const int h = i / D, j = i % D;
-    float f[1] = {s_l[h] > 0.f ? s_o[h][j] * a.oscale / s_l[h] : 0.f};
-    if ((a.v.signs[j >> 5] >> (j & 31)) & 1) f[0] = -f[0];
-    store_elems<IO, 1>(a.out.data, b * a.out.token_stride + (kv * nq + h) * a.out.head_stride + j, f, false);
+  if (NH == 8 || !(g & 1)) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) *(v4f*)(out + 16 + (c * kLanes + at) * 4) = acc[c];
   }
-  if (a.lse && tid < (int)nq)
-    a.lse[(uint64_t)b * a.layout.kv_heads * nq + kv * nq + tid] = s_l[tid] > 0.f ? (s_m[tid] + log2f(s_l[tid])) * kLn2 : -__builtin_inff();
+}
+
+// Joins the partial results of each pair of sequence and KV head that no wave or workgroup of paged_attn wrote as a whole, and
+// writes zeros for an empty sequence. A workgroup of paged_attn has left two of them at most, the merged last parts and one that
+// ends inside a wave's run: a lane each looks up whether it is there, its maxima and sums; then the waves add up the accumulators.
+constexpr int kJoinWaves = 8;
+template <int NH, int IO>
+__global__ __launch_bounds__(64 * kJoinWaves) void paged_join(PagedAttnArgs a) {
+  constexpr int kLanes = NH == 4 ? 32 : 64;
+  __shared__ v4f s_acc[kJoinWaves - 1][NC][kLanes];
+  const uint32_t heads = a.layout.kv_heads, b = blockIdx.x / heads, kv = blockIdx.x - b * heads;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const uint32_t wid = __builtin_amdgcn_readfirstlane(tid >> 6), upper = g & 1 ? ~0u : 0u;
+  const uint32_t* const pref = (const uint32_t*)a.ws;
+  const uint32_t p0 = pref[b], tiles = pref[b + 1] - p0, total = pref[a.sequences] * heads;
+  const float* const ws = a.ws + ((a.sequences + 4u) & ~3u);
+  const int at = NH == 8 ? lane : n + 16 * (g >> 1);
+  float M[NH], l[NH];
+  v4f acc[NC];
+#pragma unroll
+  for (int h = 0; h < NH; ++h) {
+    M[h] = -__FLT_MAX__;
+    l[h] = 0.f;
+  }
+#pragma unroll
+  for (int c = 0; c < NC; ++c) acc[c] = v4f{0.f, 0.f, 0.f, 0.f};
+  if (tiles) {
+    const uint32_t s = p0 * heads + kv * tiles, e = s + tiles, per_group = group_tiles(total, a);
+    const uint32_t first = s / per_group, last = (e - 1) / per_group, parts = 2 * (last - first + 1);
+    for (uint32_t c0 = 0; c0 < parts; c0 += 64) {
+      // part c0 + lane: the merged last parts (even) of a workgroup or the one that ends inside a wave's run (odd)
+      const uint32_t c = c0 + lane, grp = min(first + (c >> 1), last), g0 = grp * per_group, g1 = min(g0 + per_group, total);
+      const uint32_t per_wave = wave_tiles(total, per_group, grp), from = max(s, g0), to = min(e, g1);
+      const uint32_t wa = (from - g0) / per_wave, wb = (to - 1 - g0) / per_wave;
+      const uint32_t wa0 = g0 + wa * per_wave, wb1 = min(g0 + (wb + 1) * per_wave, g1);   // the runs' begin and end
+      const bool inside = wb1 > e;             // the pair ends inside the last wave's run: it is no last part there
+      // written by a wave, or by the workgroup that merged all of it
+      if (__any((wa == wb && wa0 <= s && wb1 >= e) || (!inside && wa0 <= s && to == e))) return;
+      const bool there = c < parts && (c & 1 ? inside : !inside || wb > wa);
+      const uint32_t slot = c & 1 ? 2 * (grp * W + wb) + 1 : 2 * (grp * W + wa);
+      const float* const in = ws + (uint64_t)slot * slot_floats(NH);
+      float pm[NH], pl[NH], mx[NH];
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        pm[h] = there ? in[h] : -__FLT_MAX__;
+        pl[h] = there ? in[8 + h] : 0.f;
+      }
+      wave_max_heads(pm, mx);
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const float m = fmax_hw(M[h], mx[h]), al = __builtin_amdgcn_exp2f(M[h] - m);
+        pm[h] = __builtin_amdgcn_exp2f(pm[h] - m);
+        l[h] = __builtin_fmaf(l[h], al, wave_sum(pl[h] * pm[h]));
+        M[h] = m;
+#pragma unroll
+        for (int k = 0; k < NC; ++k)
+          if (h < 4) {
+            acc[k][h & 3] *= NH == 8 && (g & 1) ? 1.f : al;
+          } else {
+            acc[k][h & 3] *= (g & 1) ? al : 1.f;
+          }
+      }
+      uint64_t left = __ballot(there);
+      uint32_t i = 0;
+      while (left) {
+        const int k = __builtin_ctzll(left);
+        left &= left - 1;
+        if ((i++ % kJoinWaves) != wid) continue;
+        const float* const part = ws + (uint64_t)__builtin_amdgcn_readlane(slot, k) * slot_floats(NH) + 16;
+        float f[NH];
+#pragma unroll
+        for (int h = 0; h < NH; ++h) f[h] = lane_value(pm[h], k);
+#pragma unroll
+        for (int x = 0; x < NC; ++x) {
+          const v4f y = *(const v4f*)(part + (x * kLanes + at) * 4);
+#pragma unroll
+          for (int v = 0; v < 4; ++v) acc[x][v] = __builtin_fmaf(y[v], NH == 8 ? pick(upper, f[v], f[NH - 4 + v]) : f[v], acc[x][v]);
+        }
+      }
+    }
+  }
+  if (wid > 0 && (NH == 8 || !(g & 1))) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) s_acc[wid - 1][c][at] = acc[c];
+  }
+  __syncthreads();
+  if (wid != 0) return;
+#pragma unroll
+  for (int w = 0; w < kJoinWaves - 1; ++w)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[c] += s_acc[w][c][at];
+  write_output<NH, IO>(a, b, kv, acc, M, l, lane);
+}
+
+// ---------------------------------------------------------------------------------------------------- launch
+template <int KB, int VB, int NH, int IO>
+hipError_t launch_one(const PagedAttnArgs& a, hipStream_t s) {
+  using L = Lds<KB, VB, NH, IO == 1>;
+  constexpr uint32_t most = 4u * L::words(kPagedMostSequences);
+  static_assert(most <= 160u * 1024u, "LDS of one workgroup");
+  static_assert(slot_floats(NH) <= paged_slot_floats(D, NH), "a partial result fits its slot");
+  const uint32_t bytes = 4u * L::words(a.sequences);
+  if (bytes > 65536u) {   // a property of the kernel, not of the launch: every call sets the largest (as pitch_attn_codes.hip)
+    const hipError_t e = hipFuncSetAttribute((const void*)paged_attn<KB, VB, NH, IO>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL((paged_attn<KB, VB, NH, IO>), dim3(a.groups), dim3(64 * W), bytes, s, a);
+  hipLaunchKernelGGL((paged_join<NH, IO>), dim3(a.sequences * a.layout.kv_heads), dim3(64 * kJoinWaves), 0, s, a);
+  return hipGetLastError();
+}
+template <int VB>
+hipError_t launch_heads(const PagedAttnArgs& a, uint32_t io, hipStream_t s) {
+  if (a.nq <= 4) return io == 1 ? launch_one<PITCH_KB, VB, 4, 1>(a, s) : launch_one<PITCH_KB, VB, 4, 2>(a, s);
+  return io == 1 ? launch_one<PITCH_KB, VB, 8, 1>(a, s) : launch_one<PITCH_KB, VB, 8, 2>(a, s);
 }
 
 }  // namespace
 
-#define PITCH_CAT_(a, b) a##b
-#define PITCH_CAT(a, b) PITCH_CAT_(a, b)
-hipError_t PITCH_CAT(launch_paged_attention_d, PITCH_DIM)(const PagedAttnArgs& a, uint32_t io, hipStream_t s) {
-  const dim3 grid(a.sequences * a.layout.kv_heads);
-  if (io == 1) hipLaunchKernelGGL((paged_attn<1>), grid, dim3(kChunk), 0, s, a);
-  else hipLaunchKernelGGL((paged_attn<2>), grid, dim3(kChunk), 0, s, a);
-  return hipGetLastError();
+#define PITCH_CAT4_(a, b, c, d) a##b##c##d
+#define PITCH_CAT4(a, b, c, d) PITCH_CAT4_(a, b, c, d)
+hipError_t PITCH_CAT4(launch_paged_attention_d, PITCH_DIM, _k, PITCH_KB)(const PagedAttnArgs& a0, uint32_t io, hipStream_t s) {
+  PagedAttnArgs a = a0;
+  a.kfactor = pitch_f16_factor(ilog2(D), a.k.polar, (int)a.k.bits);
+  a.vfactor = pitch_f16_factor(ilog2(D), a.v.polar, (int)a.v.bits);
+  a.kinv = 1.f / a.kfactor;
+  a.vinv = 1.f / a.vfactor;
+  a.groups_r = 0xFFFFFFFFu / a.groups;
+  a.kpage = (uint32_t)a.layout.page_stride * a.k.row_bytes;
+  a.vpage = (uint32_t)a.layout.page_stride * a.v.row_bytes;
+  a.khead = a.layout.head_step * a.k.row_bytes;
+  a.vhead = a.layout.head_step * a.v.row_bytes;
+  a.kslot = a.layout.slot_step * a.k.row_bytes;
+  a.vslot = a.layout.slot_step * a.v.row_bytes;
+  a.page_r = 0xFFFFFFFFu / (a.layout.page_size / 16);
+  a.tile_cols = 64 / a.layout.page_size;
+  a.tile_rest = 64 % a.layout.page_size;
+  switch (a.v.bits) {
+    case 2: return launch_heads<2>(a, io, s);
+    case 3: return launch_heads<3>(a, io, s);
+    case 4: return launch_heads<4>(a, io, s);
+    default: return launch_heads<0>(a, io, s);
+  }
 }
 
 }  // namespace pitch

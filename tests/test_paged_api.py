@@ -127,7 +127,7 @@ CACHE_FAULTS = [
     (_set("cache", page_stride=HEADS * PAGE - 1), _lib.ERR_INVALID_INPUT, "page stride"),
     (_set("cache", page_stride=HEADS * PAGE + 1), _lib.ERR_INVALID_INPUT, "key codes"),
     (_set("cache", page_stride=1 << 63), _lib.ERR_INVALID_INPUT, "page stride"),
-    (_set("cache", pages=1 << 26, page_stride=1 << 39), _lib.ERR_INVALID_INPUT, "page stride"),
+    (_set("cache", pages=1 << 26, page_stride=1 << 25), _lib.ERR_INVALID_INPUT, "page stride"),
     (_set("cache", value_scales=None), _lib.ERR_INVALID_INPUT, "value scales"),
     (_set("cache", value_codes_bytes=48 * PAGES * HEADS * PAGE - 1), _lib.ERR_INVALID_INPUT, "value codes"),
 ]
@@ -158,14 +158,14 @@ DECODE_FAULTS = [
 ]
 ATTENTION_FAULTS = [
     (_set("call", io_type=_lib.IO_F32), "float16 or bfloat16"), (_set("call", io_type=9), "element type"),
-    (_set("call", sequences=0), "sequences"), (_set("call", q_per_kv=0), "query heads"), (_set("call", q_per_kv=9), "query heads"),
+    (_set("call", sequences=0), "sequences"), (_set("call", sequences=2049), "sequences"), (_set("call", q_per_kv=0), "query heads"), (_set("call", q_per_kv=9), "query heads"),
     (_set("call", q_per_kv=5), "buffer"), (_set("call", sequences=B + 1), "buffer has"),
     (_set("call", output__data=None), "output"), (_set("call", output__token_stride=0), "overlap"),
     (_set("call", queries__head_stride=3), "multiples of 4"), (_set("call", block_tables=None), "page tables"),
     (_set("call", table_width=1 << 40), "width"), (_set("call", lengths_bytes=4 * B - 1), "lengths"),
     (_set("call", slopes_bytes=4), "slopes"), (_set("call", lse_bytes=4), "lse"), (_set("call", scale=float("nan")), "scale"),
     (_set("call", scale=float("inf")), "scale"), (_set("call", softcap=-1.0), "softcap"), (_set("call", softcap=float("nan")), "softcap"),
-    (_set("call", window=1 << 31), "window"),
+    (_set("call", window=1 << 31), "window"), (_set("call", table_width=1 << 26, block_tables_bytes=1 << 40), "too many tokens"),
 ]
 
 
