@@ -414,11 +414,12 @@ int pitch_enqueue_paged_append(const pitch_paged_cache_t* cache, const pitch_pag
 /* Reads tokens back. Row r of the outputs, row_starts[b] <= r < row_starts[b + 1], is token first_tokens[b] + r -
  * row_starts[b] of sequence b, found in page block_tables[b][token / page_size]; it is decoded as pitch_enqueue_decode_io
  * decodes it. row_starts does not decrease. Rows outside the sequences' ranges, and rows whose page lies outside the pool or
- * the table, are left as they were. keys or values may have null data (not read back). */
+ * the table, are left as they were. keys or values may have null data (not read back); their token strides are at most 2^22
+ * elements. */
 typedef struct pitch_paged_decode {
   uint32_t io_type;   /* PITCH_IO_* of the outputs */
   uint32_t sequences; /* at least 1 */
-  uint64_t rows;      /* rows of the outputs, 1 .. 2^31 - 1 */
+  uint64_t rows;      /* rows of the outputs, at least 1; rows * ceil(kv_heads / 4) <= 2^28 */
   const void* block_tables; /* int32 [sequences][table_width] */
   uint64_t block_tables_bytes;
   uint64_t table_width; /* at least 1 */

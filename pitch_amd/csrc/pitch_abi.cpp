@@ -1462,6 +1462,8 @@ int pitch_enqueue_paged_decode(const pitch_paged_cache_t* cache, const pitch_pag
   PITCH_TRY(check_io(call->io_type));
   const uint32_t dim = cache->key_config.dim, esize = io_bytes(call->io_type);
   if (call->rows < 1 || call->rows > 0x7FFFFFFFull) return fail(PITCH_ERR_INVALID_INPUT, "rows must be in 1...2^31 - 1");
+  if (call->rows * ((cache->kv_heads + 3u) / 4u) > 1ull << 28)   // (one launch's workgroups)
+    return fail(PITCH_ERR_INVALID_INPUT, "rows times groups of four heads exceed 2^28");
   PITCH_TRY(check_tables(call->block_tables, call->block_tables_bytes, call->table_width, call->sequences));
   PITCH_TRY(check_aligned(call->row_starts, call->row_starts_bytes, (call->sequences + 1ull) * 4u, 4, "row starts"));
   if (call->first_tokens)
@@ -1470,6 +1472,8 @@ int pitch_enqueue_paged_decode(const pitch_paged_cache_t* cache, const pitch_pag
   if (call->keys.data) PITCH_TRY(paged_vectors(call->keys, call->rows, cache->kv_heads, dim, esize, true, "keys", &a.out[0]));
   if (call->values.data)
     PITCH_TRY(paged_vectors(call->values, call->rows, cache->kv_heads, dim, esize, true, "values", &a.out[1]));
+  for (const pitch::PagedVectors& o : a.out)   // (a workgroup's rows are addressed by 32-bit offsets)
+    if (o.data && o.token_stride > 1u << 22) return fail(PITCH_ERR_INVALID_INPUT, "a token stride of the outputs exceeds 2^22");
   int dev = 0;
   PITCH_TRY(current_device(&dev));
   BatchDeviceCheck check(dev);

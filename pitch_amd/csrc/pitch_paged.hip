@@ -232,83 +232,244 @@ __global__ __launch_bounds__(kBlock) void paged_append(PagedAppendArgs a) {
 }
 
 // ----------------------------------------------------------------------------------------------------
-// Read back. Row r of the output is token first_tokens[b] + r - row_starts[b] of the sequence b whose range holds it.
+// Read back. Row r of the output is token first_tokens[b] + r - row_starts[b] of the sequence b whose range holds it. A workgroup
+// takes kReadRows rows of up to four KV heads, keys or values: it looks their pages up once (a chain of three loads), then asks
+// for the codes and scales of all its heads, and decodes two vectors per team at a time, whose transforms share the cross-lane
+// instructions. The arithmetic and its order are those of vec_decode (pitch_vector.hip), so a row's bytes are those of the
+// contiguous decode. Bound by the writes: a read waits long behind them, which is what asking for four heads at once hides
+// (with one head at a time 39-49 us, with the stores under a branch, which makes the next reads' wait one for all stores
+// before them, 40-54 us). Measured: 31,616 rows of 8 heads, d = 128 bf16, 4 / 3 bits: 36.8 us for 156 MB (4.2 TB/s); 32,767
+// rows of 12 heads, d = 64 float32: 52.3 us for 227 MB (4.3 TB/s; 57 us when each store instruction writes every other
+// 16 bytes).
 
-// The sequence whose rows hold row: the last b with row_starts[b] <= row (row_starts does not decrease).
-__device__ __forceinline__ uint32_t sequence_of(const int32_t* row_starts, uint32_t sequences, int32_t row) {
-  uint32_t lo = 0, hi = sequences;   // row_starts[lo] <= row < row_starts[hi], where the row is in the ranges at all
+// The sequence whose rows hold row: the last b with starts[b] <= row (starts does not decrease).
+template <typename P>
+__device__ __forceinline__ uint32_t sequence_of(P starts, uint32_t sequences, int32_t row) {
+  uint32_t lo = 0, hi = sequences;
   while (hi - lo > 1) {
     const uint32_t mid = (lo + hi) / 2;
-    if (row_starts[mid] <= row) lo = mid;
+    if (starts[mid] <= row) lo = mid;
     else hi = mid;
   }
   return lo;
 }
 
-__device__ __forceinline__ void decode_vectors(const PagedDecodeArgs& a, const PagedPool& p, const PagedVectors& out,
-                                               uint32_t head, uint32_t row, int t, float* s_tab) {
-  const uint32_t b = sequence_of(a.row_starts, a.sequences, (int32_t)row);
-  const int64_t begin = a.row_starts[b], end = a.row_starts[b + 1];
+constexpr uint32_t kStarts = 1024;   // row starts that are kept in LDS
+constexpr uint64_t kNoVector = ~0ull;
+constexpr uint32_t kRangeBytes = 0x7FFFFF00u;   // of the buffer that a workgroup's rows are written through
+
+// The vector (of head 0) that a row reads, kNoVector if its page lies outside the pool or the row outside the ranges.
+__device__ __forceinline__ uint64_t vector_of(const PagedDecodeArgs& a, const int32_t* s_starts, uint32_t row) {
+  const bool local = a.sequences < kStarts;
+  const uint32_t b = local ? sequence_of(s_starts, a.sequences, (int32_t)row) : sequence_of(a.row_starts, a.sequences, (int32_t)row);
+  const int64_t begin = local ? s_starts[b] : a.row_starts[b], end = local ? s_starts[b + 1] : a.row_starts[b + 1];
   const int64_t token = (int64_t)row - begin + (a.first_tokens ? a.first_tokens[b] : 0);
-  bool good = (int64_t)row >= begin && (int64_t)row < end && token >= 0;
-  const uint64_t col = (uint64_t)token / a.layout.page_size, slot = (uint64_t)token - col * a.layout.page_size;
-  good = good && col < a.table_width;
-  const int32_t page = good ? a.tables[(uint64_t)b * a.table_width + col] : 0;
-  good = good && (uint32_t)page < a.layout.pages;
-  const uint64_t v = good ? (uint64_t)page * a.layout.page_stride + (uint64_t)head * a.layout.head_step + slot * a.layout.slot_step
-                          : 0;
-  // the lane's eight codes: `bits` bytes, read as eight that stay inside the row
-  const uint32_t at = (uint32_t)t * p.bits, lo = min(at, p.row_bytes - 8u);
-  uint64_t w = *(const u64_any*)(p.codes + v * p.row_bytes + lo);
-  w >>= 8u * (at - lo);
-  const float scale = p.scales[v];
-  const uint32_t levels = 1u << p.bits, mask = levels - 1;
-  float y[8];
-  if (!p.polar) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = s_tab[(uint32_t)(w >> (p.bits * e)) & mask];
-  } else {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float r = s_tab[(uint32_t)(w >> (2 * p.bits * q)) & mask];
-      const uint32_t k = (uint32_t)(w >> (2 * p.bits * q + p.bits)) & mask;
-      y[2 * q] = r * s_tab[levels + k];
-      y[2 * q + 1] = r * s_tab[2 * levels + k];
-    }
-  }
-  fwht_contig<8, T, float>(y, t);
-  // as dec_out of pitch_vector.hip: the same bytes as the decode of a contiguous cache (a zero is +0 before its sign)
-  const float f = scale * (float)kInvSqrtD;
-  const uint32_t signs = lane_signs(p, t);
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    y[e] = __uint_as_float(__float_as_uint(__builtin_fmaf(y[e], f, 0.f)) ^ ((signs >> e) & 1u) << 31);
-  if (good) store_elems<IO, 8>(out.data, row * out.token_stride + head * out.head_stride + 8u * t, y, false);
+  if (row >= a.rows || (int64_t)row < begin || (int64_t)row >= end || token < 0 || token > 0x7FFFFFFF) return kNoVector;
+  const uint32_t col = (uint32_t)token / a.layout.page_size, slot = (uint32_t)token - col * a.layout.page_size;
+  if (col >= a.table_width) return kNoVector;
+  const int32_t page = a.tables[(uint64_t)b * a.table_width + col];
+  if ((uint32_t)page >= a.layout.pages) return kNoVector;
+  return (uint64_t)(uint32_t)page * a.layout.page_stride + (uint64_t)slot * a.layout.slot_step;
 }
 
-__global__ __launch_bounds__(kBlock) void paged_decode(PagedDecodeArgs a) {
-  __shared__ float s_tab[3 * 256];
-  const int tid = threadIdx.x, lane = tid & 63, t = lane & (T - 1), team = (tid >> 6) * V + lane / T;
-  const uint32_t kind = blockIdx.z, head = blockIdx.y;
-  const PagedPool& p = a.pool[kind];
-  if (!a.out[kind].data) return;
-  const int levels = 1 << p.bits;
-  if (p.polar) {
-    const int off = pitch_polar_offset(p.bits);
-    for (int i = tid; i < levels; i += kBlock) {
-      s_tab[i] = pitch_polar_radius_tab[off + i];
-      s_tab[levels + i] = pitch_polar_cos_tab[off + i];
-      s_tab[2 * levels + i] = pitch_polar_sin_tab[off + i];
+// The value of the lane of this quad that a DPP quad permutation names.
+template <int P>
+__device__ __forceinline__ float quad_of(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), P, 0xF, 0xF, true));
+}
+
+// Tables of the read-back: four two-bit codes, or two codes of up to five bits, look up the values of their coordinates with the
+// transform's first stages applied (as DecTab of pitch_vector.hip); wider codes look up one value each (PolarQuant: radius,
+// cosine and sine).
+template <int B, bool POLAR>
+struct ReadTab {
+  static constexpr int L = 1 << B, G = B == 2 && !POLAR ? 4 : B <= 5 ? 2 : 1;
+  static constexpr int kEntries = G == 4 ? 256 : G == 2 ? L * L : L, kFloats = G == 1 ? (POLAR ? 3 * L : L) : kEntries * G;
+  __device__ static __forceinline__ void build(float* tab, int tid) {
+    const float* const book = pitch_codebook_tab + pitch_codebook_offset(ilog2(D), B);
+    const float *const radius = pitch_polar_radius_tab + pitch_polar_offset(B), *const cosine = pitch_polar_cos_tab + pitch_polar_offset(B),
+                *const sine = pitch_polar_sin_tab + pitch_polar_offset(B);
+    for (int i = tid; i < kEntries; i += kBlock) {
+      if constexpr (G == 4) {
+        const float q0 = book[i & 3], q1 = book[(i >> 2) & 3], q2 = book[(i >> 4) & 3], q3 = book[i >> 6];
+        const float a0 = q0 + q1, a1 = q0 - q1, a2 = q2 + q3, a3 = q2 - q3;
+        *(f32x4*)(tab + 4 * i) = f32x4{a0 + a2, a1 + a3, a0 - a2, a1 - a3};
+      } else if constexpr (G == 2) {
+        const int c0 = i & (L - 1), c1 = i >> B;
+        const float x = POLAR ? radius[c0] * cosine[c1] : book[c0], y = POLAR ? radius[c0] * sine[c1] : book[c1];
+        *(f32x2*)(tab + 2 * i) = f32x2{x + y, x - y};
+      } else if constexpr (POLAR) {
+        tab[i] = radius[i];
+        tab[L + i] = cosine[i];
+        tab[2 * L + i] = sine[i];
+      } else {
+        tab[i] = book[i];
+      }
     }
-  } else {
-    const int off = pitch_codebook_offset(ilog2(D), p.bits);
-    for (int i = tid; i < levels; i += kBlock) s_tab[i] = pitch_codebook_tab[off + i];
+  }
+  // The values of the eight codes in x, with the first log2 G stages applied.
+  template <typename X>
+  __device__ static __forceinline__ void look(const float* tab, X x, float* y) {
+    if constexpr (G == 1) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const uint32_t c0 = (uint32_t)(x >> (B * e)) & (L - 1), c1 = (uint32_t)(x >> (B * (e + 1))) & (L - 1);
+        const float u = tab[c0];
+        y[e] = POLAR ? u * tab[L + c1] : u;
+        y[e + 1] = POLAR ? u * tab[2 * L + c1] : tab[c1];
+      }
+    } else {
+      constexpr uint32_t kMask = (uint32_t)(kEntries - 1) * (4 * G);   // an entry's byte offset
+#pragma unroll
+      for (int k = 0; k < 8 / G; ++k) {
+        constexpr int up = G == 4 ? 4 : 3;
+        const int pos = G * B * k;
+        const uint32_t at = (pos >= up ? (uint32_t)(x >> (pos >= up ? pos - up : 0)) : (uint32_t)x << (up - pos)) & kMask;
+        if constexpr (G == 4) {
+          const f32x4 v = *(const f32x4*)((const char*)tab + at);
+          y[4 * k] = v.x; y[4 * k + 1] = v.y; y[4 * k + 2] = v.z; y[4 * k + 3] = v.w;
+        } else {
+          const f32x2 v = *(const f32x2*)((const char*)tab + at);
+          y[2 * k] = v.x; y[2 * k + 1] = v.y;
+        }
+      }
+    }
+  }
+};
+constexpr int kReadTabFloats = 2048;
+
+// Keys or values of B bits of the workgroup's rows, heads [head, head + count): the codes and scales of all of them are asked for
+// at once, since a read takes long among the writes.
+template <int B, bool POLAR, int H>
+__device__ __forceinline__ void decode_rows(const PagedDecodeArgs& a, const PagedPool& p, const PagedVectors& out, uint32_t head,
+                                            uint32_t count, uint32_t row0, const uint64_t* s_vec, const float* s_tab) {
+  using TB = ReadTab<B, POLAR>;
+  static_assert(TB::kFloats <= kReadTabFloats, "table");
+  constexpr int kLoad = B == 2 ? 2 : B <= 4 ? 4 : 8, kRow = D * B / 8;   // bytes of a load, of a row
+  using X = std::conditional_t<(B <= 4), uint32_t, uint64_t>;
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, t = lane & (T - 1), team = lane / T;
+  const uint32_t at = (uint32_t)(t * B), lo = min(at, (uint32_t)(kRow - kLoad)), sh = 8u * (at - lo);
+  // dpp_lane_sign_bit<D, 8, true>: the transform's results are negated on some lanes
+  const uint32_t lane_sign = (uint32_t)(__builtin_popcount((unsigned)(t & 11)) & 1) << 31;
+  const uint32_t signs = lane_signs(p, t);
+  uint32_t flip[IO == 0 ? 8 : 4];   // of the values, or of the pairs of 16-bit values
+#pragma unroll
+  for (int e = 0; e < (IO == 0 ? 8 : 4); ++e)
+    flip[e] = IO == 0 ? signs << (31 - e) & 0x80000000u : (signs >> (2 * e) & 1u) << 15 | (signs >> (2 * e + 1) & 1u) << 31;
+  const uint64_t step = a.layout.head_step;
+  X w[H][2];
+  float scale[H][2];
+  uint32_t o[2];   // byte offsets from the workgroup's first row, past the range for rows that are not written
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t r = (uint32_t)((wid * 2 + i) * V + team);
+    const uint64_t v = s_vec[r];
+    const bool good = v != kNoVector;
+    const uint64_t u = (good ? v : 0) + (uint64_t)head * step;
+    const uint8_t* const q = p.codes + u * kRow + lo;
+    const float* const f = p.scales + u;
+    o[i] = good ? (r * (uint32_t)out.token_stride + (IO == 0 ? 8u * (t & ~3) + 4u * (t & 3) : 8u * t)) * Io<IO>::kBytes : kRangeBytes;
+#pragma unroll
+    for (int n = 0; n < H; ++n) {
+      const uint64_t s = min((uint32_t)n, count - 1) * step;
+      const uint8_t* const c = q + s * kRow;
+      w[n][i] = kLoad == 2 ? *(const u16_any*)c : kLoad == 4 ? *(const u32_any*)c : (X) * (const u64_any*)c;
+      scale[n][i] = f[s];
+    }
+  }
+  const float s1 = t & 1 ? -1.f : 1.f, s2 = t & 2 ? -1.f : 1.f, s8 = t & 8 ? -1.f : 1.f;
+#pragma unroll
+  for (int n = 0; n < H; ++n) {
+    if ((uint32_t)n >= count) break;
+    const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(
+        (char*)out.data + (row0 * out.token_stride + (head + n) * out.head_stride) * Io<IO>::kBytes, 0, kRangeBytes, 0x00027000);
+    float y[16];
+    TB::look(s_tab, (X)(w[n][0] >> sh), y);
+    TB::look(s_tab, (X)(w[n][1] >> sh), y + 8);
+#pragma unroll
+    for (int m = TB::G; m < 8; m *= 2)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (!(e & m)) {
+          const float u = y[e], v = y[e | m];
+          y[e] = u + v;
+          y[e | m] = u - v;
+        }
+    fmac_dpp16<1, 0>(y, s1);
+    fmac_dpp16<2, 0>(y, s2);
+    bfly4_dpp8<0>(y);
+    bfly4_dpp8<8>(y);
+    if constexpr (T == 16) fmac_dpp16<8, 0>(y, s8);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float fac = __uint_as_float(__float_as_uint(scale[n][i] * (float)kInvSqrtD) ^ lane_sign);
+      float r[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = __builtin_fmaf(y[8 * i + e], fac, 0.f);
+      if constexpr (IO == 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = __uint_as_float(__float_as_uint(r[e]) ^ flip[e]);
+        // four lanes exchange their halves: each of the two stores then writes 64 bytes in a row instead of four times 16
+        f32x4 z[2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float lo0 = quad_of<0x50>(r[e]), hi0 = quad_of<0x50>(r[4 + e]), lo1 = quad_of<0xFA>(r[e]), hi1 = quad_of<0xFA>(r[4 + e]);
+          z[0][e] = t & 1 ? hi0 : lo0;
+          z[1][e] = t & 1 ? hi1 : lo1;
+        }
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, z[0]), to, (int)o[i], 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, z[1]), to, (int)(o[i] + 64), 0, 0);
+      } else {   // (rounding to nearest even commutes with the sign)
+        const u32x4 v{narrow2<IO>(r[0], r[1]) ^ flip[0], narrow2<IO>(r[2], r[3]) ^ flip[1], narrow2<IO>(r[4], r[5]) ^ flip[2],
+                      narrow2<IO>(r[6], r[7]) ^ flip[3]};
+        __builtin_amdgcn_raw_buffer_store_b128(v, to, (int)o[i], 0, 0);
+      }
+    }
+  }
+}
+
+constexpr int kReadRows = 2 * VPB;   // of a workgroup: two vectors per team
+// Heads of a workgroup where these leave two workgroups per compute unit and kind, else one: at 16,384 rows of 8 heads, d = 128
+// bf16 (2 per unit), four take 12.0 us and one 13.2, at 8,192 rows 8.8 and 8.5, at 2,048 rows 5.9 and 4.8.
+constexpr uint32_t kReadHeads = 4;
+
+template <int H>
+__global__ __launch_bounds__(kBlock) void paged_decode(PagedDecodeArgs a, uint32_t groups) {
+  __shared__ __attribute__((aligned(16))) float s_tab[kReadTabFloats];
+  __shared__ int32_t s_starts[kStarts];
+  __shared__ uint64_t s_vec[kReadRows];
+  const int tid = threadIdx.x, kind = (int)blockIdx.y;
+  const uint32_t block = blockIdx.x / groups, head = (blockIdx.x - block * groups) * H, count = min((uint32_t)H, a.layout.kv_heads - head);
+  const uint32_t row0 = block * kReadRows;
+  const PagedVectors& out = a.out[kind];
+  if (!out.data) return;
+  const PagedPool& p = a.pool[kind];
+  if (a.sequences < kStarts)
+    for (uint32_t i = tid; i <= a.sequences; i += kBlock) s_starts[i] = a.row_starts[i];
+#define PITCH_PAGED_WIDTHS(F) F(2) F(3) F(4) F(5) F(6) F(7) F(8)
+#define PITCH_PAGED_TAB(B)                                \
+  case B:                                                 \
+    if (p.polar) ReadTab<B, true>::build(s_tab, tid);     \
+    else ReadTab<B, false>::build(s_tab, tid);            \
+    break;
+#define PITCH_PAGED_DECODE(B)                                                                   \
+  case B:                                                                                       \
+    if (p.polar) decode_rows<B, true, H>(a, p, out, head, count, row0, s_vec, s_tab);           \
+    else decode_rows<B, false, H>(a, p, out, head, count, row0, s_vec, s_tab);                  \
+    break;
+  switch (p.bits) {
+    PITCH_PAGED_WIDTHS(PITCH_PAGED_TAB)
+    default: break;
   }
   __syncthreads();
-  for (uint64_t base = (uint64_t)blockIdx.x * VPB; base < a.rows; base += (uint64_t)gridDim.x * VPB) {
-    const uint64_t row = base + team;
-    if (row < a.rows) decode_vectors(a, p, a.out[kind], head, (uint32_t)row, t, s_tab);
+  if (tid < kReadRows) s_vec[tid] = vector_of(a, s_starts, row0 + tid);
+  __syncthreads();
+  switch (p.bits) {
+    PITCH_PAGED_WIDTHS(PITCH_PAGED_DECODE)
+    default: break;
   }
+#undef PITCH_PAGED_DECODE
+#undef PITCH_PAGED_TAB
 }
 
 }  // namespace
@@ -337,8 +498,12 @@ hipError_t PITCH_CAT4(launch_paged_append_d, PITCH_DIM, _io, PITCH_IO)(const Pag
 }
 
 hipError_t PITCH_CAT4(launch_paged_decode_d, PITCH_DIM, _io, PITCH_IO)(const PagedDecodeArgs& a, hipStream_t s) {
-  const uint64_t need = ((uint64_t)a.rows + VPB - 1) / VPB, most = 8ull * (uint64_t)device_cu_count();
-  hipLaunchKernelGGL(paged_decode, dim3((uint32_t)(need < most ? need : most), a.layout.kv_heads, 2), dim3(kBlock), 0, s, a);
+  const uint32_t heads = a.layout.kv_heads, cus = (uint32_t)device_cu_count(), blocks = (a.rows + kReadRows - 1) / kReadRows;
+  const uint32_t groups = (heads + kReadHeads - 1) / kReadHeads;
+  if ((uint64_t)blocks * groups >= 2ull * cus)
+    hipLaunchKernelGGL(paged_decode<kReadHeads>, dim3(blocks * groups, 2), dim3(kBlock), 0, s, a, groups);
+  else
+    hipLaunchKernelGGL(paged_decode<1>, dim3(blocks * heads, 2), dim3(kBlock), 0, s, a, heads);
   return hipGetLastError();
 }
 

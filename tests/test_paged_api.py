@@ -154,7 +154,9 @@ DECODE_FAULTS = [
     (_set("call", row_starts_bytes=4 * B), "row starts"), (_set("call", first_tokens_bytes=4), "first tokens"),
     (_set("call", keys__data=None, values__data=None), "both null"), (_set("call", keys__bytes=64), "keys buffer"),
     (_set("call", keys__head_stride=0), "overlap"), (_set("call", values__token_stride=DIM), "overlap"),
-    (_set("call", rows=N + 1), "buffer has"),
+    (_set("call", rows=N + 1), "buffer has"), (_set("call", rows=(1 << 28) + 1), "2^28"),
+    (_set("call", keys__token_stride=(1 << 22) + 4, keys__bytes=1 << 40), "token stride"),
+    (_set("call", values__token_stride=1 << 23, values__bytes=1 << 40), "token stride"),
 ]
 ATTENTION_FAULTS = [
     (_set("call", io_type=_lib.IO_F32), "float16 or bfloat16"), (_set("call", io_type=9), "element type"),
