@@ -43,7 +43,6 @@ struct PagedAppendArgs {
   uint64_t table_rows;
   uint32_t tokens, q_heads, rotary;
   float eps;
-  uint32_t first[4];         // workgroups [first[i], first[i + 1]) take the keys, the values, the queries
 };
 
 struct PagedDecodeArgs {

@@ -54,41 +54,94 @@ __device__ __forceinline__ void store_bytes(uint8_t* p, uint64_t w, uint32_t byt
 // what float32 costs, so a code is that of the exact vector unless a value lies within 1e-15 of an edge: the write does not
 // depend on how the work is split. The norm's factor 1 / rms multiplies every coordinate alike: it changes no code and only
 // scales the stored norm (TurboQuant) or largest radius (PolarQuant). Queries are computed in float32 and rounded once.
+// A team takes one token and H of its heads: the token's weights and rotation are read and multiplied once, all heads are
+// loaded at once, and a rotation's partner coordinates come from their lane. Bound by arithmetic beside the copies: 8,191
+// tokens of 8 KV and 32 query heads (d = 128 bf16, norms, full rotation, 4 bits), 185 MB, take 54 us (3.4 TB/s); the queries
+// alone 34, keys and values alone 34. One token 4.1 us, 64 tokens 5.0.
 
-// y = w . x rotated to position pos, for this lane's coordinates; ss = sum of the x^2 over the vector (with a norm).
-template <typename F>
-__device__ __forceinline__ void norm_rotate(const PagedAppendArgs& a, const void* x, uint64_t at, const void* weight,
-                                            uint64_t pos, int t, F (&y)[8], F& ss) {
-  float f[8];
-  load_elems<IO, 8>(x, at + 8u * t, f);
+// Eight coordinates as they lie in memory.
+constexpr int kRawWords = IO == 0 ? 8 : 4;
+struct Raw {
+  uint32_t w[kRawWords];
+};
+__device__ __forceinline__ Raw load_raw(const void* base, uint64_t i) {
+  Raw r;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = (F)f[e];
-  if (weight) {
-    ss = F(0);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fma_t(y[e], y[e], ss);
-    ss = team_reduce<T>(ss, [](F p, F q) { return p + q; });
-    load_elems<IO, 8>(weight, 8u * t, f);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] *= (F)f[e];
+  for (int k = 0; k < kRawWords; k += 4) {
+    const u32x4 v = *(const u32x4*)((const char*)base + i * Io<IO>::kBytes + 4 * k);
+    r.w[k] = v.x; r.w[k + 1] = v.y; r.w[k + 2] = v.z; r.w[k + 3] = v.w;
   }
-  if (a.positions && 8u * t < a.rotary) {
-    // the partner coordinates are another lane's: read again (they are in the nearest cache)
-    const uint32_t half = a.rotary / 2, j = 8u * t, pj = j < half ? j + half : j - half;
-    float p[8], c[8], s[8];
-    load_elems<IO, 8>(x, at + pj, p);
-    load_elems<0, 8>(a.cos, pos * a.rotary + j, c);
-    load_elems<0, 8>(a.sin, pos * a.rotary + j, s);
-    if (weight) load_elems<IO, 8>(weight, pj, f);
+  return r;
+}
+__device__ __forceinline__ void widen(const Raw& r, float (&f)[8]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      F q = (F)p[e];
-      if (weight) q *= (F)f[e];
-      q = j < half ? -q : q;
-      y[e] = fma_t(y[e], (F)c[e], q * (F)s[e]);
-    }
+  for (int k = 0; k < 8; ++k) {
+    if constexpr (IO == 0) f[k] = __uint_as_float(r.w[k]);
+    else if (k % 2 == 0) widen2<IO>(r.w[k / 2], f[k], f[k + 1]);
   }
 }
+
+// The norm's weights and the rotation of one token, for this lane's coordinates: y = own . x + other . x of the partner lane.
+template <typename F>
+struct Turn {
+  F own[8], other[8];
+  int partner;    // lane (times 4) that holds the coordinates turned with these
+  bool scaled, turned;   // uniform: weights or a rotation are given; this lane's coordinates are rotated
+
+  __device__ __forceinline__ void set(const PagedAppendArgs& a, const void* weight, uint64_t pos, int lane, int t) {
+    const uint32_t half = a.rotary / 16;   // in lanes
+    scaled = weight || a.positions;
+    turned = a.positions && 2u * half > (uint32_t)t;
+    const int pt = turned ? ((uint32_t)t < half ? t + (int)half : t - (int)half) : t;
+    partner = (lane - t + pt) * 4;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      own[e] = F(1);
+      other[e] = F(0);
+    }
+    if (weight) {
+      float f[8];
+      load_elems<IO, 8>(weight, 8u * t, f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) own[e] = (F)f[e];
+    }
+    if (turned) {
+      float c[8], s[8], f[8];
+      load_elems<0, 8>(a.cos, pos * a.rotary + 8u * t, c);
+      load_elems<0, 8>(a.sin, pos * a.rotary + 8u * t, s);
+      if (weight) load_elems<IO, 8>(weight, 8u * pt, f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        own[e] *= (F)c[e];
+        other[e] = (uint32_t)t < half ? -(F)s[e] : (F)s[e];
+        if (weight) other[e] *= (F)f[e];
+      }
+    }
+  }
+  // ss = sum of the x^2 over the vector (where norm).
+  __device__ __forceinline__ void apply(const Raw& r, bool norm, F (&y)[8], F& ss) const {
+    float f[8];
+    widen(r, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (F)f[e];
+    if (norm) {
+      ss = F(0);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fma_t(y[e], y[e], ss);
+      ss = team_reduce<T>(ss, [](F p, F q) { return p + q; });
+    }
+    if (!scaled) return;
+    Raw o;
+#pragma unroll
+    for (int k = 0; k < kRawWords; ++k) o.w[k] = (uint32_t)__builtin_amdgcn_ds_bpermute(partner, (int)r.w[k]);
+    widen(o, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const F u = y[e] * own[e];
+      y[e] = turned ? fma_t((F)f[e], other[e], u) : u;
+    }
+  }
+};
 
 // The radius and angle codes of a pair near a rounding point, in float64 and the definition's order (see
 // polar_codes_exact in pitch_vector.hip; here the number of levels is a run-time value).
@@ -102,133 +155,176 @@ __device__ __attribute__((noinline)) uint32_t polar_pair_exact(double a, double 
   return (uint32_t)rq | (((uint32_t)tq & (levels - 1)) << 8);
 }
 
-// Keys (kind 0) or values (kind 1) of the workgroup's vectors.
-__device__ __forceinline__ void append_vectors(const PagedAppendArgs& a, const PagedPool& p, const PagedVectors& in,
-                                               const void* weight, bool rotate, uint32_t block, uint32_t blocks,
-                                               uint2* s_lut) {
-  const int tid = threadIdx.x, lane = tid & 63, t = lane & (T - 1), team = (tid >> 6) * V + lane / T;
-  const uint32_t heads = a.layout.kv_heads, count = a.tokens * heads;   // below 2^32 (checked by the caller)
-  const uint32_t signs = lane_signs(p, t);
-  if (!p.polar) {
+// The codes of this lane's eight coordinates of a vector, given in float64; scale = the vector's scale.
+template <bool POLAR>
+__device__ __forceinline__ uint64_t quantise(const PagedPool& p, double (&y)[8], uint32_t signs, int t, const uint2* s_lut,
+                                             double& scale) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = (signs >> e) & 1u ? -y[e] : y[e];
+  uint64_t w = 0;
+  if (!POLAR || !p.polar) {
+    double n2 = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) n2 = __builtin_fma(y[e], y[e], n2);
+    n2 = team_reduce<T>(n2, [](double x, double z) { return x + z; });
+    const double nrm = __builtin_sqrt(n2), us = (1.0 / (nrm > 0.0 ? nrm : 1.0)) * kInvSqrtD;
+    scale = nrm;
+    fwht_contig<8, T, double>(y, t);
+    // bucket u * 2^m + off holds at most one edge: code = edges below the bucket + [u > edge]
+    const double um = us * p.lut_scale;
+    uint2 entry[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int j = (int)__builtin_fma(y[e], um, p.lut_off);
+      entry[e] = s_lut[min(max(j, 0), p.lut_entries - 1)];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t code = entry[e].y + (y[e] * us > (double)__uint_as_float(entry[e].x) ? 1u : 0u);
+      w |= (uint64_t)code << (p.bits * e);
+    }
+    return w;
+  }
+  fwht_contig<8, T, double>(y, t);
+  double r2[4], top = 0.0;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    r2[q] = __builtin_fma(y[2 * q], y[2 * q], y[2 * q + 1] * y[2 * q + 1]);
+    top = r2[q] > top ? r2[q] : top;
+  }
+  top = team_reduce<T>(top, [](double x, double z) { return x > z ? x : z; });
+  const double rmax = __builtin_sqrt(top), safe = rmax > 0.0 ? rmax : 1.0, inv = 1.0 / safe;
+  scale = rmax * kInvSqrtD;
+  const uint32_t levels = 1u << p.bits;
+  const float fl = (float)levels;
+  uint32_t code[4], need = 0u;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    // float32 on the pair relative to the largest radius; what lies near a rounding point is decided in float64
+    const float af = (float)(y[2 * q] * inv), cf = (float)(y[2 * q + 1] * inv);
+    const float rf = __builtin_amdgcn_sqrtf(__builtin_fmaf(af, af, cf * cf));
+    bool ok = r2[q] > 0.0;
+    const float kr = guarded_floor(__builtin_fmaf(rf, fl - 1.f, 0.5f), ok);
+    const float ka = guarded_floor(__builtin_fmaf(angle_turns<8>(cf, af), fl, 0.5f), ok);
+    code[q] = min((uint32_t)kr, levels - 1) | (((uint32_t)ka & (levels - 1)) << 8);
+    need |= ok ? 0u : 1u << q;
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (need & (1u << q)) code[q] = polar_pair_exact(y[2 * q], y[2 * q + 1], r2[q], safe, levels);
+    w |= (uint64_t)(code[q] & 255u) << (2 * p.bits * q) | (uint64_t)(code[q] >> 8) << (2 * p.bits * q + p.bits);
+  }
+  return w;
+}
+
+// A team's token and its H heads from head on.
+struct Item {
+  uint32_t token, head;
+  bool any;
+  __device__ __forceinline__ Item(uint32_t block, int team, uint32_t tokens, uint32_t heads, int h) {
+    const uint32_t groups = (heads + h - 1) / h, count = tokens * groups, nominal = block * VPB + (uint32_t)team;
+    const uint32_t v = min(nominal, count - 1);
+    any = nominal < count;
+    token = v / groups;
+    head = (v - token * groups) * h;
+  }
+};
+template <int H>
+__device__ __forceinline__ void load_heads(const PagedVectors& in, const Item& it, uint32_t heads, int t, Raw (&x)[H]) {
+#pragma unroll
+  for (int n = 0; n < H; ++n)
+    x[n] = load_raw(in.data, it.token * in.token_stride + min(it.head + n, heads - 1) * in.head_stride + 8u * t);
+}
+// The token's row of the rotation tables; false if it lies outside them.
+__device__ __forceinline__ bool position_of(const PagedAppendArgs& a, uint32_t token, uint64_t& pos) {
+  pos = 0;
+  if (!a.positions) return true;
+  pos = (uint64_t)a.positions[token];
+  const bool ok = pos < a.table_rows;
+  pos = ok ? pos : 0;
+  return ok;
+}
+
+// Keys (normed and rotated) or values.
+template <int H, bool POLAR, bool KEYS>
+__device__ __forceinline__ void append_vectors(const PagedAppendArgs& a, uint32_t block, uint2* s_lut) {
+  const PagedPool& p = a.pool[KEYS ? 0 : 1];
+  const int tid = threadIdx.x, lane = tid & 63, t = lane & (T - 1);
+  const uint32_t heads = a.layout.kv_heads;
+  const Item it(block, (tid >> 6) * V + lane / T, a.tokens, heads, H);
+  Raw x[H];
+  load_heads<H>(a.in[KEYS ? 0 : 1], it, heads, t, x);
+  const int64_t slot = a.slots[it.token];
+  uint64_t pos;
+  const bool write = it.any & position_of(a, it.token, pos) & ((uint64_t)slot < (uint64_t)a.layout.pages * a.layout.page_size);
+  const void* const weight = KEYS ? a.k_norm : nullptr;
+  Turn<double> turn;
+  if constexpr (KEYS) turn.set(a, weight, pos, lane, t);
+  if (!POLAR || !p.polar) {
     for (int i = tid; i < p.lut_entries; i += kBlock) s_lut[i] = ((const uint2*)pitch_lut_tab)[p.lut + i];
     __syncthreads();
   }
-  for (uint32_t base = block * VPB; base < count; base += blocks * VPB) {
-    const uint32_t nominal = base + team, v = min(nominal, count - 1);
-    const uint32_t tok = v / heads, head = v - tok * heads;
-    const int64_t slot = a.slots[tok];
-    bool write = nominal < count && (uint64_t)slot < (uint64_t)a.layout.pages * a.layout.page_size;
-    uint64_t pos = 0;
-    if (a.positions) {
-      pos = (uint64_t)a.positions[tok];
-      write = write && pos < a.table_rows;
-      pos = pos < a.table_rows ? pos : 0;
-    }
-    double y[8], ss = 0.0;
-    if (rotate) {
-      norm_rotate<double>(a, in.data, tok * in.token_stride + head * in.head_stride, weight, pos, t, y, ss);
+  const uint32_t signs = lane_signs(p, t);
+  const uint64_t page = (uint64_t)slot / a.layout.page_size, in_page = (uint64_t)slot - page * a.layout.page_size;
+  uint64_t row = page * a.layout.page_stride + (uint64_t)it.head * a.layout.head_step + in_page * a.layout.slot_step;
+#pragma unroll 1
+  for (int n = 0; n < H; ++n) {
+    double y[8], ss = 0.0, scale;
+    if constexpr (KEYS) {
+      turn.apply(x[0], weight != nullptr, y, ss);
     } else {
       float f[8];
-      load_elems<IO, 8>(in.data, tok * in.token_stride + head * in.head_stride + 8u * t, f);
+      widen(x[0], f);
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = (double)f[e];
     }
-    const double r = weight ? 1.0 / __builtin_sqrt(ss * (1.0 / D) + (double)a.eps) : 1.0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = (signs >> e) & 1u ? -y[e] : y[e];
-    uint64_t w = 0;
-    double scale;
-    if (!p.polar) {
-      double n2 = 0.0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) n2 = __builtin_fma(y[e], y[e], n2);
-      n2 = team_reduce<T>(n2, [](double x, double z) { return x + z; });
-      const double nrm = __builtin_sqrt(n2), us = (1.0 / (nrm > 0.0 ? nrm : 1.0)) * kInvSqrtD;
-      scale = nrm * r;
-      fwht_contig<8, T, double>(y, t);
-      // bucket u * 2^m + off holds at most one edge: code = edges below the bucket + [u > edge]
-      const double um = us * p.lut_scale;
-      uint2 entry[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int j = (int)__builtin_fma(y[e], um, p.lut_off);
-        entry[e] = s_lut[min(max(j, 0), p.lut_entries - 1)];
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t code = entry[e].y + (y[e] * us > (double)__uint_as_float(entry[e].x) ? 1u : 0u);
-        w |= (uint64_t)code << (p.bits * e);
-      }
-    } else {
-      fwht_contig<8, T, double>(y, t);
-      double r2[4], top = 0.0;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        r2[q] = __builtin_fma(y[2 * q], y[2 * q], y[2 * q + 1] * y[2 * q + 1]);
-        top = r2[q] > top ? r2[q] : top;
-      }
-      top = team_reduce<T>(top, [](double x, double z) { return x > z ? x : z; });
-      const double rmax = __builtin_sqrt(top), safe = rmax > 0.0 ? rmax : 1.0, inv = 1.0 / safe;
-      scale = rmax * kInvSqrtD * r;
-      const uint32_t levels = 1u << p.bits;
-      const float fl = (float)levels;
-      uint32_t code[4], need = 0u;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        // float32 on the pair relative to the largest radius; what lies near a rounding point is decided in float64
-        const float af = (float)(y[2 * q] * inv), cf = (float)(y[2 * q + 1] * inv);
-        const float rf = __builtin_amdgcn_sqrtf(__builtin_fmaf(af, af, cf * cf));
-        bool ok = r2[q] > 0.0;
-        const float kr = guarded_floor(__builtin_fmaf(rf, fl - 1.f, 0.5f), ok);
-        const float ka = guarded_floor(__builtin_fmaf(angle_turns<8>(cf, af), fl, 0.5f), ok);
-        code[q] = min((uint32_t)kr, levels - 1) | (((uint32_t)ka & (levels - 1)) << 8);
-        need |= ok ? 0u : 1u << q;
-      }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (need & (1u << q)) code[q] = polar_pair_exact(y[2 * q], y[2 * q + 1], r2[q], safe, levels);
-        w |= (uint64_t)(code[q] & 255u) << (2 * p.bits * q) | (uint64_t)(code[q] >> 8) << (2 * p.bits * q + p.bits);
-      }
-    }
-    if (write) {
-      const uint64_t page = (uint64_t)slot / a.layout.page_size, in_page = (uint64_t)slot - page * a.layout.page_size;
-      const uint64_t row = page * a.layout.page_stride + (uint64_t)head * a.layout.head_step + in_page * a.layout.slot_step;
+    const uint64_t w = quantise<POLAR>(p, y, signs, t, s_lut, scale);
+    if (weight) scale *= 1.0 / __builtin_sqrt(ss * (1.0 / D) + (double)a.eps);
+    if (write && it.head + n < heads) {
       store_bytes(p.codes + row * p.row_bytes + (uint32_t)t * p.bits, w, p.bits);
       if (t == 0) p.scales[row] = (float)scale;
     }
+    row += a.layout.head_step;
+#pragma unroll
+    for (int i = 0; i + 1 < H; ++i) x[i] = x[i + 1];
   }
 }
 
-__device__ __forceinline__ void append_queries(const PagedAppendArgs& a, uint32_t block, uint32_t blocks) {
-  const int tid = threadIdx.x, lane = tid & 63, t = lane & (T - 1), team = (tid >> 6) * V + lane / T;
-  const uint32_t heads = a.q_heads, count = a.tokens * heads;
-  for (uint32_t base = block * VPB; base < count; base += blocks * VPB) {
-    const uint32_t nominal = base + team, v = min(nominal, count - 1);
-    const uint32_t tok = v / heads, head = v - tok * heads;
-    bool write = nominal < count;
-    uint64_t pos = 0;
-    if (a.positions) {
-      pos = (uint64_t)a.positions[tok];
-      write = write && pos < a.table_rows;
-      pos = pos < a.table_rows ? pos : 0;
-    }
+template <int H>
+__device__ __forceinline__ void append_queries(const PagedAppendArgs& a, uint32_t block) {
+  const int tid = threadIdx.x, lane = tid & 63, t = lane & (T - 1);
+  const Item it(block, (tid >> 6) * V + lane / T, a.tokens, a.q_heads, H);
+  Raw x[H];
+  load_heads<H>(a.q, it, a.q_heads, t, x);
+  uint64_t pos;
+  const bool write = it.any & position_of(a, it.token, pos);
+  Turn<float> turn;
+  turn.set(a, a.q_norm, pos, lane, t);
+#pragma unroll
+  for (int n = 0; n < H; ++n) {
     float y[8], ss = 0.f;
-    norm_rotate<float>(a, a.q.data, tok * a.q.token_stride + head * a.q.head_stride, a.q_norm, pos, t, y, ss);
+    turn.apply(x[n], a.q_norm != nullptr, y, ss);
     if (a.q_norm) {
       const float r = 1.f / __builtin_sqrtf(ss * (1.f / D) + a.eps);
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] *= r;
     }
-    if (write) store_elems<IO, 8>(a.q_out.data, tok * a.q_out.token_stride + head * a.q_out.head_stride + 8u * t, y, false);
+    if (write && it.head + n < a.q_heads)
+      store_elems<IO, 8>(a.q_out.data, it.token * a.q_out.token_stride + (it.head + n) * a.q_out.head_stride + 8u * t, y, false);
   }
 }
 
-__global__ __launch_bounds__(kBlock) void paged_append(PagedAppendArgs a) {
+// Workgroups take keys, values and q_turn times queries in turn, so that the keys' and values' arithmetic runs beside the queries'
+// copies; queries that are left come last. (POLAR: a pool is PolarQuant's. Its exact path's call costs registers.)
+template <int H, bool POLAR>
+__global__ __launch_bounds__(kBlock) void paged_append(PagedAppendArgs a, uint32_t kv_blocks, uint32_t q_blocks, uint32_t q_turn) {
   __shared__ uint2 s_lut[2048];
-  const uint32_t b = blockIdx.x;
-  if (b < a.first[1]) append_vectors(a, a.pool[0], a.in[0], a.k_norm, true, b, a.first[1], s_lut);
-  else if (b < a.first[2]) append_vectors(a, a.pool[1], a.in[1], nullptr, false, b - a.first[1], a.first[2] - a.first[1], s_lut);
-  else append_queries(a, b - a.first[2], a.first[3] - a.first[2]);
+  const uint32_t mixed = kv_blocks * (2 + q_turn), cycle = blockIdx.x / (2 + q_turn);
+  const uint32_t part = blockIdx.x < mixed ? (blockIdx.x - cycle * (2 + q_turn) + cycle) % (2 + q_turn) : 2;
+  const uint32_t q = blockIdx.x < mixed ? cycle * q_turn + part - 2 : blockIdx.x - 2 * kv_blocks;
+  if (part == 0 && cycle < kv_blocks) append_vectors<H, POLAR, true>(a, cycle, s_lut);
+  else if (part == 1 && cycle < kv_blocks) append_vectors<H, POLAR, false>(a, cycle, s_lut);
+  else if (part >= 2 && q < q_blocks) append_queries<H>(a, q);
 }
 
 // ----------------------------------------------------------------------------------------------------
@@ -486,15 +582,30 @@ hipError_t PITCH_CAT4(launch_paged_append_d, PITCH_DIM, _io, PITCH_IO)(const Pag
     p.lut_scale = li.scale;
     p.lut_off = li.off;
   }
-  const uint64_t most = 8ull * (uint64_t)device_cu_count();
-  const uint64_t kv = ((uint64_t)a.tokens * a.layout.kv_heads + VPB - 1) / VPB, q = ((uint64_t)a.tokens * a.q_heads + VPB - 1) / VPB;
-  const uint32_t nkv = (uint32_t)(kv < most ? kv : most), nq = (uint32_t)(q < 2 * most ? q : 2 * most);
-  a.first[0] = 0;
-  a.first[1] = nkv;
-  a.first[2] = 2 * nkv;
-  a.first[3] = 2 * nkv + nq;
-  hipLaunchKernelGGL(paged_append, dim3(a.first[3]), dim3(kBlock), 0, s, a);
-  return hipGetLastError();
+  // Four heads per team where these make eight workgroups per compute unit, else one: 8 KV and 32 query heads, d = 128 bf16, take
+  // 54 us and 98 at 8,191 tokens, 21 and 20 at 2,048, 9.8 and 7.6 at 512. PolarQuant takes one, whose kernel holds more waves (2 KV
+  // and 12 query heads at 8,000 tokens: 25 us, 35 with four). Among the keys and values come up to three workgroups of queries
+  // each (54 us; with one 56, with all of them last 65; an even number would give one XCD all of the keys).
+  const bool polar = a.pool[0].polar || a.pool[1].polar;
+  const uint32_t most = 1u << 25, slice = most / max(a.layout.kv_heads, a.q_heads);   // tokens of a launch, whose grid has a limit
+  for (uint32_t left = a0.tokens; left;) {
+    a.tokens = min(left, slice);
+    auto blocks = [&](uint32_t heads, uint32_t h) { return (uint32_t)(((uint64_t)a.tokens * ((heads + h - 1) / h) + VPB - 1) / VPB); };
+    const bool four = !polar && 2ull * blocks(a.layout.kv_heads, 4) + blocks(a.q_heads, 4) >= 8ull * (uint64_t)device_cu_count();
+    const uint32_t h = four ? 4 : 1, nkv = blocks(a.layout.kv_heads, h), nq = blocks(a.q_heads, h);
+    const uint32_t turn = min(3u, (nq + nkv - 1) / nkv) | 1u, grid = nkv * (2 + turn) + (nq > nkv * turn ? nq - nkv * turn : 0u);
+    void (*const kernel)(PagedAppendArgs, uint32_t, uint32_t, uint32_t) =
+        four ? paged_append<4, false> : polar ? paged_append<1, true> : paged_append<1, false>;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kBlock), 0, s, a, nkv, nq, turn);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    left -= a.tokens;
+    for (PagedVectors* v : {&a.in[0], &a.in[1], &a.q, &a.q_out})
+      if (v->data) v->data = (char*)v->data + (uint64_t)a.tokens * v->token_stride * Io<IO>::kBytes;
+    a.slots += a.tokens;
+    if (a.positions) a.positions += a.tokens;
+  }
+  return hipSuccess;
 }
 
 hipError_t PITCH_CAT4(launch_paged_decode_d, PITCH_DIM, _io, PITCH_IO)(const PagedDecodeArgs& a, hipStream_t s) {

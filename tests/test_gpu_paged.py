@@ -468,6 +468,29 @@ def test_pool_past_32_bits(q):
     assert int(cache.keyCodes[1].max()) == 0 and int(cache.keyCodes[-2].max()) == 0
 
 
+def test_append_of_more_tokens_than_one_launch_takes(q):
+    """2^25 + 3 tokens of one head, most of them with no slot: the first, the last of the first launch and those after it."""
+    import torch
+    import pitch_amd as P
+    n, d = (1 << 25) + 3, 64
+    cfg = q.config("turboQuant", d, 2)
+    cache = _cache(q, cfg, cfg, 1, 16, 1, "head")
+    one = torch.randn(1, 1, d, device="cuda", dtype=torch.float16)
+    slots = torch.full((n,), -1, dtype=torch.int64, device="cuda")
+    at = [0, (1 << 25) - 1, 1 << 25, (1 << 25) + 2]
+    for i, tok in enumerate(at):
+        slots[tok] = 3 * i
+    cache.enqueueAppend(one.expand(n, 1, d), one.expand(n, 1, d), slots)
+    codes, scales = torch.empty(16, dtype=torch.uint8, device="cuda"), torch.empty(1, device="cuda")
+    q.enqueueEncode(one.reshape(1, d), codes, scales, 1, cfg)
+    written = [3 * i for i in range(len(at))]
+    for t, ref in ((cache.keyCodes, codes), (cache.valueCodes, codes), (cache.keyScales, scales), (cache.valueScales, scales)):
+        got = t.reshape(16, -1).cpu()
+        for slot in range(16):
+            same = torch.equal(got[slot], ref.cpu())
+            assert same == (slot in written), slot
+
+
 def test_step_graph_replays_match_eager(q):
     """A layer's step (append with norms and rotation, attention of the rotated queries, a read-back) captured once on a stream of
     its own and replayed with new inputs, eager work in between: every replay writes what the same calls write eagerly."""
