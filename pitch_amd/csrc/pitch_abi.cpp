@@ -1504,7 +1504,7 @@ int pitch_paged_attention_workspace_size(const pitch_paged_cache_t* cache, const
   if (!bytes) return fail(PITCH_ERR_INVALID_INPUT, "bytes is null");
   int dev = 0;
   PITCH_TRY(current_device(&dev));
-  *bytes = 4u * pitch::paged_attention_workspace_floats(cache->key_config.dim, call->q_per_kv, call->sequences,
+  *bytes = 4u * pitch::paged_attention_workspace_floats(cache->key_config.dim, call->q_per_kv,
                                                         (uint32_t)pitch::device_cu_count());
   return ok();
 }
@@ -1535,7 +1535,7 @@ int pitch_enqueue_paged_attention(const pitch_paged_cache_t* cache, const pitch_
   int dev = 0;
   PITCH_TRY(current_device(&dev));
   const uint32_t cus = (uint32_t)pitch::device_cu_count();
-  const uint64_t ws = 4u * pitch::paged_attention_workspace_floats(dim, call->q_per_kv, call->sequences, cus);
+  const uint64_t ws = 4u * pitch::paged_attention_workspace_floats(dim, call->q_per_kv, cus);
   PITCH_TRY(check_aligned(call->workspace, call->workspace_bytes, ws, 16, "workspace"));
   BatchDeviceCheck check(dev);
   PITCH_TRY(paged_cache_device(cache, check));

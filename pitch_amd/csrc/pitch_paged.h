@@ -89,13 +89,14 @@ PITCH_DECLARE_PAGED(128, 1)
 PITCH_DECLARE_PAGED(128, 2)
 #undef PITCH_DECLARE_PAGED
 
-// Attention: most sequences of a call (their tiles' prefix sum lies in LDS), most waves of a workgroup, floats of a partial
-// result (maxima and sums of eight heads, accumulators of nh heads), floats of workspace of a call.
+// Attention: most sequences of a call (32 per lane of a wave), waves of a workgroup, floats of a partial result (maxima and sums
+// of eight heads, accumulators of nh heads), floats of workspace of a call (four words and two slots per workgroup, one slot per
+// wave; the same whatever the sequences are).
 constexpr uint32_t kPagedMostSequences = 2048;
 constexpr uint32_t kPagedAttnWaves = 8;
 constexpr uint32_t paged_slot_floats(uint32_t dim, uint32_t nh) { return 16 + dim * nh; }
-constexpr uint64_t paged_attention_workspace_floats(uint32_t dim, uint32_t nq, uint32_t sequences, uint32_t groups) {
-  return ((sequences + 4ull) & ~3ull) + 2ull * groups * kPagedAttnWaves * paged_slot_floats(dim, nq <= 4 ? 4 : 8);
+constexpr uint64_t paged_attention_workspace_floats(uint32_t dim, uint32_t nq, uint32_t groups) {
+  return groups * (4ull + (2ull + kPagedAttnWaves) * paged_slot_floats(dim, nq <= 4 ? 4 : 8));
 }
 #define PITCH_DECLARE_PAGED_ATTN(K)                                                             \
   hipError_t launch_paged_attention_d64_k##K(const PagedAttnArgs& a, uint32_t io, hipStream_t s); \

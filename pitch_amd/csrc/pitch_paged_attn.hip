@@ -243,38 +243,63 @@ __device__ __forceinline__ uint32_t length_of(const PagedAttnArgs& a, uint32_t b
   return len < 0 ? 0u : min((uint32_t)len, a.most_tokens);
 }
 
-// pref[i] = tiles of the sequences before i (one KV head), i = 0 .. sequences; lens[i] = their lengths. `part`: a word per wave.
-// The line's tiles, and its tiles times KV heads, are below 2^31 (checked by the caller).
-__device__ __forceinline__ void scan_tiles(const PagedAttnArgs& a, uint32_t* pref, uint32_t* lens, uint32_t* part, int tid) {
-  const uint32_t n = a.sequences, per = (n + 64 * W - 1) / (64 * W), first = min((uint32_t)tid * per, n), last = min(first + per, n);
-  uint32_t len = first < last ? length_of(a, first) : 0u;
-  uint32_t sum = 0;
-  for (uint32_t i = first; i < last; ++i) {
-    const uint32_t t = span_of(a, len).tiles;
-    lens[i] = len;
-    pref[i] = t;
-    sum += t;
-    if (i + 1 < last) len = length_of(a, i + 1);
-  }
-  uint32_t inc = sum;
-  const int lane = tid & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint32_t o = (uint32_t)__builtin_amdgcn_ds_bpermute((lane - d) << 2, (int)inc);
-    inc += lane >= d ? o : 0u;
-  }
-  if (lane == 63) part[tid >> 6] = inc;
-  __syncthreads();
-  uint32_t before = inc - sum;
-  for (int w = 0; w < tid >> 6; ++w) before += part[w];
-  for (uint32_t i = first; i < last; ++i) {
-    const uint32_t t = pref[i];
-    pref[i] = before;
-    before += t;
-  }
-  if (last == n && first < n) pref[n] = before;   // one thread has the last sequence
-  __syncthreads();
+// Sums over the lanes up to and with this one.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xF, 0xF, false);   // row_shr 1, 2, 4, 8
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xF, 0xF, false);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xF, 0xF, false);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xF, 0xF, false);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false);   // row_bcast 15, 31
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false);
+  return x;
 }
+
+// The sequences along the line, in the lanes of a wave (no barrier: every wave looks the lengths up by itself). Up to 64 sequences
+// have a lane each; of more, a lane sums `per` sequences, and the lane group that a wave's run is in is looked up one by one.
+// The line's tiles, and its tiles times KV heads, are below 2^31 (checked by the caller).
+struct Line {
+  uint32_t per, sums, total;               // sequences of a lane; tiles (of one KV head) before this lane's, of all
+  uint32_t first, count, len, before, end; // the window: lane i has the length of sequence first + i and the tiles before it
+
+  __device__ __forceinline__ void load(const PagedAttnArgs& a, int lane) {
+    const uint32_t n = a.sequences;
+    per = (n + 63u) >> 6;
+    uint32_t sum = 0;
+    first = 0;
+    count = n;
+    if (per == 1) {
+      len = (uint32_t)lane < n ? length_of(a, lane) : 0u;
+      sum = span_of(a, len).tiles;
+    } else {
+      const uint32_t at = lane * per;
+#pragma unroll 4
+      for (uint32_t i = 0; i < per; ++i) {
+        const uint32_t l = length_of(a, min(at + i, n - 1));
+        sum += at + i < n ? span_of(a, l).tiles : 0u;
+      }
+    }
+    const uint32_t inc = wave_scan(sum);
+    sums = inc - sum;
+    total = __builtin_amdgcn_readlane(inc, 63);
+    before = sums;
+    end = per == 1 ? total : 0u;
+  }
+  // The window over the tile x of the line.
+  __device__ __forceinline__ void move(const PagedAttnArgs& a, uint32_t x, int lane) {
+    if (x < end * a.layout.kv_heads) return;   // (x only grows)
+    const uint32_t at = (uint32_t)__builtin_popcountll(__ballot(sums * a.layout.kv_heads <= x)) - 1u;   // empty lanes are passed over
+    first = at * per;
+    count = min(per, a.sequences - first);
+    len = (uint32_t)lane < count ? length_of(a, first + lane) : 0u;
+    const uint32_t sum = span_of(a, len).tiles, inc = wave_scan(sum), base = __builtin_amdgcn_readlane(sums, at);
+    before = base + inc - sum;
+    end = base + __builtin_amdgcn_readlane(inc, 63);
+  }
+  // The window's lane whose sequence the tile x is in.
+  __device__ __forceinline__ uint32_t find(uint32_t x, uint32_t heads, int lane) const {
+    return (uint32_t)__builtin_popcountll(__ballot((uint32_t)lane < count && before * heads <= x)) - 1u;
+  }
+};
 
 // How the line of n tiles is cut: tiles per workgroup, and of a workgroup's tiles per wave.
 // x / d for x < 2^31, with r = floor((2^32 - 1) / d): one too small at most before the correction.
@@ -289,9 +314,13 @@ __device__ __forceinline__ uint32_t wave_tiles(uint32_t n, uint32_t per_group, u
   return (min(n - g * per_group, per_group) + W - 1) / W;
 }
 
-// The workspace: the prefix (sequences + 1 words, rounded up to 4), then two slots per wave of partial results: maxima and sums of
-// eight heads, and the accumulators as the lanes hold them. The last partial result of a wave (merged with its neighbours': of the
-// first of them) has its first slot, that of a pair which ends inside the wave's run its second.
+// The workspace: four words per workgroup, then slots of partial results (maxima and sums of eight heads, and the accumulators as
+// the lanes hold them): of each workgroup one of the pair that comes from the workgroups before and ends in it, one of the pair
+// that goes on behind it; then one per wave, of the pair that ends inside its run. The four words: the last workgroup of the pair
+// that begins in this one and goes on behind it, plus one (0: there is none), its sequence and its KV head.
+constexpr uint32_t left_slot(uint32_t group) { return 2 * group; }
+constexpr uint32_t right_slot(uint32_t group) { return 2 * group + 1; }
+__device__ __forceinline__ uint32_t wave_slot(uint32_t groups, uint32_t group, uint32_t wave) { return 2 * groups + group * W + wave; }
 constexpr uint32_t slot_floats(int nh) { return 16 + NC * 4 * (nh == 4 ? 32 : 64); }
 
 // ---------------------------------------------------------------------------------------------------- output
@@ -361,7 +390,7 @@ struct Lds {  // dwords
   static constexpr uint32_t kTab = tables_bytes(KB, VB, TWO) / 4;
   static constexpr uint32_t kMerge = W * (2 * NH + NC * 4 * (NH == 4 ? 32 : 64));
   static constexpr uint32_t kHead = kTab > kMerge ? kTab : kMerge;
-  static constexpr uint32_t words(uint32_t sequences) { return kHead + W * 4 * kPRow + 2 * W + 2 * sequences + 1; }
+  static constexpr uint32_t kWords = kHead + W * 4 * kPRow + W;
 };
 
 template <int KB, int VB, int NH, int IO>
@@ -374,10 +403,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   constexpr int VW = VB == 0 && D == 128 ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) uint32_t s_mem[];   // at LDS address 0
   uint32_t* const s_stage = s_mem + L::kHead;
-  uint32_t* const s_part = s_stage + W * 4 * kPRow;
-  uint32_t* const s_key = s_part + W;
-  uint32_t* const s_pref = s_key + W;
-  uint32_t* const s_len = s_pref + a.sequences + 1;
+  uint32_t* const s_key = s_stage + W * 4 * kPRow;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const uint32_t wid = __builtin_amdgcn_readfirstlane(tid >> 6), upper = g & 1 ? ~0u : 0u;
   const uint32_t heads = a.layout.kv_heads;
@@ -386,19 +412,18 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   Table<VB, false> vtab;
   ktab.load(a.k, tid);
   vtab.load(a.v, tid);
-  scan_tiles(a, s_pref, s_len, s_part, tid);
-  auto before = [&](uint32_t i) { return __builtin_amdgcn_readfirstlane(s_pref[i]) * heads; };
-  const uint32_t total = before(a.sequences);
-  if (blockIdx.x == 0)
-    for (uint32_t i = tid; i <= a.sequences; i += 64 * W) ((uint32_t*)a.ws)[i] = s_pref[i];
-  const uint32_t per_group = group_tiles(total, a), g0 = blockIdx.x * per_group;
-  if (g0 >= total) return;
+  Line line;
+  line.load(a, lane);
+  const uint32_t total = line.total * heads, per_group = group_tiles(total, a), g0 = blockIdx.x * per_group;
+  if (g0 >= total) {
+    if (tid == 0) ((uint32_t*)a.ws)[4 * blockIdx.x] = 0u;
+    return;
+  }
   const uint32_t per_wave = wave_tiles(total, per_group, blockIdx.x), g1 = min(g0 + per_group, total);
 
   uint32_t x0 = g0 + wid * per_wave;
   const uint32_t x1 = min(x0 + per_wave, g1);
-  float* const ws = a.ws + ((a.sequences + 4u) & ~3u);
-  const uint32_t slot = blockIdx.x * W + wid;
+  float* const ws = a.ws + 4 * a.groups;
   const uint32_t klb = lane_byte<KB, TWO>(lane) + key_base(KB, VB, TWO), vlb = lane_byte<VB, false>(lane) + value_base(KB, VB, TWO);
   uint32_t* const s_w = s_stage + wid * 4 * kPRow;
 
@@ -426,25 +451,14 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
 
   // ---- the loads run a tile ahead of the computation: the part of the next tile to load, this lane's page and offset (of its 16
   // tokens) in it
-  uint32_t xl = x0, seq = 0, tok = 0, col = 0, off = 0, run_end = 0, page = ~0u, span_begin = 0, span_end = 0;
+  uint32_t xl = x0, tok = 0, col = 0, off = 0, run_end = 0, page = ~0u, span_begin = 0, span_end = 0;
   Part part{};
   const int32_t* table = a.tables;
-  if (x0 < x1) {  // the sequence of the first tile
-    uint32_t lo = 0, hi = a.sequences;
-    while (hi - lo > 1) {
-      const uint32_t mid = (lo + hi) / 2;
-      if (before(mid) <= x0) lo = mid;
-      else hi = mid;
-    }
-    seq = lo;
-  }
   auto begin_part = [&]() __attribute__((always_inline)) {
-    Span sp;
-    for (;; ++seq) {   // (empty sequences have no tiles)
-      sp = span_of(a, __builtin_amdgcn_readfirstlane(s_len[seq]));
-      if (xl < before(seq + 1)) break;
-    }
-    const uint32_t into = xl - before(seq);
+    line.move(a, xl, lane);
+    const uint32_t at = line.find(xl, heads, lane), seq = line.first + at;
+    const Span sp = span_of(a, (uint32_t)__builtin_amdgcn_readlane(line.len, at));
+    const uint32_t into = xl - (uint32_t)__builtin_amdgcn_readlane(line.before, at) * heads;
     part.seq = seq;
     part.kv = into / sp.tiles;
     const uint32_t tile = into - part.kv * sp.tiles;
@@ -470,9 +484,10 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   Part loaded{};
   auto load_keys = [&]() __attribute__((always_inline)) {
     loaded = part;
-    safe = page < a.layout.pages ? page : 0u;
-    offs = off;
-    in = page < a.layout.pages && tok + n < span_end && tok + n >= span_begin;
+    const bool there = page < a.layout.pages;
+    safe = there ? page : safe;
+    offs = there ? off : offs;
+    in = there && tok + n < span_end && tok + n >= span_begin;
     dist = (float)(int32_t)(tok + n - (span_end - 1u));
     // the first row of this lane's 16 tokens; of all four groups of 16 in scalar registers
     const uint64_t row = (uint64_t)(a.k.codes + (uint64_t)part.kv * a.khead) + (uint64_t)safe * a.kpage + (uint64_t)(offs * a.kslot);
@@ -838,7 +853,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
     } else if (cur.end == x1) {
       tail = true;
     } else {
-      float* const out = ws + (uint64_t)(2 * slot + 1) * slot_floats(NH);
+      float* const out = ws + (uint64_t)(wid ? wave_slot(a.groups, blockIdx.x, wid) : left_slot(blockIdx.x)) * slot_floats(NH);
       if (lane == 0) {
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
@@ -871,18 +886,18 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
     prepare();
     for (uint32_t xc = x0;;) {
       compute();
+      if (++xc == x1) break;
       load_values();
       __builtin_amdgcn_sched_barrier(0);
-      if (++xc == cur.end) {
-        const bool more = xc < x1;
+      if (xc == cur.end) {
         const Part next = loaded;
-        if (more) load_queries(next);
+        load_queries(next);
         finish();
-        if (!more) break;
         cur = next;
         prepare();
       }
     }
+    finish();
   }
   const uint32_t key = tail ? cur.seq * heads + cur.kv : ~0u;   // (pairs with tiles: below 2^31)
 
@@ -908,67 +923,122 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   }
   __syncthreads();
   auto key_of = [&](uint32_t w) { return (uint32_t)__builtin_amdgcn_readfirstlane(s_key[w]); };
-  if (!tail || (wid > 0 && key_of(wid - 1) == key)) return;   // (uniform per wave; no barrier follows)
-  uint32_t last = wid + 1;
-  while (last < W && key_of(last) == key) ++last;
+  uint32_t first = wid, last = wid;
+  if (tail) {
+    ++last;
+    while (first > 0 && key_of(first - 1) == key) --first;
+    while (last < W && key_of(last) == key) ++last;
+  }
+  // the waves [first, last) have the pair's tiles [begin, end); the next one may have the rest of it, which ends inside its run
+  const uint32_t begin = g0 + first * per_wave, end = min(g0 + last * per_wave, g1);
+  const bool rest = tail && end < g1 && cur.pair_end > end;
+  const bool whole = tail && begin <= cur.pair_begin && (rest || end >= cur.pair_end);
+  const float* const rest_in = ws + (uint64_t)wave_slot(a.groups, blockIdx.x, last) * slot_floats(NH);
+  float* const out = ws + (uint64_t)(cur.pair_end <= g1 ? left_slot(blockIdx.x) : right_slot(blockIdx.x)) * slot_floats(NH);
   float mm[NH], lm[NH];
+  if (tail) {
+    // maxima and sums: lane NH w + h has head h's of wave w
+    const uint32_t lw = (uint32_t)lane / NH, lh = (uint32_t)lane % NH;
+    const bool mine = lw >= first && lw < last;
+    const uint32_t from = mine ? lw : wid;
+    const float pm = mine ? s_ml[from * kMl + lh] : -__FLT_MAX__, pl = mine ? s_ml[from * kMl + NH + lh] : 0.f;
+    const float rm = rest ? rest_in[lh] : -__FLT_MAX__, rl = rest ? rest_in[8 + lh] : 0.f;
+    auto other = [&](float x, int d) { return __uint_as_float((uint32_t)__builtin_amdgcn_ds_bpermute((lane ^ d) << 2, (int)__float_as_uint(x))); };
+    float top = fmax_hw(pm, rm);
 #pragma unroll
-  for (int h = 0; h < NH; ++h) mm[h] = M[h];
-  for (uint32_t w = wid + 1; w < last; ++w)
+    for (int d = NH; d < NH * W; d *= 2) top = fmax_hw(top, other(top, d));
+    const float pe = mine ? __builtin_amdgcn_exp2f(pm - top) : 0.f, re = __builtin_amdgcn_exp2f(rm - top);
+    float sum = pl * pe;
 #pragma unroll
-    for (int h = 0; h < NH; ++h) mm[h] = fmax_hw(mm[h], s_ml[w * kMl + h]);
-#pragma unroll
-  for (int h = 0; h < NH; ++h) lm[h] = 0.f;
-#pragma unroll
-  for (int c = 0; c < NC; ++c) acc[c] = v4f{0.f, 0.f, 0.f, 0.f};
-  for (uint32_t w = wid; w < last; ++w) {
-    float e[NH];
+    for (int d = NH; d < NH * W; d *= 2) sum += other(sum, d);
+    sum = __builtin_fmaf(rl, re, sum);
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
-      e[h] = __builtin_amdgcn_exp2f(s_ml[w * kMl + h] - mm[h]);
-      lm[h] = __builtin_fmaf(s_ml[w * kMl + NH + h], e[h], lm[h]);
+      mm[h] = lane_value(top, h);
+      lm[h] = lane_value(sum, h);
     }
+    if (last - first == 1 && !rest) {   // nothing to add
+      if (!whole && (NH == 8 || !(g & 1))) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const v4f x = s_acc[(w * NC + c) * kLanes + at];
+        for (int c = 0; c < NC; ++c) *(v4f*)(out + 16 + (c * kLanes + at) * 4) = acc[c];
+      }
+    } else
+    // the accumulators' columns, shared out over these waves: column c is read and written by one wave alone
+    for (uint32_t c = wid - first; c < NC; c += last - first) {
+      v4f x[W], col{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int v = 0; v < 4; ++v) acc[c][v] = __builtin_fmaf(x[v], NH == 8 ? pick(upper, e[v], e[NH - 4 + v]) : e[v], acc[c][v]);
+      for (int w = 0; w < W; ++w) x[w] = s_acc[(w * NC + c) * kLanes + at];
+      if (rest) {
+        const v4f y = *(const v4f*)(rest_in + 16 + (c * kLanes + at) * 4);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) col[v] = y[v] * (NH == 8 ? pick(upper, lane_value(re, v), lane_value(re, NH - 4 + v)) : lane_value(re, v));
+      }
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const bool in = (uint32_t)w >= first && (uint32_t)w < last;   // (uniform; other waves' words are not looked at)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const float e = NH == 8 ? pick(upper, lane_value(pe, NH * w + v), lane_value(pe, NH * w + NH - 4 + v)) : lane_value(pe, NH * w + v);
+          col[v] = __builtin_fmaf(in ? x[w][v] : 0.f, e, col[v]);
+        }
+      }
+      if (NH == 8 || !(g & 1)) {
+        if (whole) s_acc[(first * NC + c) * kLanes + at] = col;
+        else *(v4f*)(out + 16 + (c * kLanes + at) * 4) = col;
+      }
     }
   }
-  const uint32_t begin = g0 + wid * per_wave, end = min(g0 + last * per_wave, g1);
-  if (begin <= cur.pair_begin && end >= cur.pair_end) {
+  __syncthreads();
+  if (x0 < x1 && x1 == g1 && lane == 0) {
+    const bool more = cur.pair_end > g1 && cur.pair_begin >= g0;
+    *(w4*)((uint32_t*)a.ws + 4 * blockIdx.x) = w4{more ? (cur.pair_end - 1) / per_group + 1 : 0u, cur.seq, cur.kv, 0u};
+  }
+  if (!tail || first != wid) return;
+  if (whole) {
+    if (last - first > 1 || rest)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) acc[c] = s_acc[(first * NC + c) * kLanes + at];
     write_output<NH, IO>(a, cur.seq, cur.kv, acc, mm, lm, lane);
-    return;
-  }
-  float* const out = ws + (uint64_t)(2 * slot) * slot_floats(NH);
-  if (lane == 0) {
+  } else if (lane == 0) {
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
       out[h] = mm[h];
       out[8 + h] = lm[h];
     }
   }
-  if (NH == 8 || !(g & 1)) {
-#pragma unroll
-    for (int c = 0; c < NC; ++c) *(v4f*)(out + 16 + (c * kLanes + at) * 4) = acc[c];
-  }
 }
 
-// Joins the partial results of each pair of sequence and KV head that no wave or workgroup of paged_attn wrote as a whole, and
-// writes zeros for an empty sequence. A workgroup of paged_attn has left two of them at most, the merged last parts and one that
-// ends inside a wave's run: a lane each looks up whether it is there, its maxima and sums; then the waves add up the accumulators.
+// Joins the partial results of the pair of sequence and KV head that begins in a workgroup of paged_attn and goes on behind it: the
+// waves share its parts out, a lane each has a part's maxima and sums. The waves also write the zeros of empty sequences.
 constexpr int kJoinWaves = 8;
+constexpr int kJoinParts = 4;   // of a wave at a time
 template <int NH, int IO>
 __global__ __launch_bounds__(64 * kJoinWaves) void paged_join(PagedAttnArgs a) {
-  constexpr int kLanes = NH == 4 ? 32 : 64;
+  constexpr int kLanes = NH == 4 ? 32 : 64, kAtOnce = kJoinWaves * kJoinParts;
   __shared__ v4f s_acc[kJoinWaves - 1][NC][kLanes];
-  const uint32_t heads = a.layout.kv_heads, b = blockIdx.x / heads, kv = blockIdx.x - b * heads;
+  const uint32_t heads = a.layout.kv_heads;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const uint32_t wid = __builtin_amdgcn_readfirstlane(tid >> 6), upper = g & 1 ? ~0u : 0u;
-  const uint32_t* const pref = (const uint32_t*)a.ws;
-  const uint32_t p0 = pref[b], tiles = pref[b + 1] - p0, total = pref[a.sequences] * heads;
-  const float* const ws = a.ws + ((a.sequences + 4u) & ~3u);
+  const w4 pair = *(const w4*)((const uint32_t*)a.ws + 4 * blockIdx.x);
+  const float* const ws = a.ws + 4 * a.groups;
   const int at = NH == 8 ? lane : n + 16 * (g >> 1);
+  for (uint32_t b = blockIdx.x * kJoinWaves + wid; b < a.sequences; b += a.groups * kJoinWaves) {
+    if (span_of(a, length_of(a, b)).tiles) continue;
+    for (uint32_t kv = 0; kv < heads; ++kv) {
+      v4f acc[NC];
+      float m[NH], l[NH];
+#pragma unroll
+      for (int h = 0; h < NH; ++h) m[h] = l[h] = 0.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) acc[c] = v4f{0.f, 0.f, 0.f, 0.f};
+      write_output<NH, IO>(a, b, kv, acc, m, l, lane);
+    }
+  }
+  if (!pair[0]) return;   // (uniform over the workgroup)
+  const uint32_t parts = pair[0] - blockIdx.x;
+  auto part_of = [&](uint32_t c) {   // the last one ends in its workgroup
+    return ws + (uint64_t)(c + 1 < parts ? right_slot(blockIdx.x + c) : left_slot(blockIdx.x + c)) * slot_floats(NH);
+  };
   float M[NH], l[NH];
   v4f acc[NC];
 #pragma unroll
@@ -978,58 +1048,52 @@ __global__ __launch_bounds__(64 * kJoinWaves) void paged_join(PagedAttnArgs a) {
   }
 #pragma unroll
   for (int c = 0; c < NC; ++c) acc[c] = v4f{0.f, 0.f, 0.f, 0.f};
-  if (tiles) {
-    const uint32_t s = p0 * heads + kv * tiles, e = s + tiles, per_group = group_tiles(total, a);
-    const uint32_t first = s / per_group, last = (e - 1) / per_group, parts = 2 * (last - first + 1);
-    for (uint32_t c0 = 0; c0 < parts; c0 += 64) {
-      // part c0 + lane: the merged last parts (even) of a workgroup or the one that ends inside a wave's run (odd)
-      const uint32_t c = c0 + lane, grp = min(first + (c >> 1), last), g0 = grp * per_group, g1 = min(g0 + per_group, total);
-      const uint32_t per_wave = wave_tiles(total, per_group, grp), from = max(s, g0), to = min(e, g1);
-      const uint32_t wa = (from - g0) / per_wave, wb = (to - 1 - g0) / per_wave;
-      const uint32_t wa0 = g0 + wa * per_wave, wb1 = min(g0 + (wb + 1) * per_wave, g1);   // the runs' begin and end
-      const bool inside = wb1 > e;             // the pair ends inside the last wave's run: it is no last part there
-      // written by a wave, or by the workgroup that merged all of it
-      if (__any((wa == wb && wa0 <= s && wb1 >= e) || (!inside && wa0 <= s && to == e))) return;
-      const bool there = c < parts && (c & 1 ? inside : !inside || wb > wa);
-      const uint32_t slot = c & 1 ? 2 * (grp * W + wb) + 1 : 2 * (grp * W + wa);
-      const float* const in = ws + (uint64_t)slot * slot_floats(NH);
-      float pm[NH], pl[NH], mx[NH];
+  for (uint32_t c0 = 0; c0 < parts; c0 += kAtOnce) {
+    const bool there = lane < kAtOnce && c0 + lane < parts;
+    const float* const in = part_of(min(c0 + (uint32_t)lane % kAtOnce, parts - 1));
+    float pm[NH], pl[NH], mx[NH];
 #pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        pm[h] = there ? in[h] : -__FLT_MAX__;
-        pl[h] = there ? in[8 + h] : 0.f;
+    for (int h = 0; h < NH; h += 4) {
+      const v4f x = *(const v4f*)(in + h), y = *(const v4f*)(in + 8 + h);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        pm[h + k] = there ? x[k] : -__FLT_MAX__;
+        pl[h + k] = there ? y[k] : 0.f;
       }
-      wave_max_heads(pm, mx);
+    }
+    v4f y[kJoinParts][NC];   // (parts that are not there are read as the last one, and weigh nothing)
 #pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        const float m = fmax_hw(M[h], mx[h]), al = __builtin_amdgcn_exp2f(M[h] - m);
-        pm[h] = __builtin_amdgcn_exp2f(pm[h] - m);
-        l[h] = __builtin_fmaf(l[h], al, wave_sum(pl[h] * pm[h]));
-        M[h] = m;
+    for (int k = 0; k < kJoinParts; ++k) {
+      const float* const part = part_of(min(c0 + k * kJoinWaves + wid, parts - 1)) + 16;
 #pragma unroll
-        for (int k = 0; k < NC; ++k)
-          if (h < 4) {
-            acc[k][h & 3] *= NH == 8 && (g & 1) ? 1.f : al;
-          } else {
-            acc[k][h & 3] *= (g & 1) ? al : 1.f;
-          }
-      }
-      uint64_t left = __ballot(there);
-      uint32_t i = 0;
-      while (left) {
-        const int k = __builtin_ctzll(left);
-        left &= left - 1;
-        if ((i++ % kJoinWaves) != wid) continue;
-        const float* const part = ws + (uint64_t)__builtin_amdgcn_readlane(slot, k) * slot_floats(NH) + 16;
-        float f[NH];
+      for (int c = 0; c < NC; ++c) y[k][c] = *(const v4f*)(part + (c * kLanes + at) * 4);
+    }
+    wave_max_heads(pm, mx);
 #pragma unroll
-        for (int h = 0; h < NH; ++h) f[h] = lane_value(pm[h], k);
+    for (int h = 0; h < NH; ++h) {
+      const float m = fmax_hw(M[h], mx[h]), al = __builtin_amdgcn_exp2f(M[h] - m);
+      pm[h] = there ? __builtin_amdgcn_exp2f(pm[h] - m) : 0.f;
+      l[h] = __builtin_fmaf(l[h], al, wave_sum(pl[h] * pm[h]));
+      M[h] = m;
+      mx[h] = al;
+    }
 #pragma unroll
-        for (int x = 0; x < NC; ++x) {
-          const v4f y = *(const v4f*)(part + (x * kLanes + at) * 4);
+    for (int v = 0; v < 4; ++v) {
+      const float f = NH == 8 ? pick(upper, mx[v], mx[NH - 4 + v]) : mx[v];
 #pragma unroll
-          for (int v = 0; v < 4; ++v) acc[x][v] = __builtin_fmaf(y[v], NH == 8 ? pick(upper, f[v], f[NH - 4 + v]) : f[v], acc[x][v]);
-        }
+      for (int c = 0; c < NC; ++c) acc[c][v] *= f;
+    }
+#pragma unroll
+    for (int k = 0; k < kJoinParts; ++k) {
+      if (c0 + k * kJoinWaves + wid >= parts) break;
+      float f[NH];
+#pragma unroll
+      for (int h = 0; h < NH; ++h) f[h] = lane_value(pm[h], (int)(k * kJoinWaves + wid));
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float fv = NH == 8 ? pick(upper, f[v], f[NH - 4 + v]) : f[v];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) acc[c][v] = __builtin_fmaf(y[k][c][v], fv, acc[c][v]);
       }
     }
   }
@@ -1043,23 +1107,22 @@ __global__ __launch_bounds__(64 * kJoinWaves) void paged_join(PagedAttnArgs a) {
   for (int w = 0; w < kJoinWaves - 1; ++w)
 #pragma unroll
     for (int c = 0; c < NC; ++c) acc[c] += s_acc[w][c][at];
-  write_output<NH, IO>(a, b, kv, acc, M, l, lane);
+  write_output<NH, IO>(a, pair[1], pair[2], acc, M, l, lane);
 }
 
 // ---------------------------------------------------------------------------------------------------- launch
 template <int KB, int VB, int NH, int IO>
 hipError_t launch_one(const PagedAttnArgs& a, hipStream_t s) {
   using L = Lds<KB, VB, NH, IO == 1>;
-  constexpr uint32_t most = 4u * L::words(kPagedMostSequences);
-  static_assert(most <= 160u * 1024u, "LDS of one workgroup");
+  constexpr uint32_t bytes = 4u * L::kWords;
+  static_assert(bytes <= 160u * 1024u, "LDS of one workgroup");
   static_assert(slot_floats(NH) <= paged_slot_floats(D, NH), "a partial result fits its slot");
-  const uint32_t bytes = 4u * L::words(a.sequences);
-  if (bytes > 65536u) {   // a property of the kernel, not of the launch: every call sets the largest (as pitch_attn_codes.hip)
-    const hipError_t e = hipFuncSetAttribute((const void*)paged_attn<KB, VB, NH, IO>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+  if constexpr (bytes > 65536u) {
+    const hipError_t e = hipFuncSetAttribute((const void*)paged_attn<KB, VB, NH, IO>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e != hipSuccess) return e;
   }
   hipLaunchKernelGGL((paged_attn<KB, VB, NH, IO>), dim3(a.groups), dim3(64 * W), bytes, s, a);
-  hipLaunchKernelGGL((paged_join<NH, IO>), dim3(a.sequences * a.layout.kv_heads), dim3(64 * kJoinWaves), 0, s, a);
+  hipLaunchKernelGGL((paged_join<NH, IO>), dim3(a.groups), dim3(64 * kJoinWaves), 0, s, a);
   return hipGetLastError();
 }
 template <int VB>
