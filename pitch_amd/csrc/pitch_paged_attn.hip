@@ -255,64 +255,114 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 }
 
 // The sequences along the line, in the lanes of a wave (no barrier: every wave looks the lengths up by itself). Up to 64 sequences
-// have a lane each; of more, a lane sums `per` sequences, and the lane group that a wave's run is in is looked up one by one.
-// The line's tiles, and its tiles times KV heads, are below 2^31 (checked by the caller).
+// have a lane each; of more, a lane sums `per` sequences, and the group that a place lies in is looked up one by one. Places on the
+// line are counted twice: in tiles, and in units, of which a pair has one more than tiles, in front of them: its queries, its
+// output. Runs are cut in units. The line's units, times KV heads, are below 2^31 (checked by the caller).
+struct Place {
+  uint32_t lane, kv, tile, x;   // of the window; KV head; tile of the pair; tiles of the line before it
+};
 struct Line {
-  uint32_t per, sums, total;               // sequences of a lane; tiles (of one KV head) before this lane's, of all
-  uint32_t first, count, len, before, end; // the window: lane i has the length of sequence first + i and the tiles before it
+  uint32_t per, tsums, usums, tiles, units;   // sequences of a lane; tiles and units (of one KV head) before this lane's, and of all
+  uint32_t first, count, len, own, tbefore, ubefore;   // the window: lane i has sequence first + i's length, tiles, and those before it
+  uint32_t begin, end;                        // its units
 
   __device__ __forceinline__ void load(const PagedAttnArgs& a, int lane) {
     const uint32_t n = a.sequences;
     per = (n + 63u) >> 6;
-    uint32_t sum = 0;
-    first = 0;
+    uint32_t t = 0, u = 0;
+    first = begin = end = 0;
     count = n;
     if (per == 1) {
       len = (uint32_t)lane < n ? length_of(a, lane) : 0u;
-      sum = span_of(a, len).tiles;
+      own = t = span_of(a, len).tiles;
+      u = t + (t != 0);
     } else {
       const uint32_t at = lane * per;
 #pragma unroll 4
       for (uint32_t i = 0; i < per; ++i) {
-        const uint32_t l = length_of(a, min(at + i, n - 1));
-        sum += at + i < n ? span_of(a, l).tiles : 0u;
+        const uint32_t l = length_of(a, min(at + i, n - 1)), x = at + i < n ? span_of(a, l).tiles : 0u;
+        t += x;
+        u += x + (x != 0);
       }
     }
-    const uint32_t inc = wave_scan(sum);
-    sums = inc - sum;
-    total = __builtin_amdgcn_readlane(inc, 63);
-    before = sums;
-    end = per == 1 ? total : 0u;
+    const uint32_t ti = wave_scan(t), ui = wave_scan(u);
+    tbefore = tsums = ti - t;
+    ubefore = usums = ui - u;
+    tiles = __builtin_amdgcn_readlane(ti, 63);
+    units = __builtin_amdgcn_readlane(ui, 63);
+    if (per == 1) end = units;
   }
-  // The window over the tile x of the line.
-  __device__ __forceinline__ void move(const PagedAttnArgs& a, uint32_t x, int lane) {
-    if (x < end * a.layout.kv_heads) return;   // (x only grows)
-    const uint32_t at = (uint32_t)__builtin_popcountll(__ballot(sums * a.layout.kv_heads <= x)) - 1u;   // empty lanes are passed over
+  // The group of sequences of lane `at` as the window.
+  __device__ __forceinline__ void window(const PagedAttnArgs& a, uint32_t at, int lane) {
     first = at * per;
     count = min(per, a.sequences - first);
     len = (uint32_t)lane < count ? length_of(a, first + lane) : 0u;
-    const uint32_t sum = span_of(a, len).tiles, inc = wave_scan(sum), base = __builtin_amdgcn_readlane(sums, at);
-    before = base + inc - sum;
-    end = base + __builtin_amdgcn_readlane(inc, 63);
+    own = span_of(a, len).tiles;
+    const uint32_t u = own + (own != 0), ti = wave_scan(own), ui = wave_scan(u);
+    begin = __builtin_amdgcn_readlane(usums, at);
+    tbefore = __builtin_amdgcn_readlane(tsums, at) + ti - own;
+    ubefore = begin + ui - u;
+    end = begin + __builtin_amdgcn_readlane(ui, 63);
   }
-  // The window's lane whose sequence the tile x is in.
-  __device__ __forceinline__ uint32_t find(uint32_t x, uint32_t heads, int lane) const {
-    return (uint32_t)__builtin_popcountll(__ballot((uint32_t)lane < count && before * heads <= x)) - 1u;
+  // Where unit u of the line, below all of them, lies. (The last lane with no more units before it: empty ones are passed over.)
+  __device__ __forceinline__ Place find(const PagedAttnArgs& a, uint32_t u, int lane) {
+    const uint32_t heads = a.layout.kv_heads;
+    if (u < begin * heads || u >= end * heads) window(a, (uint32_t)__builtin_popcountll(__ballot(usums * heads <= u)) - 1u, lane);
+    Place p;
+    p.lane = (uint32_t)__builtin_popcountll(__ballot((uint32_t)lane < count && ubefore * heads <= u)) - 1u;
+    const uint32_t t = __builtin_amdgcn_readlane(own, p.lane), into = u - (uint32_t)__builtin_amdgcn_readlane(ubefore, p.lane) * heads;
+    p.kv = into / (t + 1);
+    const uint32_t r = into - p.kv * (t + 1);
+    p.tile = r ? r - 1 : 0u;
+    p.x = (uint32_t)__builtin_amdgcn_readlane(tbefore, p.lane) * heads + p.kv * t + p.tile;
+    return p;
+  }
+  // The first tile of the pair behind p's; there is one.
+  __device__ __forceinline__ void next(const PagedAttnArgs& a, Place& p, int lane) {
+    p.tile = 0;
+    if (++p.kv < a.layout.kv_heads) return;
+    p.kv = 0;
+    for (;;) {
+      const uint64_t more = __ballot((uint32_t)lane > p.lane && (uint32_t)lane < count && own != 0);
+      if (more) {
+        p.lane = (uint32_t)__builtin_ctzll(more);
+        return;
+      }
+      window(a, first / per + 1, lane);
+      if (__builtin_amdgcn_readlane(own, 0)) {
+        p.lane = 0;
+        return;
+      }
+      p.lane = 0;
+    }
   }
 };
 
-// How the line of n tiles is cut: tiles per workgroup, and of a workgroup's tiles per wave.
 // x / d for x < 2^31, with r = floor((2^32 - 1) / d): one too small at most before the correction.
 __device__ __forceinline__ uint32_t quotient(uint32_t x, uint32_t d, uint32_t r) {
   const uint32_t q = __umulhi(x, r);
   return x - q * d >= d ? q + 1u : q;
 }
-__device__ __forceinline__ uint32_t group_tiles(uint32_t n, const PagedAttnArgs& a) {
-  return quotient(n + a.groups - 1, a.groups, a.groups_r);
-}
-__device__ __forceinline__ uint32_t wave_tiles(uint32_t n, uint32_t per_group, uint32_t g) {
-  return (min(n - g * per_group, per_group) + W - 1) / W;
-}
+// How the line of n units is cut: workgroup b begins at ceil(b n / groups), so that a workgroup has one unit more than another at
+// most, and the one at the front of a pair that fills several has it; up to `groups` units, the first workgroups have one each.
+struct Cut {
+  uint32_t n, base, rest;
+  __device__ __forceinline__ Cut(uint32_t units, const PagedAttnArgs& a) : n(units) {
+    base = quotient(n, a.groups, a.groups_r);
+    rest = n - base * a.groups;
+  }
+  __device__ __forceinline__ uint32_t begin(uint32_t b, const PagedAttnArgs& a) const {
+    return base ? b * base + quotient(b * rest + a.groups - 1, a.groups, a.groups_r) : min(b, n);
+  }
+  __device__ __forceinline__ uint32_t group_of(uint32_t u, const PagedAttnArgs& a) const {
+    if (!base) return u;
+    uint32_t b = min((uint32_t)((float)u * (float)a.groups / (float)n), a.groups - 1);   // off by one at most
+    if (begin(b, a) > u) --b;
+    return begin(b + 1, a) <= u ? b + 1 : b;
+  }
+};
+// Unit of a workgroup's run of n units at which wave w begins (no empty wave lies between others).
+__device__ __forceinline__ uint32_t wave_begin(uint32_t n, uint32_t w) { return n < W ? min(w, n) : w * (n / W) + (w * (n % W) + W - 1) / W; }
 
 // The workspace: four words per workgroup, then slots of partial results (maxima and sums of eight heads, and the accumulators as
 // the lanes hold them): of each workgroup one of the pair that comes from the workgroups before and ends in it, one of the pair
@@ -390,7 +440,7 @@ struct Lds {  // dwords
   static constexpr uint32_t kTab = tables_bytes(KB, VB, TWO) / 4;
   static constexpr uint32_t kMerge = W * (2 * NH + NC * 4 * (NH == 4 ? 32 : 64));
   static constexpr uint32_t kHead = kTab > kMerge ? kTab : kMerge;
-  static constexpr uint32_t kWords = kHead + W * 4 * kPRow + W;
+  static constexpr uint32_t kWords = kHead + W * 4 * kPRow + 2 * W + 1;
 };
 
 template <int KB, int VB, int NH, int IO>
@@ -404,6 +454,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint32_t s_mem[];   // at LDS address 0
   uint32_t* const s_stage = s_mem + L::kHead;
   uint32_t* const s_key = s_stage + W * 4 * kPRow;
+  uint32_t* const s_run = s_key + W;   // the waves' first tiles, and the last one's end
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const uint32_t wid = __builtin_amdgcn_readfirstlane(tid >> 6), upper = g & 1 ? ~0u : 0u;
   const uint32_t heads = a.layout.kv_heads;
@@ -414,15 +465,18 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   vtab.load(a.v, tid);
   Line line;
   line.load(a, lane);
-  const uint32_t total = line.total * heads, per_group = group_tiles(total, a), g0 = blockIdx.x * per_group;
-  if (g0 >= total) {
+  const uint32_t total = line.units * heads;
+  const Cut cut(total, a);
+  const uint32_t u0 = cut.begin(blockIdx.x, a), u1 = cut.begin(blockIdx.x + 1, a);
+  if (u0 >= u1) {
     if (tid == 0) ((uint32_t*)a.ws)[4 * blockIdx.x] = 0u;
     return;
   }
-  const uint32_t per_wave = wave_tiles(total, per_group, blockIdx.x), g1 = min(g0 + per_group, total);
-
-  uint32_t x0 = g0 + wid * per_wave;
-  const uint32_t x1 = min(x0 + per_wave, g1);
+  const uint32_t from = u0 + wave_begin(u1 - u0, wid), to = u0 + wave_begin(u1 - u0, wid + 1);
+  const uint32_t x1 = to < total ? line.find(a, to, lane).x : line.tiles * heads;
+  Place place{0u, 0u, 0u, x1};
+  if (from < to) place = line.find(a, from, lane);
+  const uint32_t x0 = place.x;   // this wave's tiles: [x0, x1) of the line
   float* const ws = a.ws + 4 * a.groups;
   const uint32_t klb = lane_byte<KB, TWO>(lane) + key_base(KB, VB, TWO), vlb = lane_byte<VB, false>(lane) + value_base(KB, VB, TWO);
   uint32_t* const s_w = s_stage + wid * 4 * kPRow;
@@ -455,13 +509,11 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   Part part{};
   const int32_t* table = a.tables;
   auto begin_part = [&]() __attribute__((always_inline)) {
-    line.move(a, xl, lane);
-    const uint32_t at = line.find(xl, heads, lane), seq = line.first + at;
-    const Span sp = span_of(a, (uint32_t)__builtin_amdgcn_readlane(line.len, at));
-    const uint32_t into = xl - (uint32_t)__builtin_amdgcn_readlane(line.before, at) * heads;
+    const Span sp = span_of(a, (uint32_t)__builtin_amdgcn_readlane(line.len, place.lane));
+    const uint32_t tile = place.tile;
+    const uint32_t seq = line.first + place.lane;
     part.seq = seq;
-    part.kv = into / sp.tiles;
-    const uint32_t tile = into - part.kv * sp.tiles;
+    part.kv = place.kv;
     part.pair_begin = xl - tile;
     part.pair_end = part.pair_begin + sp.tiles;
     part.end = min(part.pair_end, x1);
@@ -532,7 +584,10 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
       off -= a.layout.page_size;
       ++col;
     }
-    if (xl < x1 && xl == part.end) begin_part();
+    if (xl < x1 && xl == part.end) {
+      line.next(a, place, lane);
+      begin_part();
+    }
     page = page_of();
   };
   // values: a lane group takes the 16 tokens of its own page, so that a lane's rows follow each other
@@ -907,7 +962,11 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   float* const s_ml = (float*)s_mem;
   v4f* const s_acc = (v4f*)(s_mem + W * kMl);
   const int at = NH == 8 ? lane : n + 16 * (g >> 1);
-  if (lane == 0) s_key[wid] = key;
+  if (lane == 0) {
+    s_key[wid] = key;
+    s_run[wid] = x0;
+    if (wid == W - 1) s_run[W] = x1;
+  }
   if (tail) {
     if (lane == 0) {
 #pragma unroll
@@ -930,7 +989,8 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
     while (last < W && key_of(last) == key) ++last;
   }
   // the waves [first, last) have the pair's tiles [begin, end); the next one may have the rest of it, which ends inside its run
-  const uint32_t begin = g0 + first * per_wave, end = min(g0 + last * per_wave, g1);
+  auto run_of = [&](uint32_t w) { return (uint32_t)__builtin_amdgcn_readfirstlane(s_run[w]); };
+  const uint32_t g0 = run_of(0), g1 = run_of(W), begin = run_of(first), end = run_of(last);
   const bool rest = tail && end < g1 && cur.pair_end > end;
   const bool whole = tail && begin <= cur.pair_begin && (rest || end >= cur.pair_end);
   const float* const rest_in = ws + (uint64_t)wave_slot(a.groups, blockIdx.x, last) * slot_floats(NH);
@@ -991,7 +1051,10 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   __syncthreads();
   if (x0 < x1 && x1 == g1 && lane == 0) {
     const bool more = cur.pair_end > g1 && cur.pair_begin >= g0;
-    *(w4*)((uint32_t*)a.ws + 4 * blockIdx.x) = w4{more ? (cur.pair_end - 1) / per_group + 1 : 0u, cur.seq, cur.kv, 0u};
+    const uint32_t unit = to + (cur.pair_end - x1);   // (the run ends inside the pair: only tiles are left of it)
+    *(w4*)((uint32_t*)a.ws + 4 * blockIdx.x) = w4{more ? cut.group_of(unit - 1, a) + 1 : 0u, cur.seq, cur.kv, 0u};
+  } else if (g0 == g1 && tid == 0) {
+    ((uint32_t*)a.ws)[4 * blockIdx.x] = 0u;
   }
   if (!tail || first != wid) return;
   if (whole) {
