@@ -18,7 +18,8 @@
 // coordinates of a token on the contraction axis; for the values a pair's two coordinates of one token side by side on it, with
 // the weight at the one or the other: rows 0 - 7 weigh the first coordinate, rows 8 - 15 the second. What rows remain hold the
 // operands' rest after rounding to float16: up to four heads, queries and weights both in two parts (22 bits); five to eight
-// heads, the queries in two, the weights in one (11 bits). TurboQuant's table values are stored times a factor at which they
+// heads, the queries in two and the weights in one (11 bits), or with float16 queries, whose outputs resolve that, in two by a
+// second instruction. TurboQuant's table values are stored times a factor at which they
 // nearly are float16 values (gen_tables.py: 4e-5 of a codebook's size for four bits, instead of 2e-4). With float16 queries the
 // keys' table values have two parts as well, whose products are added by a second instruction: a rounding of 2e-4 in the keys
 // moves a score of size 5 by 1e-3, several times what float16 outputs resolve (bfloat16: a quarter).
@@ -26,6 +27,8 @@
 // The table's entry of a pair (four codes for two bits) is 256 bytes long, copies for the keys in its first half and for the
 // values in its second (float16 queries: a table each): lanes read copies in different banks, and where the index is a byte of
 // the row, one v_perm makes the address.
+#include <atomic>
+
 #include "pitch_attn_shared.h"
 #include "pitch_paged.h"
 
@@ -439,8 +442,9 @@ template <int KB, int VB, int NH, bool TWO>
 struct Lds {  // dwords
   static constexpr uint32_t kTab = tables_bytes(KB, VB, TWO) / 4;
   static constexpr uint32_t kMerge = W * (2 * NH + NC * 4 * (NH == 4 ? 32 : 64));
+  static constexpr uint32_t kRows = TWO && NH == 8 ? 8 : 4;   // of staged weights per wave
   static constexpr uint32_t kHead = kTab > kMerge ? kTab : kMerge;
-  static constexpr uint32_t kWords = kHead + W * 4 * kPRow + 2 * W + 1;
+  static constexpr uint32_t kWords = kHead + W * kRows * kPRow + 2 * W + 1;
 };
 
 template <int KB, int VB, int NH, int IO>
@@ -453,7 +457,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   constexpr int VW = VB == 0 && D == 128 ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) uint32_t s_mem[];   // at LDS address 0
   uint32_t* const s_stage = s_mem + L::kHead;
-  uint32_t* const s_key = s_stage + W * 4 * kPRow;
+  uint32_t* const s_key = s_stage + W * L::kRows * kPRow;
   uint32_t* const s_run = s_key + W;   // the waves' first tiles, and the last one's end
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const uint32_t wid = __builtin_amdgcn_readfirstlane(tid >> 6), upper = g & 1 ? ~0u : 0u;
@@ -479,7 +483,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   const uint32_t x0 = place.x;   // this wave's tiles: [x0, x1) of the line
   float* const ws = a.ws + 4 * a.groups;
   const uint32_t klb = lane_byte<KB, TWO>(lane) + key_base(KB, VB, TWO), vlb = lane_byte<VB, false>(lane) + value_base(KB, VB, TWO);
-  uint32_t* const s_w = s_stage + wid * 4 * kPRow;
+  uint32_t* const s_w = s_stage + wid * L::kRows * kPRow;
 
   // A part of a pair of sequence and KV head: tiles [.., end) of the line belong to it and to this wave's run.
   struct Part {
@@ -528,7 +532,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   };
   auto page_of = [&]() __attribute__((always_inline)) { return tok < run_end ? (uint32_t)table[col] : ~0u; };   // no page beyond the part is looked up
   // A tile's loads run ahead of its computation: the keys' are issued when the tile before has its scores, the values' and the
-  // scales' when it is done. A page outside the pool, or past the run, is read as page 0 (in bounds, weight zero); there is no
+  // scales' when it is done. A page outside the pool, or past the run, is read as the one before it (first: 0; in bounds, weight zero); there is no
   // branch around a load, so that the compiler knows how many are in flight.
   uint32_t kw[4][KW], vw[16][VW], safe = 0, offs = 0;
   float nk = 0.f, nv = 0.f, dist = 0.f;
@@ -822,14 +826,22 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
     }
 #pragma unroll
     for (int h = 0; h < NH; ++h) l[h] += p[h];
-    // row r of the staged weights: four heads, head r's two parts; eight, the weights of heads r and r + 4
+    // row r of the staged weights: four heads, head r's two parts; eight, the weights of heads r and r + 4 (float16: row 4 + r
+    // their rests)
+    constexpr bool REST = TWO && NH == 8;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       if constexpr (NH == 4) {
         const float hi = (float)(_Float16)y[r];
         s_w[r * kPRow + lane] = f16_pair(hi, (y[r] - hi) * kLoScale);
       } else {
-        s_w[r * kPRow + lane] = f16_pair(y[r], y[r + 4]);
+        const uint32_t hi = f16_pair(y[r], y[r + 4]);
+        s_w[r * kPRow + lane] = hi;
+        if constexpr (REST) {
+          float p0, p1;
+          widen2<1>(hi, p0, p1);
+          s_w[(4 + r) * kPRow + lane] = f16_pair(y[r] - p0, y[r + 4] - p1);
+        }
       }
     }
     wave_lds_fence();
@@ -852,10 +864,11 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
     // a step: the pairs c (two bits: c and c + 1, which one table read gives) of four tokens
     constexpr int PC = VB == 2 ? 2 : 1, NS = 4 * NC / PC, kAhead = VB == 0 ? 1 : 2;
     uint32_t v[4][4][PC], none[PC];
-    w4 d[4], wa{};
+    w4 d[4], dr[4], wa{}, wr{};
     auto look = [&](int k) __attribute__((always_inline)) {
       const int m = k / (NC / PC), c = k % (NC / PC) * PC;
       if (c == 0) d[m] = *(const w4*)(s_row + 4 * m);
+      if (REST && c == 0) dr[m] = *(const w4*)(s_row + 4 * kPRow + 4 * m);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if constexpr (VB != 0) {
@@ -878,10 +891,17 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
       const int m = k / (NC / PC), c = k % (NC / PC) * PC;
       if (c == 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) wa[j] = __builtin_amdgcn_perm(0u, d[m][j], sel);
+        for (int j = 0; j < 4; ++j) {
+          wa[j] = __builtin_amdgcn_perm(0u, d[m][j], sel);
+          if (REST) wr[j] = __builtin_amdgcn_perm(0u, dr[m][j], sel);
+        }
       }
 #pragma unroll
-      for (int i = 0; i < PC; ++i) acc[c + i] = mfma_f16(wa, w4{v[k & 3][0][i], v[k & 3][1][i], v[k & 3][2][i], v[k & 3][3][i]}, acc[c + i]);
+      for (int i = 0; i < PC; ++i) {
+        const w4 x{v[k & 3][0][i], v[k & 3][1][i], v[k & 3][2][i], v[k & 3][3][i]};
+        acc[c + i] = mfma_f16(wa, x, acc[c + i]);
+        if (REST) acc[c + i] = mfma_f16(wr, x, acc[c + i]);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     wave_lds_fence();
@@ -1180,9 +1200,17 @@ hipError_t launch_one(const PagedAttnArgs& a, hipStream_t s) {
   constexpr uint32_t bytes = 4u * L::kWords;
   static_assert(bytes <= 160u * 1024u, "LDS of one workgroup");
   static_assert(slot_floats(NH) <= paged_slot_floats(D, NH), "a partial result fits its slot");
-  if constexpr (bytes > 65536u) {
-    const hipError_t e = hipFuncSetAttribute((const void*)paged_attn<KB, VB, NH, IO>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if constexpr (bytes > 65536u) {   // once per device and kernel: the call takes as long as a launch
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
     if (e != hipSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev > 63 || !(done.load(std::memory_order_relaxed) & bit)) {
+      e = hipFuncSetAttribute((const void*)paged_attn<KB, VB, NH, IO>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+      if (e != hipSuccess) return e;
+      if (dev <= 63) done.fetch_or(bit, std::memory_order_relaxed);
+    }
   }
   hipLaunchKernelGGL((paged_attn<KB, VB, NH, IO>), dim3(a.groups), dim3(64 * W), bytes, s, a);
   hipLaunchKernelGGL((paged_join<NH, IO>), dim3(a.groups), dim3(64 * kJoinWaves), 0, s, a);

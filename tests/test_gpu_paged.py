@@ -379,6 +379,26 @@ def test_attention(q, case):
     assert torch.equal(again, out), "the same call gives other bits"
 
 
+def _lengths(n, most, empty, seed):
+    rng = np.random.default_rng(seed)
+    return [int(x) if rng.random() >= empty else 0 for x in rng.integers(1, most + 1, n)]
+
+
+MANY = [   # more sequences than a wave has lanes, runs of empty ones, pairs that fill several workgroups beside short ones
+    (64, 2, 4, ("turboQuant", 4), ("turboQuant", 4), 16, "head", "bfloat16", [0] * 30 + [100] * 5 + [0] * 25 + [37, 0, 0, 900, 1], 0, 0, False),
+    (64, 3, 2, ("turboQuant", 4), ("turboQuant", 3), 32, "token", "float16", [0] * 80 + _lengths(140, 300, 0.4, 1) + [0] * 80, 0, 50, True),
+    (64, 1, 1, ("turboQuant", 3), ("turboQuant", 4), 16, "head", "bfloat16", _lengths(2048, 40, 0.3, 2), 0, 0, False),
+    (128, 5, 3, ("turboQuant", 4), ("turboQuant", 4), 16, "head", "bfloat16", [1] * 513, 0, 0, False),
+    (128, 1, 8, ("turboQuant", 4), ("turboQuant", 3), 64, "head", "float16", [40000, 0, 5], 0, 0, False),
+    (64, 2, 5, ("turboQuant", 4), ("turboQuant", 4), 16, "token", "bfloat16", [5000] + [1] * 100 + [7000, 0], 0, 0, False),
+]
+
+
+@pytest.mark.parametrize("case", MANY, ids=lambda c: f"d{c[0]}-kv{c[1]}x{c[2]}-{c[6]}-{c[7]}-{len(c[8])}seq")
+def test_attention_of_many_sequences(q, case):
+    test_attention(q, case)
+
+
 def test_attention_ignores_what_lies_outside(q):
     """NaN and infinite scales behind the length, in front of the window and in pages outside the pool's range weigh nothing;
     a length past the table is cut to it; several sequences may share pages."""
