@@ -51,6 +51,10 @@ constexpr float kTop = 32768.f;  // largest weight in an operand
 
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint64_t u64_any __attribute__((aligned(1)));
+// (an address made of integers is a flat one, which counts as an LDS access too: the table reads would wait for it)
+typedef __attribute__((address_space(1))) uint8_t global_u8;
+template <typename V>
+using global = __attribute__((address_space(1))) V;
 typedef __attribute__((address_space(3))) const uint32_t lds_cu32;
 typedef __attribute__((address_space(3))) const u2 lds_cu2;
 typedef __attribute__((address_space(3))) const w4 lds_cw4;
@@ -555,18 +559,18 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
     }
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
-      const uint8_t* const base = (const uint8_t*)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)row, 16 * m) |
+      const global_u8* const base = (const global_u8*)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)row, 16 * m) |
                                                    (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(row >> 32), 16 * m) << 32);
       if constexpr (KB != 0) {
-        const uint32_t* const q = (const uint32_t*)(base + k0[0]);
+        const global<uint32_t>* const q = (const global<uint32_t>*)(base + k0[0]);
         if constexpr (KW == 4) {
-          const u32x4 v = *(const u32x4*)q;
+          const u32x4 v = *(const global<u32x4>*)q;
           kw[m][0] = v.x; kw[m][1] = v.y; kw[m][2] = v.z; kw[m][3] = v.w;
         } else if constexpr (KW == 3) {
-          const u32x3 v = *(const u32x3*)q;
+          const u32x3 v = *(const global<u32x3>*)q;
           kw[m][0] = v.x; kw[m][1] = v.y; kw[m][2] = v.z;
         } else if constexpr (KW == 2) {
-          const u32x2 v = *(const u32x2*)q;
+          const u32x2 v = *(const global<u32x2>*)q;
           kw[m][0] = v.x; kw[m][1] = v.y;
         } else {
           kw[m][0] = *q;
@@ -574,7 +578,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
       } else {
 #pragma unroll
         for (int i = 0; i < KW / 2; ++i) {
-          const uint64_t v = *(const u64_any*)(base + k0[i]);
+          const uint64_t v = *(const global<u64_any>*)(base + k0[i]);
           kw[m][2 * i] = (uint32_t)v;
           kw[m][2 * i + 1] = (uint32_t)(v >> 32);
         }
