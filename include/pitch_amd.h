@@ -441,13 +441,13 @@ int pitch_enqueue_paged_decode(const pitch_paged_cache_t* cache, const pitch_pag
  * pitch_enqueue_attention_decode, which the reference does not have (README.md:96). */
 typedef struct pitch_paged_attention {
   uint32_t io_type;   /* PITCH_IO_F16 or PITCH_IO_BF16 */
-  uint32_t sequences; /* at least 1 */
+  uint32_t sequences; /* 1..2048 */
   uint32_t q_per_kv;  /* 1..8 */
   uint32_t window;    /* tokens; 0: all */
   pitch_paged_vectors_t queries, output; /* token = sequence, head = query head */
   const void* block_tables; /* int32 [sequences][table_width] */
   uint64_t block_tables_bytes;
-  uint64_t table_width;
+  uint64_t table_width; /* at least 1; (table_width * page_size / 64 + 2) * sequences * kv_heads < 2^31 */
   const void* lengths; /* int32 [sequences] */
   uint64_t lengths_bytes;
   const void* slopes; /* fp32 [q_per_kv * kv_heads], or null */

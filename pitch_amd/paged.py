@@ -214,7 +214,7 @@ class PagedDecode:
     """Reads tokens back: row r of keysOut / valuesOut [rows][kvHeads][dim] (one may be left out) with rowStarts[b] <= r <
     rowStarts[b + 1] (int32, sequences + 1 of them, not decreasing) is token firstTokens[b] (int32, default 0) + r -
     rowStarts[b] of sequence b, whose page is blockTables[b][token // pageSize] (int32). Other rows, and rows whose page lies
-    outside the pool or the table, are left as they were."""
+    outside the pool or the table, are left as they were. The outputs' token strides are at most 2^22 elements."""
 
     def __init__(self, cache: PagedCache, blockTables, rowStarts, keysOut=None, valuesOut=None, firstTokens=None):
         torch = _torch()
@@ -246,8 +246,8 @@ class PagedDecode:
 
 class PagedAttention:
     """One new token of every sequence over its pages: q and output [sequences][heads][dim] float16 or bfloat16 (heads =
-    kvHeads * 1..8; strided as in PagedAppend), blockTables int32 [sequences][pages], lengths int32 [sequences] with the new
-    token counted. The scores are softcap * tanh(scale q.k / softcap) (softcap 0: scale q.k; scale defaults to 1 / sqrt(dim))
+    kvHeads * 1..8; strided as in PagedAppend; at most 2,048 sequences), blockTables int32 [sequences][pages], lengths
+    int32 [sequences] with the new token counted. The scores are softcap * tanh(scale q.k / softcap) (softcap 0: scale q.k; scale defaults to 1 / sqrt(dim))
     plus slopes[h] * (t - (length - 1)) (float32 [heads]) over the last ``window`` tokens (0: all). lse, float32
     [sequences][heads], receives the natural-log sum of exp. A sequence of length 0 gives zeros (and minus infinity). Without
     a workspace one is allocated and held; two calls that may run at the same time must not share one."""
