@@ -587,7 +587,7 @@ hipError_t PITCH_CAT4(launch_paged_append_d, PITCH_DIM, _io, PITCH_IO)(const Pag
   // and 12 query heads at 8,000 tokens: 25 us, 35 with four). Among the keys and values come up to three workgroups of queries
   // each (54 us; with one 56, with all of them last 65; an even number would give one XCD all of the keys).
   const bool polar = a.pool[0].polar || a.pool[1].polar;
-  const uint32_t most = 1u << 25, slice = most / max(a.layout.kv_heads, a.q_heads);   // tokens of a launch, whose grid has a limit
+  const uint32_t most = 1u << 25, slice = max(1u, most / max(a.layout.kv_heads, a.q_heads));   // tokens of a launch, whose grid has a limit
   for (uint32_t left = a0.tokens; left;) {
     a.tokens = min(left, slice);
     auto blocks = [&](uint32_t heads, uint32_t h) { return (uint32_t)(((uint64_t)a.tokens * ((heads + h - 1) / h) + VPB - 1) / VPB); };

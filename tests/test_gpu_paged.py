@@ -260,6 +260,50 @@ def test_read(q, case):
     assert (wide[:, kv] == -5.0).all()
 
 
+@pytest.mark.parametrize("d,kv,nq,method,dtype,layout", [(128, 5, 7, "turboQuant", "bfloat16", "head"),
+                                                         (64, 6, 9, "turboQuant", "float32", "token"),
+                                                         (128, 7, 2, "polarQuant", "float16", "token"),
+                                                         (64, 9, 0, "turboQuant", "float16", "head")])
+def test_long_calls_equal_short_ones(q, d, kv, nq, method, dtype, layout):
+    """Long calls give a workgroup four heads of its tokens, here with groups that are not full, short calls one: the same codes,
+    scales, queries and vectors, bit for bit, and rows and slots that are not named stay as they were."""
+    import torch
+    n, page, dt = 12000, 64, _torch_dtype(dtype)
+    kcfg, vcfg = q.config(method, d, 5), q.config("turboQuant", d, 4)
+    torch.manual_seed(d + kv)
+    x = torch.randn(n, kv + nq, d, device="cuda").to(dt)
+    keys, values, queries = x[:, :kv], x[:, :kv].flip(0).contiguous(), x[:, kv:]
+    cos, sin = (torch.rand(n, d // 2, device="cuda") for _ in range(2))
+    weight = (torch.rand(d, device="cuda") + 0.5).to(dt)
+    pages = n // page + 2
+    slots = torch.randperm(pages * page, device="cuda")[:n]
+    slots[5::11] = -1
+    results = []
+    for step in (n, 500):
+        cache = _cache(q, kcfg, vcfg, pages, page, kv, layout)
+        out = torch.full((n, max(nq, 1), d), -3.0, dtype=dt, device="cuda")
+        for i in range(0, n, step):
+            at = slice(i, i + step)
+            more = dict(queries=queries[at], queriesOut=out[at], queryNorm=weight) if nq else {}
+            cache.enqueueAppend(keys[at], values[at], slots[at], keyNorm=weight, cos=cos, sin=sin,
+                                positions=torch.arange(n, device="cuda")[at], **more)
+        results.append([cache.keyCodes, cache.valueCodes, cache.keyScales, cache.valueScales, out])
+        back = [torch.full((n, kv + 1, d), -5.0, dtype=dt, device="cuda") for _ in range(2)]
+        table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+        for i in range(0, n, step):
+            m = min(step, n - i)
+            cache.enqueueDecode(table, torch.tensor([1, m - 1], dtype=torch.int32, device="cuda"), keysOut=back[0][i:i + m, :kv],
+                                valuesOut=back[1][i:i + m, :kv], firstTokens=torch.tensor([i + 1], dtype=torch.int32, device="cuda"))
+        inner = torch.ones(n, dtype=torch.bool, device="cuda")
+        inner[0::500] = inner[499::500] = False
+        for t in back:
+            assert (t[0] == -5).all() and (t[-1] == -5).all() and (t[:, kv] == -5).all()
+        results[-1] += [t[inner] for t in back]
+    torch.cuda.synchronize()
+    for name, a, b in zip(("key codes", "value codes", "key scales", "value scales", "queries", "keys", "values"), *results):
+        assert torch.equal(a, b), name
+
+
 # ----------------------------------------------------------------------------------------- attention
 def _attention64(cache, pool, tables, lengths, Q, scale, softcap, window, slopes):
     """(out, lse, sum of p |v|, largest scale |q| |k|) per sequence and query head, in float64."""
