@@ -254,10 +254,8 @@ __device__ __forceinline__ Span span_of(const PagedAttnArgs& a, uint32_t len) {
   s.tiles = s.end > s.base ? (s.end - s.base + 63u) >> 6 : 0u;
   return s;
 }
-__device__ __forceinline__ uint32_t length_of(const PagedAttnArgs& a, uint32_t b) {
-  const int32_t len = a.lengths[b];
-  return len < 0 ? 0u : min((uint32_t)len, a.most_tokens);
-}
+__device__ __forceinline__ uint32_t cut_length(const PagedAttnArgs& a, int32_t len) { return len < 0 ? 0u : min((uint32_t)len, a.most_tokens); }
+__device__ __forceinline__ uint32_t length_of(const PagedAttnArgs& a, uint32_t b) { return cut_length(a, a.lengths[b]); }
 
 // Sums over the lanes up to and with this one.
 __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
@@ -282,14 +280,15 @@ struct Line {
   uint32_t first, count, len, own, tbefore, ubefore;   // the window: lane i has sequence first + i's length, tiles, and those before it
   uint32_t begin, end;                        // its units
 
-  __device__ __forceinline__ void load(const PagedAttnArgs& a, int lane) {
+  // raw: lengths[lane], of the last sequence for lanes behind it.
+  __device__ __forceinline__ void load(const PagedAttnArgs& a, int32_t raw, int lane) {
     const uint32_t n = a.sequences;
     per = (n + 63u) >> 6;
     uint32_t t = 0, u = 0;
     first = begin = end = 0;
     count = n;
     if (per == 1) {
-      len = (uint32_t)lane < n ? length_of(a, lane) : 0u;
+      len = (uint32_t)lane < n ? cut_length(a, raw) : 0u;
       own = t = span_of(a, len).tiles;
       u = t + (t != 0);
     } else {
@@ -476,12 +475,14 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   const uint32_t wid = __builtin_amdgcn_readfirstlane(tid >> 6), upper = g & 1 ? ~0u : 0u;
   const uint32_t heads = a.layout.kv_heads;
 
+  const int32_t raw = a.lengths[min((uint32_t)lane, a.sequences - 1)];   // (in front of the tables' loads: they return in order)
+  __builtin_amdgcn_sched_barrier(0);
   Table<KB, TWO> ktab;
   Table<VB, false> vtab;
   ktab.load(a.k, tid);
   vtab.load(a.v, tid);
   Line line;
-  line.load(a, lane);
+  line.load(a, raw, lane);
   const uint32_t total = line.units * heads;
   const Cut cut(total, a);
   const uint32_t u0 = cut.begin(blockIdx.x, a), u1 = cut.begin(blockIdx.x + 1, a);
@@ -961,11 +962,15 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
     page = page_of();
     cur = part;
     load_queries(cur);
+  }
+  // the tables are written while the page is looked up
+  ktab.write(s_mem + key_base(KB, VB, TWO) / 4, a.k, a.kfactor, tid);
+  vtab.write(s_mem + value_base(KB, VB, TWO) / 4, a.v, a.vfactor, tid);
+  __builtin_amdgcn_sched_barrier(0);
+  if (x0 < x1) {
     load_keys();
     load_values();
   }
-  ktab.write(s_mem + key_base(KB, VB, TWO) / 4, a.k, a.kfactor, tid);
-  vtab.write(s_mem + value_base(KB, VB, TWO) / 4, a.v, a.vfactor, tid);
   // (orders LDS only: the loads of the first tile stay on their way)
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
   __builtin_amdgcn_s_barrier();
