@@ -75,6 +75,7 @@ struct PagedAttnArgs {
   uint32_t groups;           // workgroups
   uint32_t groups_r, page_r; // floor((2^32 - 1) / d) of groups and of page_size / 16 (set by the launcher, as the next two)
   uint32_t tile_cols, tile_rest;  // 64 tokens as pages and the rest
+  uint32_t whole;            // workgroups take whole pairs of sequence and KV head: no join
   uint32_t kpage, vpage, khead, vhead, kslot, vslot;  // bytes of codes from page to page, head to head, slot to slot
 };
 

@@ -12,7 +12,8 @@
 // sequence and KV head, whose queries and output cost about a tile (200 sequences of 1 to 500 tokens, 12 heads: 34 us, 41 by tiles
 // alone). A wave goes through its run by itself (scores, online softmax, weighted values; no barrier), pair by pair. A pair that
 // lies in one wave is written by it; the parts of one that several waves of a workgroup share are merged at the end through LDS,
-// and paged_join merges what crosses workgroups through the workspace, in an order fixed by the lengths alone.
+// and paged_join merges what crosses workgroups through the workspace, in an order fixed by the lengths alone. Where no pair can
+// have more than a tile per wave, workgroups take whole pairs and there is no join.
 //
 // What bounds it: HBM in between (5.1 TB/s while all waves run), and the chain of latencies at either end, which is half of the time
 // even of the longest calls: lengths, page, codes, tables and the queries' rotation (6 us before the first score), the slowest
@@ -273,7 +274,7 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 // line are counted twice: in tiles, and in units, of which a pair has one more than tiles, in front of them: its queries, its
 // output. Runs are cut in units. The line's units, times KV heads, are below 2^31 (checked by the caller).
 struct Place {
-  uint32_t lane, kv, tile, x;   // of the window; KV head; tile of the pair; tiles of the line before it
+  uint32_t lane, kv, unit, tile, x;   // of the window; KV head; unit and tile of the pair; tiles of the line before it
 };
 struct Line {
   uint32_t per, tsums, usums, tiles, units;   // sequences of a lane; tiles and units (of one KV head) before this lane's, and of all
@@ -328,6 +329,7 @@ struct Line {
     const uint32_t t = __builtin_amdgcn_readlane(own, p.lane), into = u - (uint32_t)__builtin_amdgcn_readlane(ubefore, p.lane) * heads;
     p.kv = into / (t + 1);
     const uint32_t r = into - p.kv * (t + 1);
+    p.unit = r;
     p.tile = r ? r - 1 : 0u;
     p.x = (uint32_t)__builtin_amdgcn_readlane(tbefore, p.lane) * heads + p.kv * t + p.tile;
     return p;
@@ -449,6 +451,15 @@ __device__ __forceinline__ void write_output(const PagedAttnArgs& a, uint32_t b,
   }
 }
 
+// The outputs of an empty sequence.
+__device__ __forceinline__ void write_zeros(const PagedAttnArgs& a, uint32_t b, int lane) {
+  const uint32_t heads = a.layout.kv_heads * a.nq;
+  for (uint32_t h = 0; h < heads; ++h)
+    if (lane < D / 2) *((uint32_t*)((uint16_t*)a.out.data + b * a.out.token_stride + h * a.out.head_stride) + lane) = 0u;
+  if (a.lse)
+    for (uint32_t h = lane; h < heads; h += 64) a.lse[(uint64_t)b * heads + h] = -__builtin_inff();
+}
+
 // ---------------------------------------------------------------------------------------------------- the kernel
 template <int KB, int VB, int NH, bool TWO>
 struct Lds {  // dwords
@@ -476,6 +487,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   const uint32_t heads = a.layout.kv_heads;
 
   const int32_t raw = a.lengths[min((uint32_t)lane, a.sequences - 1)];   // (in front of the tables' loads: they return in order)
+  int32_t raw_own = a.lengths[min(blockIdx.x * W + wid, a.sequences - 1)];
   __builtin_amdgcn_sched_barrier(0);
   Table<KB, TWO> ktab;
   Table<VB, false> vtab;
@@ -484,15 +496,24 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   Line line;
   line.load(a, raw, lane);
   const uint32_t total = line.units * heads;
+  // empty sequences: zeros
+  for (uint32_t b = blockIdx.x * W + wid; b < a.sequences; b += a.groups * W) {
+    if (span_of(a, cut_length(a, raw_own)).tiles == 0) write_zeros(a, b, lane);
+    raw_own = a.lengths[min(b + a.groups * W, a.sequences - 1)];
+  }
   const Cut cut(total, a);
-  const uint32_t u0 = cut.begin(blockIdx.x, a), u1 = cut.begin(blockIdx.x + 1, a);
+  uint32_t u0 = cut.begin(blockIdx.x, a), u1 = cut.begin(blockIdx.x + 1, a);
+  if (a.whole) {
+    if (u0 < total) u0 -= line.find(a, u0, lane).unit;
+    if (u1 < total) u1 -= line.find(a, u1, lane).unit;
+  }
   if (u0 >= u1) {
     if (tid == 0) ((uint32_t*)a.ws)[4 * blockIdx.x] = 0u;
     return;
   }
   const uint32_t from = u0 + wave_begin(u1 - u0, wid), to = u0 + wave_begin(u1 - u0, wid + 1);
   const uint32_t x1 = to < total ? line.find(a, to, lane).x : line.tiles * heads;
-  Place place{0u, 0u, 0u, x1};
+  Place place{0u, 0u, 0u, 0u, x1};
   if (from < to) place = line.find(a, from, lane);
   const uint32_t x0 = place.x;   // this wave's tiles: [x0, x1) of the line
   float* const ws = a.ws + 4 * a.groups;
@@ -1110,7 +1131,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
 }
 
 // Joins the partial results of the pair of sequence and KV head that begins in a workgroup of paged_attn and goes on behind it: the
-// waves share its parts out, a lane each has a part's maxima and sums. The waves also write the zeros of empty sequences.
+// waves share its parts out, a lane each has a part's maxima and sums.
 constexpr int kJoinWaves = 8;
 constexpr int kJoinParts = 4;   // of a wave at a time
 template <int NH, int IO>
@@ -1123,18 +1144,6 @@ __global__ __launch_bounds__(64 * kJoinWaves) void paged_join(PagedAttnArgs a) {
   const w4 pair = *(const w4*)((const uint32_t*)a.ws + 4 * blockIdx.x);
   const float* const ws = a.ws + 4 * a.groups;
   const int at = NH == 8 ? lane : n + 16 * (g >> 1);
-  for (uint32_t b = blockIdx.x * kJoinWaves + wid; b < a.sequences; b += a.groups * kJoinWaves) {
-    if (span_of(a, length_of(a, b)).tiles) continue;
-    for (uint32_t kv = 0; kv < heads; ++kv) {
-      v4f acc[NC];
-      float m[NH], l[NH];
-#pragma unroll
-      for (int h = 0; h < NH; ++h) m[h] = l[h] = 0.f;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) acc[c] = v4f{0.f, 0.f, 0.f, 0.f};
-      write_output<NH, IO>(a, b, kv, acc, m, l, lane);
-    }
-  }
   if (!pair[0]) return;   // (uniform over the workgroup)
   const uint32_t parts = pair[0] - blockIdx.x;
   auto part_of = [&](uint32_t c) {   // the last one ends in its workgroup
@@ -1231,7 +1240,7 @@ hipError_t launch_one(const PagedAttnArgs& a, hipStream_t s) {
     }
   }
   hipLaunchKernelGGL((paged_attn<KB, VB, NH, IO>), dim3(a.groups), dim3(64 * W), bytes, s, a);
-  hipLaunchKernelGGL((paged_join<NH, IO>), dim3(a.groups), dim3(64 * kJoinWaves), 0, s, a);
+  if (!a.whole) hipLaunchKernelGGL((paged_join<NH, IO>), dim3(a.groups), dim3(64 * kJoinWaves), 0, s, a);
   return hipGetLastError();
 }
 template <int VB>
@@ -1257,6 +1266,11 @@ hipError_t PITCH_CAT4(launch_paged_attention_d, PITCH_DIM, _k, PITCH_KB)(const P
   a.vhead = a.layout.head_step * a.v.row_bytes;
   a.kslot = a.layout.slot_step * a.k.row_bytes;
   a.vslot = a.layout.slot_step * a.v.row_bytes;
+  const uint32_t most = a.window ? min(a.window + 15u, a.most_tokens) : a.most_tokens;
+  // Pairs of a tile per wave at most: workgroups take whole ones, and there is no join (one sequence of up to 500 tokens and 8 KV
+  // heads 13.9 us, 14.6 with the join; 100 22.9 and 24.5; 200 of 12 heads of 64 30 and 33). At 16 tiles one sequence takes 16.7 and
+  // 15.0 us, 64 of eight bits 37 and 32: the waves of the longest pair are what the call waits for.
+  a.whole = (most + 63) / 64 <= (uint32_t)W;
   a.page_r = 0xFFFFFFFFu / (a.layout.page_size / 16);
   a.tile_cols = 64 / a.layout.page_size;
   a.tile_rest = 64 % a.layout.page_size;

@@ -435,6 +435,12 @@ MANY = [   # more sequences than a wave has lanes, runs of empty ones, pairs tha
     (128, 5, 3, ("turboQuant", 4), ("turboQuant", 4), 16, "head", "bfloat16", [1] * 513, 0, 0, False),
     (128, 1, 8, ("turboQuant", 4), ("turboQuant", 3), 64, "head", "float16", [40000, 0, 5], 0, 0, False),
     (64, 2, 5, ("turboQuant", 4), ("turboQuant", 4), 16, "token", "bfloat16", [5000] + [1] * 100 + [7000, 0], 0, 0, False),
+    # short tables or windows: workgroups take whole pairs
+    (128, 8, 4, ("turboQuant", 4), ("turboQuant", 4), 16, "head", "bfloat16", [430], 0, 0, False),
+    (64, 3, 8, ("turboQuant", 8), ("turboQuant", 4), 16, "token", "float16", [2000, 0, 3, 490, 1, 0], 0, 480, False),
+    (64, 12, 1, ("polarQuant", 3), ("turboQuant", 2), 32, "head", "bfloat16", [0] * 70 + _lengths(130, 470, 0.1, 3), 0, 0, True),
+    (128, 1, 2, ("turboQuant", 2), ("turboQuant", 3), 16, "head", "float16", [0, 0, 17, 0], 30.0, 0, False),
+    (128, 40, 2, ("turboQuant", 4), ("turboQuant", 3), 16, "head", "bfloat16", [300, 20, 0], 0, 16, False),
 ]
 
 
