@@ -9,7 +9,7 @@
 // Work split. The sequences' tiles of 64 tokens, sequence by sequence and KV head by KV head, form one line that is cut into
 // equal runs, one per workgroup (one per compute unit), and each run into equal runs of its waves: a batch of any lengths loads
 // every wave alike, and only the host-known number of workgroups is launched. What is cut equally is tiles and one more per pair of
-// sequence and KV head, whose queries and output cost about a tile (200 sequences of 1 to 500 tokens, 12 heads: 34 us, 41 by tiles
+// sequence and KV head, whose queries and output cost about a tile (200 sequences of 1 to 500 tokens, 12 heads: 34 us then, 41 by tiles
 // alone). A wave goes through its run by itself (scores, online softmax, weighted values; no barrier), pair by pair. A pair that
 // lies in one wave is written by it; the parts of one that several waves of a workgroup share are merged at the end through LDS,
 // and paged_join merges what crosses workgroups through the workspace, in an order fixed by the lengths alone. Where no pair can
@@ -19,7 +19,7 @@
 // even of the longest calls: lengths, page, codes, tables and the queries' rotation (6 us before the first score), the slowest
 // wave, the merge and the join (4 and 5 us). d = 128 bf16, 4 queries per KV head: 32 sequences of up to 8,000 tokens (138 MB)
 // 47 us, 131,072 tokens of one (126 MB) 48 us, 777 tokens 15 us. Heads of 64: eight bits and float16 (two table parts, window of
-// 1,000 tokens, 64 sequences) 32 us and the short sequences above 34, bound by the arithmetic of the lookups. Two tiles in
+// 1,000 tokens, 64 sequences) 30 us and the short sequences above 30, bound by the arithmetic of the lookups. Two tiles in
 // registers, 12 or 16 waves (spills), priorities for the waves behind, non-temporal reads and a touch of the second tile's lines at
 // the start were no faster.
 //
@@ -184,10 +184,17 @@ __device__ __forceinline__ uint32_t product(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, a) * __builtin_bit_cast(f16x2, b));
 }
 
-// The COUNT pairs of 2 COUNT codes: the N words w hold the codes from bit `at` on (constants); the widths above four bits have
-// them in w[0], w[1], `bits` bits each. hi: the pairs' float16 values, lo (TWO): their rests.
+// Four codes of 5 to 7 bits as bytes.
+__device__ __forceinline__ uint32_t spread(uint32_t x, uint32_t bits) {
+  const uint32_t two = (1u << 2 * bits) - 1u, one = ((1u << bits) - 1u) * 0x10001u;
+  const uint32_t t = (x & two) | (x >> 2 * bits & two) << 16;
+  return (t & one) | (t & one << bits) << (8u - bits);
+}
+
+// The COUNT pairs of 2 COUNT codes: the N words w hold the codes from bit `at` on (constants); the widths above four bits have a
+// byte per code. hi: the pairs' float16 values, lo (TWO): their rests.
 template <int B, bool TWO, int COUNT, int N>
-__device__ __forceinline__ void look_pairs(const uint32_t (&w)[N], int at, uint32_t lb, uint32_t bits, bool polar, uint32_t (&hi)[COUNT],
+__device__ __forceinline__ void look_pairs(const uint32_t (&w)[N], int at, uint32_t lb, bool polar, uint32_t (&hi)[COUNT],
                                            uint32_t (&lo)[COUNT]) {
   constexpr uint32_t kSel = 0x0C060004u;   // bytes: the lane's, a byte of the codes, the table's base above 64 KB, 0
   if constexpr (B == 2) {
@@ -218,12 +225,11 @@ __device__ __forceinline__ void look_pairs(const uint32_t (&w)[N], int at, uint3
       }
     }
   } else {
-    uint64_t x = w[0];
-    if constexpr (N > 1) x |= (uint64_t)w[1] << 32;
-    const uint32_t mask8 = ((1u << bits) - 1u) << 8;
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) {
-      const uint32_t a0 = ((uint32_t)(x >> (bits * (2 * i))) << 8 & mask8) | lb, a1 = ((uint32_t)(x >> (bits * (2 * i + 1))) << 8 & mask8) | lb;
+      const int p = at + 16 * i;
+      const uint32_t a0 = __builtin_amdgcn_perm(lb, w[p >> 5], kSel | (uint32_t)((p & 31) >> 3) << 8);
+      const uint32_t a1 = __builtin_amdgcn_perm(lb, w[p >> 5], kSel | (uint32_t)((p & 31) / 8 + 1) << 8);
       if constexpr (!TWO) {
         hi[i] = product(*(lds_cu32*)(uintptr_t)a0, *(lds_cu32*)(uintptr_t)(a1 + 64u));
       } else if (polar) {   // the copies' bytes: 16 of four, then 16 of eight
@@ -750,11 +756,12 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
     for (int m = 0; m < 4; ++m) {
       cs[m] = v4f{0.f, 0.f, 0.f, 0.f};
       if constexpr (KB == 0) {
+        if (a.k.bits == 8) continue;   // a row's words are whole codes
 #pragma unroll
         for (int j = 0; j < KW / 2; ++j) {
           const uint64_t v = ((uint64_t)kw[m][2 * j + 1] << 32 | kw[m][2 * j]) >> ksh[j];
-          kw[m][2 * j] = (uint32_t)v;
-          kw[m][2 * j + 1] = (uint32_t)(v >> 32);
+          kw[m][2 * j] = spread((uint32_t)v, a.k.bits);
+          kw[m][2 * j + 1] = spread((uint32_t)(v >> 4 * a.k.bits), a.k.bits);
         }
       } else if constexpr (GC * KB % 32 != 0) {
 #pragma unroll
@@ -766,12 +773,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
       uint32_t hi[4][4], lo[4][4];
       auto look = [&](int k) {
         const int s = k >> 2, m = k & 3;
-        if constexpr (KB == 0) {
-          const uint32_t w[2] = {kw[m][2 * s], kw[m][2 * s + 1]};
-          look_pairs<KB, TWO, 4>(w, 0, klb, a.k.bits, a.k.polar != 0, hi[k & 3], lo[k & 3]);
-        } else {
-          look_pairs<KB, TWO, 4>(kw[m], 8 * KB * s, klb, 0u, false, hi[k & 3], lo[k & 3]);
-        }
+        look_pairs<KB, TWO, 4>(kw[m], 8 * (KB ? KB : 8) * s, klb, a.k.polar != 0, hi[k & 3], lo[k & 3]);
       };
       constexpr int kAhead = KB == 0 ? 1 : 2;
 #pragma unroll
@@ -882,15 +884,16 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
     wave_lds_fence();
 
     // ---- weighted values: the accumulators' rows 0 - 7 weigh a pair's first coordinate, 8 - 15 its second
-    if constexpr (kShiftV) {
+    if (kShiftV && (VB != 0 || a.v.bits != 8)) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         if constexpr (VW == 2) {
           const uint64_t v = ((uint64_t)vw[j][1] << 32 | vw[j][0]) >> vsh;
-          vw[j][0] = (uint32_t)v;
-          vw[j][1] = (uint32_t)(v >> 32);
+          vw[j][0] = spread((uint32_t)v, a.v.bits);
+          vw[j][1] = spread((uint32_t)(v >> 4 * a.v.bits), a.v.bits);
         } else {
           vw[j][0] >>= vsh;
+          if constexpr (VB == 0) vw[j][0] = spread(vw[j][0], a.v.bits);
         }
       }
     }
@@ -906,15 +909,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
       if (REST && c == 0) dr[m] = *(const w4*)(s_row + 4 * kPRow + 4 * m);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if constexpr (VB != 0) {
-          look_pairs<VB, false, PC>(vw[4 * m + j], 2 * VB * c, vlb, 0u, false, v[k & 3][j], none);
-        } else {
-          uint64_t x = vw[4 * m + j][0];
-          if constexpr (VW == 2) x |= (uint64_t)vw[4 * m + j][VW - 1] << 32;
-          x >>= a.v.bits * (2 * c);
-          const uint32_t w[2] = {(uint32_t)x, (uint32_t)(x >> 32)};
-          look_pairs<VB, false, PC>(w, 0, vlb, a.v.bits, false, v[k & 3][j], none);
-        }
+        look_pairs<VB, false, PC>(vw[4 * m + j], 2 * (VB ? VB : 8) * c, vlb, a.v.polar != 0, v[k & 3][j], none);
       }
     };
 #pragma unroll
