@@ -56,8 +56,23 @@ __device__ __forceinline__ void store_bytes(uint8_t* p, uint64_t w, uint32_t byt
 // scales the stored norm (TurboQuant) or largest radius (PolarQuant). Queries are computed in float32 and rounded once.
 // A team takes one token and H of its heads: the token's weights and rotation are read and multiplied once, all heads are
 // loaded at once, and a rotation's partner coordinates come from their lane. Bound by arithmetic beside the copies: 8,191
-// tokens of 8 KV and 32 query heads (d = 128 bf16, norms, full rotation, 4 bits), 185 MB, take 54 us (3.4 TB/s); the queries
-// alone 34, keys and values alone 34. One token 4.1 us, 64 tokens 5.0.
+// tokens of 8 KV and 32 query heads (d = 128 bf16, norms, full rotation, 4 bits), 185 MB, take 50 us (3.7 TB/s); the queries
+// alone about 32, keys and values alone 32. One token 4.0 us, 64 tokens 5.0.
+
+// 1 / sqrt(x) of a normal positive x, to 2^-51: the hardware's estimate and two steps of Newton's, a third of what a division by
+// the correctly rounded root takes.
+__device__ __forceinline__ double inv_sqrt(double x) {
+  const double h = 0.5 * x;
+  double r = __builtin_amdgcn_rsq(x);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) r = __builtin_fma(r, __builtin_fma(-(h * r), r, 0.5), r);
+  return r;
+}
+// The same in float32, to 2^-23 (the hardware's, which takes no subnormal numbers).
+__device__ __forceinline__ float inv_sqrt(float x) {
+  const bool tiny = x < 0x1p-96f;
+  return __builtin_amdgcn_rsqf(tiny ? x * 0x1p96f : x) * (tiny ? 0x1p48f : 1.f);
+}
 
 // Eight coordinates as they lie in memory.
 constexpr int kRawWords = IO == 0 ? 8 : 4;
@@ -155,20 +170,29 @@ __device__ __attribute__((noinline)) uint32_t polar_pair_exact(double a, double 
   return (uint32_t)rq | (((uint32_t)tq & (levels - 1)) << 8);
 }
 
-// The codes of this lane's eight coordinates of a vector, given in float64; scale = the vector's scale.
-template <bool POLAR>
-__device__ __forceinline__ uint64_t quantise(const PagedPool& p, double (&y)[8], uint32_t signs, int t, const uint2* s_lut,
-                                             double& scale) {
+// Eight codes of p.bits bits each as the bytes of a row.
+__device__ __forceinline__ uint64_t pack(const uint32_t (&c)[8], uint32_t bits) {
+  uint32_t lo = c[0], hi = c[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = (signs >> e) & 1u ? -y[e] : y[e];
-  uint64_t w = 0;
+  for (int e = 1; e < 4; ++e) {
+    lo |= c[e] << (bits * e);
+    hi |= c[4 + e] << (bits * e);
+  }
+  return (uint64_t)lo | (uint64_t)hi << (4 * bits);
+}
+
+// The codes of this lane's eight coordinates of a vector, given in float64 times their signs; scale = the vector's scale.
+template <bool POLAR>
+__device__ __forceinline__ uint64_t quantise(const PagedPool& p, double (&y)[8], int t, const uint2* s_lut, double& scale) {
+  uint32_t codes[8];
   if (!POLAR || !p.polar) {
     double n2 = 0.0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) n2 = __builtin_fma(y[e], y[e], n2);
     n2 = team_reduce<T>(n2, [](double x, double z) { return x + z; });
-    const double nrm = __builtin_sqrt(n2), us = (1.0 / (nrm > 0.0 ? nrm : 1.0)) * kInvSqrtD;
-    scale = nrm;
+    const bool some = n2 > 0.0 && n2 < (double)__builtin_inf();
+    const double inv = some ? inv_sqrt(n2) : 1.0, us = inv * kInvSqrtD;
+    scale = some ? n2 * inv : n2;
     fwht_contig<8, T, double>(y, t);
     // bucket u * 2^m + off holds at most one edge: code = edges below the bucket + [u > edge]
     const double um = us * p.lut_scale;
@@ -180,10 +204,9 @@ __device__ __forceinline__ uint64_t quantise(const PagedPool& p, double (&y)[8],
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const uint32_t code = entry[e].y + (y[e] * us > (double)__uint_as_float(entry[e].x) ? 1u : 0u);
-      w |= (uint64_t)code << (p.bits * e);
+      codes[e] = entry[e].y + (y[e] * us > (double)__uint_as_float(entry[e].x) ? 1u : 0u);
     }
-    return w;
+    return pack(codes, p.bits);
   }
   fwht_contig<8, T, double>(y, t);
   double r2[4], top = 0.0;
@@ -212,9 +235,10 @@ __device__ __forceinline__ uint64_t quantise(const PagedPool& p, double (&y)[8],
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     if (need & (1u << q)) code[q] = polar_pair_exact(y[2 * q], y[2 * q + 1], r2[q], safe, levels);
-    w |= (uint64_t)(code[q] & 255u) << (2 * p.bits * q) | (uint64_t)(code[q] >> 8) << (2 * p.bits * q + p.bits);
+    codes[2 * q] = code[q] & 255u;
+    codes[2 * q + 1] = code[q] >> 8;
   }
-  return w;
+  return pack(codes, p.bits);
 }
 
 // A team's token and its H heads from head on.
@@ -259,17 +283,32 @@ __device__ __forceinline__ void append_vectors(const PagedAppendArgs& a, uint32_
   const bool write = it.any & position_of(a, it.token, pos) & ((uint64_t)slot < (uint64_t)a.layout.pages * a.layout.page_size);
   const void* const weight = KEYS ? a.k_norm : nullptr;
   Turn<double> turn;
-  if constexpr (KEYS) turn.set(a, weight, pos, lane, t);
+  const uint32_t signs = lane_signs(p, t);
+  if constexpr (KEYS) {
+    turn.set(a, weight, pos, lane, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {   // the vector's signs go with the factors, without any onto the words as they lie in memory
+      turn.own[e] = (signs >> e) & 1u ? -turn.own[e] : turn.own[e];
+      turn.other[e] = (signs >> e) & 1u ? -turn.other[e] : turn.other[e];
+    }
+  }
+  uint32_t flip[kRawWords];
+#pragma unroll
+  for (int k = 0; k < kRawWords; ++k) {
+    flip[k] = IO == 0 ? signs << (31 - k) & 0x80000000u : (signs >> (2 * k) & 1u) << 15 | (signs >> (2 * k + 1) & 1u) << 31;
+    if (KEYS && turn.scaled) flip[k] = 0u;
+  }
   if (!POLAR || !p.polar) {
     for (int i = tid; i < p.lut_entries; i += kBlock) s_lut[i] = ((const uint2*)pitch_lut_tab)[p.lut + i];
     __syncthreads();
   }
-  const uint32_t signs = lane_signs(p, t);
   const uint64_t page = (uint64_t)slot / a.layout.page_size, in_page = (uint64_t)slot - page * a.layout.page_size;
   uint64_t row = page * a.layout.page_stride + (uint64_t)it.head * a.layout.head_step + in_page * a.layout.slot_step;
 #pragma unroll 1
   for (int n = 0; n < H; ++n) {
     double y[8], ss = 0.0, scale;
+#pragma unroll
+    for (int k = 0; k < kRawWords; ++k) x[0].w[k] ^= flip[k];
     if constexpr (KEYS) {
       turn.apply(x[0], weight != nullptr, y, ss);
     } else {
@@ -278,8 +317,8 @@ __device__ __forceinline__ void append_vectors(const PagedAppendArgs& a, uint32_
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = (double)f[e];
     }
-    const uint64_t w = quantise<POLAR>(p, y, signs, t, s_lut, scale);
-    if (weight) scale *= 1.0 / __builtin_sqrt(ss * (1.0 / D) + (double)a.eps);
+    const uint64_t w = quantise<POLAR>(p, y, t, s_lut, scale);
+    if (weight) scale *= inv_sqrt(ss * (1.0 / D) + (double)a.eps);
     if (write && it.head + n < heads) {
       store_bytes(p.codes + row * p.row_bytes + (uint32_t)t * p.bits, w, p.bits);
       if (t == 0) p.scales[row] = (float)scale;
@@ -305,7 +344,7 @@ __device__ __forceinline__ void append_queries(const PagedAppendArgs& a, uint32_
     float y[8], ss = 0.f;
     turn.apply(x[n], a.q_norm != nullptr, y, ss);
     if (a.q_norm) {
-      const float r = 1.f / __builtin_sqrtf(ss * (1.f / D) + a.eps);
+      const float r = inv_sqrt(ss * (1.f / D) + a.eps);
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] *= r;
     }
