@@ -57,7 +57,7 @@ __device__ __forceinline__ void store_bytes(uint8_t* p, uint64_t w, uint32_t byt
 // A team takes one token and H of its heads: the token's weights and rotation are read and multiplied once, all heads are
 // loaded at once, and a rotation's partner coordinates come from their lane. Bound by arithmetic beside the copies: 8,191
 // tokens of 8 KV and 32 query heads (d = 128 bf16, norms, full rotation, 4 bits), 185 MB, take 50 us (3.7 TB/s); the queries
-// alone about 32, keys and values alone 32. One token 4.0 us, 64 tokens 5.0.
+// alone 33, keys and values alone 31. One token 4.0 us, 64 tokens 5.0.
 
 // 1 / sqrt(x) of a normal positive x, to 2^-51: the hardware's estimate and two steps of Newton's, a third of what a division by
 // the correctly rounded root takes.

@@ -466,6 +466,14 @@ __device__ __forceinline__ void write_zeros(const PagedAttnArgs& a, uint32_t b, 
     for (uint32_t h = lane; h < heads; h += 64) a.lse[(uint64_t)b * heads + h] = -__builtin_inff();
 }
 
+// The kernel's arguments read again where they are used: what a part or the end of a run needs is not kept in scalar registers (or
+// spilled from them) through the tiles' loop.
+__device__ __forceinline__ const PagedAttnArgs& again() {
+  auto p = (const __attribute__((address_space(4))) PagedAttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const PagedAttnArgs*)p;
+}
+
 // ---------------------------------------------------------------------------------------------------- the kernel
 template <int KB, int VB, int NH, bool TWO>
 struct Lds {  // dwords
@@ -522,7 +530,6 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   Place place{0u, 0u, 0u, 0u, x1};
   if (from < to) place = line.find(a, from, lane);
   const uint32_t x0 = place.x;   // this wave's tiles: [x0, x1) of the line
-  float* const ws = a.ws + 4 * a.groups;
   const uint32_t klb = lane_byte<KB, TWO>(lane) + key_base(KB, VB, TWO), vlb = lane_byte<VB, false>(lane) + value_base(KB, VB, TWO);
   uint32_t* const s_w = s_stage + wid * L::kRows * kPRow;
 
@@ -554,6 +561,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   Part part{};
   const int32_t* table = a.tables;
   auto begin_part = [&]() __attribute__((always_inline)) {
+    const PagedAttnArgs& a = again();
     const Span sp = span_of(a, (uint32_t)__builtin_amdgcn_readlane(line.len, place.lane));
     const uint32_t tile = place.tile;
     const uint32_t seq = line.first + place.lane;
@@ -630,7 +638,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
       ++col;
     }
     if (xl < x1 && xl == part.end) {
-      line.next(a, place, lane);
+      line.next(again(), place, lane);
       begin_part();
     }
     page = page_of();
@@ -663,6 +671,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   // Queries: a lane (head, group) loads eight coordinates from 32 t + 8 g of its head for every t, the other operand of the rotation.
   uint32_t yraw[KS][4];
   auto load_queries = [&](const Part& p) __attribute__((always_inline)) {
+    const PagedAttnArgs& a = again();
     const uint32_t h = NH == 4 ? n & 3 : n & 7;
     const uint16_t* const q = (const uint16_t*)a.q.data + p.seq * a.q.token_stride + (p.kv * a.nq + min(h, a.nq - 1u)) * a.q.head_stride + 8 * g;
 #pragma unroll
@@ -679,6 +688,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   Part cur{};
   // ---- a part begins: the score operand of its queries, which are in yraw
   auto prepare = [&]() __attribute__((always_inline)) {
+    const PagedAttnArgs& a = again();
     {
       const uint32_t h = NH == 4 ? n & 3 : n & 7, part = NH == 4 ? n >> 2 : n >> 3;
       // H (s q) on the matrix cores, exactly: rows of +1 and -1 times the raw queries with their signs flipped. Instruction b
@@ -939,6 +949,8 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
 
   // ---- a part is done: sums over the lanes, parts added, factors taken out
   auto finish = [&]() __attribute__((always_inline)) {
+    const PagedAttnArgs& a = again();
+    float* const ws = a.ws + 4 * a.groups;
 #pragma unroll
     for (int h = 0; h < NH; ++h) l[h] = wave_sum(l[h]);
 #pragma unroll
@@ -1010,6 +1022,8 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   }
   const uint32_t key = tail ? cur.seq * heads + cur.kv : ~0u;   // (pairs with tiles: below 2^31)
 
+  const PagedAttnArgs& e = again();
+  float* const ws = e.ws + 4 * e.groups;
   // ---- the last parts of neighbouring waves, where they are of one pair, merge through LDS (the tables' space)
   __syncthreads();
   constexpr int kMl = 2 * NH, kLanes = NH == 4 ? 32 : 64;
@@ -1047,7 +1061,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   const uint32_t g0 = run_of(0), g1 = run_of(W), begin = run_of(first), end = run_of(last);
   const bool rest = tail && end < g1 && cur.pair_end > end;
   const bool whole = tail && begin <= cur.pair_begin && (rest || end >= cur.pair_end);
-  const float* const rest_in = ws + (uint64_t)wave_slot(a.groups, blockIdx.x, last) * slot_floats(NH);
+  const float* const rest_in = ws + (uint64_t)wave_slot(e.groups, blockIdx.x, last) * slot_floats(NH);
   float* const out = ws + (uint64_t)(cur.pair_end <= g1 ? left_slot(blockIdx.x) : right_slot(blockIdx.x)) * slot_floats(NH);
   float mm[NH], lm[NH];
   if (tail) {
@@ -1106,16 +1120,16 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   if (x0 < x1 && x1 == g1 && lane == 0) {
     const bool more = cur.pair_end > g1 && cur.pair_begin >= g0;
     const uint32_t unit = to + (cur.pair_end - x1);   // (the run ends inside the pair: only tiles are left of it)
-    *(w4*)((uint32_t*)a.ws + 4 * blockIdx.x) = w4{more ? cut.group_of(unit - 1, a) + 1 : 0u, cur.seq, cur.kv, 0u};
+    *(w4*)((uint32_t*)e.ws + 4 * blockIdx.x) = w4{more ? cut.group_of(unit - 1, e) + 1 : 0u, cur.seq, cur.kv, 0u};
   } else if (g0 == g1 && tid == 0) {
-    ((uint32_t*)a.ws)[4 * blockIdx.x] = 0u;
+    ((uint32_t*)e.ws)[4 * blockIdx.x] = 0u;
   }
   if (!tail || first != wid) return;
   if (whole) {
     if (last - first > 1 || rest)
 #pragma unroll
       for (int c = 0; c < NC; ++c) acc[c] = s_acc[(first * NC + c) * kLanes + at];
-    write_output<NH, IO>(a, cur.seq, cur.kv, acc, mm, lm, lane);
+    write_output<NH, IO>(e, cur.seq, cur.kv, acc, mm, lm, lane);
   } else if (lane == 0) {
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
