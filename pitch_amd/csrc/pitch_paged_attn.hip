@@ -9,19 +9,19 @@
 // Work split. The sequences' tiles of 64 tokens, sequence by sequence and KV head by KV head, form one line that is cut into
 // equal runs, one per workgroup (one per compute unit), and each run into equal runs of its waves: a batch of any lengths loads
 // every wave alike, and only the host-known number of workgroups is launched. What is cut equally is tiles and one more per pair of
-// sequence and KV head, whose queries and output cost about a tile (200 sequences of 1 to 500 tokens, 12 heads: 34 us then, 41 by tiles
-// alone). A wave goes through its run by itself (scores, online softmax, weighted values; no barrier), pair by pair. A pair that
+// sequence and KV head, whose queries and output cost about a tile (200 sequences of 1 to 500 tokens, 12 heads: 34 us, by tiles alone 41,
+// both with a join). A wave goes through its run by itself (scores, online softmax, weighted values; no barrier), pair by pair. A pair that
 // lies in one wave is written by it; the parts of one that several waves of a workgroup share are merged at the end through LDS,
 // and paged_join merges what crosses workgroups through the workspace, in an order fixed by the lengths alone. Where no pair can
 // have more than a tile per wave, workgroups take whole pairs and there is no join.
 //
-// What bounds it: HBM in between (5.1 TB/s while all waves run), and the chain of latencies at either end, which is half of the time
-// even of the longest calls: lengths, page, codes, tables and the queries' rotation (6 us before the first score), the slowest
-// wave, the merge and the join (4 and 5 us). d = 128 bf16, 4 queries per KV head: 32 sequences of up to 8,000 tokens (138 MB)
-// 47 us, 131,072 tokens of one (126 MB) 48 us, 777 tokens 15 us. Heads of 64: eight bits and float16 (two table parts, window of
-// 1,000 tokens, 64 sequences) 30 us and the short sequences above 30, bound by the arithmetic of the lookups. Two tiles in
-// registers, 12 or 16 waves (spills), priorities for the waves behind, non-temporal reads and a touch of the second tile's lines at
-// the start were no faster.
+// What bounds it: HBM in between (5.1 TB/s while all waves run), and the chain of latencies at either end, which is nearly half of
+// the time even of the longest calls: lengths, page, codes, tables and the queries' rotation (5 us before the first score), the
+// slowest wave, the merge and the join (4 and 5 us). d = 128 bf16, 4 queries per KV head: 32 sequences of up to 8,000 tokens
+// (138 MB) 45 us, 131,072 tokens of one (126 MB) 47 us, 777 tokens 14.4 us. Heads of 64: eight bits and float16 (two table parts,
+// a window of 1,000 tokens, 64 sequences) 29.5 us and the short sequences above 29, bound by the arithmetic of the lookups. Two
+// tiles in registers, 12 or 16 waves (spills), priorities for the waves behind, non-temporal reads and a touch of the second tile's
+// lines at the start were no faster.
 //
 // Contractions on the 16-bit matrix cores (v_mfma_f32_16x16x32_f16), 16 rows of one operand for a KV head's query heads. A code
 // pair is looked up in LDS as two float16 values, which are operand words as they are: for the scores two neighbouring

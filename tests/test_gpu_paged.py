@@ -627,6 +627,44 @@ def test_step_graph_replays_match_eager(q):
         _ = (torch.randn(1024, device=dev) * 2).sum().item()
 
 
+def test_graphs_that_share_a_workspace(q):
+    """Two captured attentions of different shapes over one workspace, pairs that cross workgroups, lengths that change between
+    the replays (to nothing, to the whole table): each replay writes what an eager call with a workspace of its own writes."""
+    import torch
+    import pitch_amd as P
+    dev, page, kv, d, width = q.device, 64, 2, 64, 40
+    rng = np.random.default_rng(5)
+    cache, _ = _filled(q, P.QuantConfig("turboQuant", d, 4, 1), P.QuantConfig("turboQuant", d, 3, 2), 6 * width, page, kv, "head", rng)
+    tables = torch.from_numpy(rng.permutation(6 * width).reshape(6, width).astype(np.int32)).to(dev)
+    sides = []
+    need = max(cache.attentionWorkspaceBytes(b, nq) for b, nq in ((4, 4), (2, 8)))
+    shared = torch.full((need,), 0xFF, dtype=torch.uint8, device=dev)   # (NaN wherever it is read before it is written)
+    for at, b, nq in ((0, 4, 4), (4, 2, 8)):
+        H = kv * nq
+        s = dict(q=torch.randn(b, H, d, device=dev).to(torch.bfloat16), lengths=torch.full((b,), 70, dtype=torch.int32, device=dev),
+                 out=torch.zeros(b, H, d, device=dev, dtype=torch.bfloat16), ref=torch.zeros(b, H, d, device=dev, dtype=torch.bfloat16))
+        s["run"] = P.PagedAttention(cache, s["q"], tables[at:at + b], s["lengths"], s["out"], workspace=shared)
+        s["eager"] = P.PagedAttention(cache, s["q"], tables[at:at + b], s["lengths"], s["ref"])
+        s["eager"].enqueue()
+        torch.cuda.synchronize()
+        s["graph"] = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(s["graph"], stream=torch.cuda.Stream()):
+            s["run"].enqueue()
+        sides.append(s)
+    for i, lengths in enumerate(([2560, 0, 1, 999], [0, 0, 0, 0], [2560] * 4, [64, 65, 63, 1500], [1, 0, 0, 0], [3, 2000, 0, 9999])):
+        for s in sides:
+            s["lengths"].copy_(torch.tensor(lengths[:len(s["lengths"])], dtype=torch.int32))
+            s["q"].copy_(torch.randn(s["q"].shape).to(torch.bfloat16))
+        torch.cuda.synchronize()
+        for s in sides:
+            s["graph"].replay()
+        torch.cuda.synchronize()
+        for s in sides:
+            s["eager"].enqueue()
+            torch.cuda.synchronize()
+            assert s["ref"].isfinite().all() and torch.equal(s["out"], s["ref"]), i
+
+
 def test_calls_on_a_stream_of_their_own(q):
     """The operators run on the stream they are given, behind work that it already holds; attention there takes a workspace."""
     import torch
