@@ -437,7 +437,9 @@ int pitch_enqueue_paged_decode(const pitch_paged_cache_t* cache, const pitch_pag
  * over the tokens t of [0, L), of [L - window, L) with a window; cap(x) = softcap * tanh(x / softcap), x itself with
  * softcap 0. Queries and outputs are float16 or bfloat16: the products run on the 16-bit matrix cores. A length of 0 or
  * less gives zeros and an lse of minus infinity; lengths are cut to table_width * page_size tokens; tokens of pages
- * outside the pool (-1) take no part. Page tables need be right only up to the sequences' lengths. Extends
+ * outside the pool (-1) take no part, nor do scores of minus infinity; a query, a visible token's scale or a score of plus
+ * infinity that is no number gives NaN to the heads that it reaches. Page tables need be right only up to the sequences'
+ * lengths. Extends
  * pitch_enqueue_attention_decode, which the reference does not have (README.md:96). */
 typedef struct pitch_paged_attention {
   uint32_t io_type;   /* PITCH_IO_F16 or PITCH_IO_BF16 */

@@ -398,7 +398,8 @@ constexpr uint32_t slot_floats(int nh) { return 16 + NC * 4 * (nh == 4 ? 32 : 64
 
 // ---------------------------------------------------------------------------------------------------- output
 // acc: a lane (n, g) has coordinates 2 (NC n + c) + (g >> 1) of head v (NH = 4) or v + 4 (g & 1); the transform back runs over its
-// registers and across lanes.
+// registers and across lanes. A sum of weights of zero (all that was visible had scores of minus infinity) gives zeros; one that is
+// NaN (a query, a scale or a score of plus infinity that is no number) gives NaN.
 template <int NH, int IO>
 __device__ __forceinline__ void write_output(const PagedAttnArgs& a, uint32_t b, uint32_t kv, v4f (&acc)[NC], const float (&m)[NH],
                                              const float (&l)[NH], int lane) {
@@ -408,12 +409,12 @@ __device__ __forceinline__ void write_output(const PagedAttnArgs& a, uint32_t b,
 #pragma unroll
   for (int v = 0; v < 4; ++v) {
     const float total = NH == 8 ? pick(upper, l[v], l[NH - 4 + v]) : l[v];
-    const float f = total > 0.f ? a.oscale / total : 0.f;
+    const float f = total != 0.f ? a.oscale / total : 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[c][v]), __float_as_uint(acc[c][v]), false, false);
       const float x = __uint_as_float(r[0]), y = __uint_as_float(r[1]);
-      acc[c][v] = total > 0.f ? (g >= 2 ? x - y : x + y) * f : 0.f;
+      acc[c][v] = total != 0.f ? (g >= 2 ? x - y : x + y) * f : 0.f;
     }
   }
 #pragma unroll
@@ -453,7 +454,7 @@ __device__ __forceinline__ void write_output(const PagedAttnArgs& a, uint32_t b,
 #pragma unroll
     for (int h = 0; h < NH; ++h)
       if (h < (int)a.nq)
-        a.lse[((uint64_t)b * a.layout.kv_heads + kv) * a.nq + h] = l[h] > 0.f ? (m[h] + log2f(l[h])) * kLn2 : -__builtin_inff();
+        a.lse[((uint64_t)b * a.layout.kv_heads + kv) * a.nq + h] = l[h] != 0.f ? (m[h] + log2f(l[h])) * kLn2 : -__builtin_inff();
   }
 }
 

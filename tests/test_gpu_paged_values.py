@@ -1,0 +1,106 @@
+"""Paged attention against float64 where its outputs are large beside their bars (paged_reference.py), and at the edges of its
+value range: infinities and NaN, caps of every size, value scales of any range."""
+import math
+
+import numpy as np
+import pytest
+
+import paged_reference as R
+
+TURBO = "turboQuant"
+
+
+def _pool(rng, dim, kv, keys, values, page, pages, spread=0.5):
+    return R.Pool(rng, keys + (3,), values + (4,), pages, page, kv, spread).fill(dim)
+
+
+def _attend(q, pool, layout, tables, lengths, Q, dtype, **more):
+    """(out, lse) in float64 of one call over a cache of the pool's contents."""
+    import torch
+    import pitch_amd as P
+    dev, d = q.device, pool.dim
+    cfgs = [P.QuantConfig(m, d, b, s) for m, b, s in (pool.kcfg, pool.vcfg)]
+    cache = P.PagedCache(q, *cfgs, pages=pool.pages, pageSize=pool.page, kvHeads=pool.kv, layout=layout)
+    pool.load(cache)
+    qs = torch.from_numpy(Q).to(getattr(torch, dtype)).to(dev)
+    out = torch.full(qs.shape, -9.0, dtype=qs.dtype, device=dev)
+    lse = torch.full(qs.shape[:2], -9.0, device=dev)
+    slopes = more.pop("slopes", None)
+    cache.enqueueAttention(qs, torch.from_numpy(np.ascontiguousarray(tables)).to(dev),
+                           torch.tensor([int(n) for n in lengths], dtype=torch.int32, device=dev), out, lse=lse,
+                           slopes=None if slopes is None else torch.from_numpy(slopes).to(dev), **more)
+    torch.cuda.synchronize()
+    return out.double().cpu().numpy(), lse.double().cpu().numpy()
+
+
+def _typed(Q, dtype):
+    """Q rounded to the type, as float64."""
+    import torch
+    return torch.from_numpy(Q).to(getattr(torch, dtype)).double().numpy()
+
+
+def _signed_pairs(rng, B, kv, nq, d):
+    """Queries in pairs x and -x."""
+    x = rng.normal(size=(B, kv, nq // 2, d))
+    return np.concatenate([x, -x], 2).reshape(B, kv * nq, d)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+@pytest.mark.parametrize("lengths", [[64, 65, 1], [300, 64], [9000, 700]], ids=["tiles", "whole pairs", "joined"])
+@pytest.mark.parametrize("d,nq,bits,dtype", [(128, 4, 4, "bfloat16"), (64, 8, 4, "float16"), (64, 8, 8, "bfloat16"), (128, 2, 3, "float16")])
+def test_infinities_and_nan(q, d, nq, bits, dtype, lengths, softcap):
+    """What is not a number is not answered with a number. Two KV heads; in the first sequence the first head's token in the middle has a
+    key scale of NaN or infinity (a score of minus infinity takes no part, of plus infinity gives NaN; a cap makes them finite), or a value scale that is not finite;
+    or a query has an element that is none. Other heads and sequences do not notice."""
+    rng = np.random.default_rng(d + nq + len(lengths))
+    B, page = len(lengths), 16
+    tables, pages = R.tables_of(rng, lengths, page)
+    pool = _pool(rng, d, 2, (TURBO, bits), (TURBO, bits), page, pages)
+    Q = _typed(_signed_pairs(rng, B, 2, nq, d), dtype)
+    scale = float(np.float32(0.11))
+    ref = R.reference(pool, tables, lengths, Q, dtype, scale, softcap)
+    t = lengths[0] // 2
+    at = int(tables[0, t // page]) * page + t % page
+    unit, _ = pool.vectors("k", np.array([at]), 0)
+    plus = Q[0, :nq] @ unit[0] > 0
+    others = np.ones((B, 2 * nq), bool)
+    others[0, :nq] = False
+
+    def run(key=1.0, value=1.0, element=None):
+        k, v, x = pool.ks[at, 0], pool.vs[at, 0], Q.copy()
+        pool.ks[at, 0], pool.vs[at, 0] = k * np.float32(key), v * np.float32(value)
+        if element is not None:
+            x[0, 1, 5] = element
+        out, lse = _attend(q, pool, "head", tables, lengths, x, dtype, scale=scale, softcap=softcap)
+        pool.ks[at, 0], pool.vs[at, 0] = k, v
+        return out, lse
+
+    def right(out, lse, which, r=ref):
+        bad = [tuple(x) for x in R.wrong(out, lse, r) if which[tuple(x)]]
+        assert not bad, bad[:5]
+
+    for key in (math.inf, math.nan):
+        out, lse = run(key=key)
+        right(out, lse, others)
+        if key == math.inf:
+            less = R.reference(pool, tables, lengths, Q, dtype, scale, softcap, lost=lambda b, u: (u == t) & (b == 0))
+            minus = np.zeros_like(others)
+            minus[0, :nq] = ~plus
+            if not softcap:
+                right(out, lse, minus, less)
+                assert np.isnan(out[0, :nq][plus]).all() and np.isnan(lse[0, :nq][plus]).all()
+        else:
+            assert np.isnan(out[0, :nq]).all() and np.isnan(lse[0, :nq]).all()
+    for value in (math.inf, math.nan):
+        out, lse = run(value=value)
+        right(out, lse, others)
+        assert not np.isfinite(out[0, :nq]).any()
+        right(np.where(np.isfinite(out), out, ref["out"]), lse, ~others)      # the log-sum-exp does not depend on the values
+    for element in (math.nan, math.inf, -math.inf):
+        out, lse = run(element=element)
+        one = np.zeros_like(others)
+        one[0, 1] = True
+        right(out, lse, ~one)
+        if element != element or not softcap:
+            assert np.isnan(out[0, 1]).all() and np.isnan(lse[0, 1])
