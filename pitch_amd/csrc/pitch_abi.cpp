@@ -12,6 +12,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <algorithm>
+#include <limits>
 #include <mutex>
 #include <vector>
 #include <string>
@@ -1557,12 +1558,12 @@ int pitch_enqueue_paged_attention(const pitch_paged_cache_t* cache, const pitch_
   a.window = call->window;
   a.most_tokens = (uint32_t)most;
   a.groups = cus;
-  // the softmax scale, the key decode's 1 / sqrt(d) and log2(e) (scores in log2 units) are folded into the queries; with a
-  // cap the queries give 2 log2(e) x instead, so that exp2 of a product is exp(2 x) of tanh(x) = 1 - 2 / (1 + exp(2 x))
-  constexpr double kLog2E = 1.4426950408889634;
-  const double s = (double)call->scale / __builtin_sqrt((double)dim);
-  a.qscale = (float)(call->softcap > 0.f ? s / call->softcap * 2.0 * kLog2E : s * kLog2E);
-  a.cap = (float)(call->softcap * kLog2E);
+  // the softmax scale, the key decode's 1 / sqrt(d) and log2(e) (scores in log2 units) are folded into the queries
+  constexpr double kLog2E = 1.4426950408889634, kMost = std::numeric_limits<float>::max();
+  a.qscale = (float)((double)call->scale / __builtin_sqrt((double)dim) * kLog2E);
+  const double cap = call->softcap * kLog2E;
+  a.cap = (float)std::min(cap, kMost);
+  a.cap_r = call->softcap > 0.f ? (float)std::min(1.0 / cap, kMost) : 0.f;
   a.slope_scale = (float)kLog2E;
   a.oscale = (float)(1.0 / __builtin_sqrt((double)dim));
   static constexpr hipError_t (*kLaunch[2][4])(const pitch::PagedAttnArgs&, uint32_t, hipStream_t) = {

@@ -67,7 +67,7 @@ struct PagedAttnArgs {
   uint32_t table_width, sequences, nq, window;
   uint32_t most_tokens;      // table_width * page_size
   float qscale;              // what the rotated queries are multiplied by
-  float cap;                 // scores are cap * tanh(x) when positive (log2 units), else x
+  float cap, cap_r;          // scores x are cap * tanh(x * cap_r) when cap is positive (log2 units), else x
   float slope_scale;         // log2(e): slopes to log2 units
   float oscale;              // 1 / sqrt(dim) of the value decode
   float kfactor, vfactor;    // the tables' factors and their reciprocals (set by the launcher)

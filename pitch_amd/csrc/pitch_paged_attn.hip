@@ -823,9 +823,32 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
 #pragma unroll
     for (int h = 0; h < NH; ++h) z[h] *= qs[h] * now_nk;
     if (a.cap > 0.f) {
-      asm volatile("");   // a branch: the exponentials are not computed where no score is capped
+      asm volatile("");   // a branch: no instruction of it runs where no score is capped
+      // cap tanh(t), t = z / cap. Up to 0.4 the odd series, whose next term is 2^-24 of the value: the score keeps its bits however
+      // large the cap is (1 - 2 / (1 + exp(2 t)) cancels: 1e-7 of the cap, 0.1 of a score at a cap of 1e6). The exponentials only
+      // where a tile has a larger t.
+      bool far = false;
 #pragma unroll
-      for (int h = 0; h < NH; ++h) z[h] = a.cap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z[h])));
+      for (int h = 0; h < NH; ++h) far |= now_in && !(__builtin_fabsf(z[h] * a.cap_r) <= 0.4f);
+      auto series = [](float t) {
+        const float s = t * t;
+        float x = __builtin_fmaf(s, -1382.f / 155925.f, 62.f / 2835.f);
+        x = __builtin_fmaf(s, x, -17.f / 315.f);
+        x = __builtin_fmaf(s, x, 2.f / 15.f);
+        x = __builtin_fmaf(s, x, -1.f / 3.f);
+        return __builtin_fmaf(s, x, 1.f);
+      };
+      if (!__any(far)) {
+#pragma unroll
+        for (int h = 0; h < NH; ++h) z[h] *= series(z[h] * a.cap_r);
+      } else {
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          const float t = z[h] * a.cap_r;
+          const float y = a.cap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(t * 2.885390082f)));   // 2 log2(e)
+          z[h] = __builtin_fabsf(t) <= 0.4f ? z[h] * series(t) : y;
+        }
+      }
     }
 #pragma unroll
     for (int h = 0; h < NH; ++h) z[h] = now_in ? __builtin_fmaf(slope[h], now_dist, z[h]) : -__builtin_inff();

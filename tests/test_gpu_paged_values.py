@@ -104,3 +104,25 @@ def test_infinities_and_nan(q, d, nq, bits, dtype, lengths, softcap):
         right(out, lse, ~one)
         if element != element or not softcap:
             assert np.isnan(out[0, 1]).all() and np.isnan(lse[0, 1])
+
+
+CAPS = [1e-30, 1e-3, 0.5, 3.0, 50.0, 1e3, 1e4, 1e5, 1e6, 1e8, 1e20, 3e38]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,nq,dtype", [(128, 4, "float16"), (64, 8, "float16"), (64, 2, "bfloat16")])
+def test_soft_caps_of_any_size(q, d, nq, dtype):
+    """A cap far above the scores leaves them as they are; a cap far below them leaves their signs."""
+    rng = np.random.default_rng(d)
+    lengths = [900, 64, 1]
+    tables, pages = R.tables_of(rng, lengths, 16)
+    pool = _pool(rng, d, 2, (TURBO, 4), (TURBO, 4), 16, pages)
+    scale = float(np.float32(0.11))
+    Q = _typed(R.queries_of(rng, pool, tables, lengths, 2 * nq, scale), dtype)
+    for cap in CAPS:
+        print(cap, flush=True)
+        cap = float(np.float32(cap))
+        ref = R.reference(pool, tables, lengths, Q, dtype, scale, cap)
+        out, lse = _attend(q, pool, "head", tables, lengths, Q, dtype, scale=scale, softcap=cap)
+        bad = R.wrong(out, lse, ref)
+        assert not len(bad), (cap, bad[:5], np.abs(lse - ref["lse"]).max())
