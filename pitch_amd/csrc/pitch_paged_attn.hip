@@ -870,18 +870,19 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
         const float m = fmax_hw(M[h], mx[h]), al = __builtin_amdgcn_exp2f(M[h] - m);
         M[h] = m;
         l[h] *= al;
-        f[h] = al;
+        f[h] = al >= 0x1p-126f ? al : 0.f;
         p[h] = __builtin_amdgcn_exp2f(z[h] - m);
         y[h] = __builtin_fabsf(p[h] * n_t);
       }
       wave_max_heads(y, mx);
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
-        // the accumulators are relative to M and times S: a new maximum leaves them as they are with S / al
+        // the accumulators are relative to M and times S: a new maximum leaves them as they are with S / al. Otherwise S follows the
+        // tile's largest weight (from 2^-127 on; without any, it waits at 2^60 for the next), and the accumulators never grow.
         const float keep = S[h] * __builtin_amdgcn_rcpf(f[h]);
         float s_new = keep, fac = 1.f;
         if (!(keep <= 0x1p60f && mx[h] * keep <= kTop)) {
-          s_new = mx[h] > 0.f ? pow2i(min(13 - max(exponent_of(mx[h]), -100), 60)) : 1.f;
+          s_new = fmin_hw(pow2i(mx[h] > 0.f ? min(13 - max(exponent_of(mx[h]), -100), 113) : 60), keep);
           fac = f[h] * s_new * __builtin_amdgcn_rcpf(S[h]);
         }
         S[h] = s_new;

@@ -126,3 +126,45 @@ def test_soft_caps_of_any_size(q, d, nq, dtype):
         out, lse = _attend(q, pool, "head", tables, lengths, Q, dtype, scale=scale, softcap=cap)
         bad = R.wrong(out, lse, ref)
         assert not len(bad), (cap, bad[:5], np.abs(lse - ref["lse"]).max())
+
+
+RANGES = ["zero values first", "zero values with the highest score", "huge scale without weight", "wide scales", "tiny scales"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,copies", [(64, 1), (65, 1), (129, 1), (129, 600), (1100, 1), (1100, 400), (4200, 100)])
+@pytest.mark.parametrize("d,nq", [(128, 4), (64, 8), (128, 5)])
+@pytest.mark.parametrize("what", RANGES)
+def test_range_of_weights(q, what, d, nq, tokens, copies):
+    """A token's share of the output is its softmax weight times its value scale, which may be zero over whole tiles, differ
+    by 2^80, or lie near the smallest float32. In float32 none of that costs precision. (Copies: sequences over the same pages, so
+    that a wave goes through several tiles of a sequence.)"""
+    rng = np.random.default_rng(tokens + d)
+    tables, pages = R.tables_of(rng, [tokens], 16)
+    pool = _pool(rng, d, 1, (TURBO, 4), (TURBO, 3), 16, pages)
+    _, _, at = R.visible(pool, tables, [tokens], 0, 0)
+    scale = float(np.float32(0.11))
+    Q = R.queries_of(rng, pool, tables, [tokens], nq, scale)
+    score, token = None, 3
+    if what == "zero values first":
+        pool.vs[at] = np.exp(rng.uniform(-1, 1, (tokens, 1))) * 1e-7
+        pool.vs[at[:max(tokens - 70, 1)]] = 0.0
+    elif what == "zero values with the highest score":
+        pool.vs[at] = np.exp(rng.uniform(-1, 1, (tokens, 1))) * 1e-7
+        token = tokens // 2
+        pool.vs[at[token // 64 * 64:token // 64 * 64 + 63]] = 0.0
+        score = 40.0
+    elif what == "huge scale without weight":
+        pool.vs[at[3]], score = 2.0 ** 60, -60.0
+    elif what == "wide scales":
+        pool.vs[at] = np.exp2(rng.uniform(-40, 40, (tokens, 1)))
+    else:
+        pool.vs[at] = np.exp2(rng.uniform(-116, -114, (tokens, 1)))
+    if score is not None:
+        k, _ = pool.vectors("k", at[token:token + 1], 0)
+        Q[0] += np.outer(score / scale - Q[0] @ k[0], k[0] / (k[0] @ k[0]))
+    Q = _typed(Q, "bfloat16")
+    ref = R.reference(pool, tables, [tokens], Q, "bfloat16", scale)
+    out, lse = _attend(q, pool, "head", tables.repeat(copies, 0), [tokens] * copies, Q.repeat(copies, 0), "bfloat16", scale=scale)
+    ratio, ratio_lse = np.linalg.norm(out - ref["out"], axis=-1) / ref["bar"], np.abs(lse - ref["lse"]) / ref["lse_bar"]
+    assert (ratio <= 1).all() and (ratio_lse <= 1).all(), (ratio.max(), ratio_lse.max())
