@@ -6,8 +6,9 @@ import numpy as np
 import pytest
 
 import paged_reference as R
+from oracle import pitch_oracle as O
 
-TURBO = "turboQuant"
+TURBO, POLAR = "turboQuant", "polarQuant"
 
 
 def _pool(rng, dim, kv, keys, values, page, pages, spread=0.5):
@@ -37,6 +38,120 @@ def _typed(Q, dtype):
     """Q rounded to the type, as float64."""
     import torch
     return torch.from_numpy(Q).to(getattr(torch, dtype)).double().numpy()
+
+
+LONG = [   # dim, kv, q per kv, keys, values, page, layout, dtype, lengths, softcap, window, slopes
+    (64, 2, 4, (TURBO, 4), (TURBO, 3), 32, "head", "float16", [20000], 0.0, 0, False),
+    (64, 1, 5, (TURBO, 2), (TURBO, 4), 16, "token", "bfloat16", [6000, 1, 8000], 0.0, 0, False),
+    (128, 1, 8, (TURBO, 4), (TURBO, 3), 64, "head", "float16", [16000, 0, 5], 0.0, 0, False),
+    (128, 2, 4, (TURBO, 4), (TURBO, 4), 64, "head", "bfloat16", [7000] + [3] * 70 + [5000, 0], 0.0, 0, False),
+    (128, 1, 6, (POLAR, 4), (POLAR, 3), 48, "head", "float16", [6000, 900], 50.0, 0, False),
+    (64, 2, 8, (TURBO, 8), (POLAR, 6), 16, "token", "float16", [3000, 2500, 64, 65], 0.0, 1100, False),
+    (64, 3, 1, (POLAR, 6), (TURBO, 5), 32, "head", "bfloat16", [4000, 700], 0.0, 0, True),
+    (128, 2, 3, (TURBO, 3), (TURBO, 7), 80, "token", "float16", [2000, 1, 2, 63, 64, 65, 500], 0.0, 0, True),
+    (128, 1, 2, (TURBO, 6), (TURBO, 2), 16, "head", "bfloat16", [400] * 40, 30.0, 0, False),
+    (64, 4, 2, (POLAR, 3), (TURBO, 2), 16, "head", "float16", [130] * 90, 0.0, 77, False),
+]
+
+
+def _long(case, **mistakes):
+    """(pool, tables, lengths, Q, call's arguments, reference)."""
+    d, kv, nq, keys, values, page, _, dtype, lengths, softcap, window, sloped = case
+    rng = np.random.default_rng(d * nq + sum(lengths))
+    tables, pages = R.tables_of(rng, lengths, page)
+    pool = _pool(rng, d, kv, keys, values, page, pages)
+    slopes = (0.02 * 2.0 ** -np.arange(kv * nq)).astype(np.float32) if sloped else None
+    scale = float(np.float32(0.11))
+    Q = _typed(R.queries_of(rng, pool, tables, lengths, kv * nq, scale, window, softcap=softcap, slopes=slopes), dtype)
+    more = dict(scale=scale, softcap=softcap, window=window, slopes=slopes)
+    ref = R.reference(pool, tables, lengths, Q, dtype, **dict(more, slopes=None if slopes is None else slopes.astype(np.float64)), **mistakes)
+    return pool, tables, lengths, Q, more, ref
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", LONG, ids=lambda c: f"d{c[0]}-kv{c[1]}x{c[2]}-{c[3][0][0]}{c[3][1]}{c[4][0][0]}{c[4][1]}-{c[7]}-{len(c[8])}seq")
+def test_long_and_many(q, case):
+    """Pairs split over waves and workgroups, merged and joined, with bars below a tenth of what comes out."""
+    pool, tables, lengths, Q, more, ref = _long(case)
+    seen = np.array(lengths) > 0
+    assert (ref["bar"] < 0.1 * np.linalg.norm(ref["out"], axis=-1))[seen].all(), "a bar that finds nothing"
+    out, lse = _attend(q, pool, case[6], tables, lengths, Q, case[7], **more)
+    bad = R.wrong(out, lse, ref)
+    assert not len(bad), (bad[:5], [(np.linalg.norm(out[b, h] - ref["out"][b, h]), ref["bar"][b, h], lse[b, h] - ref["lse"][b, h],
+                                     ref["lse_bar"][b, h]) for b, h in bad[:5]])
+
+
+@pytest.mark.parametrize("i", [0, 1, 3, 8])
+def test_the_bars_find_mistakes(i):
+    """On the CPU: a tile of 64 tokens that is lost, or whose values are not weighed, is beyond the bars of its sequence."""
+    case = LONG[i]
+    b, L = int(np.argmax(case[8])), max(case[8])
+    *_, ref = _long(case)
+
+    def tile(seq, t):
+        return (seq == b) & (t >= L // 2 // 64 * 64) & (t < L // 2 // 64 * 64 + 64)
+
+    lost, unweighed = _long(case, lost=tile)[-1], _long(case, unweighed=tile)[-1]
+    even = {(b, h) for h in range(0, case[1] * case[2], 2)}     # (the others' weight may lie at one token)
+    assert even <= {tuple(x) for x in R.wrong(lost["out"], lost["lse"], ref)}
+    assert even <= {tuple(x) for x in R.wrong(unweighed["out"], None, ref)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,nq,keys", [(128, 4, (TURBO, 4)), (64, 8, (TURBO, 3)), (128, 8, (POLAR, 4)), (64, 3, (TURBO, 8)),
+                                       (128, 2, (POLAR, 6)), (64, 5, (TURBO, 2))])
+def test_a_single_token_gives_its_score(q, d, nq, keys):
+    """The log-sum-exp of one token is its score: float16 queries and their keys' table values count in two parts each."""
+    pool, tables, lengths, Q, ref = _singles(d, nq, keys)
+    out, lse = _attend(q, pool, "head", tables, lengths, Q, "float16", scale=0.11)
+    assert not len(R.wrong(out, lse, ref))
+
+
+def _singles(d, nq, keys, values=(TURBO, 4), dtype="float16"):
+    rng = np.random.default_rng(d + nq)
+    lengths = [1] * 64
+    tables, pages = R.tables_of(rng, lengths, 16)
+    pool = _pool(rng, d, 2, keys, values, 16, pages)
+    Q = _typed(rng.normal(size=(64, 2 * nq, d)), dtype)
+    return pool, tables, lengths, Q, R.reference(pool, tables, lengths, Q, dtype, float(np.float32(0.11)))
+
+
+@pytest.mark.parametrize("what", ["keys", "queries"])
+def test_scores_of_one_part_are_found(what):
+    """On the CPU: a table value or a rotated query rounded to one float16 is beyond the bars of most scores."""
+    pool, tables, lengths, Q, ref = _singles(128, 4, (TURBO, 4))
+    lse = np.empty_like(ref["lse"])
+    for b in range(64):
+        _, _, at = R.visible(pool, tables, lengths, b, 0)
+        for h in range(8):
+            _, k = pool.vectors("k", at, h // 4)
+            n = float(pool.ks[at[0], h // 4])
+            y = O.rotate(Q[b, h][None], 3)
+            if what == "keys":
+                k = (k / n * 4096.0).astype(np.float16).astype(np.float64) / 4096.0 * n
+            else:
+                y = y.astype(np.float16).astype(np.float64)
+            lse[b, h] = float(np.float32(0.11)) * float((k * y).sum())
+    assert len(R.wrong(ref["out"], lse, ref)) > 300    # of 512
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq", [1, 4, 5, 8])
+def test_weights_have_two_parts(q, nq):
+    """float16 outputs: of a single token, output over value is 1 up to the output's rounding, averaged over the coordinates, and
+    what is left of four-bit table values (4e-5). A weight of one float16 alone would be off by 2e-4 (root mean square)."""
+    pool, tables, lengths, Q, ref = _singles(128, nq, (TURBO, 4))
+    out, _ = _attend(q, pool, "head", tables, lengths, Q, "float16", scale=0.11)
+    o = ref["out"]
+    size = (o * o).sum(-1)
+    off = (out * o).sum(-1) / size - 1
+    step = R.rounding("float16", 2.0 ** np.ceil(np.log2(np.abs(o) + 1e-30))) / 2    # half of a step at least, of these values
+    expected = np.sqrt(((2 * step / math.sqrt(3) * o) ** 2).sum(-1)) / size
+    bar = 1.5 * math.sqrt((expected ** 2).mean()) + 4e-5
+    n = np.repeat(np.stack([pool.vs[R.visible(pool, tables, lengths, b, 0)[2][0]] for b in range(64)]), nq, 1).astype(np.float64)
+    planted = n.astype(np.float16).astype(np.float64) / n - 1
+    assert math.sqrt((planted ** 2).mean()) > 1.3 * bar, "a bar that finds nothing"
+    assert math.sqrt((off ** 2).mean()) <= bar
 
 
 def _signed_pairs(rng, B, kv, nq, d):
@@ -168,3 +283,22 @@ def test_range_of_weights(q, what, d, nq, tokens, copies):
     out, lse = _attend(q, pool, "head", tables.repeat(copies, 0), [tokens] * copies, Q.repeat(copies, 0), "bfloat16", scale=scale)
     ratio, ratio_lse = np.linalg.norm(out - ref["out"], axis=-1) / ref["bar"], np.abs(lse - ref["lse"]) / ref["lse_bar"]
     assert (ratio <= 1).all() and (ratio_lse <= 1).all(), (ratio.max(), ratio_lse.max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,dtype", [(5, "bfloat16"), (4, "float16")])
+def test_scores_beyond_exp(q, nq, dtype):
+    """Scores of several hundred, one token far ahead of the others, key scales of zero."""
+    rng = np.random.default_rng(6)
+    lengths = [640, 334, 333]
+    pool = _pool(rng, 64, 1, (TURBO, 4), (TURBO, 4), 16, 40)
+    tables = np.arange(40, dtype=np.int32)[None].repeat(3, 0)
+    pool.ks[:, 0] = np.exp(rng.normal(size=640)) * 0.1
+    pool.ks[100:200] = 0.0
+    pool.ks[333] = 300.0
+    Q = _typed(np.where(np.arange(nq)[None, :, None] % 2, -1.0, 1.0) * rng.normal(size=(3, 1, 64)).repeat(nq, 1), dtype)
+    ref = R.reference(pool, tables, lengths, Q, dtype, 1.0)
+    reach = np.abs(ref["lse"])
+    assert reach[1].max() > 100
+    out, lse = _attend(q, pool, "head", tables, lengths, Q, dtype, scale=1.0)
+    assert not len(R.wrong(out, lse, ref)), (out - ref["out"], lse - ref["lse"])
