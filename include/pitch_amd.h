@@ -386,8 +386,9 @@ typedef struct pitch_paged_vectors {
  * rotary_dim coordinates are then rotated: x * cos[p] + rotate_half(x) * sin[p], rotate_half over these coordinates
  * (-x[rotary_dim / 2:], x[:rotary_dim / 2]), p = positions[t], cos and sin [rows][rotary_dim] fp32. A key is not rounded
  * between these steps and its codes. Queries (q_heads per token, 0 for none) are normed with query_norm and rotated alike,
- * in float32, and written to queries_out in io_type; they may be written in place. A token whose position lies outside the
- * tables is not written, nor are its queries. Without norm and positions the codes and scales are those of
+ * in float32, and written to queries_out in io_type; they may be written in place (queries_out the same vectors), and else
+ * queries_out must not overlap what the call reads. A token whose position lies outside the tables is not written, nor are
+ * its queries. Without norm and positions the codes and scales are those of
  * pitch_enqueue_encode_io, up to values within 1e-11 of an edge between two codes (relative to the vector's norm).
  * For a decode step's or a prompt's write (README.md:65-71 appends with one PITCH.enqueueEncode per cache). */
 typedef struct pitch_paged_append {

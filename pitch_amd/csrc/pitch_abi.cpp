@@ -13,6 +13,7 @@
 #include <cstdlib>
 #include <algorithm>
 #include <limits>
+#include <numeric>
 #include <mutex>
 #include <vector>
 #include <string>
@@ -1360,6 +1361,38 @@ int paged_vectors(const pitch_paged_vectors_t& v, uint64_t tokens, uint64_t head
   return PITCH_OK;
 }
 
+// Memory that a call names: `heads` runs of `bytes` for each of `tokens`, with distances in bytes (0: one of them).
+struct Spread {
+  uint64_t base, token_stride, head_stride, tokens, heads, bytes;
+  Spread(const pitch_paged_vectors_t& v, uint64_t tokens, uint64_t heads, uint32_t dim, uint32_t esize)
+      : base((uintptr_t)v.data), token_stride(tokens > 1 ? v.token_stride * esize : 0), head_stride(heads > 1 ? v.head_stride * esize : 0),
+        tokens(tokens), heads(heads), bytes(dim * esize) {}
+  Spread(const void* p, uint64_t bytes) : base((uintptr_t)p), token_stride(0), head_stride(0), tokens(1), heads(1), bytes(bytes) {}
+  uint64_t of_token() const { return (heads - 1) * head_stride + bytes; }   // from a token's first byte to its last
+  uint64_t of_head() const { return (tokens - 1) * token_stride + bytes; }
+  uint64_t end() const { return base + (tokens - 1) * token_stride + of_token(); }
+  bool same(const Spread& o) const {
+    return base == o.base && token_stride == o.token_stride && head_stride == o.head_stride && tokens == o.tokens && heads == o.heads;
+  }
+};
+// Whether a and b are known to share no byte: one lies behind the other, or between the other's vectors, tokens or heads: slices of
+// one buffer. (Runs that begin at multiples of g from their first share none where one's fit between the other's, modulo g.)
+bool apart(const Spread& a, const Spread& b) {
+  if (a.end() <= b.base || b.end() <= a.base) return true;
+  auto between = [&](uint64_t g, uint64_t run_a, uint64_t run_b) {
+    if (!g) return false;
+    const uint64_t r = b.base >= a.base ? (b.base - a.base) % g : (g - (a.base - b.base) % g) % g;
+    return r >= run_a && r + run_b <= g;
+  };
+  const uint64_t tokens = std::gcd(a.token_stride, b.token_stride), heads = std::gcd(a.head_stride, b.head_stride);
+  return between(std::gcd(tokens, heads), a.bytes, b.bytes) || between(tokens, a.of_token(), b.of_token()) ||
+         between(heads, a.of_head(), b.of_head());
+}
+int check_apart(const Spread& out, const char* out_name, const Spread& in, const char* name) {
+  if (apart(out, in)) return PITCH_OK;
+  return fail(PITCH_ERR_INVALID_INPUT, "%s and %s overlap", out_name, name);
+}
+
 int check_aligned(const void* ptr, uint64_t bytes, uint64_t need, uint32_t align, const char* name) {
   PITCH_TRY(check_buffer(ptr, bytes, 0, need, name));
   if ((uintptr_t)ptr % align) return fail(PITCH_ERR_INVALID_INPUT, "%s buffer must be aligned to %u bytes", name, align);
@@ -1419,6 +1452,21 @@ int pitch_enqueue_paged_append(const pitch_paged_cache_t* cache, const pitch_pag
     a.table_rows = call->table_bytes / row;
   } else if (call->cos || call->sin || call->rotary_dim) {
     return fail(PITCH_ERR_INVALID_INPUT, "RoPE tables need positions");
+  }
+  if (call->q_heads) {   // workgroups of queries, keys and values run in no order: what one reads, none may write
+    const Spread out(call->queries_out, n, call->q_heads, dim, esize), in(call->queries, n, call->q_heads, dim, esize);
+    const char* const name = "queries' output";
+    if (!out.same(in)) PITCH_TRY(check_apart(out, name, in, "queries"));
+    PITCH_TRY(check_apart(out, name, Spread(call->keys, n, cache->kv_heads, dim, esize), "keys"));
+    PITCH_TRY(check_apart(out, name, Spread(call->values, n, cache->kv_heads, dim, esize), "values"));
+    PITCH_TRY(check_apart(out, name, Spread(call->slots, n * 8u), "slots"));
+    if (call->query_norm) PITCH_TRY(check_apart(out, name, Spread(call->query_norm, dim * esize), "query norm"));
+    if (call->key_norm) PITCH_TRY(check_apart(out, name, Spread(call->key_norm, dim * esize), "key norm"));
+    if (call->positions) {
+      PITCH_TRY(check_apart(out, name, Spread(call->positions, n * 8u), "positions"));
+      PITCH_TRY(check_apart(out, name, Spread(call->cos, call->table_bytes), "RoPE cos"));
+      PITCH_TRY(check_apart(out, name, Spread(call->sin, call->table_bytes), "RoPE sin"));
+    }
   }
   int dev = 0;
   PITCH_TRY(current_device(&dev));

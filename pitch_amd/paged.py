@@ -162,7 +162,8 @@ class PagedAppend:
     Two tokens must not have the same slot. With keyNorm (dim weights of the vectors' type) a key is first divided by
     sqrt(mean(x^2) + eps) and multiplied by the weights; with positions (int64) and the model's tables cos, sin (float32
     [positions][rotaryDim]) its first rotaryDim coordinates are rotated (rotate_half over them). Queries [tokens][heads][dim]
-    are normed with queryNorm, rotated and written to queriesOut (may be the queries themselves). Tokens with positions
+    are normed with queryNorm, rotated and written to queriesOut (the queries themselves, or memory that the call does not
+    read; slices of one buffer that share no element are). Tokens with positions
     outside the tables are left out. All vectors have one element type; their first two dimensions take any stride."""
 
     def __init__(self, cache: PagedCache, keys, values, slots, queries=None, queriesOut=None, queryNorm=None, keyNorm=None,
