@@ -54,6 +54,15 @@ def test_slices_of_one_buffer_are_taken(lib, form):  # noqa: F811
     assert _stopped_at_the_device(*_issue(lib, _append, "pitch_enqueue_paged_append", _append_at(wide, q, k, v)))
 
 
+def _inside(name, shift=0):
+    """An input and the queries' output in a buffer of their own."""
+    def change(call, mem):
+        at = mem(1 << 16) + 4096
+        setattr(call, name, at)
+        call.queries_out.data = at + shift
+    return change
+
+
 OVERLAPS = [
     (_append_at(FUSED[0], (DIM, ROW * DIM, DIM), None, None), "queries"),                        # one head off
     (_append_at((DIM, ROW * DIM, DIM), None, FUSED[1], FUSED[2]), "keys"),
@@ -62,12 +71,8 @@ OVERLAPS = [
     (_append_at((0, Q * DIM, DIM), (0, DIM, N * DIM), None, None), "queries"),                    # in place, transposed
     (_append_at((2, ROW * DIM, DIM), FUSED[0], None, None), "queries"),                           # two elements off
     (_append_at((0, ROW * DIM, DIM), None, (DIM - 2, ROW * DIM, DIM), None), "keys"),
-    (lambda call, mem: setattr(call.queries_out, "data", call.slots), "slots"),
-    (lambda call, mem: setattr(call.queries_out, "data", call.query_norm), "query norm"),
-    (lambda call, mem: setattr(call.queries_out, "data", call.key_norm - 8), "key norm"),
-    (lambda call, mem: setattr(call.queries_out, "data", call.positions), "positions"),
-    (lambda call, mem: setattr(call.queries_out, "data", call.cos + 4), "RoPE cos"),
-    (lambda call, mem: setattr(call.queries_out, "data", call.sin), "RoPE sin"),
+    (_inside("slots"), "slots"), (_inside("query_norm"), "query norm"), (_inside("key_norm", -8), "key norm"),
+    (_inside("positions"), "positions"), (_inside("cos", 4), "RoPE cos"), (_inside("sin"), "RoPE sin"),
 ]
 
 
