@@ -416,7 +416,7 @@ int pitch_enqueue_paged_append(const pitch_paged_cache_t* cache, const pitch_pag
  * row_starts[b] of sequence b, found in page block_tables[b][token / page_size]; it is decoded as pitch_enqueue_decode_io
  * decodes it. row_starts does not decrease. Rows outside the sequences' ranges, and rows whose page lies outside the pool or
  * the table, are left as they were. keys or values may have null data (not read back); their token strides are at most 2^22
- * elements. */
+ * elements, and they share no element. */
 typedef struct pitch_paged_decode {
   uint32_t io_type;   /* PITCH_IO_* of the outputs */
   uint32_t sequences; /* at least 1 */
@@ -447,7 +447,8 @@ typedef struct pitch_paged_attention {
   uint32_t sequences; /* 1..2048 */
   uint32_t q_per_kv;  /* 1..8 */
   uint32_t window;    /* tokens; 0: all */
-  pitch_paged_vectors_t queries, output; /* token = sequence, head = query head */
+  /* token = sequence, head = query head; the output may be the queries' own vectors, else the two share no element */
+  pitch_paged_vectors_t queries, output;
   const void* block_tables; /* int32 [sequences][table_width] */
   uint64_t block_tables_bytes;
   uint64_t table_width; /* at least 1; (table_width * page_size / 64 + 2) * sequences * kv_heads < 2^31 */

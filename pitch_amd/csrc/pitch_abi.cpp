@@ -1523,6 +1523,9 @@ int pitch_enqueue_paged_decode(const pitch_paged_cache_t* cache, const pitch_pag
     PITCH_TRY(paged_vectors(call->values, call->rows, cache->kv_heads, dim, esize, true, "values", &a.out[1]));
   for (const pitch::PagedVectors& o : a.out)   // (a workgroup's rows are addressed by 32-bit offsets)
     if (o.data && o.token_stride > 1u << 22) return fail(PITCH_ERR_INVALID_INPUT, "a token stride of the outputs exceeds 2^22");
+  if (call->keys.data && call->values.data)
+    PITCH_TRY(check_apart(Spread(call->keys, call->rows, cache->kv_heads, dim, esize), "keys",
+                          Spread(call->values, call->rows, cache->kv_heads, dim, esize), "values"));
   int dev = 0;
   PITCH_TRY(current_device(&dev));
   BatchDeviceCheck check(dev);
@@ -1572,6 +1575,10 @@ int pitch_enqueue_paged_attention(const pitch_paged_cache_t* cache, const pitch_
   PITCH_TRY(check_aligned(call->lengths, call->lengths_bytes, call->sequences * 4ull, 4, "lengths"));
   if (call->slopes) PITCH_TRY(check_aligned(call->slopes, call->slopes_bytes, heads * 4ull, 4, "slopes"));
   if (call->lse) PITCH_TRY(check_aligned(call->lse, call->lse_bytes, (uint64_t)call->sequences * heads * 4u, 4, "lse"));
+  // a pair of sequence and KV head is written when all of its queries are read, in any order among the pairs
+  const Spread out(call->output, call->sequences, heads, dim, 2), in(call->queries, call->sequences, heads, dim, 2);
+  if (!out.same(in)) PITCH_TRY(check_apart(out, "output", in, "query"));
+  if (call->lse) PITCH_TRY(check_apart(out, "output", Spread(call->lse, (uint64_t)call->sequences * heads * 4u), "lse"));
   if (!(call->scale >= -3.0e38f && call->scale <= 3.0e38f)) return fail(PITCH_ERR_INVALID_INPUT, "scale must be finite");
   if (!(call->softcap >= 0.f && call->softcap <= 3.0e38f))
     return fail(PITCH_ERR_INVALID_INPUT, "softcap must be finite and not negative");

@@ -215,7 +215,8 @@ class PagedDecode:
     """Reads tokens back: row r of keysOut / valuesOut [rows][kvHeads][dim] (one may be left out) with rowStarts[b] <= r <
     rowStarts[b + 1] (int32, sequences + 1 of them, not decreasing) is token firstTokens[b] (int32, default 0) + r -
     rowStarts[b] of sequence b, whose page is blockTables[b][token // pageSize] (int32). Other rows, and rows whose page lies
-    outside the pool or the table, are left as they were. The outputs' token strides are at most 2^22 elements."""
+    outside the pool or the table, are left as they were. The outputs' token strides are at most 2^22 elements; the two may be
+    slices of one buffer that share no element."""
 
     def __init__(self, cache: PagedCache, blockTables, rowStarts, keysOut=None, valuesOut=None, firstTokens=None):
         torch = _torch()
@@ -247,7 +248,7 @@ class PagedDecode:
 
 class PagedAttention:
     """One new token of every sequence over its pages: q and output [sequences][heads][dim] float16 or bfloat16 (heads =
-    kvHeads * 1..8; strided as in PagedAppend; at most 2,048 sequences), blockTables int32 [sequences][pages], lengths
+    kvHeads * 1..8; strided as in PagedAppend; at most 2,048 sequences; the output may be q itself), blockTables int32 [sequences][pages], lengths
     int32 [sequences] with the new token counted. The scores are softcap * tanh(scale q.k / softcap) (softcap 0: scale q.k; scale defaults to 1 / sqrt(dim))
     plus slopes[h] * (t - (length - 1)) (float32 [heads]) over the last ``window`` tokens (0: all). lse, float32
     [sequences][heads], receives the natural-log sum of exp. A sequence of length 0 gives zeros (and minus infinity). Without

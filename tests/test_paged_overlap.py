@@ -6,7 +6,7 @@ import random
 import pytest
 
 from pitch_amd import _lib
-from test_paged_api import DIM, HEADS, N, Memory, _append, _cache, lib  # noqa: F401 (a fixture)
+from test_paged_api import B, DIM, HEADS, N, Memory, _append, _attention, _cache, _decode, lib  # noqa: F401 (a fixture)
 
 Q = 4                    # query heads of an append
 ROW = Q + 2 * HEADS      # heads of a fused projection
@@ -112,3 +112,51 @@ def test_no_shared_byte_is_taken(lib):  # noqa: F811
             refused += 1
             assert "queries' output and keys overlap" in why, why
     assert refused > 100 and taken > 100
+
+
+def _decode_at(keys, values):
+    def change(call, mem):
+        base = mem(1 << 20)
+        call.keys, call.values = _vectors(base, *keys), _vectors(base, *values)
+    return change
+
+
+@pytest.mark.parametrize("keys,values,good", [
+    ((0, 2 * HEADS * DIM, DIM), (HEADS * DIM, 2 * HEADS * DIM, DIM), True),                 # [row][keys, values][head]
+    ((0, 2 * HEADS * DIM, 2 * DIM), (DIM, 2 * HEADS * DIM, 2 * DIM), True),                 # [row][head][key, value]
+    ((0, DIM, N * DIM), (HEADS * N * DIM, DIM, N * DIM), True),
+    ((0, HEADS * DIM, DIM), (0, HEADS * DIM, DIM), False),
+    ((0, HEADS * DIM, DIM), ((N - 1) * HEADS * DIM, HEADS * DIM, DIM), False),
+    ((0, 2 * HEADS * DIM, DIM), (DIM, 2 * HEADS * DIM, DIM), False),
+])
+def test_read_back_outputs(lib, keys, values, good):  # noqa: F811
+    rc, why = _issue(lib, _decode, "pitch_enqueue_paged_decode", _decode_at(keys, values))
+    assert _stopped_at_the_device(rc, why) if good else rc == _lib.ERR_INVALID_INPUT and "keys and values overlap" in why, (rc, why)
+
+
+H = 4 * HEADS   # query heads of an attention
+
+
+@pytest.mark.parametrize("output,queries,good", [
+    ((0, H * DIM, DIM), (0, H * DIM, DIM), True),                   # in place
+    ((0, 2 * H * DIM, DIM), (H * DIM, 2 * H * DIM, DIM), True),
+    ((0, 2 * H * DIM, 2 * DIM), (DIM, 2 * H * DIM, 2 * DIM), True),
+    ((0, H * DIM, DIM), (DIM, H * DIM, DIM), False),                # one head off
+    ((0, H * DIM, DIM), (H * DIM, H * DIM, DIM), False),            # one sequence off
+    ((0, H * DIM, DIM), (0, DIM, B * DIM), False),                  # the same memory in another order
+    ((0, H * DIM, DIM), (0, 0, DIM), False),                        # one sequence's queries for all
+])
+def test_attention_outputs(lib, output, queries, good):  # noqa: F811
+    def change(call, mem):
+        base = mem(1 << 20)
+        call.output, call.queries = _vectors(base, *output), _vectors(base, *queries)
+    rc, why = _issue(lib, _attention, "pitch_enqueue_paged_attention", change)
+    assert _stopped_at_the_device(rc, why) if good else rc == _lib.ERR_INVALID_INPUT and "output and query overlap" in why, (rc, why)
+
+
+def test_attention_lse_in_the_output(lib):  # noqa: F811
+    def change(call, mem):
+        base = mem(1 << 16)
+        call.output, call.lse = _vectors(base, 2048, H * DIM, DIM), base + 4096 + 512
+    rc, why = _issue(lib, _attention, "pitch_enqueue_paged_attention", change)
+    assert rc == _lib.ERR_INVALID_INPUT and "output and lse overlap" in why, (rc, why)
