@@ -252,7 +252,8 @@ class PagedAttention:
     int32 [sequences] with the new token counted. The scores are softcap * tanh(scale q.k / softcap) (softcap 0: scale q.k; scale defaults to 1 / sqrt(dim))
     plus slopes[h] * (t - (length - 1)) (float32 [heads]) over the last ``window`` tokens (0: all). lse, float32
     [sequences][heads], receives the natural-log sum of exp. A sequence of length 0 gives zeros (and minus infinity). Without
-    a workspace one is allocated and held; two calls that may run at the same time must not share one."""
+    a workspace one is allocated and held, and a call on another stream waits for the work of the stream that it was allocated on;
+    a graph needs the object as long as it is replayed. Two calls that may run at the same time must not share a workspace."""
 
     def __init__(self, cache: PagedCache, q, blockTables, lengths, output, scale: float | None = None, softcap: float = 0.0,
                  window: int = 0, slopes=None, lse=None, workspace=None):
@@ -275,9 +276,14 @@ class PagedAttention:
         c.lse, c.lse_bytes = _flat(lse, "lse", torch.float32, c.sequences * heads)
         c.scale = 1.0 / math.sqrt(cache.dim) if scale is None else float(scale)
         c.softcap = float(softcap)
+        # the handles of the streams that may use the workspace as it is (None: all, the caller's workspace is the caller's to order)
+        self._own, self._ready = None, None
         if workspace is None:
             n = cache.attentionWorkspaceBytes(c.sequences, c.q_per_kv)
-            workspace = torch.empty(n, dtype=torch.uint8, device=cache.pitch.device) if n else None
+            if n:
+                workspace = torch.empty(n, dtype=torch.uint8, device=cache.pitch.device)
+                self._own = torch.cuda.current_stream(cache.pitch.device)
+                self._ready = {self._own.cuda_stream}
         if workspace is not None:
             c.workspace, c.workspace_bytes = _buf(workspace, "workspace")
         self._held = (q, blockTables, lengths, output, slopes, lse, workspace)
@@ -285,6 +291,25 @@ class PagedAttention:
         self._fn, self._device = cache.pitch._lib.pitch_enqueue_paged_attention, cache.pitch.device
 
     def enqueue(self, stream=None) -> None:
-        rc = self._fn(self._pool, self._ref, _stream_handle(stream, self._device))
+        handle = _stream_handle(stream, self._device)
+        if self._ready is not None and handle not in self._ready:
+            self._admit(stream, handle)
+        rc = self._fn(self._pool, self._ref, handle)
         if rc:
             _raise_for(rc)
+
+    def _admit(self, stream, handle: int) -> None:
+        """Lets another stream use a workspace allocated here: behind the work that the allocation's stream holds (the memory may
+        have been freed by it just before), and known to torch's allocator, which else hands it out again on its own stream
+        as soon as this object is gone."""
+        torch = _torch()
+        if stream is None:
+            stream = torch.cuda.current_stream(self._device)
+        elif not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(handle, device=self._device) if handle else torch.cuda.default_stream(self._device)
+        self._held[-1].record_stream(stream)
+        with torch.cuda.stream(stream):
+            capturing = torch.cuda.is_current_stream_capturing()
+        if not capturing:   # (a graph waits for no work outside of it: it is replayed later than that work was issued)
+            stream.wait_event(self._own.record_event())
+            self._ready.add(handle)
