@@ -26,6 +26,13 @@ def _int(v, name: str, least: int = 0) -> int:
     return int(v)
 
 
+def _float(v, name: str) -> float:
+    try:
+        return float(v)
+    except (TypeError, ValueError):
+        raise InvalidInput(f"{name} {v!r} must be a number") from None
+
+
 def _device_tensor(t, name: str, dtypes=None):
     torch = _torch()
     if not isinstance(t, torch.Tensor):
@@ -183,7 +190,7 @@ class PagedAppend:
         if (queries is None) != (queriesOut is None):
             raise InvalidInput("queries and queriesOut go together")
         if queries is not None:
-            if queries.dim() != 3 or queries.shape[1] < 1:
+            if _device_tensor(queries, "queries").dim() != 3 or queries.shape[1] < 1:
                 raise InvalidInput(f"queries must be [tokens][heads][dim], got {list(queries.shape)}")
             c.q_heads = queries.shape[1]
             c.queries = _vectors(queries, "queries", c.q_heads, d, keys.dtype)
@@ -192,10 +199,12 @@ class PagedAppend:
                 raise InvalidInput("queries and queriesOut need the keys' tokens")
         c.query_norm, c.query_norm_bytes = _flat(queryNorm, "queryNorm", keys.dtype, d)
         c.key_norm, c.key_norm_bytes = _flat(keyNorm, "keyNorm", keys.dtype, d)
-        c.eps = float(eps)
+        c.eps = _float(eps, "eps")
         if positions is not None:
-            if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or cos.shape[0] < 1:
+            if cos is None or sin is None:
                 raise InvalidInput("positions need tables cos and sin [positions][rotaryDim]")
+            if _device_tensor(cos, "cos").dim() != 2 or cos.shape != _device_tensor(sin, "sin").shape or cos.shape[0] < 1:
+                raise InvalidInput("cos and sin must be [positions][rotaryDim], both the same")
             c.positions, c.positions_bytes = _flat(positions, "positions", torch.int64, n)
             c.cos, c.table_bytes = _flat(cos, "cos", torch.float32, None)
             c.sin, _ = _flat(sin, "sin", torch.float32, None)
@@ -274,8 +283,8 @@ class PagedAttention:
         c.lengths, c.lengths_bytes = _flat(lengths, "lengths", torch.int32, c.sequences)
         c.slopes, c.slopes_bytes = _flat(slopes, "slopes", torch.float32, heads)
         c.lse, c.lse_bytes = _flat(lse, "lse", torch.float32, c.sequences * heads)
-        c.scale = 1.0 / math.sqrt(cache.dim) if scale is None else float(scale)
-        c.softcap = float(softcap)
+        c.scale = 1.0 / math.sqrt(cache.dim) if scale is None else _float(scale, "scale")
+        c.softcap = _float(softcap, "softcap")
         # the handles of the streams that may use the workspace as it is (None: all, the caller's workspace is the caller's to order)
         self._own, self._ready = None, None
         if workspace is None:
