@@ -436,7 +436,9 @@ int pitch_enqueue_paged_decode(const pitch_paged_cache_t* cache, const pitch_pag
  * among them; query head h of its q_per_kv * kv_heads heads reads KV head h / q_per_kv:
  *   out = softmax(z) V,  lse = log sum exp(z),  z_t = cap(scale * q . k_t) + slopes[h] * (t - (L - 1))
  * over the tokens t of [0, L), of [L - window, L) with a window; cap(x) = softcap * tanh(x / softcap), x itself with
- * softcap 0. Queries and outputs are float16 or bfloat16: the products run on the 16-bit matrix cores. A length of 0 or
+ * softcap 0. Queries and outputs are float16 or bfloat16: the products run on the 16-bit matrix cores. With float16 every operand
+ * has two float16 parts and the outputs are the exact result's rounding; with bfloat16 the vectors that the codes stand for
+ * have one (11 bits, PolarQuant of 5 to 8 bits about 10), which moves an lse by up to 2e-3. A length of 0 or
  * less gives zeros and an lse of minus infinity; lengths are cut to table_width * page_size tokens; tokens of pages
  * outside the pool (-1) take no part, nor do scores of minus infinity; a query, a visible token's scale or a score of plus
  * infinity that is no number gives NaN to the heads that it reaches. Page tables need be right only up to the sequences'

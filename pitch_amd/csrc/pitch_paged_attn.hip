@@ -19,7 +19,7 @@
 // the time even of the longest calls: lengths, page, codes, tables and the queries' rotation (5 us before the first score), the
 // slowest wave, the merge and the join (4 and 5 us). d = 128 bf16, 4 queries per KV head: 32 sequences of up to 8,000 tokens
 // (138 MB) 45 us, 131,072 tokens of one (126 MB) 47 us, 777 tokens 14.4 us. Heads of 64: eight bits and float16 (two table parts,
-// a window of 1,000 tokens, 64 sequences) 29.5 us and the short sequences above 29, bound by the arithmetic of the lookups. Two
+// a window of 1,000 tokens, 64 sequences) 31 us and the short sequences above 29, bound by the arithmetic of the lookups. Two
 // tiles in registers, 12 or 16 waves (spills), priorities for the waves behind, non-temporal reads and a touch of the second tile's
 // lines at the start were no faster.
 //
@@ -31,8 +31,13 @@
 // heads, the queries in two and the weights in one (11 bits), or with float16 queries, whose outputs resolve that, in two by a
 // second instruction. TurboQuant's table values are stored times a factor at which they
 // nearly are float16 values (gen_tables.py: 4e-5 of a codebook's size for four bits, instead of 2e-4). With float16 queries the
-// keys' table values have two parts as well, whose products are added by a second instruction: a rounding of 2e-4 in the keys
-// moves a score of size 5 by 1e-3, several times what float16 outputs resolve (bfloat16: a quarter).
+// keys' and the values' table values have two parts as well, whose products are added by a second instruction: a rounding of 2e-4
+// in the keys moves a score of size 5 by 1e-3, several times what float16 outputs resolve (bfloat16: a quarter), and one in
+// the values is as large as the output's own. Errors of outputs relative to their norm, 4 sequences of up to 900 tokens: float16
+// 2.0e-4, the rounding of the exact result (values in one part: up to 1.25 times that for eight bits, 1.6 for PolarQuant); bfloat16,
+// one part each, 1.6e-3, at most 6 % above the rounding (PolarQuant of 8 bits, whose pairs are a product of two rounded values, else 0.8 %).
+// The log-sum-exps are off by 3e-6 with float16 queries, with bfloat16 by up to 4e-4 (TurboQuant) and 2e-3 (PolarQuant).
+// The second parts of the values cost 5 % (64 sequences, window of 1,000, 8 heads of 64 of eight bits: 31.1 us, 29.6 without).
 //
 // The table's entry of a pair (four codes for two bits) is 256 bytes long, copies for the keys in its first half and for the
 // values in its second (float16 queries: a table each): lanes read copies in different banks, and where the index is a byte of
@@ -77,7 +82,7 @@ __device__ __forceinline__ uint32_t f16_pair(float a, float b) { return narrow2<
 // ---------------------------------------------------------------------------------------------------- tables
 // Bytes of LDS of a table: 256 bytes per entry.
 constexpr uint32_t table_bytes(int b) { return b == 3 ? 64u * 256u : 65536u; }
-// With two parts of the keys the tables follow each other, else they share their entries. A table of 64 KB begins at a multiple
+// With two parts the keys' and the values' tables follow each other, else they share their entries. A table of 64 KB begins at a multiple
 // of its size: its lane bytes hold the base in their third byte, which v_perm passes on.
 constexpr uint32_t key_base(int kb, int vb, bool two) { return two && kb == 3 && vb != 3 ? 65536u : 0u; }
 constexpr uint32_t value_base(int kb, int vb, bool two) { return !two ? 128u : kb != 3 ? 65536u : vb != 3 ? 0u : 16384u; }
@@ -93,7 +98,7 @@ __device__ __forceinline__ u2 split_pair(float x, float y) {
   return u2{hi, f16_pair(x - a, y - b)};
 }
 
-// A table for codes of B bits (0: p.bits), of the values (TWO false) or of keys in two parts (TWO), in two steps: a thread's
+// A table for codes of B bits (0: p.bits), of values in one part or in two (TWO), in two steps: a thread's
 // source values are loaded when the kernel begins, and written to LDS when other loads are on their way.
 //   B = 3, 4, two codes: 32 copies of the pair, or of its two parts
 //   B = 2, four codes: 16 copies of two pairs, or of their two parts
@@ -505,7 +510,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   int32_t raw_own = a.lengths[min(blockIdx.x * W + wid, a.sequences - 1)];
   __builtin_amdgcn_sched_barrier(0);
   Table<KB, TWO> ktab;
-  Table<VB, false> vtab;
+  Table<VB, TWO> vtab;
   ktab.load(a.k, tid);
   vtab.load(a.v, tid);
   Line line;
@@ -531,7 +536,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
   Place place{0u, 0u, 0u, 0u, x1};
   if (from < to) place = line.find(a, from, lane);
   const uint32_t x0 = place.x;   // this wave's tiles: [x0, x1) of the line
-  const uint32_t klb = lane_byte<KB, TWO>(lane) + key_base(KB, VB, TWO), vlb = lane_byte<VB, false>(lane) + value_base(KB, VB, TWO);
+  const uint32_t klb = lane_byte<KB, TWO>(lane) + key_base(KB, VB, TWO), vlb = lane_byte<VB, TWO>(lane) + value_base(KB, VB, TWO);
   uint32_t* const s_w = s_stage + wid * L::kRows * kPRow;
 
   // A part of a pair of sequence and KV head: tiles [.., end) of the line belong to it and to this wave's run.
@@ -936,7 +941,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
     const uint32_t sel = n < 8 ? (n & 4 ? 0x0C0C0302u : 0x0C0C0100u) : (n & 4 ? 0x03020C0Cu : 0x01000C0Cu);
     // a step: the pairs c (two bits: c and c + 1, which one table read gives) of four tokens
     constexpr int PC = VB == 2 ? 2 : 1, NS = 4 * NC / PC, kAhead = VB == 0 ? 1 : 2;
-    uint32_t v[4][4][PC], none[PC];
+    uint32_t v[4][4][PC], rest[4][4][PC];
     w4 d[4], dr[4], wa{}, wr{};
     auto look = [&](int k) __attribute__((always_inline)) {
       const int m = k / (NC / PC), c = k % (NC / PC) * PC;
@@ -944,7 +949,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
       if (REST && c == 0) dr[m] = *(const w4*)(s_row + 4 * kPRow + 4 * m);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        look_pairs<VB, false, PC>(vw[4 * m + j], 2 * (VB ? VB : 8) * c, vlb, a.v.polar != 0, v[k & 3][j], none);
+        look_pairs<VB, TWO, PC>(vw[4 * m + j], 2 * (VB ? VB : 8) * c, vlb, a.v.polar != 0, v[k & 3][j], rest[k & 3][j]);
       }
     };
 #pragma unroll
@@ -966,6 +971,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn(PagedAttnArgs a) {
         const w4 x{v[k & 3][0][i], v[k & 3][1][i], v[k & 3][2][i], v[k & 3][3][i]};
         acc[c + i] = mfma_f16(wa, x, acc[c + i]);
         if (REST) acc[c + i] = mfma_f16(wr, x, acc[c + i]);
+        if (TWO) acc[c + i] = mfma_f16(wa, w4{rest[k & 3][0][i], rest[k & 3][1][i], rest[k & 3][2][i], rest[k & 3][3][i]}, acc[c + i]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }

@@ -11,8 +11,9 @@ then holds about half of the weight. The bars follow the roundings' sizes:
   scores' errors of a sequence's tokens are independent of each other. Six of these are allowed for sums over tokens. For float16 queries keys have
   two parts: 2^-21 instead.
 * Fixed parts: float32 sums and two-part operands, 2^-21 sum_j |q_j k_j| of a score, 2^-20 of a score itself and 2^-22 of a bias.
-* Values' table values are one float16: at most 2^-11 (three times that for PolarQuant of more than four bits) of the weighted
-  sum of the values' norms. Weights have two parts, or one (bfloat16, five heads and more): 2^-11 / sqrt(3) each, independent.
+* Values' table values are one float16 for bfloat16 outputs: at most 2^-11 (three times that for PolarQuant of more than four bits)
+  of the weighted sum of the values' norms; two parts for float16 outputs: 2^-21. Weights have two parts, or one (bfloat16, five
+  heads and more): 2^-11 / sqrt(3) each, independent.
 * The output's own rounding, and 2^-18 for exponentials and sums over tokens.
 """
 import math
@@ -124,6 +125,7 @@ def reference(pool, tables, lengths, Q, dtype, scale, softcap=0.0, window=0, slo
     wide_k = 3.0 if pool.kcfg[0] == "polarQuant" and pool.kcfg[1] > 4 else 1.0
     wide_v = 3.0 if pool.vcfg[0] == "polarQuant" and pool.vcfg[1] > 4 else 1.0
     key_step = (2.0 ** -21 if dtype == "float16" else wide_k * 2.0 ** -11) / math.sqrt(3)
+    value_step = 2.0 ** -21 if dtype == "float16" else wide_v * 2.0 ** -11
     one_part = dtype == "bfloat16" and nq > 4
     for b in range(B):
         L, t, at = visible(pool, tables, lengths, b, window)
@@ -159,7 +161,7 @@ def reference(pool, tables, lengths, Q, dtype, scale, softcap=0.0, window=0, slo
                                       + 2.0 ** -19 * (1 + abs(r["lse"][b, h])))
                 weight = 2.0 ** -11 / math.sqrt(3) * SIGMAS * math.sqrt((p * p * vn * vn).sum()) if one_part else 2.0 ** -21 * (p @ vn)
                 r["bar"][b, h] = (SIGMAS * math.sqrt((p * p * sigma * sigma * far * far).sum()) + sigma.max() ** 2 * (p @ vn)
-                                  + (p * fixed) @ far + (wide_v * 2.0 ** -11 + 2.0 ** -18) * (p @ vn) + weight
+                                  + (p * fixed) @ far + (value_step + 2.0 ** -18) * (p @ vn) + weight
                                   + np.linalg.norm(rounding(dtype, o)))
     return r
 

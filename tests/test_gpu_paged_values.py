@@ -138,7 +138,7 @@ def test_scores_of_one_part_are_found(what):
 @pytest.mark.gpu
 @pytest.mark.parametrize("nq", [1, 4, 5, 8])
 def test_weights_have_two_parts(q, nq):
-    """float16 outputs: of a single token, output over value is 1 up to the output's rounding, averaged over the coordinates, and
+    """float16 outputs, of a single token: output over value is 1 up to the output's rounding, averaged over the coordinates, and
     what is left of four-bit table values (4e-5). A weight of one float16 alone would be off by 2e-4 (root mean square)."""
     pool, tables, lengths, Q, ref = _singles(128, nq, (TURBO, 4))
     out, _ = _attend(q, pool, "head", tables, lengths, Q, "float16", scale=0.11)
@@ -152,6 +152,41 @@ def test_weights_have_two_parts(q, nq):
     planted = n.astype(np.float16).astype(np.float64) / n - 1
     assert math.sqrt((planted ** 2).mean()) > 1.3 * bar, "a bar that finds nothing"
     assert math.sqrt((off ** 2).mean()) <= bar
+
+
+def _coordinate_bar(o):
+    """Of a single token's float16 output: half of its step (2^-25 at least), and 2^-20 of the vector's norm for what two parts,
+    weights and the rotation in float32 leave."""
+    half = np.exp2(np.maximum(np.floor(np.log2(np.abs(o) + 1e-30)) - 11, -25))
+    return 1.0001 * half + 2.0 ** -20 * np.linalg.norm(o, axis=-1, keepdims=True)
+
+
+VALUES = [(TURBO, 2), (TURBO, 4), (TURBO, 5), (TURBO, 8), (POLAR, 2), (POLAR, 4), (POLAR, 5), (POLAR, 8)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,nq", [(128, 4), (64, 8), (128, 7), (64, 1)])
+@pytest.mark.parametrize("values", VALUES, ids=lambda v: f"{v[0]}{v[1]}")
+def test_values_have_two_parts(q, d, nq, values):
+    """float16 outputs: of a single token, the value that its codes stand for, rounded once."""
+    pool, tables, lengths, Q, ref = _singles(d, nq, (TURBO, 3), values)
+    out, _ = _attend(q, pool, "head", tables, lengths, Q, "float16", scale=0.11)
+    off = np.abs(out - ref["out"])
+    assert (off <= _coordinate_bar(ref["out"])).all(), (off / _coordinate_bar(ref["out"])).max()
+
+
+def test_values_of_one_part_are_found():
+    """On the CPU: table values of eight bits rounded to one float16 put one of twenty coordinates beyond the bar."""
+    pool, tables, lengths, Q, ref = _singles(128, 4, (TURBO, 3), (TURBO, 8))
+    out = np.empty_like(ref["out"])
+    for b in range(64):
+        _, _, at = R.visible(pool, tables, lengths, b, 0)
+        for h in range(8):
+            _, v = pool.vectors("v", at, h // 4)
+            n = float(pool.vs[at[0], h // 4])
+            v = (v / n * 4096.0).astype(np.float16).astype(np.float64) / 4096.0 * n
+            out[b, h] = O.unrotate(v, 4)[0].astype(np.float16)
+    assert (np.abs(out - ref["out"]) > _coordinate_bar(ref["out"])).mean() > 0.05
 
 
 def _signed_pairs(rng, B, kv, nq, d):
