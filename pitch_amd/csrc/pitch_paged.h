@@ -13,7 +13,6 @@ struct PagedPool {
   uint8_t* codes;
   float* scales;
   uint32_t polar, bits, row_bytes;
-  uint32_t seed;
   uint32_t signs[4];         // rotation signs: bit i of the 128 is 1 where coordinate i has sign -1
   int32_t lut, lut_entries;  // TurboQuant's bucket table (pitch_lut_tab), its scale and offset
   double lut_scale, lut_off;

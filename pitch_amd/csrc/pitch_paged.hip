@@ -56,8 +56,8 @@ __device__ __forceinline__ void store_bytes(uint8_t* p, uint64_t w, uint32_t byt
 // scales the stored norm (TurboQuant) or largest radius (PolarQuant). Queries are computed in float32 and rounded once.
 // A team takes one token and H of its heads: the token's weights and rotation are read and multiplied once, all heads are
 // loaded at once, and a rotation's partner coordinates come from their lane. Bound by arithmetic beside the copies: 8,191
-// tokens of 8 KV and 32 query heads (d = 128 bf16, norms, full rotation, 4 bits), 185 MB, take 50 us (3.7 TB/s); the queries
-// alone 33, keys and values alone 31. One token 4.0 us, 64 tokens 5.0.
+// tokens of 8 KV and 32 query heads (d = 128 bf16, norms, full rotation, 4 bits), 185 MB, take 48 us (3.9 TB/s); the queries
+// alone 36, keys and values alone 28. One token 4.8 us, 64 tokens 4.9. (Times in this file are those of a call among others.)
 
 // 1 / sqrt(x) of a normal positive x, to 2^-51: the hardware's estimate and two steps of Newton's, a third of what a division by
 // the correctly rounded root takes.
@@ -372,9 +372,9 @@ __global__ __launch_bounds__(kBlock) void paged_append(PagedAppendArgs a, uint32
 // for the codes and scales of all its heads, and decodes two vectors per team at a time, whose transforms share the cross-lane
 // instructions. The arithmetic and its order are those of vec_decode (pitch_vector.hip), so a row's bytes are those of the
 // contiguous decode. Bound by the writes: a read waits long behind them, which is what asking for four heads at once hides
-// (with one head at a time 39-49 us, with the stores under a branch, which makes the next reads' wait one for all stores
-// before them, 40-54 us). Measured: 31,616 rows of 8 heads, d = 128 bf16, 4 / 3 bits: 36.8 us for 156 MB (4.2 TB/s); 32,767
-// rows of 12 heads, d = 64 float32: 52.3 us for 227 MB (4.3 TB/s; 57 us when each store instruction writes every other
+// (with one head at a time 47 us, with the stores under a branch, which makes the next reads' wait one for all stores
+// before them, 40-54 us). Measured: 31,616 rows of 8 heads, d = 128 bf16, 4 / 3 bits: 36.9 us for 156 MB (4.2 TB/s); 32,767
+// rows of 12 heads, d = 64 float32: 52.5 us for 227 MB (4.3 TB/s; 57 us when each store instruction writes every other
 // 16 bytes).
 
 // The sequence whose rows hold row: the last b with starts[b] <= row (starts does not decrease).
@@ -565,7 +565,7 @@ __device__ __forceinline__ void decode_rows(const PagedDecodeArgs& a, const Page
 
 constexpr int kReadRows = 2 * VPB;   // of a workgroup: two vectors per team
 // Heads of a workgroup where these leave two workgroups per compute unit and kind, else one: at 16,384 rows of 8 heads, d = 128
-// bf16 (2 per unit), four take 12.0 us and one 13.2, at 8,192 rows 8.8 and 8.5, at 2,048 rows 5.9 and 4.8.
+// bf16, four take 16.4 us and one 18.4, at 8,192 rows (2 per unit) 10.9 and 11.9, at 4,096 rows 7.9 and 7.7, at 2,048 6.2 and 5.5.
 constexpr uint32_t kReadHeads = 4;
 
 template <int H>
@@ -622,9 +622,10 @@ hipError_t PITCH_CAT4(launch_paged_append_d, PITCH_DIM, _io, PITCH_IO)(const Pag
     p.lut_off = li.off;
   }
   // Four heads per team where these make eight workgroups per compute unit, else one: 8 KV and 32 query heads, d = 128 bf16, take
-  // 54 us and 98 at 8,191 tokens, 21 and 20 at 2,048, 9.8 and 7.6 at 512. PolarQuant takes one, whose kernel holds more waves (2 KV
-  // and 12 query heads at 8,000 tokens: 25 us, 35 with four). Among the keys and values come up to three workgroups of queries
-  // each (54 us; with one 56, with all of them last 65; an even number would give one XCD all of the keys).
+  // 48 us and 65 at 8,191 tokens, 27 and 32 at 4,096, 17.3 and 17.0 at 2,048, 8.6 and 7.0 at 512. PolarQuant takes one, whose kernel
+  // holds more waves (2 KV and 12 query heads at 8,000 tokens: 23 us, 32 with four). Among the keys and values come up to three
+  // workgroups of queries each (48 us; with one 49, with all of them last 53; an even number gives one XCD all of the keys: with
+  // two 62).
   const bool polar = a.pool[0].polar || a.pool[1].polar;
   const uint32_t most = 1u << 25, slice = max(1u, most / max(a.layout.kv_heads, a.q_heads));   // tokens of a launch, whose grid has a limit
   for (uint32_t left = a0.tokens; left;) {

@@ -9,19 +9,20 @@
 // Work split. The sequences' tiles of 64 tokens, sequence by sequence and KV head by KV head, form one line that is cut into
 // equal runs, one per workgroup (one per compute unit), and each run into equal runs of its waves: a batch of any lengths loads
 // every wave alike, and only the host-known number of workgroups is launched. What is cut equally is tiles and one more per pair of
-// sequence and KV head, whose queries and output cost about a tile (200 sequences of 1 to 500 tokens, 12 heads: 34 us, by tiles alone 41,
-// both with a join). A wave goes through its run by itself (scores, online softmax, weighted values; no barrier), pair by pair. A pair that
+// sequence and KV head, whose queries and output cost about a tile (200 sequences of 1 to 500 tokens, 12 heads, with a join: 34 us
+// then, 31 now, by tiles alone 41). A wave goes through its run by itself (scores, online softmax, weighted values; no barrier), pair by pair. A pair that
 // lies in one wave is written by it; the parts of one that several waves of a workgroup share are merged at the end through LDS,
 // and paged_join merges what crosses workgroups through the workspace, in an order fixed by the lengths alone. Where no pair can
 // have more than a tile per wave, workgroups take whole pairs and there is no join.
 //
-// What bounds it: HBM in between (5.1 TB/s while all waves run), and the chain of latencies at either end, which is nearly half of
-// the time even of the longest calls: lengths, page, codes, tables and the queries' rotation (5 us before the first score), the
-// slowest wave, the merge and the join (4 and 5 us). d = 128 bf16, 4 queries per KV head: 32 sequences of up to 8,000 tokens
-// (138 MB) 45 us, 131,072 tokens of one (126 MB) 47 us, 777 tokens 14.4 us. Heads of 64: eight bits and float16 (two table parts,
-// a window of 1,000 tokens, 64 sequences) 31 us and the short sequences above 29, bound by the arithmetic of the lookups. Two
-// tiles in registers, 12 or 16 waves (spills), priorities for the waves behind, non-temporal reads and a touch of the second tile's
-// lines at the start were no faster.
+// What bounds it: HBM in between, and latencies at either end, which are half of the time even of the longest calls. 32 sequences of
+// up to 8,000 tokens, d = 128 bf16, 4 queries per KV head (138 MB, 45 us with the join), by stamps of the waves: lengths known after
+// 0.7 us, page looked up 1.7, tables written 2.6, first loads asked for 4.8, queries rotated 6.2, first tile done 9.6; then 120 MB
+// until the median wave ends at 30 us (5.8 TB/s), the first at 25 and the last at 36; merged at 39; the join 5.2. 131,072 tokens of
+// one sequence (126 MB) 47 us, 777 tokens 14.7 us. Heads of 64: eight bits and float16 (two parts, a window of 1,000 tokens, 64
+// sequences) 31 us and the short sequences above 28, bound by the arithmetic of the lookups. Writing the tables takes 0.3 to 1 us of
+// a wave; without it calls were 0 to 2.3 us shorter. Two tiles in registers, 12 or 16 waves (spills), priorities for the waves
+// behind, non-temporal reads and a touch of the second tile's lines at the start were no faster.
 //
 // Contractions on the 16-bit matrix cores (v_mfma_f32_16x16x32_f16), 16 rows of one operand for a KV head's query heads. A code
 // pair is looked up in LDS as two float16 values, which are operand words as they are: for the scores two neighbouring
@@ -35,7 +36,7 @@
 // in the keys moves a score of size 5 by 1e-3, several times what float16 outputs resolve (bfloat16: a quarter), and one in
 // the values is as large as the output's own. Errors of outputs relative to their norm, 4 sequences of up to 900 tokens: float16
 // 2.0e-4, the rounding of the exact result (values in one part: up to 1.25 times that for eight bits, 1.6 for PolarQuant); bfloat16,
-// one part each, 1.6e-3, at most 6 % above the rounding (PolarQuant of 8 bits, whose pairs are a product of two rounded values, else 0.8 %).
+// one part each, 1.6e-3, at most 6 % above the rounding (PolarQuant of 6 and 8 bits, whose pairs are a product of two rounded values, else 0.8 %).
 // The log-sum-exps are off by 3e-6 with float16 queries, with bfloat16 by up to 4e-4 (TurboQuant) and 2e-3 (PolarQuant).
 // The second parts of the values cost 5 % (64 sequences, window of 1,000, 8 heads of 64 of eight bits: 31.1 us, 29.6 without).
 //
@@ -1308,8 +1309,8 @@ hipError_t PITCH_CAT4(launch_paged_attention_d, PITCH_DIM, _k, PITCH_KB)(const P
   a.vslot = a.layout.slot_step * a.v.row_bytes;
   const uint32_t most = a.window ? min(a.window + 15u, a.most_tokens) : a.most_tokens;
   // Pairs of a tile per wave at most: workgroups take whole ones, and there is no join (one sequence of up to 500 tokens and 8 KV
-  // heads 13.9 us, 14.6 with the join; 100 22.9 and 24.5; 200 of 12 heads of 64 30 and 33). At 16 tiles one sequence takes 16.7 and
-  // 15.0 us, 64 of eight bits 37 and 32: the waves of the longest pair are what the call waits for.
+  // heads 13.0 us, 13.7 with the join; 100 22.3 and 23.8; 200 of 12 heads of 64 28 and 31). At 16 tiles one sequence takes 15.9 and
+  // 14.0 us, 64 of eight bits 37 and 31: the waves of the longest pair are what the call waits for.
   a.whole = (most + 63) / 64 <= (uint32_t)W;
   a.page_r = 0xFFFFFFFFu / (a.layout.page_size / 16);
   a.tile_cols = 64 / a.layout.page_size;
