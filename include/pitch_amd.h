@@ -389,7 +389,8 @@ typedef struct pitch_paged_vectors {
  * in float32, and written to queries_out in io_type; they may be written in place (queries_out the same vectors), and else
  * queries_out must not overlap what the call reads. A token whose position lies outside the tables is not written, nor are
  * its queries. Without norm and positions the codes and scales are those of
- * pitch_enqueue_encode_io, up to values within 1e-11 of an edge between two codes (relative to the vector's norm).
+ * pitch_enqueue_encode_io, up to values within 1e-11 of an edge between two codes (relative to the vector's norm). A vector
+ * with an element that is not finite gets a scale that is not finite.
  * For a decode step's or a prompt's write (README.md:65-71 appends with one PITCH.enqueueEncode per cache). */
 typedef struct pitch_paged_append {
   uint32_t io_type; /* PITCH_IO_*: keys, values, queries, norm weights */

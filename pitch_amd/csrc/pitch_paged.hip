@@ -213,9 +213,9 @@ __device__ __forceinline__ uint64_t quantise(const PagedPool& p, double (&y)[8],
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     r2[q] = __builtin_fma(y[2 * q], y[2 * q], y[2 * q + 1] * y[2 * q + 1]);
-    top = r2[q] > top ? r2[q] : top;
+    top = r2[q] <= top ? top : r2[q];   // (NaN is kept: every transformed coordinate of a vector that is not finite is infinite or NaN)
   }
-  top = team_reduce<T>(top, [](double x, double z) { return x > z ? x : z; });
+  top = team_reduce<T>(top, [](double x, double z) { return x <= z ? z : x; });
   const double rmax = __builtin_sqrt(top), safe = rmax > 0.0 ? rmax : 1.0, inv = 1.0 / safe;
   scale = rmax * kInvSqrtD;
   const uint32_t levels = 1u << p.bits;
