@@ -319,6 +319,6 @@ class PagedAttention:
         self._held[-1].record_stream(stream)
         with torch.cuda.stream(stream):
             capturing = torch.cuda.is_current_stream_capturing()
-        if not capturing:   # (a graph waits for no work outside of it: it is replayed later than that work was issued)
+        if not capturing:   # (a graph cannot wait for work outside of it; torch.cuda.graph begins with a synchronisation)
             stream.wait_event(self._own.record_event())
             self._ready.add(handle)
