@@ -472,6 +472,51 @@ int pitch_paged_attention_workspace_size(const pitch_paged_cache_t* cache, const
                                          uint64_t* bytes);
 int pitch_enqueue_paged_attention(const pitch_paged_cache_t* cache, const pitch_paged_attention_t* call, void* stream);
 
+/* Attention over whole prompts, or chunks of them, packed one behind the other: the step between the append of a prompt's
+ * tokens and the first new token's pitch_enqueue_paged_attention (no counterpart in the reference, whose next step is attention,
+ * README.md:96). Sequence b has the queries row_starts[b] <= r < row_starts[b + 1] and the keys and values key_starts[b] <= r <
+ * key_starts[b + 1]; its nq queries are the last of its nk tokens: query i is at position p = nk - nq + i. Query head h of
+ * q_heads reads KV head h / (q_heads / kv_heads):
+ *   out = softmax(z) V,  lse = log sum exp(z),  z_j = cap(scale * q . k_j) + slopes[h] * (j - p)
+ * over the sequence's keys j, with causal those j <= p, with a window those j > p - window; cap(x) = softcap * tanh(x / softcap), x
+ * itself with softcap 0. Keys and values may be the projection's (slices of one buffer), or rows that pitch_enqueue_paged_decode read
+ * back: with its row_starts as key_starts a chunk attends to all of its cached tokens. Products run on the 16-bit matrix cores and are
+ * summed in float32; the softmax's weights are rounded to the vectors' type. A query that sees no key (more queries than keys) gives
+ * zeros and an lse of minus infinity; scores of minus infinity take no part; what is hidden from a query has no effect on it, also
+ * where it is not finite; a visible value that is not finite gives what its sum is, a score that is NaN or plus infinity gives NaN to
+ * its query. Rows of no sequence are left as they were. row_starts and key_starts do not decrease; they lie in device memory, are cut
+ * to the buffers' rows and taken on trust no further. Kernels only: captured into graphs like the others. */
+typedef struct pitch_prompt_attention {
+  uint32_t io_type;   /* PITCH_IO_F16 or PITCH_IO_BF16 */
+  uint32_t dim;       /* 64 or 128 */
+  uint32_t sequences; /* at least 1; (rows * q_heads / 128 / kv_heads + sequences) * kv_heads < 2^24 */
+  uint32_t q_heads, kv_heads; /* q_heads a multiple of kv_heads, both at least 1 */
+  uint32_t causal;    /* 0 or 1 */
+  uint32_t window;    /* tokens, below 2^31; 0: all. Needs causal, as slopes do */
+  uint32_t reserved;  /* 0 */
+  uint64_t rows;      /* tokens of queries and output, at least 1; rows * q_heads < 2^31 */
+  uint64_t key_rows;  /* tokens of keys and values, at least 1, below 2^31 */
+  /* data and strides are multiples of 16 bytes; the token strides of keys and values are at most 2^22 elements. The output may be
+   * the queries' own vectors, and else shares no element with what the call reads */
+  pitch_paged_vectors_t queries, keys, values, output;
+  const void* row_starts; /* int32 [sequences + 1] */
+  uint64_t row_starts_bytes;
+  const void* key_starts; /* int32 [sequences + 1] */
+  uint64_t key_starts_bytes;
+  const void* slopes; /* fp32 [q_heads], or null */
+  uint64_t slopes_bytes;
+  void* lse; /* fp32 [rows][q_heads], or null */
+  uint64_t lse_bytes;
+  float scale;
+  float softcap; /* 0: none */
+  void* workspace; /* pitch_prompt_attention_workspace_size bytes (null for none); not used by another call until this one has completed */
+  uint64_t workspace_bytes;
+} pitch_prompt_attention_t;
+/* Bytes of device workspace pitch_enqueue_prompt_attention needs on the current device (0 where no keys are split) for these
+ * dim, sequences, heads, rows and key_rows. */
+int pitch_prompt_attention_workspace_size(const pitch_prompt_attention_t* call, uint64_t* bytes);
+int pitch_enqueue_prompt_attention(const pitch_prompt_attention_t* call, void* stream);
+
 /* Packs count rows of dim unpacked codes (one uint8 per code, each < 2^bits) into count * code_stride
  * bytes, code i at bits [i * bits, i * bits + bits) of the row's little-endian 32-bit words.
  * Replaces pack_codes (reference/pitch_reference.py:68-78). */

@@ -18,5 +18,6 @@ from .api import (  # noqa: F401
     turbo_decode, turbo_encode, unpack_codes,
 )
 from .paged import PagedAppend, PagedAttention, PagedCache, PagedDecode  # noqa: F401
+from .prompt import PromptAttention  # noqa: F401
 
 __version__ = "0.1.0"

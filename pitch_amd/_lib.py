@@ -76,6 +76,14 @@ class PitchPagedAttentionC(ctypes.Structure):
                 + [("scale", ctypes.c_float), ("softcap", ctypes.c_float)] + _with_bytes("workspace"))
 
 
+class PitchPromptAttentionC(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_uint32) for n in ("io_type", "dim", "sequences", "q_heads", "kv_heads", "causal", "window", "reserved")]
+                + [("rows", ctypes.c_uint64), ("key_rows", ctypes.c_uint64)]
+                + [(n, PitchPagedVectorsC) for n in ("queries", "keys", "values", "output")]
+                + _with_bytes("row_starts", "key_starts", "slopes", "lse")
+                + [("scale", ctypes.c_float), ("softcap", ctypes.c_float)] + _with_bytes("workspace"))
+
+
 class PitchKeyBiasC(ctypes.Structure):
     _fields_ = [("bias", ctypes.c_void_p), ("bias_bytes", ctypes.c_uint64), ("cos", ctypes.c_void_p),
                 ("sin", ctypes.c_void_p), ("table_bytes", ctypes.c_uint64), ("first_position", ctypes.c_uint64),
@@ -162,6 +170,8 @@ SIGNATURES = {
     "pitch_paged_attention_workspace_size": (_int, [ctypes.POINTER(PitchPagedCacheC),
                                                     ctypes.POINTER(PitchPagedAttentionC), ctypes.POINTER(_u64)]),
     "pitch_enqueue_paged_attention": (_int, [ctypes.POINTER(PitchPagedCacheC), ctypes.POINTER(PitchPagedAttentionC), _vp]),
+    "pitch_prompt_attention_workspace_size": (_int, [ctypes.POINTER(PitchPromptAttentionC), ctypes.POINTER(_u64)]),
+    "pitch_enqueue_prompt_attention": (_int, [ctypes.POINTER(PitchPromptAttentionC), _vp]),
     "pitch_enqueue_pack_codes": (_int, [_u32, _u32, _vp, _u64, _u64, _vp, _u64, _u64, _u64, _vp]),
     "pitch_enqueue_unpack_codes": (_int, [_u32, _u32, _vp, _u64, _u64, _vp, _u64, _u64, _u64, _vp]),
     "pitch_selftest_reciprocal": (_int, [ctypes.POINTER(_u64)]),

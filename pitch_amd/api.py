@@ -802,6 +802,16 @@ class PITCH:
         _raise_for(rc)
 
     # ---- attention over compressed caches (no counterpart in the reference; README.md:96)
+    def enqueuePromptAttention(self, q, k, v, rowStarts, output, stream=None, workspace=None, **more) -> None:
+        """One PromptAttention call: packed sequences of queries over their keys and values. On a stream of the caller's, the caller's
+        workspace has to be given, if the call needs one: one that is made here returns to torch's allocator when the call
+        returns, which orders its next use with the current stream only."""
+        from .prompt import PromptAttention
+        call = PromptAttention(self, q, k, v, rowStarts, output, workspace=workspace, **more)
+        if stream is not None and workspace is None and call.workspaceBytes:
+            raise InvalidInput("a call on a stream of its own needs a workspace of its own")
+        call.enqueue(stream)
+
     def enqueueAttentionDecode(self, q, keyCodes, keyScales, valueCodes, valueScales, output, tokens: int,
                                keyConfig: QuantConfig, valueConfig: QuantConfig | None = None, qPerKv: int = 1,
                                kvHeads: int = 1, tokenStride: int = 1, headStride: int | None = None,

@@ -6,8 +6,8 @@ Steps: generate csrc/pitch_tables.inc from data/codebooks.json, compile csrc/pit
 dimension and element type of the uncompressed vectors (-DPITCH_DIM=2..1024, -DPITCH_IO=0/1/2 for
 float32/float16/bfloat16), csrc/pitch_channel.hip once per element type, csrc/pitch_attention.hip once per
 attention dimension (64, 128), csrc/pitch_attn_codes.hip once per attention dimension and kind of caches, csrc/pitch_paged.hip once per
-attention dimension and element type, csrc/pitch_paged_attn.hip once per attention dimension and width of the key codes, and csrc/pitch_abi.cpp, and link the
-shared library next to this file. Object files go to <repo>/_build/.
+attention dimension and element type, csrc/pitch_paged_attn.hip once per attention dimension and width of the key codes,
+csrc/pitch_prompt.hip once per attention dimension and 16-bit type, and csrc/pitch_abi.cpp, and link the shared library next to this file. Object files go to <repo>/_build/.
 Also builds libpitch_calib.so from csrc/pitch_calib.hip: the measurement kernels bench.py times beside the
 codec (not part of the codec's C ABI).
 """
@@ -73,6 +73,8 @@ def units() -> list[tuple[Path, Path, list[str], int]]:
               for d in ATTENTION_DIMS for io in IO_TYPES]
     units += [(CSRC / "pitch_paged_attn.hip", BUILD / f"paged_attn_d{d}_k{k}.o", [f"-DPITCH_DIM={d}", f"-DPITCH_KB={k}"],
                1024 + d) for d in ATTENTION_DIMS for k in PAGED_KEY_BITS]
+    units += [(CSRC / "pitch_prompt.hip", BUILD / f"prompt_d{d}_io{io}.o", [f"-DPITCH_DIM={d}", f"-DPITCH_IO={io}"], 512 + d)
+              for d in ATTENTION_DIMS for io in IO_TYPES[1:]]
     # largest dims first: they take longest to compile
     return sorted(units, key=lambda u: -u[3])
 

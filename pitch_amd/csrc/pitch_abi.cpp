@@ -22,6 +22,7 @@
 #include "../../include/pitch_amd.h"
 #include "pitch_launch.h"
 #include "pitch_paged.h"
+#include "pitch_prompt.h"
 
 namespace {
 
@@ -1627,6 +1628,153 @@ int pitch_enqueue_paged_attention(const pitch_paged_cache_t* cache, const pitch_
       {pitch::launch_paged_attention_d128_k2, pitch::launch_paged_attention_d128_k3, pitch::launch_paged_attention_d128_k4,
        pitch::launch_paged_attention_d128_k0}};
   const hipError_t e = kLaunch[dim == 128][std::min(a.k.bits, 5u) - 2](a, call->io_type, (hipStream_t)stream);
+  if (e != hipSuccess) return fail(PITCH_ERR_DECODING_FAILED, "Attention failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------------------------------- prompts
+namespace {
+
+int validate_prompt(const pitch_prompt_attention_t* c) {
+  if (!c) return fail(PITCH_ERR_INVALID_INPUT, "call is null");
+  if (c->dim != 64 && c->dim != 128)
+    return fail(PITCH_ERR_INVALID_DIMENSION, "Invalid dimension %u. Prompt attention takes vectors of 64 or 128.", c->dim);
+  if (c->q_heads < 1 || c->kv_heads < 1 || c->q_heads % c->kv_heads)
+    return fail(PITCH_ERR_INVALID_INPUT, "query heads %u must be a multiple of KV heads %u", c->q_heads, c->kv_heads);
+  if (c->rows < 1 || c->rows > 0x7FFFFFFFull / c->q_heads)
+    return fail(PITCH_ERR_INVALID_INPUT, "rows times query heads must be in 1...2^31 - 1");
+  if (c->key_rows < 1 || c->key_rows > 0x7FFFFFFFull - 64) return fail(PITCH_ERR_INVALID_INPUT, "key rows must be in 1...2^31 - 65");
+  if (c->sequences < 1 || (c->rows * (c->q_heads / c->kv_heads) / pitch::kPromptRows + c->sequences) * c->kv_heads >= 1u << 24)
+    return fail(PITCH_ERR_INVALID_INPUT, "sequences must be at least 1, and the tiles of all KV heads fewer than 2^24");
+  return PITCH_OK;
+}
+
+pitch::PromptPlan plan_of(const pitch_prompt_attention_t* c) {
+  return pitch::prompt_plan((uint32_t)c->rows, (uint32_t)c->key_rows, c->sequences, c->kv_heads, c->q_heads / c->kv_heads, c->dim,
+                            (uint32_t)pitch::device_cu_count());
+}
+
+// Vectors that are loaded 16 bytes at a time.
+int wide_vectors(const pitch_paged_vectors_t& v, uint64_t tokens, uint64_t heads, uint32_t dim, bool write, const char* name,
+                 pitch::PagedVectors* out) {
+  PITCH_TRY(paged_vectors(v, tokens, heads, dim, 2, write, name, out));
+  if ((uintptr_t)v.data % 16 || (tokens > 1 && v.token_stride % 8) || (heads > 1 && v.head_stride % 8))
+    return fail(PITCH_ERR_INVALID_INPUT, "%s: the buffer and its strides must be multiples of 16 bytes", name);
+  if (tokens == 1) out->token_stride = 0;
+  if (heads == 1) out->head_stride = 0;
+  return PITCH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pitch_prompt_attention_workspace_size(const pitch_prompt_attention_t* call, uint64_t* bytes) {
+  PITCH_TRY(validate_prompt(call));
+  if (!bytes) return fail(PITCH_ERR_INVALID_INPUT, "bytes is null");
+  int dev = 0;
+  PITCH_TRY(current_device(&dev));
+  *bytes = 4u * plan_of(call).ws_floats;
+  return ok();
+}
+
+int pitch_enqueue_prompt_attention(const pitch_prompt_attention_t* call, void* stream) {
+  PITCH_TRY(validate_prompt(call));
+  PITCH_TRY(check_io(call->io_type));
+  if (call->io_type == PITCH_IO_F32) return fail(PITCH_ERR_INVALID_INPUT, "prompt attention takes float16 or bfloat16 vectors");
+  if (call->causal > 1) return fail(PITCH_ERR_INVALID_INPUT, "causal must be 0 or 1");
+  if (call->reserved) return fail(PITCH_ERR_INVALID_INPUT, "reserved must be 0");
+  if (call->window > 0x7FFFFFFFu) return fail(PITCH_ERR_INVALID_INPUT, "window must be below 2^31");
+  if (!call->causal && (call->window || call->slopes))
+    return fail(PITCH_ERR_INVALID_INPUT, "a window or slopes need causal attention");
+  pitch::PromptArgs a{};
+  const uint32_t dim = call->dim, qh = call->q_heads, kvh = call->kv_heads;
+  PITCH_TRY(wide_vectors(call->queries, call->rows, qh, dim, false, "query", &a.q));
+  PITCH_TRY(wide_vectors(call->keys, call->key_rows, kvh, dim, false, "key", &a.k));
+  PITCH_TRY(wide_vectors(call->values, call->key_rows, kvh, dim, false, "value", &a.v));
+  PITCH_TRY(wide_vectors(call->output, call->rows, qh, dim, true, "output", &a.out));
+  if (a.k.token_stride > 1u << 22 || a.v.token_stride > 1u << 22)   // (a tile's rows are addressed by 32-bit offsets)
+    return fail(PITCH_ERR_INVALID_INPUT, "a token stride of keys or values exceeds 2^22");
+  const uint64_t starts = (call->sequences + 1ull) * 4u, lse_bytes = call->rows * qh * 4u;
+  PITCH_TRY(check_aligned(call->row_starts, call->row_starts_bytes, starts, 4, "row starts"));
+  PITCH_TRY(check_aligned(call->key_starts, call->key_starts_bytes, starts, 4, "key starts"));
+  if (call->slopes) PITCH_TRY(check_aligned(call->slopes, call->slopes_bytes, qh * 4ull, 4, "slopes"));
+  if (call->lse) PITCH_TRY(check_aligned(call->lse, call->lse_bytes, lse_bytes, 4, "lse"));
+  if (!(call->scale >= -3.0e38f && call->scale <= 3.0e38f)) return fail(PITCH_ERR_INVALID_INPUT, "scale must be finite");
+  if (!(call->softcap >= 0.f && call->softcap <= 3.0e38f))
+    return fail(PITCH_ERR_INVALID_INPUT, "softcap must be finite and not negative");
+  // a tile's output is written when its queries are read; tiles run in any order
+  const Spread out(call->output, call->rows, qh, dim, 2), in(call->queries, call->rows, qh, dim, 2);
+  const Spread keys(call->keys, call->key_rows, kvh, dim, 2), values(call->values, call->key_rows, kvh, dim, 2);
+  if (!out.same(in)) PITCH_TRY(check_apart(out, "output", in, "query"));
+  auto check_written = [&](const Spread& w, const char* name) {
+    PITCH_TRY(check_apart(w, name, keys, "key"));
+    PITCH_TRY(check_apart(w, name, values, "value"));
+    PITCH_TRY(check_apart(w, name, Spread(call->row_starts, starts), "row starts"));
+    PITCH_TRY(check_apart(w, name, Spread(call->key_starts, starts), "key starts"));
+    if (call->slopes) PITCH_TRY(check_apart(w, name, Spread(call->slopes, qh * 4ull), "slopes"));
+    return PITCH_OK;
+  };
+  PITCH_TRY(check_written(out, "output"));
+  if (call->lse) {
+    const Spread lse(call->lse, lse_bytes);
+    PITCH_TRY(check_apart(lse, "lse", out, "output"));
+    PITCH_TRY(check_apart(lse, "lse", in, "query"));
+    PITCH_TRY(check_written(lse, "lse"));
+  }
+  int dev = 0;
+  PITCH_TRY(current_device(&dev));
+  const pitch::PromptPlan plan = plan_of(call);
+  BatchDeviceCheck check(dev);
+  PITCH_TRY(check(call->queries.data, "query"));
+  PITCH_TRY(check(call->keys.data, "key"));
+  PITCH_TRY(check(call->values.data, "value"));
+  PITCH_TRY(check(call->output.data, "output"));
+  PITCH_TRY(check(call->row_starts, "row starts"));
+  PITCH_TRY(check(call->key_starts, "key starts"));
+  if (call->slopes) PITCH_TRY(check(call->slopes, "slopes"));
+  if (call->lse) PITCH_TRY(check(call->lse, "lse"));
+  if (plan.ws_floats) {
+    PITCH_TRY(check_aligned(call->workspace, call->workspace_bytes, plan.ws_floats * 4u, 16, "workspace"));
+    PITCH_TRY(check(call->workspace, "workspace"));
+    const Spread ws(call->workspace, plan.ws_floats * 4u);
+    PITCH_TRY(check_apart(ws, "workspace", out, "output"));
+    PITCH_TRY(check_apart(ws, "workspace", in, "query"));
+    if (call->lse) PITCH_TRY(check_apart(ws, "workspace", Spread(call->lse, lse_bytes), "lse"));
+    PITCH_TRY(check_written(ws, "workspace"));
+  }
+  a.row_starts = (const int32_t*)call->row_starts;
+  a.key_starts = (const int32_t*)call->key_starts;
+  a.slopes = (const float*)call->slopes;
+  a.lse = (float*)call->lse;
+  a.ws = (float*)call->workspace;
+  a.rows = (uint32_t)call->rows;
+  a.keys = (uint32_t)call->key_rows;
+  a.sequences = call->sequences;
+  a.kv_heads = kvh;
+  a.nq = qh / kvh;
+  a.causal = call->causal;
+  a.window = call->window;
+  a.tiles = plan.tiles;
+  a.splits = plan.splits;
+  // scores in log2 units; hidden scores are minus infinity, which a factor of zero would make NaN
+  constexpr double kLog2E = 1.4426950408889634, kMost = std::numeric_limits<float>::max();
+  const double to_log2 = std::max(-kMost, std::min(kMost, (double)call->scale * kLog2E));
+  if (call->slopes || call->softcap > 0.f) {
+    const double cap = call->softcap * kLog2E;
+    a.pre = (float)to_log2;
+    a.c = 1.f;
+    a.cap = (float)std::min(cap, kMost);
+    a.cap_r = call->softcap > 0.f ? (float)std::min(2.0 * kLog2E / cap, kMost) : 0.f;   // e^(2 x / cap) as a power of two
+  } else {
+    a.negate = call->scale < 0.f;
+    a.c = (float)std::max(std::abs(to_log2), 1e-37);
+  }
+  static constexpr hipError_t (*kLaunch[2][2])(const pitch::PromptArgs&, hipStream_t) = {
+      {pitch::launch_prompt_d64_io1, pitch::launch_prompt_d64_io2}, {pitch::launch_prompt_d128_io1, pitch::launch_prompt_d128_io2}};
+  const hipError_t e = kLaunch[dim == 128][call->io_type - 1](a, (hipStream_t)stream);
   if (e != hipSuccess) return fail(PITCH_ERR_DECODING_FAILED, "Attention failed: %s", hipGetErrorString(e));
   return ok();
 }

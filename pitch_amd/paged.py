@@ -255,7 +255,45 @@ class PagedDecode:
             _raise_for(rc)
 
 
-class PagedAttention:
+class WorkspaceCall:
+    """A call with a workspace: the caller's, or one that is allocated and held here."""
+
+    def _hold_workspace(self, c, workspace, needed: int, device) -> None:
+        torch = _torch()
+        # the handles of the streams that may use the workspace as it is (None: all, the caller's workspace is the caller's to order)
+        self._own, self._ready = None, None
+        if workspace is None and needed:
+            workspace = torch.empty(needed, dtype=torch.uint8, device=device)
+            self._own = torch.cuda.current_stream(device)
+            self._ready = {self._own.cuda_stream}
+        if workspace is not None:
+            c.workspace, c.workspace_bytes = _buf(workspace, "workspace")
+        self._workspace = workspace
+
+    def enqueue(self, stream=None) -> None:
+        handle = _stream_handle(stream, self._device)
+        if self._ready is not None and handle not in self._ready:
+            self._admit(stream, handle)
+        self._issue(handle)
+
+    def _admit(self, stream, handle: int) -> None:
+        """Lets another stream use a workspace allocated here: behind the work that the allocation's stream holds (the memory may
+        have been freed by it just before), and known to torch's allocator, which else hands it out again on its own stream
+        as soon as this object is gone."""
+        torch = _torch()
+        if stream is None:
+            stream = torch.cuda.current_stream(self._device)
+        elif not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(handle, device=self._device) if handle else torch.cuda.default_stream(self._device)
+        self._workspace.record_stream(stream)
+        with torch.cuda.stream(stream):
+            capturing = torch.cuda.is_current_stream_capturing()
+        if not capturing:   # (a graph cannot wait for work outside of it; torch.cuda.graph begins with a synchronisation)
+            stream.wait_event(self._own.record_event())
+            self._ready.add(handle)
+
+
+class PagedAttention(WorkspaceCall):
     """One new token of every sequence over its pages: q and output [sequences][heads][dim] float16 or bfloat16 (heads =
     kvHeads * 1..8; strided as in PagedAppend; at most 2,048 sequences; the output may be q itself), blockTables int32 [sequences][pages], lengths
     int32 [sequences] with the new token counted. The scores are softcap * tanh(scale q.k / softcap) (softcap 0: scale q.k; scale defaults to 1 / sqrt(dim))
@@ -285,40 +323,13 @@ class PagedAttention:
         c.lse, c.lse_bytes = _flat(lse, "lse", torch.float32, c.sequences * heads)
         c.scale = 1.0 / math.sqrt(cache.dim) if scale is None else _float(scale, "scale")
         c.softcap = _float(softcap, "softcap")
-        # the handles of the streams that may use the workspace as it is (None: all, the caller's workspace is the caller's to order)
-        self._own, self._ready = None, None
-        if workspace is None:
-            n = cache.attentionWorkspaceBytes(c.sequences, c.q_per_kv)
-            if n:
-                workspace = torch.empty(n, dtype=torch.uint8, device=cache.pitch.device)
-                self._own = torch.cuda.current_stream(cache.pitch.device)
-                self._ready = {self._own.cuda_stream}
-        if workspace is not None:
-            c.workspace, c.workspace_bytes = _buf(workspace, "workspace")
-        self._held = (q, blockTables, lengths, output, slopes, lse, workspace)
+        n = cache.attentionWorkspaceBytes(c.sequences, c.q_per_kv) if workspace is None else 0
+        self._hold_workspace(c, workspace, n, cache.pitch.device)
+        self._held = (q, blockTables, lengths, output, slopes, lse)
         self._call, self._ref, self._pool = c, ctypes.byref(c), ctypes.byref(cache._cstruct)
         self._fn, self._device = cache.pitch._lib.pitch_enqueue_paged_attention, cache.pitch.device
 
-    def enqueue(self, stream=None) -> None:
-        handle = _stream_handle(stream, self._device)
-        if self._ready is not None and handle not in self._ready:
-            self._admit(stream, handle)
+    def _issue(self, handle: int) -> None:
         rc = self._fn(self._pool, self._ref, handle)
         if rc:
             _raise_for(rc)
-
-    def _admit(self, stream, handle: int) -> None:
-        """Lets another stream use a workspace allocated here: behind the work that the allocation's stream holds (the memory may
-        have been freed by it just before), and known to torch's allocator, which else hands it out again on its own stream
-        as soon as this object is gone."""
-        torch = _torch()
-        if stream is None:
-            stream = torch.cuda.current_stream(self._device)
-        elif not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(handle, device=self._device) if handle else torch.cuda.default_stream(self._device)
-        self._held[-1].record_stream(stream)
-        with torch.cuda.stream(stream):
-            capturing = torch.cuda.is_current_stream_capturing()
-        if not capturing:   # (a graph cannot wait for work outside of it; torch.cuda.graph begins with a synchronisation)
-            stream.wait_event(self._own.record_event())
-            self._ready.add(handle)
