@@ -517,6 +517,68 @@ typedef struct pitch_prompt_attention {
 int pitch_prompt_attention_workspace_size(const pitch_prompt_attention_t* call, uint64_t* bytes);
 int pitch_enqueue_prompt_attention(const pitch_prompt_attention_t* call, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Page tables in device memory: handing out a pool's pages, giving them back, sharing them between sequences and compacting them, for
+ * a program whose steps are captured into graphs (no counterpart in the reference, whose caches are one sequence's buffers,
+ * README.md:65-76). Sequence b holds the pages block_tables[b][0 .. ceil(lengths[b] / page_size) - 1]; references[p] counts the
+ * rows' entries that hold page p (a program may add its own, for a prefix that it keeps), and a page whose count is not positive is
+ * free. The tables serve all layers: their caches have pools of as many pages of the same size. Lengths are cut to
+ * 0 .. table_width * page_size; entries outside the pool are no pages; entries behind a row's length are left as they are. Where free
+ * pages are handed out, the lowest number goes first, in the order of the sequences and their tokens; where they run out, a row ends
+ * with its last token that has a page, and *missing is the number of pages that were lacking (0 where none were).
+ * Calls that share tables, pools or a workspace run one after the other. */
+typedef struct pitch_paged_tables {
+  void* block_tables; /* int32 [sequences][table_width] */
+  uint64_t block_tables_bytes;
+  uint64_t table_width; /* at least 1; table_width * page_size < 2^31 */
+  void* lengths; /* int32 [sequences] */
+  uint64_t lengths_bytes;
+  void* references; /* int32 [pages] */
+  uint64_t references_bytes;
+  void* missing; /* int32 [1], or null; written by reserve and fork */
+  uint64_t missing_bytes;
+  uint64_t pages;     /* pages * page_size < 2^32 */
+  uint32_t page_size; /* a multiple of 16, at most 65536 */
+  uint32_t sequences; /* 1..2048 */
+  void* workspace;    /* pitch_paged_tables_workspace_size bytes */
+  uint64_t workspace_bytes;
+} pitch_paged_tables_t;
+/* Bytes of device workspace that the calls on these tables need (sequences, table_width, pages and page_size are looked at). */
+int pitch_paged_tables_workspace_size(const pitch_paged_tables_t* tables, uint64_t* bytes);
+
+/* Takes new_tokens[b] (int32; 0 or less: none) further tokens into every sequence b: pages are handed out where the held ones do not
+ * suffice, and lengths grow. The call's tokens are packed in the order of the sequences, as a batch of prompts or a decode step has them: token
+ * t's slot (page * page_size + slot, for pitch_enqueue_paged_append) goes to slots[t] and its position in its sequence to positions[t]
+ * (or null). A token without a page or a place in its row has -1 in both, one whose entry of the table is no page has slot -1;
+ * so do the entries behind the last token. Tokens beyond `capacity` are not taken. */
+typedef struct pitch_paged_reserve {
+  const void* new_tokens; /* int32 [sequences] */
+  uint64_t new_tokens_bytes;
+  uint64_t capacity; /* entries of slots and positions: 1..2^31 - 1 */
+  void* slots; /* int64 [capacity] */
+  uint64_t slots_bytes;
+  void* positions; /* int64 [capacity], or null */
+  uint64_t positions_bytes;
+} pitch_paged_reserve_t;
+int pitch_enqueue_paged_reserve(const pitch_paged_tables_t* tables, const pitch_paged_reserve_t* call, void* stream);
+
+/* Cuts every sequence b to at most keep[b] tokens (int32; 0 or less: the whole sequence is given back): the pages behind lose a
+ * reference. The tokens that remain are untouched: drafted tokens that were rejected, sequences that have ended. */
+int pitch_enqueue_paged_trim(const pitch_paged_tables_t* tables, const void* keep, uint64_t keep_bytes, void* stream);
+
+/* Makes every row b a copy of row parents[b] (int32) as it was before the call: b itself leaves the row alone, a number outside the
+ * rows empties it. Whole pages are shared and counted. A last page that is partly filled goes to one row (the parent's own if that stays, else its first
+ * child); the others get a page of their own, into which its tokens are copied in all n_caches caches. Pages that lose their last
+ * reference are handed out again in the same call. */
+int pitch_enqueue_paged_fork(const pitch_paged_tables_t* tables, const pitch_paged_cache_t* caches, uint32_t n_caches,
+                             const void* parents, uint64_t parents_bytes, void* stream);
+
+/* Moves the pages in use to the lowest numbers: with U pages in use, those at U and above go into the free ones below U, the k-th to the
+ * k-th, in all n_caches caches; tables and references follow. mapping (int32 [pages], or null) receives each page's new number, -1
+ * for a free page; used (int32 [1], or null) receives U. The moved pages' old places keep their contents. */
+int pitch_enqueue_paged_compact(const pitch_paged_tables_t* tables, const pitch_paged_cache_t* caches, uint32_t n_caches,
+                                void* mapping, uint64_t mapping_bytes, void* used, uint64_t used_bytes, void* stream);
+
 /* Packs count rows of dim unpacked codes (one uint8 per code, each < 2^bits) into count * code_stride
  * bytes, code i at bits [i * bits, i * bits + bits) of the row's little-endian 32-bit words.
  * Replaces pack_codes (reference/pitch_reference.py:68-78). */

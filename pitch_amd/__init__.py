@@ -18,6 +18,7 @@ from .api import (  # noqa: F401
     turbo_decode, turbo_encode, unpack_codes,
 )
 from .paged import PagedAppend, PagedAttention, PagedCache, PagedDecode  # noqa: F401
+from .pages import PagedCompact, PagedFork, PagedReserve, PagedTables, PagedTrim  # noqa: F401
 from .prompt import PromptAttention  # noqa: F401
 
 __version__ = "0.1.0"

@@ -84,6 +84,16 @@ class PitchPromptAttentionC(ctypes.Structure):
                 + [("scale", ctypes.c_float), ("softcap", ctypes.c_float)] + _with_bytes("workspace"))
 
 
+class PitchPagedTablesC(ctypes.Structure):
+    _fields_ = (_with_bytes("block_tables") + [("table_width", ctypes.c_uint64)] + _with_bytes("lengths", "references", "missing")
+                + [("pages", ctypes.c_uint64), ("page_size", ctypes.c_uint32), ("sequences", ctypes.c_uint32)]
+                + _with_bytes("workspace"))
+
+
+class PitchPagedReserveC(ctypes.Structure):
+    _fields_ = _with_bytes("new_tokens") + [("capacity", ctypes.c_uint64)] + _with_bytes("slots", "positions")
+
+
 class PitchKeyBiasC(ctypes.Structure):
     _fields_ = [("bias", ctypes.c_void_p), ("bias_bytes", ctypes.c_uint64), ("cos", ctypes.c_void_p),
                 ("sin", ctypes.c_void_p), ("table_bytes", ctypes.c_uint64), ("first_position", ctypes.c_uint64),
@@ -170,6 +180,12 @@ SIGNATURES = {
     "pitch_paged_attention_workspace_size": (_int, [ctypes.POINTER(PitchPagedCacheC),
                                                     ctypes.POINTER(PitchPagedAttentionC), ctypes.POINTER(_u64)]),
     "pitch_enqueue_paged_attention": (_int, [ctypes.POINTER(PitchPagedCacheC), ctypes.POINTER(PitchPagedAttentionC), _vp]),
+    "pitch_paged_tables_workspace_size": (_int, [ctypes.POINTER(PitchPagedTablesC), ctypes.POINTER(_u64)]),
+    "pitch_enqueue_paged_reserve": (_int, [ctypes.POINTER(PitchPagedTablesC), ctypes.POINTER(PitchPagedReserveC), _vp]),
+    "pitch_enqueue_paged_trim": (_int, [ctypes.POINTER(PitchPagedTablesC), _vp, _u64, _vp]),
+    "pitch_enqueue_paged_fork": (_int, [ctypes.POINTER(PitchPagedTablesC), ctypes.POINTER(PitchPagedCacheC), _u32, _vp, _u64, _vp]),
+    "pitch_enqueue_paged_compact": (_int, [ctypes.POINTER(PitchPagedTablesC), ctypes.POINTER(PitchPagedCacheC), _u32, _vp, _u64,
+                                           _vp, _u64, _vp]),
     "pitch_prompt_attention_workspace_size": (_int, [ctypes.POINTER(PitchPromptAttentionC), ctypes.POINTER(_u64)]),
     "pitch_enqueue_prompt_attention": (_int, [ctypes.POINTER(PitchPromptAttentionC), _vp]),
     "pitch_enqueue_pack_codes": (_int, [_u32, _u32, _vp, _u64, _u64, _vp, _u64, _u64, _u64, _vp]),

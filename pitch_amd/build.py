@@ -7,7 +7,7 @@ dimension and element type of the uncompressed vectors (-DPITCH_DIM=2..1024, -DP
 float32/float16/bfloat16), csrc/pitch_channel.hip once per element type, csrc/pitch_attention.hip once per
 attention dimension (64, 128), csrc/pitch_attn_codes.hip once per attention dimension and kind of caches, csrc/pitch_paged.hip once per
 attention dimension and element type, csrc/pitch_paged_attn.hip once per attention dimension and width of the key codes,
-csrc/pitch_prompt.hip once per attention dimension and 16-bit type, and csrc/pitch_abi.cpp, and link the shared library next to this file. Object files go to <repo>/_build/.
+csrc/pitch_prompt.hip once per attention dimension and 16-bit type, csrc/pitch_pages.hip and csrc/pitch_abi.cpp, and link the shared library next to this file. Object files go to <repo>/_build/.
 Also builds libpitch_calib.so from csrc/pitch_calib.hip: the measurement kernels bench.py times beside the
 codec (not part of the codec's C ABI).
 """
@@ -68,7 +68,7 @@ def units() -> list[tuple[Path, Path, list[str], int]]:
               for d in ATTENTION_DIMS]
     units += [(CSRC / "pitch_attn_codes.hip", BUILD / f"attn_codes_d{d}_k{k}.o",
                [f"-DPITCH_DIM={d}", f"-DPITCH_KIND={k}"], 1024 + d) for d in ATTENTION_DIMS for k in ATTENTION_KINDS]
-    units += [(CSRC / "pitch_abi.cpp", BUILD / "abi.o", [], 0)]
+    units += [(CSRC / "pitch_abi.cpp", BUILD / "abi.o", [], 0), (CSRC / "pitch_pages.hip", BUILD / "pages.o", [], 1)]
     units += [(CSRC / "pitch_paged.hip", BUILD / f"paged_d{d}_io{io}.o", [f"-DPITCH_DIM={d}", f"-DPITCH_IO={io}"], 256 + d)
               for d in ATTENTION_DIMS for io in IO_TYPES]
     units += [(CSRC / "pitch_paged_attn.hip", BUILD / f"paged_attn_d{d}_k{k}.o", [f"-DPITCH_DIM={d}", f"-DPITCH_KB={k}"],

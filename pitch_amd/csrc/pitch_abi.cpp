@@ -12,6 +12,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <algorithm>
+#include <exception>
 #include <limits>
 #include <numeric>
 #include <mutex>
@@ -22,6 +23,7 @@
 #include "../../include/pitch_amd.h"
 #include "pitch_launch.h"
 #include "pitch_paged.h"
+#include "pitch_pages.h"
 #include "pitch_prompt.h"
 
 namespace {
@@ -1273,8 +1275,8 @@ int pitch_selftest_attention_route(uint32_t dim, uint64_t tokens, uint32_t kv_he
 // ---------------------------------------------------------------------------------------------------- paged caches
 namespace {
 
-// Checks a paged cache without device access and fills the kernels' view of it.
-int paged_cache(const pitch_paged_cache_t* c, pitch::PagedPool* k, pitch::PagedPool* v, pitch::PagedLayout* l) {
+// Checks a paged cache without device access.
+int check_paged_cache(const pitch_paged_cache_t* c) {
   if (!c) return fail(PITCH_ERR_INVALID_INPUT, "cache is null");
   PITCH_TRY(validate_config(&c->key_config));
   PITCH_TRY(validate_config(&c->value_config));
@@ -1303,20 +1305,32 @@ int paged_cache(const pitch_paged_cache_t* c, pitch::PagedPool* k, pitch::PagedP
   void* const scales[2] = {c->key_scales, c->value_scales};
   const uint64_t codes_bytes[2] = {c->key_codes_bytes, c->value_codes_bytes};
   const uint64_t scales_bytes[2] = {c->key_scales_bytes, c->value_scales_bytes};
-  pitch::PagedPool* const pool[2] = {k, v};
   for (int i = 0; i < 2; ++i) {
     const uint32_t cs = code_stride_of(dim, cfg[i]->bits);
     PITCH_TRY(check_buffer(codes[i], codes_bytes[i], 0, vectors * cs, i ? "value codes" : "key codes"));
     PITCH_TRY(check_buffer(scales[i], scales_bytes[i], 0, vectors * 4u, i ? "value scales" : "key scales"));
     if ((uintptr_t)codes[i] % 4 || (uintptr_t)scales[i] % 4)
       return fail(PITCH_ERR_INVALID_INPUT, "cache buffers must be aligned to 4 bytes");
+  }
+  return PITCH_OK;
+}
+
+// The same, and fills the kernels' view of it.
+int paged_cache(const pitch_paged_cache_t* c, pitch::PagedPool* k, pitch::PagedPool* v, pitch::PagedLayout* l) {
+  PITCH_TRY(check_paged_cache(c));
+  const uint32_t dim = c->key_config.dim;
+  const pitch_config_t* cfg[2] = {&c->key_config, &c->value_config};
+  void* const codes[2] = {c->key_codes, c->value_codes};
+  void* const scales[2] = {c->key_scales, c->value_scales};
+  pitch::PagedPool* const pool[2] = {k, v};
+  for (int i = 0; i < 2; ++i) {
     pitch::PagedPool& p = *pool[i];
     p = pitch::PagedPool{};
     p.codes = (uint8_t*)codes[i];
     p.scales = (float*)scales[i];
     p.polar = cfg[i]->method == PITCH_METHOD_POLAR;
     p.bits = cfg[i]->bits;
-    p.row_bytes = cs;
+    p.row_bytes = code_stride_of(dim, cfg[i]->bits);
     for (uint32_t j = 0; j < dim; ++j)
       if (pitch_sign_is_negative(cfg[i]->seed, j)) p.signs[j >> 5] |= 1u << (j & 31);
   }
@@ -1777,6 +1791,234 @@ int pitch_enqueue_prompt_attention(const pitch_prompt_attention_t* call, void* s
   const hipError_t e = kLaunch[dim == 128][call->io_type - 1](a, (hipStream_t)stream);
   if (e != hipSuccess) return fail(PITCH_ERR_DECODING_FAILED, "Attention failed: %s", hipGetErrorString(e));
   return ok();
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------------------------------- page tables
+namespace {
+
+// The memory that a call on page tables names, each part with its name, and whether the call writes it.
+struct Named {
+  Spread memory;
+  const char* name;
+  bool written;
+};
+
+int validate_tables(const pitch_paged_tables_t* t) {
+  if (!t) return fail(PITCH_ERR_INVALID_INPUT, "tables are null");
+  if (t->page_size < 16 || t->page_size > 65536 || t->page_size % 16 != 0)
+    return fail(PITCH_ERR_INVALID_INPUT, "page size %u must be a multiple of 16 in 16...65536", t->page_size);
+  if (t->pages < 1 || t->pages > 0x7FFFFFFFull || t->pages * t->page_size > 0xFFFFFFFFull)
+    return fail(PITCH_ERR_INVALID_INPUT, "a pool holds 1 page or more and fewer than 2^32 token slots, got %llu pages of %u",
+                (unsigned long long)t->pages, t->page_size);
+  if (t->sequences < 1 || t->sequences > pitch::kPagedMostSequences)
+    return fail(PITCH_ERR_INVALID_INPUT, "sequences must be in 1...%u", pitch::kPagedMostSequences);
+  if (t->table_width < 1 || t->table_width > 0x7FFFFFFFull / t->page_size)
+    return fail(PITCH_ERR_INVALID_INPUT, "a page table's row must hold 1 page or more and fewer than 2^31 tokens");
+  return PITCH_OK;
+}
+
+uint64_t tables_workspace(const pitch_paged_tables_t* t) {
+  return 4u * pitch::pages_workspace_words(t->pages, t->sequences, t->table_width);
+}
+
+// Checks tables without device access, fills the kernels' view and the list of their memory.
+int paged_tables(const pitch_paged_tables_t* t, pitch::PagesTables* out, std::vector<Named>* memory) {
+  PITCH_TRY(validate_tables(t));
+  PITCH_TRY(check_tables(t->block_tables, t->block_tables_bytes, t->table_width, t->sequences));
+  PITCH_TRY(check_aligned(t->lengths, t->lengths_bytes, t->sequences * 4ull, 4, "lengths"));
+  PITCH_TRY(check_aligned(t->references, t->references_bytes, t->pages * 4u, 4, "references"));
+  if (t->missing) PITCH_TRY(check_aligned(t->missing, t->missing_bytes, 4, 4, "missing"));
+  PITCH_TRY(check_aligned(t->workspace, t->workspace_bytes, tables_workspace(t), 16, "workspace"));
+  memory->push_back({Spread(t->block_tables, t->table_width * t->sequences * 4u), "page tables", true});
+  memory->push_back({Spread(t->lengths, t->sequences * 4ull), "lengths", true});
+  memory->push_back({Spread(t->references, t->pages * 4u), "references", true});
+  if (t->missing) memory->push_back({Spread(t->missing, 4), "missing", true});
+  memory->push_back({Spread(t->workspace, tables_workspace(t)), "workspace", true});
+  out->tables = (int32_t*)t->block_tables;
+  out->lengths = (int32_t*)t->lengths;
+  out->references = (int32_t*)t->references;
+  out->missing = (int32_t*)t->missing;
+  out->width = (uint32_t)t->table_width;
+  out->sequences = t->sequences;
+  out->pages = (uint32_t)t->pages;
+  out->page_size = t->page_size;
+  out->most_tokens = (uint32_t)(t->table_width * t->page_size);
+  out->segment = pitch::pages_segment(t->pages);
+  out->segments = (uint32_t)((t->pages + out->segment - 1) / out->segment);
+  out->counts = (uint32_t*)t->workspace;
+  out->plan = out->counts + pitch::kPagesMostSegments;
+  out->room = out->plan + pitch::pages_plan_words(t->sequences);
+  return PITCH_OK;
+}
+
+// The caches whose pages the tables number: their checks, and their memory for the list.
+int paged_layers(const pitch_paged_tables_t* t, const pitch_paged_cache_t* caches, uint32_t n, std::vector<Named>* memory) {
+  if (!caches || n < 1 || n > 4096) return fail(PITCH_ERR_INVALID_INPUT, "caches must be 1...4096");
+  for (uint32_t i = 0; i < n; ++i) {
+    const pitch_paged_cache_t& c = caches[i];
+    PITCH_TRY(check_paged_cache(&c));
+    if (c.pages != t->pages || c.page_size != t->page_size)
+      return fail(PITCH_ERR_CONFIGURATION_MISMATCH, "cache %u has %llu pages of %u tokens, the tables number %llu of %u", i,
+                  (unsigned long long)c.pages, c.page_size, (unsigned long long)t->pages, t->page_size);
+    const uint64_t page = (uint64_t)c.kv_heads * c.page_size;
+    auto pool = [&](const void* p, uint64_t row, const char* name) {
+      Spread s(p, page * row);
+      if (c.pages > 1) s.tokens = c.pages, s.token_stride = c.page_stride * row;
+      memory->push_back({s, name, true});
+    };
+    pool(c.key_codes, code_stride_of(c.key_config.dim, c.key_config.bits), "key codes");
+    pool(c.key_scales, 4, "key scales");
+    pool(c.value_codes, code_stride_of(c.value_config.dim, c.value_config.bits), "value codes");
+    pool(c.value_scales, 4, "value scales");
+  }
+  return PITCH_OK;
+}
+
+// No memory that the call writes may be named twice; all of it is the device's. (Pools are not compared with each other.)
+int check_tables_memory(const std::vector<Named>& memory, size_t small) {
+  for (size_t i = 0; i < small; ++i)
+    for (size_t j = i + 1; j < memory.size(); ++j)
+      if (memory[i].written || memory[j].written)
+        PITCH_TRY(check_apart(memory[i].memory, memory[i].name, memory[j].memory, memory[j].name));
+  int dev = 0;
+  PITCH_TRY(current_device(&dev));
+  BatchDeviceCheck check(dev);
+  for (const Named& m : memory) PITCH_TRY(check((const void*)m.memory.base, m.name));
+  return PITCH_OK;
+}
+
+// The copies that a call's bookkeeping has listed, in all layers.
+hipError_t copy_pages(pitch::PagesCopyArgs& a, const pitch_paged_cache_t* caches, uint32_t n, hipStream_t s) {
+  const uint32_t cus = (uint32_t)pitch::device_cu_count();
+  a.page_size = caches[0].page_size;
+  for (uint32_t first = 0; first < n; first += pitch::kPagesLayers) {
+    a.layers = std::min(n - first, pitch::kPagesLayers);
+    uint64_t largest = 0;
+    for (uint32_t i = 0; i < a.layers; ++i) {
+      const pitch_paged_cache_t& c = caches[first + i];
+      pitch::PagesLayer& l = a.layer[i];
+      l.base[0] = (uint8_t*)c.key_codes;
+      l.base[1] = (uint8_t*)c.key_scales;
+      l.base[2] = (uint8_t*)c.value_codes;
+      l.base[3] = (uint8_t*)c.value_scales;
+      l.page_stride = (uint32_t)c.page_stride;
+      l.kv_heads = c.kv_heads;
+      l.row_bytes[0] = code_stride_of(c.key_config.dim, c.key_config.bits);
+      l.row_bytes[1] = code_stride_of(c.value_config.dim, c.value_config.bits);
+      l.head_major = c.layout == PITCH_PAGES_HEAD_MAJOR;
+      largest = std::max(largest, (uint64_t)c.kv_heads * c.page_size * (l.row_bytes[0] + l.row_bytes[1] + 8u));
+    }
+    a.slices = (uint32_t)((largest + pitch::kPagesSlice - 1) / pitch::kPagesSlice);
+    const hipError_t e = pitch::launch_pages_copy(a, cus, s);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+// No exception leaves a C entry.
+template <typename F>
+int guarded(F f) {
+  try {
+    return f();
+  } catch (const std::exception& e) {
+    return fail(PITCH_ERR_INVALID_INPUT, "out of host memory: %s", e.what());
+  }
+}
+
+int finished(hipError_t e) {
+  if (e != hipSuccess) return fail(PITCH_ERR_ENCODING_FAILED, "Page tables failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+}  // namespace
+
+extern "C" {
+
+int pitch_paged_tables_workspace_size(const pitch_paged_tables_t* tables, uint64_t* bytes) {
+  PITCH_TRY(validate_tables(tables));
+  if (!bytes) return fail(PITCH_ERR_INVALID_INPUT, "bytes is null");
+  *bytes = tables_workspace(tables);
+  return ok();
+}
+
+int pitch_enqueue_paged_reserve(const pitch_paged_tables_t* tables, const pitch_paged_reserve_t* call, void* stream) {
+  return guarded([&]() -> int {
+    pitch::PagesReserveArgs a{};
+    std::vector<Named> memory;
+    PITCH_TRY(paged_tables(tables, &a.t, &memory));
+    if (!call) return fail(PITCH_ERR_INVALID_INPUT, "call is null");
+    if (call->capacity < 1 || call->capacity > 0x7FFFFFFFull) return fail(PITCH_ERR_INVALID_INPUT, "capacity must be in 1...2^31 - 1");
+    PITCH_TRY(check_aligned(call->new_tokens, call->new_tokens_bytes, tables->sequences * 4ull, 4, "new tokens"));
+    PITCH_TRY(check_aligned(call->slots, call->slots_bytes, call->capacity * 8u, 8, "slots"));
+    if (call->positions) PITCH_TRY(check_aligned(call->positions, call->positions_bytes, call->capacity * 8u, 8, "positions"));
+    memory.push_back({Spread(call->new_tokens, tables->sequences * 4ull), "new tokens", false});
+    memory.push_back({Spread(call->slots, call->capacity * 8u), "slots", true});
+    if (call->positions) memory.push_back({Spread(call->positions, call->capacity * 8u), "positions", true});
+    PITCH_TRY(check_tables_memory(memory, memory.size()));
+    a.new_tokens = (const int32_t*)call->new_tokens;
+    a.slots = (int64_t*)call->slots;
+    a.positions = (int64_t*)call->positions;
+    a.capacity = (uint32_t)call->capacity;
+    return finished(pitch::launch_pages_reserve(a, (hipStream_t)stream));
+  });
+}
+
+int pitch_enqueue_paged_trim(const pitch_paged_tables_t* tables, const void* keep, uint64_t keep_bytes, void* stream) {
+  return guarded([&]() -> int {
+    pitch::PagesTrimArgs a{};
+    std::vector<Named> memory;
+    PITCH_TRY(paged_tables(tables, &a.t, &memory));
+    PITCH_TRY(check_aligned(keep, keep_bytes, tables->sequences * 4ull, 4, "keep"));
+    memory.push_back({Spread(keep, tables->sequences * 4ull), "keep", false});
+    PITCH_TRY(check_tables_memory(memory, memory.size()));
+    a.keep = (const int32_t*)keep;
+    return finished(pitch::launch_pages_trim(a, (hipStream_t)stream));
+  });
+}
+
+int pitch_enqueue_paged_fork(const pitch_paged_tables_t* tables, const pitch_paged_cache_t* caches, uint32_t n_caches,
+                             const void* parents, uint64_t parents_bytes, void* stream) {
+  return guarded([&]() -> int {
+    pitch::PagesForkArgs a{};
+    std::vector<Named> memory;
+    PITCH_TRY(paged_tables(tables, &a.t, &memory));
+    PITCH_TRY(check_aligned(parents, parents_bytes, tables->sequences * 4ull, 4, "parents"));
+    memory.push_back({Spread(parents, tables->sequences * 4ull), "parents", false});
+    const size_t small = memory.size();
+    PITCH_TRY(paged_layers(tables, caches, n_caches, &memory));
+    PITCH_TRY(check_tables_memory(memory, small));
+    a.parents = (const int32_t*)parents;
+    pitch::PagesCopyArgs copies{};
+    const hipError_t e = pitch::launch_pages_fork(a, &copies, (hipStream_t)stream);
+    return finished(e != hipSuccess ? e : copy_pages(copies, caches, n_caches, (hipStream_t)stream));
+  });
+}
+
+int pitch_enqueue_paged_compact(const pitch_paged_tables_t* tables, const pitch_paged_cache_t* caches, uint32_t n_caches,
+                                void* mapping, uint64_t mapping_bytes, void* used, uint64_t used_bytes, void* stream) {
+  return guarded([&]() -> int {
+    pitch::PagesCompactArgs a{};
+    std::vector<Named> memory;
+    PITCH_TRY(paged_tables(tables, &a.t, &memory));
+    if (mapping) {
+      PITCH_TRY(check_aligned(mapping, mapping_bytes, tables->pages * 4u, 4, "mapping"));
+      memory.push_back({Spread(mapping, tables->pages * 4u), "mapping", true});
+    }
+    if (used) {
+      PITCH_TRY(check_aligned(used, used_bytes, 4, 4, "used"));
+      memory.push_back({Spread(used, 4), "used", true});
+    }
+    const size_t small = memory.size();
+    PITCH_TRY(paged_layers(tables, caches, n_caches, &memory));
+    PITCH_TRY(check_tables_memory(memory, small));
+    a.mapping = (int32_t*)mapping;
+    a.used = (int32_t*)used;
+    pitch::PagesCopyArgs copies{};
+    const hipError_t e = pitch::launch_pages_compact(a, &copies, (hipStream_t)stream);
+    return finished(e != hipSuccess ? e : copy_pages(copies, caches, n_caches, (hipStream_t)stream));
+  });
 }
 
 }  // extern "C"

@@ -1,0 +1,491 @@
+// The pages of a paged cache: handing out, giving back, sharing and compacting them, with tables, lengths and counts of references in
+// device memory, so that a captured graph serves every step.
+//
+// Free pages are ranked, not listed: a pool's references are counted in segments by one launch, and the next gives page number k
+// among the free ones to the k-th place that needs a page. Every order is that of the numbers, never that of arrival: the same state
+// gives the same pages. Counts of references change by atomic additions, whose order does not matter.
+#include "pitch_pages.h"
+
+namespace pitch {
+namespace {
+
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kMostSequences = 2048;
+
+__device__ __forceinline__ uint32_t lanes_below(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
+}
+__device__ __forceinline__ uint32_t pages_of(uint32_t tokens, uint32_t page) { return tokens / page + (tokens % page != 0); }
+// A sequence's length as it is taken: within its row of the table.
+__device__ __forceinline__ uint32_t length_of(const PagesTables& t, int32_t x) { return min((uint32_t)max(x, 0), t.most_tokens); }
+__device__ __forceinline__ bool in_pool(const PagesTables& t, int32_t page) { return (uint32_t)page < t.pages; }
+
+// Sums over the workgroup, in every thread.
+__device__ __forceinline__ uint32_t group_sum(uint32_t x, uint32_t* lds) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+  __syncthreads();
+  return lds[0] + lds[1] + lds[2] + lds[3];
+}
+// The sum over the threads before this one; *total gets the workgroup's.
+template <typename T>
+__device__ __forceinline__ T group_before(T x, T* lds, T* total) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  T sum = x;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const T up = __shfl_up(sum, d);
+    if (lane >= (uint32_t)d) sum += up;
+  }
+  __syncthreads();
+  if (lane == 63) lds[wave] = sum;
+  __syncthreads();
+  T before = sum - x;
+  for (uint32_t w = 0; w < wave; ++w) before += lds[w];
+  *total = lds[0] + lds[1] + lds[2] + lds[3];
+  return before;
+}
+
+// Counts a segment's pages with (USED) or without references.
+template <bool USED>
+__device__ __forceinline__ void count_segment(const PagesTables& t, uint32_t segment, uint32_t* lds) {
+  const uint32_t from = segment * t.segment, to = min(from + t.segment, t.pages);
+  uint32_t n = 0;
+  for (uint32_t p = from + threadIdx.x; p < to; p += kThreads) n += (t.references[p] > 0) == USED;
+  n = group_sum(n, lds);
+  if (threadIdx.x == 0) t.counts[segment] = n;
+}
+// The counted pages before a segment, and of the pool.
+__device__ __forceinline__ uint32_t counted_before(const PagesTables& t, uint32_t segment, uint32_t* lds, uint32_t* total) {
+  uint32_t before = 0, all = 0;
+  for (uint32_t i = threadIdx.x; i < t.segments; i += kThreads) {
+    const uint32_t n = t.counts[i];
+    all += n;
+    before += i < segment ? n : 0;
+  }
+  *total = group_sum(all, lds);
+  return group_sum(before, lds);
+}
+// Calls f(page, counted, rank) for every page of a segment, all lanes of a wave together (page t.pages for lanes behind the segment):
+// counted says whether it is one of the counted pages, rank is their number before it in the pool.
+template <bool USED, typename F>
+__device__ __forceinline__ void for_segment(const PagesTables& t, uint32_t segment, uint32_t before, uint32_t* lds, F f) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, each = t.segment / 4;
+  const uint32_t from = segment * t.segment + wave * each, end = min((segment + 1) * t.segment, t.pages), to = min(from + each, end);
+  uint32_t n = 0;
+  for (uint32_t p = from; p < to; p += 64) n += __popcll(__ballot(p + lane < to && (t.references[p + lane] > 0) == USED));
+  __syncthreads();
+  if (lane == 0) lds[wave] = n;
+  __syncthreads();
+  uint32_t rank = before;
+  for (uint32_t w = 0; w < wave; ++w) rank += lds[w];
+  for (uint32_t p = from; p < to; p += 64) {
+    const bool inside = p + lane < to, counted = inside && (t.references[p + lane] > 0) == USED;
+    const uint64_t mask = __ballot(counted);
+    f(inside ? p + lane : t.pages, counted, rank + lanes_below(mask));
+    rank += __popcll(mask);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ reserve
+// plan: [0] tokens of the call, [1] pages needed; arrays: the rows' first tokens, their tokens, the pages needed before them, their
+// lengths before the call.
+struct ReservePlan {
+  uint32_t *words, *start, *tokens, *first, *length;
+  __device__ explicit ReservePlan(const PagesTables& t)
+      : words(t.plan), start(t.plan + 8), tokens(start + t.sequences), first(tokens + t.sequences), length(first + t.sequences) {}
+};
+
+__global__ __launch_bounds__(kThreads) void pages_reserve_plan(PagesReserveArgs a) {
+  __shared__ uint32_t lds[4];
+  __shared__ uint64_t wide[4];
+  const PagesTables& t = a.t;
+  if (blockIdx.x < t.segments) {
+    count_segment<false>(t, blockIdx.x, lds);
+    return;
+  }
+  const ReservePlan plan(t);
+  uint64_t tokens = 0;
+  uint32_t pages = 0;
+  for (uint32_t base = 0; base < t.sequences; base += kThreads) {
+    const uint32_t b = base + threadIdx.x;
+    const bool row = b < t.sequences;
+    const uint32_t asked = row ? (uint32_t)max(a.new_tokens[b], 0) : 0, length = row ? length_of(t, t.lengths[b]) : 0;
+    uint64_t all;
+    const uint64_t at = tokens + group_before<uint64_t>(asked, wide, &all);
+    tokens += all;
+    const uint32_t start = (uint32_t)min(at, (uint64_t)a.capacity), n = min(asked, a.capacity - start);
+    const uint32_t need = pages_of(length + min(n, t.most_tokens - length), t.page_size) - pages_of(length, t.page_size);
+    uint32_t sum;
+    const uint32_t first = pages + group_before<uint32_t>(need, lds, &sum);
+    pages += sum;
+    if (row) {
+      plan.start[b] = start;
+      plan.tokens[b] = n;
+      plan.first[b] = first;
+      plan.length[b] = length;
+    }
+  }
+  if (threadIdx.x == 0) {
+    plan.words[0] = (uint32_t)min(tokens, (uint64_t)a.capacity);
+    plan.words[1] = pages;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void pages_reserve_place(PagesReserveArgs a) {
+  __shared__ uint32_t lds[4];
+  __shared__ uint32_t first[kMostSequences];
+  const PagesTables& t = a.t;
+  const ReservePlan plan(t);
+  const uint32_t lane = threadIdx.x & 63, page = t.page_size, needed = plan.words[1];
+  const bool rows = blockIdx.x >= t.segments;
+  uint32_t free;
+  const uint32_t before = counted_before(t, rows ? 0 : blockIdx.x, lds, &free);
+  // a row's tokens end where the free pages do
+  auto after = [&](uint32_t b) {
+    const uint32_t length = plan.length[b], fits = min(plan.tokens[b], t.most_tokens - length);
+    const uint32_t held = pages_of(length, page), need = pages_of(length + fits, page) - held, at = plan.first[b];
+    const uint32_t got = min(need, free - min(free, at));
+    return got == need ? length + fits : min(length + fits, (held + got) * page);
+  };
+  if (!rows) {
+    if (before >= needed) return;
+    for (uint32_t b = threadIdx.x; b < t.sequences; b += kThreads) first[b] = plan.first[b];
+    __syncthreads();
+    for_segment<false>(t, blockIdx.x, before, lds, [&](uint32_t p, bool is_free, uint32_t rank) {
+      const bool given = is_free && rank < needed;
+      uint32_t b = 0, at = 0;
+      if (given) {
+        uint32_t lo = 0, hi = t.sequences;   // the last row whose pages begin at this rank or before it
+        while (hi - lo > 1) {
+          const uint32_t mid = (lo + hi) / 2;
+          (first[mid] <= rank ? lo : hi) = mid;
+        }
+        b = lo;
+        at = pages_of(plan.length[b], page) + rank - first[b];
+        t.tables[(uint64_t)b * t.width + at] = (int32_t)p;
+        t.references[p] = 1;
+      }
+      // the page's tokens, page by page
+      for (uint64_t todo = __ballot(given); todo; todo &= todo - 1) {
+        const int who = __ffsll((unsigned long long)todo) - 1;
+        const uint32_t row = __builtin_amdgcn_readlane(b, who), col = __builtin_amdgcn_readlane(at, who);
+        const uint32_t number = __builtin_amdgcn_readlane(p, who), length = plan.length[row];
+        const uint32_t end = after(row), from = plan.start[row] + col * page - length;   // (a new page begins behind the length)
+        const uint32_t n = min(page, end - min(end, col * page));
+        for (uint32_t i = lane; i < n; i += 64) {
+          a.slots[from + i] = (int64_t)((uint64_t)number * page + i);
+          if (a.positions) a.positions[from + i] = col * page + i;
+        }
+      }
+    });
+    return;
+  }
+  const uint32_t waves = (gridDim.x - t.segments) * 4, wave = (blockIdx.x - t.segments) * 4 + (threadIdx.x >> 6);
+  for (uint32_t b = wave; b < t.sequences; b += waves) {
+    const uint32_t length = plan.length[b], start = plan.start[b], n = plan.tokens[b], end = after(b);
+    // tokens that the last page held before still takes, and tokens without a page
+    const uint32_t full = min(end, pages_of(length, page) * page);
+    for (uint32_t i = lane; i < full - length; i += 64) {
+      const uint32_t pos = length + i;
+      const int32_t entry = t.tables[(uint64_t)b * t.width + pos / page];
+      a.slots[start + i] = in_pool(t, entry) ? (int64_t)((uint64_t)entry * page + pos % page) : -1;
+      if (a.positions) a.positions[start + i] = pos;
+    }
+    for (uint32_t i = end - length + lane; i < n; i += 64) {
+      a.slots[start + i] = -1;
+      if (a.positions) a.positions[start + i] = -1;
+    }
+    if (lane == 0) t.lengths[b] = (int32_t)end;
+  }
+  for (uint32_t i = plan.words[0] + wave * 64 + lane; i < a.capacity; i += waves * 64) {
+    a.slots[i] = -1;
+    if (a.positions) a.positions[i] = -1;
+  }
+  if (wave == 0 && lane == 0 && t.missing) *t.missing = (int32_t)(needed - min(needed, free));
+}
+
+// ------------------------------------------------------------------------------------------------ trim
+__global__ __launch_bounds__(kThreads) void pages_trim(PagesTrimArgs a) {
+  const PagesTables& t = a.t;
+  const uint32_t lane = threadIdx.x & 63, b = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (b >= t.sequences) return;
+  const uint32_t length = length_of(t, t.lengths[b]), end = min(length, (uint32_t)max(a.keep[b], 0));
+  for (uint32_t i = pages_of(end, t.page_size) + lane; i < pages_of(length, t.page_size); i += 64) {
+    const int32_t page = t.tables[(uint64_t)b * t.width + i];
+    if (in_pool(t, page)) atomicSub(t.references + page, 1);
+  }
+  if (lane == 0) t.lengths[b] = (int32_t)end;
+}
+
+// ------------------------------------------------------------------------------------------------ fork
+// plan: [0] rows that need a copy, [1] pages copied; arrays: lengths before the call, each row's number among those that need a copy
+// (kNone: none), and the copies' sources, targets and tokens. room: the tables as they were, of the rows' lengths.
+constexpr uint32_t kNone = 0xFFFFFFFFu;
+struct ForkPlan {
+  uint32_t *words, *length, *rank, *source, *target, *tokens, *old;
+  __device__ explicit ForkPlan(const PagesTables& t)
+      : words(t.plan), length(t.plan + 8), rank(length + t.sequences), source(rank + t.sequences), target(source + t.sequences),
+        tokens(target + t.sequences), old(t.room) {}
+};
+
+// Counts of references as they will be, by one wave for each row.
+__global__ __launch_bounds__(kThreads) void pages_fork_rows(PagesForkArgs a) {
+  const PagesTables& t = a.t;
+  const ForkPlan plan(t);
+  const uint32_t lane = threadIdx.x & 63, b = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (b >= t.sequences) return;
+  const uint32_t length = length_of(t, t.lengths[b]), parent = (uint32_t)a.parents[b];
+  const int32_t* const row = t.tables + (uint64_t)b * t.width;
+  const bool changed = parent != b;
+  for (uint32_t i = lane; i < pages_of(length, t.page_size); i += 64) {
+    const int32_t page = row[i];
+    plan.old[(uint64_t)b * t.width + i] = (uint32_t)page;
+    if (changed && in_pool(t, page)) atomicSub(t.references + page, 1);
+  }
+  bool copy = false;
+  if (changed && parent < t.sequences) {
+    const uint32_t tokens = length_of(t, t.lengths[parent]), whole = tokens / t.page_size;
+    const int32_t* const from = t.tables + (uint64_t)parent * t.width;
+    // the parent's own row keeps its last page, or the first of its children does
+    bool keeps = (uint32_t)a.parents[parent] != parent;
+    for (uint32_t i = 0; i < b && keeps; i += 64)
+      keeps = !__ballot(i + lane < b && (uint32_t)a.parents[min(i + lane, b)] == parent);
+    const bool part = tokens % t.page_size != 0;
+    for (uint32_t i = lane; i < whole + (part && keeps); i += 64)
+      if (in_pool(t, from[i])) atomicAdd(t.references + from[i], 1);
+    copy = part && !keeps && in_pool(t, from[whole]);
+  }
+  if (lane == 0) {
+    plan.length[b] = length;
+    plan.rank[b] = copy ? 0 : kNone;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void pages_fork_plan(PagesForkArgs a) {
+  __shared__ uint32_t lds[4];
+  const PagesTables& t = a.t;
+  if (blockIdx.x < t.segments) {
+    count_segment<false>(t, blockIdx.x, lds);
+    return;
+  }
+  const ForkPlan plan(t);
+  uint32_t copies = 0;
+  for (uint32_t base = 0; base < t.sequences; base += kThreads) {
+    const uint32_t b = base + threadIdx.x;
+    const bool copy = b < t.sequences && plan.rank[b] != kNone;
+    uint32_t all;
+    const uint32_t rank = copies + group_before<uint32_t>(copy, lds, &all);
+    copies += all;
+    if (!copy) continue;
+    const uint32_t parent = (uint32_t)a.parents[b], tokens = plan.length[parent], whole = tokens / t.page_size;
+    plan.rank[b] = rank;
+    plan.source[rank] = plan.old[(uint64_t)parent * t.width + whole];
+    plan.target[rank] = b;       // the row, until the page is known
+    plan.tokens[rank] = tokens % t.page_size;
+  }
+  if (threadIdx.x == 0) plan.words[0] = copies;
+}
+
+__global__ __launch_bounds__(kThreads) void pages_fork_place(PagesForkArgs a) {
+  __shared__ uint32_t lds[4];
+  const PagesTables& t = a.t;
+  const ForkPlan plan(t);
+  const bool rows = blockIdx.x >= t.segments;
+  const uint32_t copies = plan.words[0];
+  uint32_t free;
+  const uint32_t before = counted_before(t, rows ? 0 : blockIdx.x, lds, &free);
+  if (!rows) {
+    if (before >= copies) return;
+    for_segment<false>(t, blockIdx.x, before, lds, [&](uint32_t p, bool is_free, uint32_t rank) {
+      if (!is_free || rank >= copies) return;
+      const uint32_t b = plan.target[rank], whole = plan.length[(uint32_t)a.parents[b]] / t.page_size;
+      t.tables[(uint64_t)b * t.width + whole] = (int32_t)p;
+      t.references[p] = 1;
+      plan.target[rank] = p;
+    });
+    return;
+  }
+  const uint32_t lane = threadIdx.x & 63, b = (blockIdx.x - t.segments) * 4 + (threadIdx.x >> 6);
+  if (b == 0 && lane == 0) {
+    plan.words[1] = min(copies, free);
+    if (t.missing) *t.missing = (int32_t)(copies - min(copies, free));
+  }
+  if (b >= t.sequences) return;
+  const uint32_t parent = (uint32_t)a.parents[b], rank = plan.rank[b];
+  if (parent == b) return;
+  uint32_t end = 0;
+  if (parent < t.sequences) {
+    end = plan.length[parent];
+    const uint32_t whole = end / t.page_size, n = rank == kNone ? pages_of(end, t.page_size) : whole;
+    for (uint32_t i = lane; i < n; i += 64) t.tables[(uint64_t)b * t.width + i] = (int32_t)plan.old[(uint64_t)parent * t.width + i];
+    if (rank != kNone && rank >= free) end = whole * t.page_size;   // no page is left for the last tokens
+  }
+  if (lane == 0) t.lengths[b] = (int32_t)end;
+}
+
+// ------------------------------------------------------------------------------------------------ compact
+// U pages are in use. Those at U and above (movers) go to the free ones below U (holes), as many, the k-th to the k-th. plan: [0] U,
+// [1] movers; room: the holes, the movers counted from the last, and for each page at U or above its number among these (kNone: free).
+struct CompactPlan {
+  uint32_t *words, *holes, *movers, *number;
+  __device__ explicit CompactPlan(const PagesTables& t)
+      : words(t.plan), holes(t.room), movers(t.room + t.pages), number(t.room + 2ull * t.pages) {}
+};
+
+__global__ __launch_bounds__(kThreads) void pages_compact_count(PagesCompactArgs a) {
+  __shared__ uint32_t lds[4];
+  count_segment<true>(a.t, blockIdx.x, lds);
+}
+
+__global__ __launch_bounds__(kThreads) void pages_compact_list(PagesCompactArgs a) {
+  __shared__ uint32_t lds[4];
+  const PagesTables& t = a.t;
+  const CompactPlan plan(t);
+  uint32_t used;
+  const uint32_t before = counted_before(t, blockIdx.x, lds, &used);
+  for_segment<true>(t, blockIdx.x, before, lds, [&](uint32_t p, bool in_use, uint32_t rank) {
+    if (p >= t.pages) return;
+    if (p == used) plan.words[1] = used - rank;   // as many lie at U and above as are missing below
+    if (p < used) {
+      if (!in_use) plan.holes[p - rank] = p;
+    } else {
+      plan.number[p] = in_use ? used - 1 - rank : kNone;
+      if (in_use) plan.movers[used - 1 - rank] = p;
+    }
+    if (a.mapping && !(in_use && p >= used)) a.mapping[p] = in_use ? (int32_t)p : -1;
+  });
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    plan.words[0] = used;
+    if (used == t.pages) plan.words[1] = 0;
+    if (a.used) *a.used = (int32_t)used;
+  }
+}
+
+// The tables' entries, and the references and mapping of the pages that move.
+__global__ __launch_bounds__(kThreads) void pages_compact_tables(PagesCompactArgs a) {
+  const PagesTables& t = a.t;
+  const CompactPlan plan(t);
+  const uint32_t used = plan.words[0], moves = plan.words[1];
+  const uint32_t all = gridDim.x * kThreads, at = blockIdx.x * kThreads + threadIdx.x;
+  for (uint32_t i = at; i < moves; i += all) {
+    const uint32_t from = plan.movers[moves - 1 - i], to = plan.holes[i];
+    t.references[to] = t.references[from];
+    t.references[from] = 0;
+    if (a.mapping) a.mapping[from] = (int32_t)to;
+  }
+  for (uint32_t b = at / 64; b < t.sequences; b += all / 64) {
+    const uint32_t n = pages_of(length_of(t, t.lengths[b]), t.page_size);
+    for (uint32_t i = at % 64; i < n; i += 64) {
+      int32_t* const entry = t.tables + (uint64_t)b * t.width + i;
+      const int32_t page = *entry;
+      if (!in_pool(t, page) || (uint32_t)page < used) continue;
+      const uint32_t number = plan.number[page];
+      if (number != kNone) *entry = (int32_t)plan.holes[moves - 1 - number];
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ copies
+typedef uint32_t w4 __attribute__((ext_vector_type(4)));
+typedef w4 w4_any __attribute__((aligned(4)));   // (buffers are aligned to 4 bytes)
+
+// Copies n16 pieces of 16 bytes of `runs` runs, run bytes apart, `used` bytes of each (a multiple of 4).
+__device__ __forceinline__ void copy_runs(const uint8_t* from, uint8_t* to, uint32_t runs, uint32_t run, uint32_t used, uint32_t first,
+                                          uint32_t last) {
+  const uint32_t each = (used + 15) / 16;
+  for (uint32_t i = first + threadIdx.x; i < last; i += kThreads) {
+    const uint32_t r = runs > 1 ? i / each : 0, at = (i - r * each) * 16, left = used - at;
+    const uint8_t* const f = from + (uint64_t)r * run + at;
+    uint8_t* const g = to + (uint64_t)r * run + at;
+    if (left >= 16) {
+      *(w4_any*)g = *(const w4_any*)f;
+    } else {
+      for (uint32_t j = 0; j < left; j += 4) *(uint32_t*)(g + j) = *(const uint32_t*)(f + j);
+    }
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void pages_copy(PagesCopyArgs a) {
+  const uint32_t count = min(*a.count, a.most);
+  const uint64_t units = (uint64_t)count * a.layers * a.slices;
+  for (uint64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const uint64_t rest = unit / a.slices;
+    const uint32_t slice = (uint32_t)(unit % a.slices), l = (uint32_t)(rest % a.layers), i = (uint32_t)(rest / a.layers);
+    const uint32_t source = a.source[a.backwards ? count - 1 - i : i], target = a.target[i];
+    const PagesLayer& layer = a.layer[l];
+    const uint32_t tokens = a.tokens ? a.tokens[i] : a.page_size;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const uint32_t row = b & 1 ? 4u : layer.row_bytes[b >> 1];
+      const uint64_t stride = (uint64_t)layer.page_stride * row;
+      // whole pages and token-major ones are one run
+      const bool split = layer.head_major && tokens != a.page_size;
+      const uint32_t runs = split ? layer.kv_heads : 1, used = tokens * row * (split ? 1 : layer.kv_heads), run = a.page_size * row;
+      const uint32_t pieces = runs * ((used + 15) / 16), each = (pieces + a.slices - 1) / a.slices;
+      copy_runs(layer.base[b] + source * stride, layer.base[b] + target * stride, runs, run, used, min(slice * each, pieces),
+                min((slice + 1) * each, pieces));
+    }
+  }
+}
+
+}  // namespace
+
+hipError_t launch_pages_reserve(const PagesReserveArgs& a, hipStream_t s) {
+  pages_reserve_plan<<<dim3(a.t.segments + 1), dim3(kThreads), 0, s>>>(a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  pages_reserve_place<<<dim3(a.t.segments + (a.t.sequences + 3) / 4), dim3(kThreads), 0, s>>>(a);
+  return hipGetLastError();
+}
+
+hipError_t launch_pages_trim(const PagesTrimArgs& a, hipStream_t s) {
+  pages_trim<<<dim3((a.t.sequences + 3) / 4), dim3(kThreads), 0, s>>>(a);
+  return hipGetLastError();
+}
+
+hipError_t launch_pages_fork(const PagesForkArgs& a, PagesCopyArgs* copies, hipStream_t s) {
+  const uint32_t rows = (a.t.sequences + 3) / 4;
+  pages_fork_rows<<<dim3(rows), dim3(kThreads), 0, s>>>(a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  pages_fork_plan<<<dim3(a.t.segments + 1), dim3(kThreads), 0, s>>>(a);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  pages_fork_place<<<dim3(a.t.segments + rows), dim3(kThreads), 0, s>>>(a);
+  copies->count = a.t.plan + 1;
+  copies->source = a.t.plan + 8 + 2ull * a.t.sequences;
+  copies->target = copies->source + a.t.sequences;
+  copies->tokens = copies->target + a.t.sequences;
+  copies->backwards = 0;
+  copies->most = a.t.sequences;
+  return hipGetLastError();
+}
+
+hipError_t launch_pages_compact(const PagesCompactArgs& a, PagesCopyArgs* copies, hipStream_t s) {
+  pages_compact_count<<<dim3(a.t.segments), dim3(kThreads), 0, s>>>(a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  pages_compact_list<<<dim3(a.t.segments), dim3(kThreads), 0, s>>>(a);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  pages_compact_tables<<<dim3((a.t.sequences + 3) / 4), dim3(kThreads), 0, s>>>(a);
+  copies->count = a.t.plan + 1;
+  copies->target = a.t.room;
+  copies->source = a.t.room + a.t.pages;
+  copies->tokens = nullptr;
+  copies->backwards = 1;
+  copies->most = a.t.pages / 2;
+  return hipGetLastError();
+}
+
+hipError_t launch_pages_copy(const PagesCopyArgs& a, uint32_t cus, hipStream_t s) {
+  const uint64_t units = (uint64_t)a.most * a.layers * a.slices, most = 8ull * cus;
+  if (units == 0) return hipSuccess;
+  pages_copy<<<dim3((uint32_t)(units < most ? units : most)), dim3(kThreads), 0, s>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace pitch

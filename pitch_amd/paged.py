@@ -270,11 +270,12 @@ class WorkspaceCall:
             c.workspace, c.workspace_bytes = _buf(workspace, "workspace")
         self._workspace = workspace
 
-    def enqueue(self, stream=None) -> None:
+    def _handle(self, stream) -> int:
+        """The stream's handle, when the stream may use the workspace."""
         handle = _stream_handle(stream, self._device)
         if self._ready is not None and handle not in self._ready:
             self._admit(stream, handle)
-        self._issue(handle)
+        return handle
 
     def _admit(self, stream, handle: int) -> None:
         """Lets another stream use a workspace allocated here: behind the work that the allocation's stream holds (the memory may
@@ -329,7 +330,7 @@ class PagedAttention(WorkspaceCall):
         self._call, self._ref, self._pool = c, ctypes.byref(c), ctypes.byref(cache._cstruct)
         self._fn, self._device = cache.pitch._lib.pitch_enqueue_paged_attention, cache.pitch.device
 
-    def _issue(self, handle: int) -> None:
-        rc = self._fn(self._pool, self._ref, handle)
+    def enqueue(self, stream=None) -> None:
+        rc = self._fn(self._pool, self._ref, self._handle(stream))
         if rc:
             _raise_for(rc)

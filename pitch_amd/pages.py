@@ -1,0 +1,152 @@
+"""Page tables in device memory (no counterpart in the reference, whose caches are one sequence's contiguous buffers,
+README.md:65-76): ``PagedTables`` holds (or allocates) the tables, lengths and counts of references of sequences whose layers'
+``PagedCache`` pools have the same pages. ``PagedReserve`` hands out pages and slots for new tokens, ``PagedTrim`` gives tokens back,
+``PagedFork`` makes rows copies of others, sharing whole pages, and ``PagedCompact`` moves the pages in use to the lowest numbers. Nothing
+is read back to the host, so a captured graph serves every step: reserve, append, attend. Like ``PagedAttention``, each keeps a
+call's checked arguments between calls; ``PagedTables.enqueueReserve`` and the like make and issue one such call.
+"""
+from __future__ import annotations
+
+import ctypes
+
+from . import _lib
+from .api import InvalidInput, _raise_for, _torch
+from .paged import PagedCache, WorkspaceCall, _device_tensor, _flat, _int, _tables
+
+
+class PagedTables(WorkspaceCall):
+    """The pages of sequences over the pools of ``caches`` (the layers' PagedCache objects, or one; all with as many pages of the same
+    size): sequence b holds blockTables[b][0 .. ceil(lengths[b] / pageSize) - 1]. blockTables int32 [sequences][width], lengths int32
+    [sequences], references int32 [pages] (how many entries hold a page; free where not positive) and missing int32 [1] (pages that the
+    last reserve or fork lacked) are allocated empty, for ``sequences`` rows (at most 2,048) of ``width`` pages, or given. A
+    program that keeps a page for itself, a prefix's say, adds 1 to its references. Free pages are handed out lowest
+    number first, in the order of the sequences and their tokens. Where they run out, a row ends with its last token that has a
+    page. Calls on the same tables run one after the other; on another stream than the one that the workspace was allocated on a call
+    waits for that stream's work."""
+
+    def __init__(self, caches, sequences: int | None = None, width: int | None = None, blockTables=None, lengths=None, references=None,
+                 missing=None):
+        torch = _torch()
+        self.caches = [caches] if isinstance(caches, PagedCache) else list(caches)
+        if not self.caches or not all(isinstance(c, PagedCache) for c in self.caches):
+            raise InvalidInput("caches must be PagedCache objects, at least one")
+        first = self.caches[0]
+        self.pitch, self.pages, self.pageSize = first.pitch, first.pages, first.pageSize
+        if any((c.pages, c.pageSize) != (self.pages, self.pageSize) for c in self.caches):
+            raise InvalidInput("all caches need as many pages of the same size")
+        device = self.pitch.device
+        if blockTables is None:
+            if sequences is None or width is None:
+                raise InvalidInput("sequences and width are needed where blockTables is not given")
+            blockTables = torch.full((_int(sequences, "sequences", 1), _int(width, "width", 1)), -1, dtype=torch.int32, device=device)
+        elif sequences is not None or width is not None:
+            raise InvalidInput("blockTables has its own sequences and width")
+        c = _lib.PitchPagedTablesC()
+        c.block_tables, c.block_tables_bytes = _tables(blockTables)
+        self.sequences, self.width = blockTables.shape
+        given = lambda t, n: torch.zeros(n, dtype=torch.int32, device=device) if t is None else t  # noqa: E731
+        lengths, references, missing = given(lengths, self.sequences), given(references, self.pages), given(missing, 1)
+        c.lengths, c.lengths_bytes = _flat(lengths, "lengths", torch.int32, self.sequences)
+        c.references, c.references_bytes = _flat(references, "references", torch.int32, self.pages)
+        c.missing, c.missing_bytes = _flat(missing, "missing", torch.int32, 1)
+        c.table_width, c.pages, c.page_size, c.sequences = self.width, self.pages, self.pageSize, self.sequences
+        self.blockTables, self.lengths, self.references, self.missing = blockTables, lengths, references, missing
+        needed = ctypes.c_uint64(0)
+        _raise_for(self.pitch._lib.pitch_paged_tables_workspace_size(ctypes.byref(c), ctypes.byref(needed)))
+        self._hold_workspace(c, None, int(needed.value), device)
+        self._cstruct, self._device = c, device
+        self._layers = (_lib.PitchPagedCacheC * len(self.caches))(*[cache._cstruct for cache in self.caches])
+
+    def enqueueReserve(self, newTokens, slots, positions=None, stream=None) -> None:
+        """One PagedReserve call."""
+        PagedReserve(self, newTokens, slots, positions=positions).enqueue(stream)
+
+    def enqueueTrim(self, keep, stream=None) -> None:
+        """One PagedTrim call."""
+        PagedTrim(self, keep).enqueue(stream)
+
+    def enqueueFork(self, parents, stream=None) -> None:
+        """One PagedFork call."""
+        PagedFork(self, parents).enqueue(stream)
+
+    def enqueueCompact(self, mapping=None, used=None, stream=None) -> None:
+        """One PagedCompact call."""
+        PagedCompact(self, mapping=mapping, used=used).enqueue(stream)
+
+
+class _TablesCall:
+    """A call on tables, whose workspace is the tables'."""
+
+    def __init__(self, tables: PagedTables):
+        if not isinstance(tables, PagedTables):
+            raise InvalidInput("tables must be a PagedTables object")
+        self.tables = tables
+        self._pool, self._lib = ctypes.byref(tables._cstruct), tables.pitch._lib
+
+    def enqueue(self, stream=None) -> None:
+        rc = self._launch(self.tables._handle(stream))
+        if rc:
+            _raise_for(rc)
+
+
+class PagedReserve(_TablesCall):
+    """Takes newTokens[b] (int32 [sequences]; 0 or less: none) further tokens into every sequence b: hands out pages where those that
+    it holds do not suffice, and adds to lengths. The tokens are packed in the order of the sequences; token t's slot (page * pageSize + slot,
+    for ``PagedAppend``) goes to slots[t] and its position in its sequence to positions[t] (int64, both as many as a step has room for).
+    A token without a page, or without a place in its row of the table, has -1 in both, and so have the entries behind the last token:
+    ``PagedAppend`` leaves them out. Tokens for which slots has no room are not taken."""
+
+    def __init__(self, tables: PagedTables, newTokens, slots, positions=None):
+        super().__init__(tables)
+        torch = _torch()
+        c = _lib.PitchPagedReserveC()
+        c.new_tokens, c.new_tokens_bytes = _flat(newTokens, "newTokens", torch.int32, tables.sequences)
+        c.slots, c.slots_bytes = _flat(slots, "slots", torch.int64, None)
+        c.capacity = slots.numel()
+        c.positions, c.positions_bytes = _flat(positions, "positions", torch.int64, c.capacity)
+        self._held, self._call, self._ref = (newTokens, slots, positions), c, ctypes.byref(c)
+
+    def _launch(self, handle: int) -> int:
+        return self._lib.pitch_enqueue_paged_reserve(self._pool, self._ref, handle)
+
+
+class PagedTrim(_TablesCall):
+    """Cuts every sequence b to at most keep[b] tokens (int32 [sequences]; 0 or less: the whole sequence is given back). The pages
+    behind lose a reference; what remains is untouched."""
+
+    def __init__(self, tables: PagedTables, keep):
+        super().__init__(tables)
+        self._held, (self._keep, self._bytes) = keep, _flat(keep, "keep", _torch().int32, tables.sequences)
+
+    def _launch(self, handle: int) -> int:
+        return self._lib.pitch_enqueue_paged_trim(self._pool, self._keep, self._bytes, handle)
+
+
+class PagedFork(_TablesCall):
+    """Makes every row b a copy of row parents[b] (int32 [sequences]) as it was before the call; b itself leaves the row alone, a number
+    outside the rows (-1) empties it. Whole pages are shared; a partly filled last page goes to one row (the parent's own if that stays, else its
+    first child), and the others get a page of their own with its tokens, in every cache of the tables."""
+
+    def __init__(self, tables: PagedTables, parents):
+        super().__init__(tables)
+        self._held, (self._parents, self._bytes) = parents, _flat(parents, "parents", _torch().int32, tables.sequences)
+
+    def _launch(self, handle: int) -> int:
+        t = self.tables
+        return self._lib.pitch_enqueue_paged_fork(self._pool, t._layers, len(t.caches), self._parents, self._bytes, handle)
+
+
+class PagedCompact(_TablesCall):
+    """Moves the pages in use to the lowest numbers: with U in use, those at U and above go into the free ones below U, the k-th to the
+    k-th, in every cache; tables and references follow. mapping (int32 [pages]) receives each page's new number, -1 for a free
+    page, and used (int32 [1]) U."""
+
+    def __init__(self, tables: PagedTables, mapping=None, used=None):
+        super().__init__(tables)
+        torch = _torch()
+        self._held = (mapping, used)
+        self._more = _flat(mapping, "mapping", torch.int32, tables.pages) + _flat(used, "used", torch.int32, 1)
+
+    def _launch(self, handle: int) -> int:
+        t = self.tables
+        return self._lib.pitch_enqueue_paged_compact(self._pool, t._layers, len(t.caches), *self._more, handle)

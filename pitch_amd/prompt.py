@@ -64,7 +64,7 @@ class PromptAttention(WorkspaceCall):
         self._call, self._ref = c, ctypes.byref(c)
         self._fn, self._device = pitch._lib.pitch_enqueue_prompt_attention, pitch.device
 
-    def _issue(self, handle: int) -> None:
-        rc = self._fn(self._ref, handle)
+    def enqueue(self, stream=None) -> None:
+        rc = self._fn(self._ref, self._handle(stream))
         if rc:
             _raise_for(rc)
