@@ -55,6 +55,30 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
 }
 __device__ __forceinline__ uint32_t of_wave(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// x *= f where `go` is not zero. The branch is inside the statement: with one around it, the compiler keeps two copies of the
+// accumulators and moves them, 64 registers there and back for every tile (2,190 us of a prompt of 16,381 tokens, 8 KV and 32 query heads; XXX without).
+// Waits: 16 states behind the matrix instructions that wrote x, two before those that read it.
+__device__ __forceinline__ void scale_where(uint64_t go, float f, v16f& x) {
+  float y[16];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) y[r] = x[r];
+  asm("s_cmp_eq_u64 %16, 0\n\t"
+      "s_cbranch_scc1 .Lkept%=\n\t"
+      "s_nop 7\n\ts_nop 7\n\t"
+      "v_mul_f32 %0, %0, %17\n\tv_mul_f32 %1, %1, %17\n\tv_mul_f32 %2, %2, %17\n\tv_mul_f32 %3, %3, %17\n\t"
+      "v_mul_f32 %4, %4, %17\n\tv_mul_f32 %5, %5, %17\n\tv_mul_f32 %6, %6, %17\n\tv_mul_f32 %7, %7, %17\n\t"
+      "v_mul_f32 %8, %8, %17\n\tv_mul_f32 %9, %9, %17\n\tv_mul_f32 %10, %10, %17\n\tv_mul_f32 %11, %11, %17\n\t"
+      "v_mul_f32 %12, %12, %17\n\tv_mul_f32 %13, %13, %17\n\tv_mul_f32 %14, %14, %17\n\tv_mul_f32 %15, %15, %17\n\t"
+      "s_nop 1\n"
+      ".Lkept%=:"
+      : "+v"(y[0]), "+v"(y[1]), "+v"(y[2]), "+v"(y[3]), "+v"(y[4]), "+v"(y[5]), "+v"(y[6]), "+v"(y[7]), "+v"(y[8]), "+v"(y[9]),
+        "+v"(y[10]), "+v"(y[11]), "+v"(y[12]), "+v"(y[13]), "+v"(y[14]), "+v"(y[15])
+      : "s"(go), "v"(f)
+      : "scc");
+#pragma unroll
+  for (int r = 0; r < 16; ++r) x[r] = y[r];
+}
+
 // A query tile: the rows [row, row + kRows) of (token, head) pairs of a sequence.
 struct Tile {
   uint32_t first_query, queries;  // the sequence's
@@ -162,8 +186,7 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void prompt_attention(PromptA
   const uint32_t wave_row = t.row + wave * NB * 32, wave_last = min(wave_row + NB * 32, rows) - 1;
   const bool wave_live = wave_row < rows;
   const int32_t wpos0 = offset + (int32_t)(wave_row / a.nq), wpos1 = offset + (int32_t)(wave_last / a.nq);
-  const int32_t whi0 = a.causal ? wpos0 : 0x7FFFFFFF, whi1 = a.causal ? wpos1 : 0x7FFFFFFF;
-  const int32_t wlo0 = window_start(wpos0, a.window), wlo1 = window_start(wpos1, a.window);
+  const int32_t whi0 = a.causal ? wpos0 : 0x7FFFFFFF, wlo1 = window_start(wpos1, a.window);
 
   const uint32_t ktb = (uint32_t)a.k.token_stride * 2, vtb = (uint32_t)a.v.token_stride * 2;
   const uint8_t* const kbase = (const uint8_t*)a.k.data + head * a.k.head_stride * 2 + (uint64_t)t.first_key * ktb;
@@ -179,7 +202,7 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void prompt_attention(PromptA
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                   :: "s"(of_wave(to + (i * kWaves + wave) * 1024)), "v"(at + i * kWaves * kLaneRows * stride), "s"(r) : "memory", "m0");
+                   :: "s"(of_wave(to + (i * kWaves + wave) * 1024)), "v"(at + i * kWaves * kLaneRows * stride), "s"(r) : "memory");
   };
   auto load = [&](int32_t k0, int buf) {
     const uint32_t more = (uint32_t)min((int32_t)t.keys - k0, kKeys) - 1;  // rows behind the sequence are zeros
@@ -196,7 +219,6 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void prompt_attention(PromptA
   const uint32_t vrow = half * 4 + ((lane >> 2) & 3), vchunk = ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1), vbyte = (lane & 1) * 8;
 
   auto tile = [&](int32_t k0, int buf, auto careful, uint32_t kind) {
-    if (!wave_live || k0 > whi1 || k0 + kKeys <= wlo0) return;
     v16f s[NB][2];
     const lds_u8* const kt = (const lds_u8*)lds[buf][0];
     const lds_u8* const vt = (const lds_u8*)lds[buf][1];
@@ -256,20 +278,29 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void prompt_attention(PromptA
             if (kind) s[n][b][r] = s[n][b][r] > kNoScore ? 1.f : 0.f;
       }
       if (!careful || !kind) {
-        float top = fmax_hw(s[n][0][0], s[n][1][0]);
+        // (the compiler does not see that the maxima below read what matrix instructions write: 16 wait states, 11 are needed)
+        asm("s_nop 7\n\ts_nop 7" : "+v"(s[n][0]), "+v"(s[n][1]));
+        float top = fmax3_hw(s[n][0][0], s[n][1][0], s[n][0][1]);
+        float top2 = fmax3_hw(s[n][1][1], s[n][0][2], s[n][1][2]);
 #pragma unroll
-        for (int r = 1; r < 16; ++r) top = fmax_hw(fmax_hw(top, s[n][0][r]), s[n][1][r]);
-        top = max32(top, top);
-        if (__ballot(__builtin_fmaf(top, a.c, -m_run[n] * a.c) > kGrow)) {
+        for (int r = 3; r < 15; r += 2) {
+          top = fmax3_hw(top, s[n][0][r], s[n][1][r]);
+          top2 = fmax3_hw(top2, s[n][0][r + 1], s[n][1][r + 1]);
+        }
+        top = fmax3_hw(top, s[n][0][15], s[n][1][15]);
+        top = max32(fmax_hw(top, top2), fmax_hw(top, top2));
+        const uint64_t grown = __ballot(__builtin_fmaf(top, a.c, -m_run[n] * a.c) > kGrow);
+        float keep = 1.f;
+        if (grown) {
           const float next = fmax_hw(m_run[n], top);
           const float nc = next == kNoScore ? 0.f : next * a.c;
-          const float keep = __builtin_amdgcn_exp2f(__builtin_fmaf(m_run[n], a.c, -nc));
-#pragma unroll
-          for (int d = 0; d < kBlocks; ++d) o[n][d] *= keep;
+          keep = __builtin_amdgcn_exp2f(__builtin_fmaf(m_run[n], a.c, -nc));
           sum[n] *= keep;
           m_run[n] = next;
           mc[n] = nc;
         }
+#pragma unroll
+        for (int d = 0; d < kBlocks; ++d) scale_where(grown, keep, o[n][d]);
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -331,6 +362,15 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void prompt_attention(PromptA
     if (lo >= hi) return;
     load(lo, 0);
     int buf = 0;
+    if (!wave_live) {   // a wave without rows loads its share for the others
+      for (int32_t k0 = lo; k0 < hi; k0 += kKeys, buf ^= 1) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (k0 + kKeys < hi) load(k0 + kKeys, buf ^ 1);
+      }
+      __syncthreads();
+      return;
+    }
     for (int32_t k0 = lo; k0 < hi; k0 += kKeys, buf ^= 1) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
