@@ -61,6 +61,7 @@ struct PagesCopyArgs {
   const uint32_t* tokens;  // of each page, or null: all of the page
   uint32_t backwards;      // 1: sources in descending order of the targets' index (source[count - 1 - i])
   uint32_t page_size, layers, slices, most;  // slices of a layer's page; the most pages there can be
+  uint32_t parts;          // 4: a unit of work is one of a layer's four buffers (set by the launcher)
   PagesLayer layer[kPagesLayers];
 };
 

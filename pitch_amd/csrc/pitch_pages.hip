@@ -156,28 +156,28 @@ __global__ __launch_bounds__(kThreads) void pages_reserve_place(PagesReserveArgs
     __syncthreads();
     for_segment<false>(t, blockIdx.x, before, lds, [&](uint32_t p, bool is_free, uint32_t rank) {
       const bool given = is_free && rank < needed;
-      uint32_t b = 0, at = 0;
+      uint32_t at = 0, from = 0, n = 0;   // the page's place in its row, its first token's in the call, its tokens
       if (given) {
         uint32_t lo = 0, hi = t.sequences;   // the last row whose pages begin at this rank or before it
         while (hi - lo > 1) {
           const uint32_t mid = (lo + hi) / 2;
           (first[mid] <= rank ? lo : hi) = mid;
         }
-        b = lo;
-        at = pages_of(plan.length[b], page) + rank - first[b];
-        t.tables[(uint64_t)b * t.width + at] = (int32_t)p;
+        const uint32_t length = plan.length[lo], end = after(lo);
+        at = pages_of(length, page) + rank - first[lo];
+        from = plan.start[lo] + at * page - length;   // (a new page begins at the length or behind it)
+        n = min(page, end - min(end, at * page));
+        t.tables[(uint64_t)lo * t.width + at] = (int32_t)p;
         t.references[p] = 1;
       }
-      // the page's tokens, page by page
+      // the tokens, page by page
       for (uint64_t todo = __ballot(given); todo; todo &= todo - 1) {
         const int who = __ffsll((unsigned long long)todo) - 1;
-        const uint32_t row = __builtin_amdgcn_readlane(b, who), col = __builtin_amdgcn_readlane(at, who);
-        const uint32_t number = __builtin_amdgcn_readlane(p, who), length = plan.length[row];
-        const uint32_t end = after(row), from = plan.start[row] + col * page - length;   // (a new page begins behind the length)
-        const uint32_t n = min(page, end - min(end, col * page));
-        for (uint32_t i = lane; i < n; i += 64) {
-          a.slots[from + i] = (int64_t)((uint64_t)number * page + i);
-          if (a.positions) a.positions[from + i] = col * page + i;
+        const uint32_t number = __builtin_amdgcn_readlane(p, who), first_token = __builtin_amdgcn_readlane(from, who);
+        const uint32_t pos = __builtin_amdgcn_readlane(at, who) * page, tokens = __builtin_amdgcn_readlane(n, who);
+        for (uint32_t i = lane; i < tokens; i += 64) {
+          a.slots[first_token + i] = (int64_t)((uint64_t)number * page + i);
+          if (a.positions) a.positions[first_token + i] = pos + i;
         }
       }
     });
@@ -392,7 +392,7 @@ __global__ __launch_bounds__(kThreads) void pages_compact_tables(PagesCompactArg
 typedef uint32_t w4 __attribute__((ext_vector_type(4)));
 typedef w4 w4_any __attribute__((aligned(4)));   // (buffers are aligned to 4 bytes)
 
-// Copies n16 pieces of 16 bytes of `runs` runs, run bytes apart, `used` bytes of each (a multiple of 4).
+// Copies pieces [first, last) of 16 bytes of `runs` runs, `run` bytes apart, `used` bytes of each (a multiple of 4).
 __device__ __forceinline__ void copy_runs(const uint8_t* from, uint8_t* to, uint32_t runs, uint32_t run, uint32_t used, uint32_t first,
                                           uint32_t last) {
   const uint32_t each = (used + 15) / 16;
@@ -408,17 +408,21 @@ __device__ __forceinline__ void copy_runs(const uint8_t* from, uint8_t* to, uint
   }
 }
 
+// A unit of work is a slice of a page of a layer, all four buffers one behind the other, or one of them.
 __global__ __launch_bounds__(kThreads) void pages_copy(PagesCopyArgs a) {
   const uint32_t count = min(*a.count, a.most);
-  const uint64_t units = (uint64_t)count * a.layers * a.slices;
+  const uint64_t units = (uint64_t)count * a.layers * a.slices * a.parts;
   for (uint64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
-    const uint64_t rest = unit / a.slices;
-    const uint32_t slice = (uint32_t)(unit % a.slices), l = (uint32_t)(rest % a.layers), i = (uint32_t)(rest / a.layers);
+    uint64_t rest = unit / a.parts;
+    const uint32_t only = (uint32_t)(unit % a.parts), slice = (uint32_t)(rest % a.slices);
+    rest /= a.slices;
+    const uint32_t l = (uint32_t)(rest % a.layers), i = (uint32_t)(rest / a.layers);
     const uint32_t source = a.source[a.backwards ? count - 1 - i : i], target = a.target[i];
     const PagesLayer& layer = a.layer[l];
     const uint32_t tokens = a.tokens ? a.tokens[i] : a.page_size;
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
+      if (a.parts > 1 && only != (uint32_t)b) continue;
       const uint32_t row = b & 1 ? 4u : layer.row_bytes[b >> 1];
       const uint64_t stride = (uint64_t)layer.page_stride * row;
       // whole pages and token-major ones are one run
@@ -481,9 +485,13 @@ hipError_t launch_pages_compact(const PagesCompactArgs& a, PagesCopyArgs* copies
   return hipGetLastError();
 }
 
-hipError_t launch_pages_copy(const PagesCopyArgs& a, uint32_t cus, hipStream_t s) {
-  const uint64_t units = (uint64_t)a.most * a.layers * a.slices, most = 8ull * cus;
-  if (units == 0) return hipSuccess;
+hipError_t launch_pages_copy(const PagesCopyArgs& call, uint32_t cus, hipStream_t s) {
+  PagesCopyArgs a = call;
+  const uint64_t slices = (uint64_t)a.most * a.layers * a.slices, most = 8ull * cus;
+  if (slices == 0) return hipSuccess;
+  // Where there are few slices, a workgroup takes one buffer of a slice: the four do not wait for each other.
+  a.parts = slices < 2ull * cus ? 4 : 1;
+  const uint64_t units = slices * a.parts;
   pages_copy<<<dim3((uint32_t)(units < most ? units : most)), dim3(kThreads), 0, s>>>(a);
   return hipGetLastError();
 }

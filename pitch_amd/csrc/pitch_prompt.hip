@@ -481,20 +481,34 @@ __global__ __launch_bounds__(256) void prompt_join(PromptArgs a) {
   for (uint32_t b = lane; b < a.sequences; b += 64)
     inside |= (int32_t)token >= a.row_starts[b] && (int32_t)token < a.row_starts[b + 1];
   if (!__ballot(inside)) return;
-  float m = kNoScore;
-  for (uint32_t p = 0; p < a.splits; ++p) {
-    const float x = a.ws[(p * all + at) * 2];
-    m = x != x ? x : fmax_hw(m, x);
-  }
+  // a lane for each part (64 at most): its maximum and its sum
+  const bool part = lane < a.splits;
+  const float mine = part ? a.ws[(lane * all + at) * 2] : kNoScore, mine_sum = part ? a.ws[(lane * all + at) * 2 + 1] : 0.f;
+  const bool nan = __ballot(mine != mine) != 0;
+  float m = wave_max(mine);
   if (m == kNoScore) m = 0.f;
-  float sum = 0.f, o[D / 64] = {};
+  const float weight = nan ? __builtin_nanf("") : __builtin_amdgcn_exp2f(mine - m);
+  const float sum = wave_sum(weight == 0.f ? 0.f : weight * mine_sum);
+  float o[D / 64] = {};
   const float* const ov = a.ws + (uint64_t)a.splits * all * 2;
-  for (uint32_t p = 0; p < a.splits; ++p) {
-    const float w = __builtin_amdgcn_exp2f(a.ws[(p * all + at) * 2] - m);
-    if (w == 0.f) continue;
-    sum = __builtin_fmaf(w, a.ws[(p * all + at) * 2 + 1], sum);
+  // (parts without a visible key have not written values that count)
+  for (uint64_t todo = __ballot(part && weight != 0.f); todo;) {
+    float w[8], x[8][D / 64];
 #pragma unroll
-    for (int d = 0; d < D / 64; ++d) o[d] = __builtin_fmaf(w, ov[(p * all + at) * D + lane * (D / 64) + d], o[d]);
+    for (int i = 0; i < 8; ++i) {   // eight parts on their way at once
+      w[i] = 0.f;
+      if (!todo) continue;
+      const int p = __ffsll((unsigned long long)todo) - 1;
+      todo &= todo - 1;
+      w[i] = lane_value(weight, p);
+#pragma unroll
+      for (int d = 0; d < D / 64; ++d) x[i][d] = ov[(p * all + at) * D + lane * (D / 64) + d];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int d = 0; d < D / 64; ++d)
+        if (w[i] != 0.f) o[d] = __builtin_fmaf(w[i], x[i][d], o[d]);
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   if (a.lse && lane == 0) a.lse[at] = sum == 0.f ? kNoScore : (m + __builtin_amdgcn_logf(sum)) * kLn2;
