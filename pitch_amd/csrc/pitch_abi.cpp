@@ -1800,9 +1800,11 @@ namespace {
 
 // The memory that a call on page tables names, each part with its name, and whether the call writes it.
 struct Named {
+  Named(const Spread& m, const char* n, bool w) : memory(m), name(n), written(w), from(m.base), to(m.end()) {}
   Spread memory;
   const char* name;
   bool written;
+  uint64_t from, to;   // all that lies between its first and last byte
 };
 
 int validate_tables(const pitch_paged_tables_t* t) {
@@ -1831,6 +1833,7 @@ int paged_tables(const pitch_paged_tables_t* t, pitch::PagesTables* out, std::ve
   PITCH_TRY(check_aligned(t->references, t->references_bytes, t->pages * 4u, 4, "references"));
   if (t->missing) PITCH_TRY(check_aligned(t->missing, t->missing_bytes, 4, 4, "missing"));
   PITCH_TRY(check_aligned(t->workspace, t->workspace_bytes, tables_workspace(t), 16, "workspace"));
+  memory->reserve(10);
   memory->push_back({Spread(t->block_tables, t->table_width * t->sequences * 4u), "page tables", true});
   memory->push_back({Spread(t->lengths, t->sequences * 4ull), "lengths", true});
   memory->push_back({Spread(t->references, t->pages * 4u), "references", true});
@@ -1856,6 +1859,7 @@ int paged_tables(const pitch_paged_tables_t* t, pitch::PagesTables* out, std::ve
 // The caches whose pages the tables number: their checks, and their memory for the list.
 int paged_layers(const pitch_paged_tables_t* t, const pitch_paged_cache_t* caches, uint32_t n, std::vector<Named>* memory) {
   if (!caches || n < 1 || n > 4096) return fail(PITCH_ERR_INVALID_INPUT, "caches must be 1...4096");
+  memory->reserve(memory->size() + 4u * n);
   for (uint32_t i = 0; i < n; ++i) {
     const pitch_paged_cache_t& c = caches[i];
     PITCH_TRY(check_paged_cache(&c));
@@ -1880,7 +1884,7 @@ int paged_layers(const pitch_paged_tables_t* t, const pitch_paged_cache_t* cache
 int check_tables_memory(const std::vector<Named>& memory, size_t small) {
   for (size_t i = 0; i < small; ++i)
     for (size_t j = i + 1; j < memory.size(); ++j)
-      if (memory[i].written || memory[j].written)
+      if ((memory[i].written || memory[j].written) && memory[i].from < memory[j].to && memory[j].from < memory[i].to)
         PITCH_TRY(check_apart(memory[i].memory, memory[i].name, memory[j].memory, memory[j].name));
   int dev = 0;
   PITCH_TRY(current_device(&dev));

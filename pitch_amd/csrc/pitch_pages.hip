@@ -9,8 +9,13 @@
 namespace pitch {
 namespace {
 
-constexpr uint32_t kThreads = 256;
+constexpr uint32_t kThreads = 256, kOneThreads = 1024, kMostWaves = kOneThreads / 64;
 constexpr uint32_t kMostSequences = 2048;
+// The largest calls whose bookkeeping one workgroup does, in one launch: it costs the host about 2 us less for each launch saved, but
+// a workgroup's wave turns to one row, or to 64 pages, after the other.
+constexpr uint32_t kReserveOnePages = 4096, kReserveOneRows = 256, kReserveOneTokens = 4096;
+constexpr uint32_t kForkOnePages = 4096, kForkOneRows = 16;
+constexpr uint32_t kCompactOnePages = 4096, kCompactOneRows = 64;
 
 __device__ __forceinline__ uint32_t lanes_below(uint64_t mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
@@ -20,6 +25,9 @@ __device__ __forceinline__ uint32_t pages_of(uint32_t tokens, uint32_t page) { r
 __device__ __forceinline__ uint32_t length_of(const PagesTables& t, int32_t x) { return min((uint32_t)max(x, 0), t.most_tokens); }
 __device__ __forceinline__ bool in_pool(const PagesTables& t, int32_t page) { return (uint32_t)page < t.pages; }
 
+// The workgroup's threads: 256, or 1,024 where one does all of a call's work.
+__device__ __forceinline__ uint32_t group_waves() { return blockDim.x >> 6; }
+
 // Sums over the workgroup, in every thread.
 __device__ __forceinline__ uint32_t group_sum(uint32_t x, uint32_t* lds) {
 #pragma unroll
@@ -27,40 +35,67 @@ __device__ __forceinline__ uint32_t group_sum(uint32_t x, uint32_t* lds) {
   __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
   __syncthreads();
-  return lds[0] + lds[1] + lds[2] + lds[3];
+  uint32_t sum = 0;
+  for (uint32_t w = 0; w < group_waves(); ++w) sum += lds[w];
+  return sum;
 }
-// The sum over the threads before this one; *total gets the workgroup's.
+// The sum over the lanes before this one; *total gets the wave's.
 template <typename T>
-__device__ __forceinline__ T group_before(T x, T* lds, T* total) {
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__device__ __forceinline__ T wave_before(T x, T* total) {
+  const uint32_t lane = threadIdx.x & 63;
   T sum = x;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const T up = __shfl_up(sum, d);
     if (lane >= (uint32_t)d) sum += up;
   }
+  *total = __shfl(sum, 63);
+  return sum - x;
+}
+// The same over the workgroup's threads.
+template <typename T>
+__device__ __forceinline__ T group_before(T x, T* lds, T* total) {
+  const uint32_t wave = threadIdx.x >> 6;
+  T own;
+  T before = wave_before(x, &own), all = 0;
   __syncthreads();
-  if (lane == 63) lds[wave] = sum;
+  if ((threadIdx.x & 63) == 0) lds[wave] = own;
   __syncthreads();
-  T before = sum - x;
-  for (uint32_t w = 0; w < wave; ++w) before += lds[w];
-  *total = lds[0] + lds[1] + lds[2] + lds[3];
+  for (uint32_t w = 0; w < group_waves(); ++w) {
+    const T n = lds[w];
+    before += w < wave ? n : 0;
+    all += n;
+  }
+  *total = all;
   return before;
 }
 
+// A page's count of references. With PAST_CACHE it is read past the compute unit's cache, which may hold what the line was before
+// this workgroup's own atomics changed it in L2.
+template <bool PAST_CACHE>
+__device__ __forceinline__ int32_t references_of(const PagesTables& t, uint32_t page) {
+  if constexpr (PAST_CACHE) return __hip_atomic_load(t.references + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return t.references[page];
+}
+
 // Counts a segment's pages with (USED) or without references.
-template <bool USED>
+template <bool USED, bool PAST_CACHE = false>
 __device__ __forceinline__ void count_segment(const PagesTables& t, uint32_t segment, uint32_t* lds) {
   const uint32_t from = segment * t.segment, to = min(from + t.segment, t.pages);
   uint32_t n = 0;
-  for (uint32_t p = from + threadIdx.x; p < to; p += kThreads) n += (t.references[p] > 0) == USED;
+#pragma unroll 4
+  for (uint32_t p = from + threadIdx.x; p < to; p += blockDim.x) n += (references_of<PAST_CACHE>(t, p) > 0) == USED;
   n = group_sum(n, lds);
   if (threadIdx.x == 0) t.counts[segment] = n;
 }
 // The counted pages before a segment, and of the pool.
 __device__ __forceinline__ uint32_t counted_before(const PagesTables& t, uint32_t segment, uint32_t* lds, uint32_t* total) {
+  if (t.segments == 1) {
+    *total = t.counts[0];
+    return 0;
+  }
   uint32_t before = 0, all = 0;
-  for (uint32_t i = threadIdx.x; i < t.segments; i += kThreads) {
+  for (uint32_t i = threadIdx.x; i < t.segments; i += blockDim.x) {
     const uint32_t n = t.counts[i];
     all += n;
     before += i < segment ? n : 0;
@@ -69,20 +104,22 @@ __device__ __forceinline__ uint32_t counted_before(const PagesTables& t, uint32_
   return group_sum(before, lds);
 }
 // Calls f(page, counted, rank) for every page of a segment, all lanes of a wave together (page t.pages for lanes behind the segment):
-// counted says whether it is one of the counted pages, rank is their number before it in the pool.
-template <bool USED, typename F>
-__device__ __forceinline__ void for_segment(const PagesTables& t, uint32_t segment, uint32_t before, uint32_t* lds, F f) {
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, each = t.segment / 4;
+// counted says whether it is one of the counted pages, rank is their number before it in the pool. Stops behind the page of rank `last`.
+template <bool USED, bool PAST_CACHE = false, typename F>
+__device__ __forceinline__ void for_segment(const PagesTables& t, uint32_t segment, uint32_t before, uint32_t last, uint32_t* lds, F f) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, each = t.segment / group_waves();
   const uint32_t from = segment * t.segment + wave * each, end = min((segment + 1) * t.segment, t.pages), to = min(from + each, end);
   uint32_t n = 0;
-  for (uint32_t p = from; p < to; p += 64) n += __popcll(__ballot(p + lane < to && (t.references[p + lane] > 0) == USED));
+  for (uint32_t p = from + lane; p < to; p += 64) n += (references_of<PAST_CACHE>(t, p) > 0) == USED;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
   __syncthreads();
   if (lane == 0) lds[wave] = n;
   __syncthreads();
   uint32_t rank = before;
   for (uint32_t w = 0; w < wave; ++w) rank += lds[w];
-  for (uint32_t p = from; p < to; p += 64) {
-    const bool inside = p + lane < to, counted = inside && (t.references[p + lane] > 0) == USED;
+  for (uint32_t p = from; p < to && rank < last; p += 64) {
+    const bool inside = p + lane < to, counted = inside && (references_of<PAST_CACHE>(t, p + lane) > 0) == USED;
     const uint64_t mask = __ballot(counted);
     f(inside ? p + lane : t.pages, counted, rank + lanes_below(mask));
     rank += __popcll(mask);
@@ -94,32 +131,29 @@ __device__ __forceinline__ void for_segment(const PagesTables& t, uint32_t segme
 // lengths before the call.
 struct ReservePlan {
   uint32_t *words, *start, *tokens, *first, *length;
-  __device__ explicit ReservePlan(const PagesTables& t)
-      : words(t.plan), start(t.plan + 8), tokens(start + t.sequences), first(tokens + t.sequences), length(first + t.sequences) {}
+  __device__ explicit ReservePlan(const PagesTables& t) : ReservePlan(t.plan, t.sequences) {}
+  __device__ ReservePlan(uint32_t* at, uint32_t rows)
+      : words(at), start(at + 8), tokens(start + rows), first(tokens + rows), length(first + rows) {}
 };
 
-__global__ __launch_bounds__(kThreads) void pages_reserve_plan(PagesReserveArgs a) {
-  __shared__ uint32_t lds[4];
-  __shared__ uint64_t wide[4];
+// The plan, by a workgroup or by one wave (whose sums take no barrier).
+template <bool WAVE>
+__device__ __forceinline__ void reserve_plan(const PagesReserveArgs& a, const ReservePlan& plan, uint32_t* lds, uint64_t* wide) {
   const PagesTables& t = a.t;
-  if (blockIdx.x < t.segments) {
-    count_segment<false>(t, blockIdx.x, lds);
-    return;
-  }
-  const ReservePlan plan(t);
+  const uint32_t width = WAVE ? 64 : blockDim.x, me = WAVE ? threadIdx.x & 63 : threadIdx.x;
   uint64_t tokens = 0;
   uint32_t pages = 0;
-  for (uint32_t base = 0; base < t.sequences; base += kThreads) {
-    const uint32_t b = base + threadIdx.x;
+  for (uint32_t base = 0; base < t.sequences; base += width) {
+    const uint32_t b = base + me;
     const bool row = b < t.sequences;
     const uint32_t asked = row ? (uint32_t)max(a.new_tokens[b], 0) : 0, length = row ? length_of(t, t.lengths[b]) : 0;
     uint64_t all;
-    const uint64_t at = tokens + group_before<uint64_t>(asked, wide, &all);
+    const uint64_t at = tokens + (WAVE ? wave_before<uint64_t>(asked, &all) : group_before<uint64_t>(asked, wide, &all));
     tokens += all;
     const uint32_t start = (uint32_t)min(at, (uint64_t)a.capacity), n = min(asked, a.capacity - start);
     const uint32_t need = pages_of(length + min(n, t.most_tokens - length), t.page_size) - pages_of(length, t.page_size);
     uint32_t sum;
-    const uint32_t first = pages + group_before<uint32_t>(need, lds, &sum);
+    const uint32_t first = pages + (WAVE ? wave_before<uint32_t>(need, &sum) : group_before<uint32_t>(need, lds, &sum));
     pages += sum;
     if (row) {
       plan.start[b] = start;
@@ -128,65 +162,66 @@ __global__ __launch_bounds__(kThreads) void pages_reserve_plan(PagesReserveArgs 
       plan.length[b] = length;
     }
   }
-  if (threadIdx.x == 0) {
+  if (me == 0) {
     plan.words[0] = (uint32_t)min(tokens, (uint64_t)a.capacity);
     plan.words[1] = pages;
   }
 }
+// A row's tokens end where the free pages do.
+__device__ __forceinline__ uint32_t reserve_end(const PagesTables& t, const ReservePlan& plan, uint32_t b, uint32_t free) {
+  const uint32_t page = t.page_size, length = plan.length[b], fits = min(plan.tokens[b], t.most_tokens - length);
+  const uint32_t held = pages_of(length, page), need = pages_of(length + fits, page) - held, at = plan.first[b];
+  const uint32_t got = min(need, free - min(free, at));
+  return got == need ? length + fits : min(length + fits, (held + got) * page);
+}
 
-__global__ __launch_bounds__(kThreads) void pages_reserve_place(PagesReserveArgs a) {
-  __shared__ uint32_t lds[4];
-  __shared__ uint32_t first[kMostSequences];
+// A page that is handed out: its first token's place in the call, its tokens, its number, its first token's position.
+struct Handed {
+  uint32_t from, tokens, page, position;
+};
+
+// Gives a wave's free ones of 64 pages to the rows that need them, and writes their tokens. `first` is the plan's, in LDS.
+__device__ __forceinline__ void reserve_pages(const PagesReserveArgs& a, const ReservePlan& plan, const uint32_t* first, Handed* handed,
+                                              uint32_t p, bool is_free, uint32_t rank, uint32_t needed, uint32_t free) {
   const PagesTables& t = a.t;
-  const ReservePlan plan(t);
-  const uint32_t lane = threadIdx.x & 63, page = t.page_size, needed = plan.words[1];
-  const bool rows = blockIdx.x >= t.segments;
-  uint32_t free;
-  const uint32_t before = counted_before(t, rows ? 0 : blockIdx.x, lds, &free);
-  // a row's tokens end where the free pages do
-  auto after = [&](uint32_t b) {
-    const uint32_t length = plan.length[b], fits = min(plan.tokens[b], t.most_tokens - length);
-    const uint32_t held = pages_of(length, page), need = pages_of(length + fits, page) - held, at = plan.first[b];
-    const uint32_t got = min(need, free - min(free, at));
-    return got == need ? length + fits : min(length + fits, (held + got) * page);
-  };
-  if (!rows) {
-    if (before >= needed) return;
-    for (uint32_t b = threadIdx.x; b < t.sequences; b += kThreads) first[b] = plan.first[b];
-    __syncthreads();
-    for_segment<false>(t, blockIdx.x, before, lds, [&](uint32_t p, bool is_free, uint32_t rank) {
-      const bool given = is_free && rank < needed;
-      uint32_t at = 0, from = 0, n = 0;   // the page's place in its row, its first token's in the call, its tokens
-      if (given) {
-        uint32_t lo = 0, hi = t.sequences;   // the last row whose pages begin at this rank or before it
-        while (hi - lo > 1) {
-          const uint32_t mid = (lo + hi) / 2;
-          (first[mid] <= rank ? lo : hi) = mid;
-        }
-        const uint32_t length = plan.length[lo], end = after(lo);
-        at = pages_of(length, page) + rank - first[lo];
-        from = plan.start[lo] + at * page - length;   // (a new page begins at the length or behind it)
-        n = min(page, end - min(end, at * page));
-        t.tables[(uint64_t)lo * t.width + at] = (int32_t)p;
-        t.references[p] = 1;
-      }
-      // the tokens, page by page
-      for (uint64_t todo = __ballot(given); todo; todo &= todo - 1) {
-        const int who = __ffsll((unsigned long long)todo) - 1;
-        const uint32_t number = __builtin_amdgcn_readlane(p, who), first_token = __builtin_amdgcn_readlane(from, who);
-        const uint32_t pos = __builtin_amdgcn_readlane(at, who) * page, tokens = __builtin_amdgcn_readlane(n, who);
-        for (uint32_t i = lane; i < tokens; i += 64) {
-          a.slots[first_token + i] = (int64_t)((uint64_t)number * page + i);
-          if (a.positions) a.positions[first_token + i] = pos + i;
-        }
-      }
-    });
-    return;
+  const uint32_t lane = threadIdx.x & 63, page = t.page_size;
+  const bool given = is_free && rank < needed;
+  const uint64_t mask = __ballot(given);
+  if (given) {
+    uint32_t lo = 0, hi = t.sequences;   // the last row whose pages begin at this rank or before it
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      (first[mid] <= rank ? lo : hi) = mid;
+    }
+    const uint32_t length = plan.length[lo], end = reserve_end(t, plan, lo, free);
+    const uint32_t at = pages_of(length, page) + rank - first[lo], pos = at * page, tokens = min(page, end - min(end, pos));
+    t.tables[(uint64_t)lo * t.width + at] = (int32_t)p;
+    t.references[p] = 1;
+    // (a new page begins at the length or behind it)
+    handed[lanes_below(mask)] = Handed{plan.start[lo] + pos - length, tokens, p, pos};
   }
-  const uint32_t waves = (gridDim.x - t.segments) * 4, wave = (blockIdx.x - t.segments) * 4 + (threadIdx.x >> 6);
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  // the pages' tokens, 64 at a time whatever the page's size
+  const uint64_t all = (uint64_t)__popcll(mask) * page;
+  for (uint64_t i = lane; i < all; i += 64) {
+    const uint32_t k = (uint32_t)(i / page), at = (uint32_t)(i - (uint64_t)k * page);
+    const Handed h = handed[k];
+    if (at >= h.tokens) continue;
+    a.slots[h.from + at] = (int64_t)((uint64_t)h.page * page + at);
+    if (a.positions) a.positions[h.from + at] = h.position + at;
+  }
+  __builtin_amdgcn_wave_barrier();
+}
+
+// The rows' tokens in pages that they held before, those without a page, the entries behind the last token, the lengths.
+__device__ __forceinline__ void reserve_rows(const PagesReserveArgs& a, const ReservePlan& plan, uint32_t free, uint32_t wave,
+                                             uint32_t waves) {
+  const PagesTables& t = a.t;
+  const uint32_t lane = threadIdx.x & 63, page = t.page_size, needed = plan.words[1];
   for (uint32_t b = wave; b < t.sequences; b += waves) {
-    const uint32_t length = plan.length[b], start = plan.start[b], n = plan.tokens[b], end = after(b);
-    // tokens that the last page held before still takes, and tokens without a page
+    const uint32_t length = plan.length[b], start = plan.start[b], n = plan.tokens[b], end = reserve_end(t, plan, b, free);
     const uint32_t full = min(end, pages_of(length, page) * page);
     for (uint32_t i = lane; i < full - length; i += 64) {
       const uint32_t pos = length + i;
@@ -205,6 +240,68 @@ __global__ __launch_bounds__(kThreads) void pages_reserve_place(PagesReserveArgs
     if (a.positions) a.positions[i] = -1;
   }
   if (wave == 0 && lane == 0 && t.missing) *t.missing = (int32_t)(needed - min(needed, free));
+}
+
+__global__ __launch_bounds__(kThreads) void pages_reserve_plan(PagesReserveArgs a) {
+  __shared__ uint32_t lds[kMostWaves];
+  __shared__ uint64_t wide[kMostWaves];
+  if (blockIdx.x < a.t.segments)
+    count_segment<false>(a.t, blockIdx.x, lds);
+  else
+    reserve_plan<false>(a, ReservePlan(a.t), lds, wide);
+}
+
+__global__ __launch_bounds__(kThreads) void pages_reserve_place(PagesReserveArgs a) {
+  __shared__ uint32_t lds[kMostWaves];
+  __shared__ uint32_t first[kMostSequences];
+  __shared__ Handed handed[kThreads / 64][64];
+  const PagesTables& t = a.t;
+  const ReservePlan plan(t);
+  const bool rows = blockIdx.x >= t.segments;
+  uint32_t free;
+  const uint32_t before = counted_before(t, rows ? 0 : blockIdx.x, lds, &free), needed = plan.words[1];
+  if (rows) {
+    reserve_rows(a, plan, free, (blockIdx.x - t.segments) * 4 + (threadIdx.x >> 6), (gridDim.x - t.segments) * 4);
+  } else if (before < needed) {
+    for (uint32_t b = threadIdx.x; b < t.sequences; b += blockDim.x) first[b] = plan.first[b];
+    __syncthreads();
+    for_segment<false>(t, blockIdx.x, before, needed, lds, [&](uint32_t p, bool is_free, uint32_t rank) {
+      reserve_pages(a, plan, first, handed[threadIdx.x >> 6], p, is_free, rank, needed, free);
+    });
+  }
+}
+
+// All of it by one workgroup: a wave holds which of its 256 pages are free while the first wave makes the plan, in LDS.
+__global__ __launch_bounds__(kOneThreads) void pages_reserve_one(PagesReserveArgs a) {
+  constexpr uint32_t kTurns = kReserveOnePages / kOneThreads;
+  __shared__ uint32_t counts[kMostWaves], room[8 + 4 * kReserveOneRows];
+  __shared__ Handed handed[kMostWaves][64];
+  const PagesTables& t = a.t;
+  const ReservePlan plan(room, t.sequences);
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, from = wave * (64 * kTurns) + lane;
+  bool is_free[kTurns];
+  uint32_t found = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < kTurns; ++i) is_free[i] = from + i * 64 < t.pages && t.references[from + i * 64] <= 0;
+#pragma unroll
+  for (uint32_t i = 0; i < kTurns; ++i) found += __popcll(__ballot(is_free[i]));
+  if (lane == 0) counts[wave] = found;
+  if (wave == 0) reserve_plan<true>(a, plan, nullptr, nullptr);
+  __syncthreads();
+  uint32_t free = 0, rank = 0;
+  for (uint32_t w = 0; w < kMostWaves; ++w) {
+    free += counts[w];
+    rank += w < wave ? counts[w] : 0;
+  }
+  reserve_rows(a, plan, free, wave, kMostWaves);
+  const uint32_t needed = plan.words[1];
+#pragma unroll
+  for (uint32_t i = 0; i < kTurns; ++i) {
+    const uint64_t mask = __ballot(is_free[i]);
+    if (rank < needed)
+      reserve_pages(a, plan, plan.first, handed[wave], from + i * 64, is_free[i], rank + lanes_below(mask), needed, free);
+    rank += __popcll(mask);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ trim
@@ -232,11 +329,10 @@ struct ForkPlan {
 };
 
 // Counts of references as they will be, by one wave for each row.
-__global__ __launch_bounds__(kThreads) void pages_fork_rows(PagesForkArgs a) {
+__device__ __forceinline__ void fork_row(const PagesForkArgs& a, uint32_t b) {
   const PagesTables& t = a.t;
   const ForkPlan plan(t);
-  const uint32_t lane = threadIdx.x & 63, b = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (b >= t.sequences) return;
+  const uint32_t lane = threadIdx.x & 63;
   const uint32_t length = length_of(t, t.lengths[b]), parent = (uint32_t)a.parents[b];
   const int32_t* const row = t.tables + (uint64_t)b * t.width;
   const bool changed = parent != b;
@@ -264,16 +360,12 @@ __global__ __launch_bounds__(kThreads) void pages_fork_rows(PagesForkArgs a) {
   }
 }
 
-__global__ __launch_bounds__(kThreads) void pages_fork_plan(PagesForkArgs a) {
-  __shared__ uint32_t lds[4];
+// Numbers the rows that need a copy.
+__device__ __forceinline__ void fork_plan(const PagesForkArgs& a, uint32_t* lds) {
   const PagesTables& t = a.t;
-  if (blockIdx.x < t.segments) {
-    count_segment<false>(t, blockIdx.x, lds);
-    return;
-  }
   const ForkPlan plan(t);
   uint32_t copies = 0;
-  for (uint32_t base = 0; base < t.sequences; base += kThreads) {
+  for (uint32_t base = 0; base < t.sequences; base += blockDim.x) {
     const uint32_t b = base + threadIdx.x;
     const bool copy = b < t.sequences && plan.rank[b] != kNone;
     uint32_t all;
@@ -289,31 +381,31 @@ __global__ __launch_bounds__(kThreads) void pages_fork_plan(PagesForkArgs a) {
   if (threadIdx.x == 0) plan.words[0] = copies;
 }
 
-__global__ __launch_bounds__(kThreads) void pages_fork_place(PagesForkArgs a) {
-  __shared__ uint32_t lds[4];
+// Gives a segment's free pages to the rows that need a copy.
+template <bool PAST_CACHE>
+__device__ __forceinline__ void fork_segment(const PagesForkArgs& a, uint32_t segment, uint32_t before, uint32_t* lds) {
   const PagesTables& t = a.t;
   const ForkPlan plan(t);
-  const bool rows = blockIdx.x >= t.segments;
   const uint32_t copies = plan.words[0];
-  uint32_t free;
-  const uint32_t before = counted_before(t, rows ? 0 : blockIdx.x, lds, &free);
-  if (!rows) {
-    if (before >= copies) return;
-    for_segment<false>(t, blockIdx.x, before, lds, [&](uint32_t p, bool is_free, uint32_t rank) {
-      if (!is_free || rank >= copies) return;
-      const uint32_t b = plan.target[rank], whole = plan.length[(uint32_t)a.parents[b]] / t.page_size;
-      t.tables[(uint64_t)b * t.width + whole] = (int32_t)p;
-      t.references[p] = 1;
-      plan.target[rank] = p;
-    });
-    return;
-  }
-  const uint32_t lane = threadIdx.x & 63, b = (blockIdx.x - t.segments) * 4 + (threadIdx.x >> 6);
+  if (before >= copies) return;
+  for_segment<false, PAST_CACHE>(t, segment, before, copies, lds, [&](uint32_t p, bool is_free, uint32_t rank) {
+    if (!is_free || rank >= copies) return;
+    const uint32_t b = plan.target[rank], whole = plan.length[(uint32_t)a.parents[b]] / t.page_size;
+    t.tables[(uint64_t)b * t.width + whole] = (int32_t)p;
+    t.references[p] = 1;
+    plan.target[rank] = p;
+  });
+}
+
+// A changed row's entries and length, by one wave.
+__device__ __forceinline__ void fork_entries(const PagesForkArgs& a, uint32_t b, uint32_t free) {
+  const PagesTables& t = a.t;
+  const ForkPlan plan(t);
+  const uint32_t lane = threadIdx.x & 63, copies = plan.words[0];
   if (b == 0 && lane == 0) {
     plan.words[1] = min(copies, free);
     if (t.missing) *t.missing = (int32_t)(copies - min(copies, free));
   }
-  if (b >= t.sequences) return;
   const uint32_t parent = (uint32_t)a.parents[b], rank = plan.rank[b];
   if (parent == b) return;
   uint32_t end = 0;
@@ -326,6 +418,45 @@ __global__ __launch_bounds__(kThreads) void pages_fork_place(PagesForkArgs a) {
   if (lane == 0) t.lengths[b] = (int32_t)end;
 }
 
+__global__ __launch_bounds__(kThreads) void pages_fork_rows(PagesForkArgs a) {
+  const uint32_t b = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (b < a.t.sequences) fork_row(a, b);
+}
+
+__global__ __launch_bounds__(kThreads) void pages_fork_plan(PagesForkArgs a) {
+  __shared__ uint32_t lds[kMostWaves];
+  if (blockIdx.x < a.t.segments)
+    count_segment<false>(a.t, blockIdx.x, lds);
+  else
+    fork_plan(a, lds);
+}
+
+__global__ __launch_bounds__(kThreads) void pages_fork_place(PagesForkArgs a) {
+  __shared__ uint32_t lds[kMostWaves];
+  const bool rows = blockIdx.x >= a.t.segments;
+  uint32_t free;
+  const uint32_t before = counted_before(a.t, rows ? 0 : blockIdx.x, lds, &free);
+  if (!rows) {
+    fork_segment<false>(a, blockIdx.x, before, lds);
+    return;
+  }
+  const uint32_t b = (blockIdx.x - a.t.segments) * 4 + (threadIdx.x >> 6);
+  if (b < a.t.sequences) fork_entries(a, b, free);
+}
+
+// All of it by one workgroup (the pool is one segment).
+__global__ __launch_bounds__(kOneThreads) void pages_fork_one(PagesForkArgs a) {
+  __shared__ uint32_t lds[kMostWaves];
+  for (uint32_t b = threadIdx.x >> 6; b < a.t.sequences; b += kMostWaves) fork_row(a, b);
+  __syncthreads();
+  count_segment<false, true>(a.t, 0, lds);
+  fork_plan(a, lds);
+  __syncthreads();
+  const uint32_t free = a.t.counts[0];
+  for (uint32_t b = threadIdx.x >> 6; b < a.t.sequences; b += kMostWaves) fork_entries(a, b, free);
+  fork_segment<true>(a, 0, 0, lds);
+}
+
 // ------------------------------------------------------------------------------------------------ compact
 // U pages are in use. Those at U and above (movers) go to the free ones below U (holes), as many, the k-th to the k-th. plan: [0] U,
 // [1] movers; room: the holes, the movers counted from the last, and for each page at U or above its number among these (kNone: free).
@@ -335,18 +466,12 @@ struct CompactPlan {
       : words(t.plan), holes(t.room), movers(t.room + t.pages), number(t.room + 2ull * t.pages) {}
 };
 
-__global__ __launch_bounds__(kThreads) void pages_compact_count(PagesCompactArgs a) {
-  __shared__ uint32_t lds[4];
-  count_segment<true>(a.t, blockIdx.x, lds);
-}
-
-__global__ __launch_bounds__(kThreads) void pages_compact_list(PagesCompactArgs a) {
-  __shared__ uint32_t lds[4];
+__device__ __forceinline__ void compact_segment(const PagesCompactArgs& a, uint32_t segment, uint32_t* lds) {
   const PagesTables& t = a.t;
   const CompactPlan plan(t);
   uint32_t used;
-  const uint32_t before = counted_before(t, blockIdx.x, lds, &used);
-  for_segment<true>(t, blockIdx.x, before, lds, [&](uint32_t p, bool in_use, uint32_t rank) {
+  const uint32_t before = counted_before(t, segment, lds, &used);
+  for_segment<true>(t, segment, before, kNone, lds, [&](uint32_t p, bool in_use, uint32_t rank) {
     if (p >= t.pages) return;
     if (p == used) plan.words[1] = used - rank;   // as many lie at U and above as are missing below
     if (p < used) {
@@ -357,7 +482,7 @@ __global__ __launch_bounds__(kThreads) void pages_compact_list(PagesCompactArgs 
     }
     if (a.mapping && !(in_use && p >= used)) a.mapping[p] = in_use ? (int32_t)p : -1;
   });
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
+  if (segment == 0 && threadIdx.x == 0) {
     plan.words[0] = used;
     if (used == t.pages) plan.words[1] = 0;
     if (a.used) *a.used = (int32_t)used;
@@ -365,11 +490,10 @@ __global__ __launch_bounds__(kThreads) void pages_compact_list(PagesCompactArgs 
 }
 
 // The tables' entries, and the references and mapping of the pages that move.
-__global__ __launch_bounds__(kThreads) void pages_compact_tables(PagesCompactArgs a) {
+__device__ __forceinline__ void compact_tables(const PagesCompactArgs& a, uint32_t at, uint32_t all) {
   const PagesTables& t = a.t;
   const CompactPlan plan(t);
   const uint32_t used = plan.words[0], moves = plan.words[1];
-  const uint32_t all = gridDim.x * kThreads, at = blockIdx.x * kThreads + threadIdx.x;
   for (uint32_t i = at; i < moves; i += all) {
     const uint32_t from = plan.movers[moves - 1 - i], to = plan.holes[i];
     t.references[to] = t.references[from];
@@ -386,6 +510,28 @@ __global__ __launch_bounds__(kThreads) void pages_compact_tables(PagesCompactArg
       if (number != kNone) *entry = (int32_t)plan.holes[moves - 1 - number];
     }
   }
+}
+
+__global__ __launch_bounds__(kThreads) void pages_compact_count(PagesCompactArgs a) {
+  __shared__ uint32_t lds[kMostWaves];
+  count_segment<true>(a.t, blockIdx.x, lds);
+}
+__global__ __launch_bounds__(kThreads) void pages_compact_list(PagesCompactArgs a) {
+  __shared__ uint32_t lds[kMostWaves];
+  compact_segment(a, blockIdx.x, lds);
+}
+__global__ __launch_bounds__(kThreads) void pages_compact_tables(PagesCompactArgs a) {
+  compact_tables(a, blockIdx.x * kThreads + threadIdx.x, gridDim.x * kThreads);
+}
+
+// All of it by one workgroup (the pool is one segment).
+__global__ __launch_bounds__(kOneThreads) void pages_compact_one(PagesCompactArgs a) {
+  __shared__ uint32_t lds[kMostWaves];
+  count_segment<true>(a.t, 0, lds);
+  __syncthreads();
+  compact_segment(a, 0, lds);
+  __syncthreads();
+  compact_tables(a, threadIdx.x, kOneThreads);
 }
 
 // ------------------------------------------------------------------------------------------------ copies
@@ -437,7 +583,17 @@ __global__ __launch_bounds__(kThreads) void pages_copy(PagesCopyArgs a) {
 
 }  // namespace
 
+// The pool as one segment, for one workgroup.
+static void as_one_segment(PagesTables& t) {
+  t.segment = (t.pages + kOneThreads - 1) / kOneThreads * kOneThreads;
+  t.segments = 1;
+}
+
 hipError_t launch_pages_reserve(const PagesReserveArgs& a, hipStream_t s) {
+  if (a.t.pages <= kReserveOnePages && a.t.sequences <= kReserveOneRows && a.capacity <= kReserveOneTokens) {
+    pages_reserve_one<<<dim3(1), dim3(kOneThreads), 0, s>>>(a);
+    return hipGetLastError();
+  }
   pages_reserve_plan<<<dim3(a.t.segments + 1), dim3(kThreads), 0, s>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
@@ -450,8 +606,20 @@ hipError_t launch_pages_trim(const PagesTrimArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-hipError_t launch_pages_fork(const PagesForkArgs& a, PagesCopyArgs* copies, hipStream_t s) {
+hipError_t launch_pages_fork(const PagesForkArgs& call, PagesCopyArgs* copies, hipStream_t s) {
+  PagesForkArgs a = call;
   const uint32_t rows = (a.t.sequences + 3) / 4;
+  copies->count = a.t.plan + 1;
+  copies->source = a.t.plan + 8 + 2ull * a.t.sequences;
+  copies->target = copies->source + a.t.sequences;
+  copies->tokens = copies->target + a.t.sequences;
+  copies->backwards = 0;
+  copies->most = a.t.sequences;
+  if (a.t.pages <= kForkOnePages && a.t.sequences <= kForkOneRows) {
+    as_one_segment(a.t);
+    pages_fork_one<<<dim3(1), dim3(kOneThreads), 0, s>>>(a);
+    return hipGetLastError();
+  }
   pages_fork_rows<<<dim3(rows), dim3(kThreads), 0, s>>>(a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
@@ -459,16 +627,22 @@ hipError_t launch_pages_fork(const PagesForkArgs& a, PagesCopyArgs* copies, hipS
   e = hipGetLastError();
   if (e != hipSuccess) return e;
   pages_fork_place<<<dim3(a.t.segments + rows), dim3(kThreads), 0, s>>>(a);
-  copies->count = a.t.plan + 1;
-  copies->source = a.t.plan + 8 + 2ull * a.t.sequences;
-  copies->target = copies->source + a.t.sequences;
-  copies->tokens = copies->target + a.t.sequences;
-  copies->backwards = 0;
-  copies->most = a.t.sequences;
   return hipGetLastError();
 }
 
-hipError_t launch_pages_compact(const PagesCompactArgs& a, PagesCopyArgs* copies, hipStream_t s) {
+hipError_t launch_pages_compact(const PagesCompactArgs& call, PagesCopyArgs* copies, hipStream_t s) {
+  PagesCompactArgs a = call;
+  copies->count = a.t.plan + 1;
+  copies->target = a.t.room;
+  copies->source = a.t.room + a.t.pages;
+  copies->tokens = nullptr;
+  copies->backwards = 1;
+  copies->most = a.t.pages / 2;
+  if (a.t.pages <= kCompactOnePages && a.t.sequences <= kCompactOneRows) {
+    as_one_segment(a.t);
+    pages_compact_one<<<dim3(1), dim3(kOneThreads), 0, s>>>(a);
+    return hipGetLastError();
+  }
   pages_compact_count<<<dim3(a.t.segments), dim3(kThreads), 0, s>>>(a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
@@ -476,12 +650,6 @@ hipError_t launch_pages_compact(const PagesCompactArgs& a, PagesCopyArgs* copies
   e = hipGetLastError();
   if (e != hipSuccess) return e;
   pages_compact_tables<<<dim3((a.t.sequences + 3) / 4), dim3(kThreads), 0, s>>>(a);
-  copies->count = a.t.plan + 1;
-  copies->target = a.t.room;
-  copies->source = a.t.room + a.t.pages;
-  copies->tokens = nullptr;
-  copies->backwards = 1;
-  copies->most = a.t.pages / 2;
   return hipGetLastError();
 }
 
