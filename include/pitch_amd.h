@@ -495,7 +495,7 @@ typedef struct pitch_prompt_attention {
   uint32_t window;    /* tokens, below 2^31; 0: all. Needs causal, as slopes do */
   uint32_t reserved;  /* 0 */
   uint64_t rows;      /* tokens of queries and output, at least 1; rows * q_heads < 2^31 */
-  uint64_t key_rows;  /* tokens of keys and values, at least 1, below 2^31 */
+  uint64_t key_rows;  /* tokens of keys and values: 1..2^31 - 1025 */
   /* data and strides are multiples of 16 bytes; the token strides of keys and values are at most 2^22 elements. The output may be
    * the queries' own vectors, and else shares no element with what the call reads */
   pitch_paged_vectors_t queries, keys, values, output;
@@ -512,8 +512,8 @@ typedef struct pitch_prompt_attention {
   void* workspace; /* pitch_prompt_attention_workspace_size bytes (null for none); not used by another call until this one has completed */
   uint64_t workspace_bytes;
 } pitch_prompt_attention_t;
-/* Bytes of device workspace pitch_enqueue_prompt_attention needs on the current device (0 where no keys are split) for these
- * dim, sequences, heads, rows and key_rows. */
+/* Bytes of device workspace pitch_enqueue_prompt_attention needs on the current device (0 for many or short sequences) for these
+ * dim, sequences, heads, rows, key_rows and window. */
 int pitch_prompt_attention_workspace_size(const pitch_prompt_attention_t* call, uint64_t* bytes);
 int pitch_enqueue_prompt_attention(const pitch_prompt_attention_t* call, void* stream);
 

@@ -1659,14 +1659,15 @@ int validate_prompt(const pitch_prompt_attention_t* c) {
     return fail(PITCH_ERR_INVALID_INPUT, "query heads %u must be a multiple of KV heads %u", c->q_heads, c->kv_heads);
   if (c->rows < 1 || c->rows > 0x7FFFFFFFull / c->q_heads)
     return fail(PITCH_ERR_INVALID_INPUT, "rows times query heads must be in 1...2^31 - 1");
-  if (c->key_rows < 1 || c->key_rows > 0x7FFFFFFFull - 64) return fail(PITCH_ERR_INVALID_INPUT, "key rows must be in 1...2^31 - 65");
+  if (c->key_rows < 1 || c->key_rows > 0x7FFFFFFFull - 1024)
+    return fail(PITCH_ERR_INVALID_INPUT, "key rows must be in 1...2^31 - 1025");
   if (c->sequences < 1 || (c->rows * (c->q_heads / c->kv_heads) / pitch::kPromptRows + c->sequences) * c->kv_heads >= 1u << 24)
     return fail(PITCH_ERR_INVALID_INPUT, "sequences must be at least 1, and the tiles of all KV heads fewer than 2^24");
   return PITCH_OK;
 }
 
 pitch::PromptPlan plan_of(const pitch_prompt_attention_t* c) {
-  return pitch::prompt_plan((uint32_t)c->rows, (uint32_t)c->key_rows, c->sequences, c->kv_heads, c->q_heads / c->kv_heads, c->dim,
+  return pitch::prompt_plan((uint32_t)c->rows, (uint32_t)c->key_rows, c->window, c->sequences, c->kv_heads, c->q_heads / c->kv_heads, c->dim,
                             (uint32_t)pitch::device_cu_count());
 }
 
@@ -1772,7 +1773,8 @@ int pitch_enqueue_prompt_attention(const pitch_prompt_attention_t* call, void* s
   a.causal = call->causal;
   a.window = call->window;
   a.tiles = plan.tiles;
-  a.splits = plan.splits;
+  a.runs = plan.runs;
+  a.parts_at = plan.parts_at;
   // scores in log2 units; hidden scores are minus infinity, which a factor of zero would make NaN
   constexpr double kLog2E = 1.4426950408889634, kMost = std::numeric_limits<float>::max();
   const double to_log2 = std::max(-kMost, std::min(kMost, (double)call->scale * kLog2E));
@@ -1781,7 +1783,8 @@ int pitch_enqueue_prompt_attention(const pitch_prompt_attention_t* call, void* s
     a.pre = (float)to_log2;
     a.c = 1.f;
     a.cap = (float)std::min(cap, kMost);
-    a.cap_r = call->softcap > 0.f ? (float)std::min(2.0 * kLog2E / cap, kMost) : 0.f;   // e^(2 x / cap) as a power of two
+    const double cap_r = call->softcap > 0.f ? 2.0 * kLog2E * call->scale / call->softcap : 0.0;   // e^(2 scale x / softcap) as a power of two
+    a.cap_r = (float)std::max(-kMost, std::min(kMost, cap_r));
   } else {
     a.negate = call->scale < 0.f;
     a.c = (float)std::max(std::abs(to_log2), 1e-37);

@@ -14,39 +14,38 @@ struct PromptArgs {
   const int32_t* key_starts;  // [sequences + 1]: keys of each sequence
   const float* slopes;        // [query heads] or null
   float* lse;                 // [rows][query heads] or null
-  float* ws;                  // partial results of a call whose keys are split
+  float* ws;                  // with runs: the line of tiles (kPromptLineHead floats and 4 per tile and one more), parts from parts_at on
   uint32_t rows, keys;        // tokens that the queries' and the keys' buffers hold
   uint32_t sequences, kv_heads, nq;
   uint32_t causal, window;    // window 0: all
   uint32_t negate;            // 1: a negative scale, whose sign the queries take
   float c;                    // |scale| log2(e): scores to log2 units (1 with a cap or slopes, which give such units)
   float pre;                  // with a cap or slopes: what a product is multiplied by first
-  float cap, cap_r;           // scores x are cap * tanh(x * cap_r) when cap is positive (log2 units), else x
-  uint32_t tiles;             // an upper bound of the query tiles of a KV head (set by the launcher, as splits)
-  uint32_t splits;            // parts of a tile's keys
+  float cap, cap_r;           // with a positive cap, products x give cap * tanh(x'), e^(2 x') = 2^(x * cap_r), in log2 units
+  uint32_t tiles;             // an upper bound of the query tiles of a KV head
+  uint32_t runs;              // workgroups of a KV head that the line of tiles is cut for; 0: every workgroup takes a query tile
+  uint64_t parts_at;
 };
 
-// Rows of (token, query head of a KV head) in a tile; tiles and parts of the keys; floats of workspace.
-constexpr uint32_t kPromptRows = 128;
+// Rows of (token, query head of a KV head) in a query tile; the most sequences of a call whose line of tiles is laid out, and the
+// keys from which that is done; tiles of keys that a cut costs a run; floats before the line's tiles.
+constexpr uint32_t kPromptRows = 128, kPromptLineSequences = 1024, kPromptLineKeys = 2048, kPromptCut = 12, kPromptLineHead = 8;
 struct PromptPlan {
-  uint32_t tiles, splits;
-  uint64_t ws_floats;
+  uint32_t tiles, runs;
+  uint64_t parts_at, ws_floats;
 };
-inline PromptPlan prompt_plan(uint32_t rows, uint32_t keys, uint32_t sequences, uint32_t kv_heads, uint32_t nq, uint32_t dim,
-                              uint32_t cus) {
+// What the host decides: with query tiles enough for four turns of every workgroup place (two on a compute unit), each takes one; else,
+// where tiles may be long, the line of tiles is laid out, and its lengths decide on the device.
+inline PromptPlan prompt_plan(uint32_t rows, uint32_t keys, uint32_t window, uint32_t sequences, uint32_t kv_heads, uint32_t nq,
+                              uint32_t dim, uint32_t cus) {
   PromptPlan p{};
   p.tiles = (uint32_t)((uint64_t)rows * nq / kPromptRows) + (sequences < rows ? sequences : rows);
-  const uint64_t groups = (uint64_t)p.tiles * kv_heads, slots = 2ull * cus;
-  uint64_t splits = 1;
-  if (groups < slots) {
-    // parts of 256 keys or more, of a sequence of twice the average length
-    const uint64_t most = 2ull * keys / sequences / 256;
-    splits = (4 * slots + groups - 1) / groups;
-    splits = splits < most ? splits : most;
-    splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
-  }
-  p.splits = (uint32_t)splits;
-  if (splits > 1) p.ws_floats = splits * rows * kv_heads * nq * (dim + 2ull);
+  const uint32_t places = 2 * cus, seen = window && window < keys ? window : keys;
+  if (sequences > kPromptLineSequences || (uint64_t)p.tiles * kv_heads >= 4ull * places || seen < kPromptLineKeys || places / kv_heads < 2)
+    return p;
+  p.runs = places / kv_heads;
+  p.parts_at = kPromptLineHead + (p.tiles + 1ull) * 4;
+  p.ws_floats = p.parts_at + (uint64_t)p.runs * kv_heads * 2 * kPromptRows * (dim + 2);
   return p;
 }
 

@@ -8,17 +8,13 @@
 #ifndef PITCH_IO
 #error "compile with -DPITCH_IO=<io type>"
 #endif
-#ifndef PITCH_PROMPT_NB
-#define PITCH_PROMPT_NB 1
-#endif
 
 namespace pitch {
 namespace {
 
 constexpr int D = PITCH_DIM;
-constexpr int kWaves = 4;
-constexpr int NB = PITCH_PROMPT_NB;  // blocks of 32 rows of a wave
-constexpr int kRows = kWaves * 32 * NB;
+constexpr int kWaves = 4;            // of a group, 32 rows each
+constexpr int kRows = kWaves * 32;  // rows of a tile of queries
 constexpr int kKeys = 64;            // keys of a tile
 constexpr int kSteps = D / 16;       // steps of the contraction over the coordinates
 constexpr int kBlocks = D / 32;      // blocks of 32 output coordinates
@@ -79,28 +75,35 @@ __device__ __forceinline__ void scale_where(uint64_t go, float f, v16f& x) {
   for (int r = 0; r < 16; ++r) x[r] = y[r];
 }
 
+// A sequence's queries and keys, within the buffers.
+struct Sequence {
+  uint32_t first_query, queries, first_key, keys, tiles;
+};
+__device__ __forceinline__ Sequence sequence(const PromptArgs& a, uint32_t b) {
+  Sequence s{};
+  if (b >= a.sequences) return s;
+  const int32_t q0 = a.row_starts[b], q1 = a.row_starts[b + 1], k0 = a.key_starts[b], k1 = a.key_starts[b + 1];
+  s.first_query = min((uint32_t)max(q0, 0), a.rows);
+  s.queries = max((int32_t)(min((uint32_t)max(q1, 0), a.rows) - s.first_query), 0);
+  s.first_key = min((uint32_t)max(k0, 0), a.keys);
+  s.keys = max((int32_t)(min((uint32_t)max(k1, 0), a.keys) - s.first_key), 0);
+  s.tiles = (s.queries * a.nq + kRows - 1) / kRows;
+  return s;
+}
+
 // A query tile: the rows [row, row + kRows) of (token, head) pairs of a sequence.
 struct Tile {
-  uint32_t first_query, queries;  // the sequence's
-  uint32_t first_key, keys;
+  Sequence s;
   uint32_t row;
   bool any;
 };
-
-// The sequence of tile number `at`, found by all of the waves alike; a sequence's last tile, whose rows see most, comes first.
+// Tile number `at` of all sequences, found by all of the waves alike; a sequence's last tile, whose rows see most, comes first.
 __device__ __forceinline__ Tile find_tile(const PromptArgs& a, uint32_t at) {
   const uint32_t lane = threadIdx.x & 63;
   Tile t{};
   for (uint32_t base = 0; base < a.sequences; base += 64) {
-    const uint32_t b = base + lane;
-    uint32_t n = 0, q0 = 0;
-    if (b < a.sequences) {
-      const int32_t lo = a.row_starts[b], hi = a.row_starts[b + 1];
-      q0 = min((uint32_t)max(lo, 0), a.rows);
-      n = max((int32_t)(min((uint32_t)max(hi, 0), a.rows) - q0), 0);
-    }
-    const uint32_t tiles = (n * a.nq + kRows - 1) / kRows;
-    uint32_t sum = tiles;
+    const Sequence s = sequence(a, base + lane);
+    uint32_t sum = s.tiles;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const uint32_t up = __shfl_up(sum, d);
@@ -109,18 +112,130 @@ __device__ __forceinline__ Tile find_tile(const PromptArgs& a, uint32_t at) {
     const uint32_t total = of_wave(__shfl(sum, 63));
     if (at < total) {
       const int who = __ffsll((unsigned long long)__ballot(sum > at)) - 1;
-      t.any = true;
-      t.first_query = of_wave(__shfl(q0, who));
-      t.queries = of_wave(__shfl(n, who));
+      t.s = Sequence{of_wave(__shfl(s.first_query, who)), of_wave(__shfl(s.queries, who)), of_wave(__shfl(s.first_key, who)),
+                     of_wave(__shfl(s.keys, who)), 0};
       t.row = (of_wave(__shfl(sum, who)) - 1 - at) * kRows;
-      const int32_t lo = a.key_starts[base + who], hi = a.key_starts[base + who + 1];
-      t.first_key = min((uint32_t)max(lo, 0), a.keys);
-      t.keys = max((int32_t)(min((uint32_t)max(hi, 0), a.keys) - t.first_key), 0);
+      t.any = true;
       return t;
     }
     at -= total;
   }
   return t;
+}
+
+// The first key that a query at position pos sees through a window (0: all). Written so that no window, however long, overflows.
+__device__ __forceinline__ int32_t window_start(int32_t pos, uint32_t window) {
+  return !window || pos < (int32_t)window ? 0 : pos - (int32_t)window + 1;
+}
+// The keys [lo, hi) of a tile, from its first row's first to its last row's last.
+struct Range {
+  int32_t lo, hi;
+};
+__device__ __forceinline__ Range keys_of(const PromptArgs& a, const Sequence& s, uint32_t row) {
+  const int32_t offset = (int32_t)s.keys - (int32_t)s.queries;   // a query's position in its sequence, less its number
+  const uint32_t last = min(row + kRows, s.queries * a.nq) - 1;
+  const int32_t pos0 = offset + (int32_t)(row / a.nq), pos1 = offset + (int32_t)(last / a.nq);
+  return Range{window_start(pos0, a.window), a.causal ? min(pos1 + 1, (int32_t)s.keys) : (int32_t)s.keys};
+}
+
+// ------------------------------------------------------------------------------------------------ the line of tiles
+// Where a KV head has few query tiles, or tiles of very different lengths, all of a KV head's tiles of keys form one line, which is cut into equal
+// runs, one per workgroup. A run that holds a query tile whole writes its output; of a tile that is cut, every run leaves its part
+// (maxima, sums, values) in the workspace, and prompt_join puts them together, in their order. A run has two such parts at most: of the
+// tile in which it begins and of the one in which it ends.
+struct LineTile {
+  uint64_t before;       // tiles of keys before this query tile's
+  uint32_t sequence, row;
+};
+struct Line {
+  uint64_t total, run;   // tiles of keys, of a run (0: a workgroup takes a whole query tile)
+  uint32_t tiles, runs;
+};
+__device__ __forceinline__ Line* line_of(const PromptArgs& a) { return (Line*)a.ws; }
+__device__ __forceinline__ LineTile* line_tiles(const PromptArgs& a) { return (LineTile*)(a.ws + kPromptLineHead); }
+constexpr uint32_t kPartFloats = kPromptRows * (PITCH_DIM + 2);   // [rows][2] maxima and sums, [rows][dim] values
+__device__ __forceinline__ float* line_part(const PromptArgs& a, uint32_t head, uint32_t run, uint32_t last) {
+  return a.ws + a.parts_at + ((uint64_t)(run * a.kv_heads + head) * 2 + last) * kPartFloats;
+}
+
+// The line's tiles, and whether it is cut: a cut costs about as much as kPromptCut tiles of keys in every run (its part written and
+// read, the join), which an uneven split over the workgroups has to outweigh.
+__global__ __launch_bounds__(1024) void prompt_line(PromptArgs a) {
+  __shared__ uint32_t first[kPromptLineSequences + 1], sums[16];
+  __shared__ uint64_t wide[16];
+  __shared__ uint32_t longest;
+  const uint32_t me = threadIdx.x, lane = me & 63, wave = me >> 6;
+  static_assert(kPromptLineSequences == 1024, "a thread for each sequence");
+  uint32_t x = sequence(a, me).tiles;
+  const uint32_t own = x;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t up = __shfl_up(x, d);
+    if (lane >= (uint32_t)d) x += up;
+  }
+  if (lane == 63) sums[wave] = x;
+  if (me == 0) longest = 0;
+  __syncthreads();
+  for (uint32_t w = 0; w < wave; ++w) x += sums[w];
+  first[me] = x - own;
+  if (me == 1023) first[1024] = x;
+  __syncthreads();
+  const uint32_t tiles = min(first[1024], a.tiles);
+  uint64_t before = 0;
+  for (uint32_t base = 0; base < tiles; base += 1024) {
+    const uint32_t i = base + me;
+    uint32_t units = 0, b = 0, row = 0;
+    if (i < tiles) {
+      uint32_t lo = 0, hi = a.sequences;   // the last sequence whose tiles begin at i or before it
+      while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        (first[mid] <= i ? lo : hi) = mid;
+      }
+      b = lo;
+      row = (i - first[b]) * kRows;
+      const Range r = keys_of(a, sequence(a, b), row);
+      units = r.lo < r.hi ? (uint32_t)(r.hi - r.lo + kKeys - 1) / kKeys : 1;   // (a tile without keys writes its zeros)
+      atomicMax(&longest, units);
+    }
+    uint64_t sum = units;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint64_t up = __shfl_up(sum, d);
+      if (lane >= (uint32_t)d) sum += up;
+    }
+    __syncthreads();
+    if (lane == 63) wide[wave] = sum;
+    __syncthreads();
+    uint64_t at = before + sum - units;
+    for (uint32_t w = 0; w < 16; ++w) {
+      at += w < wave ? wide[w] : 0;
+      before += wide[w];
+    }
+    if (i < tiles) line_tiles(a)[i] = LineTile{at, b, row};
+  }
+  __syncthreads();
+  if (me == 0) {
+    line_tiles(a)[tiles] = LineTile{before, 0, 0};
+    const uint64_t runs = a.runs, run = max((before + runs - 1) / runs, (uint64_t)4);
+    const uint64_t rounds = (tiles + a.runs - 1) / a.runs, whole = max((uint64_t)longest, tiles ? rounds * before / tiles : 0);
+    Line line{before, run, tiles, tiles};
+    if (run + kPromptCut < whole)
+      line.runs = (uint32_t)((before + run - 1) / run);
+    else
+      line.run = 0;
+    *line_of(a) = line;
+  }
+}
+
+// The query tile of the line's position `at`, below the line's total, found by the wave: 64 places at a time, then 64 tiles.
+__device__ __forceinline__ uint32_t line_find(const LineTile* tiles, uint32_t count, uint64_t at) {
+  const uint32_t lane = threadIdx.x & 63;
+  uint32_t from = 0;
+  for (uint32_t step = 4096; step; step /= 64) {
+    const uint32_t i = from + lane * step;
+    from += (__popcll(__ballot(i < count && tiles[i].before <= at)) - 1) * step;
+  }
+  return from;
 }
 
 // Chunks of 16 bytes of a tile's row lie at places that depend on the row: 16 lanes that read the same chunk of 16 rows (keys), or
@@ -132,65 +247,25 @@ __device__ __forceinline__ uint32_t value_place(uint32_t row, uint32_t chunk) {
   return D == 128 ? chunk ^ ((row & 3) << 2) : chunk ^ ((row & 2) << 1);
 }
 
-// The first key that a query at position pos sees through a window (0: all). Written so that no window, however long, overflows.
-__device__ __forceinline__ int32_t window_start(int32_t pos, uint32_t window) {
-  return !window || pos < (int32_t)window ? 0 : pos - (int32_t)window + 1;
-}
+// w x, where a weight that has become zero leaves what is not finite.
+__device__ __forceinline__ float weighed(float w, float x) { return w == 0.f && x - x == 0.f ? 0.f : w == 0.f ? x : w * x; }
 
+// A workgroup's shared memory: two tiles of keys and of values, and whether a result is not finite.
+struct Shared {
+  __align__(1024) uint8_t tile[2][2][kTileBytes];
+  uint32_t odd;
+};
+
+// Attention of a query tile over its keys [from, to) of the range that it sees. The results go to the output, or with `part` there.
 template <bool MOD>
-__global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void prompt_attention(PromptArgs a) {
-  __shared__ __align__(1024) uint8_t lds[2][2][kTileBytes];
-  __shared__ uint32_t odd;
-  const uint32_t head = blockIdx.x % a.kv_heads, part = blockIdx.x / a.kv_heads % a.splits;
-  const Tile t = find_tile(a, blockIdx.x / (a.kv_heads * a.splits));
-  if (!t.any) return;
+__device__ __forceinline__ void attend(const PromptArgs& a, Shared& shared, uint32_t head, const Tile& t, Range range, float* part) {
   const uint32_t lane = threadIdx.x & 63, wave = of_wave(threadIdx.x >> 6), half = lane >> 5;
-  const int32_t offset = (int32_t)t.keys - (int32_t)t.queries;  // a query's position in its sequence, less its number
-  const uint32_t rows = t.queries * a.nq;
-
-  // the rows of this lane, and the keys [lo, hi] that they see
-  int32_t seen_hi[NB], seen_lo[NB];
-  uint64_t q_at[NB], o_at[NB];
-  uint32_t head_of[NB], token_of[NB];
-  bool live[NB];
-  w4 q[NB][kSteps];
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    const uint32_t m = t.row + (wave * NB + n) * 32 + (lane & 31);
-    live[n] = m < rows;
-    const uint32_t mm = min(m, rows - 1), token = mm / a.nq;
-    token_of[n] = t.first_query + token;
-    head_of[n] = head * a.nq + (mm - token * a.nq);
-    const int32_t pos = offset + (int32_t)token;
-    seen_hi[n] = a.causal ? min(pos, (int32_t)t.keys - 1) : (int32_t)t.keys - 1;
-    seen_lo[n] = window_start(pos, a.window);
-    const uint16_t* const p = (const uint16_t*)a.q.data + token_of[n] * a.q.token_stride + head_of[n] * a.q.head_stride;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      q[n][s] = *(const w4*)(p + s * 16 + half * 8);
-      if (a.negate) q[n][s] ^= 0x80008000u;
-    }
-  }
-  // the tile's keys, from its first row's first to its last row's last
-  const uint32_t last_row = min(t.row + kRows, rows) - 1;
-  const int32_t pos0 = offset + (int32_t)(t.row / a.nq), pos1 = offset + (int32_t)(last_row / a.nq);
-  int32_t lo = window_start(pos0, a.window);
-  int32_t hi = a.causal ? min(pos1 + 1, (int32_t)t.keys) : (int32_t)t.keys;
-  if (a.splits > 1 && lo < hi) {   // (unsigned: the last parts may begin behind the last key)
-    const uint32_t each = (((uint32_t)(hi - lo) + a.splits - 1) / a.splits + kKeys - 1) / kKeys * kKeys;
-    const uint32_t from = (uint32_t)lo + part * each;
-    lo = (int32_t)min(from, (uint32_t)hi);
-    hi = (int32_t)min(from + each, (uint32_t)hi);
-  }
-  // the wave's own rows
-  const uint32_t wave_row = t.row + wave * NB * 32, wave_last = min(wave_row + NB * 32, rows) - 1;
-  const bool wave_live = wave_row < rows;
-  const int32_t wpos0 = offset + (int32_t)(wave_row / a.nq), wpos1 = offset + (int32_t)(wave_last / a.nq);
-  const int32_t whi0 = a.causal ? wpos0 : 0x7FFFFFFF, wlo1 = window_start(wpos1, a.window);
-
+  const int32_t offset = (int32_t)t.s.keys - (int32_t)t.s.queries;
+  const uint32_t rows = t.s.queries * a.nq;
+  const int32_t lo = range.lo, hi = range.hi;
   const uint32_t ktb = (uint32_t)a.k.token_stride * 2, vtb = (uint32_t)a.v.token_stride * 2;
-  const uint8_t* const kbase = (const uint8_t*)a.k.data + head * a.k.head_stride * 2 + (uint64_t)t.first_key * ktb;
-  const uint8_t* const vbase = (const uint8_t*)a.v.data + head * a.v.head_stride * 2 + (uint64_t)t.first_key * vtb;
+  const uint8_t* const kbase = (const uint8_t*)a.k.data + head * a.k.head_stride * 2 + (uint64_t)t.s.first_key * ktb;
+  const uint8_t* const vbase = (const uint8_t*)a.v.data + head * a.v.head_stride * 2 + (uint64_t)t.s.first_key * vtb;
   const uint32_t load_row = wave * kLaneRows + lane / (D / 8), place = lane % (D / 8);
   const uint32_t koff = load_row * ktb + key_place(load_row, place) * 16;
   const uint32_t voff = load_row * vtb + value_place(load_row, place) * 16;
@@ -205,13 +280,47 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void prompt_attention(PromptA
                    :: "s"(of_wave(to + (i * kWaves + wave) * 1024)), "v"(at + i * kWaves * kLaneRows * stride), "s"(r) : "memory");
   };
   auto load = [&](int32_t k0, int buf) {
-    const uint32_t more = (uint32_t)min((int32_t)t.keys - k0, kKeys) - 1;  // rows behind the sequence are zeros
-    load_rows(kbase + (uint64_t)(uint32_t)k0 * ktb, ktb, more, koff, (uint32_t)(uintptr_t)(lds_u8*)lds[buf][0]);
-    load_rows(vbase + (uint64_t)(uint32_t)k0 * vtb, vtb, more, voff, (uint32_t)(uintptr_t)(lds_u8*)lds[buf][1]);
+    if (k0 >= hi) return;
+    const uint32_t more = (uint32_t)min((int32_t)t.s.keys - k0, kKeys) - 1;  // rows behind the sequence are zeros
+    load_rows(kbase + (uint64_t)(uint32_t)k0 * ktb, ktb, more, koff, (uint32_t)(uintptr_t)(lds_u8*)shared.tile[buf][0]);
+    load_rows(vbase + (uint64_t)(uint32_t)k0 * vtb, vtb, more, voff, (uint32_t)(uintptr_t)(lds_u8*)shared.tile[buf][1]);
   };
+  if (threadIdx.x == 0) shared.odd = 0;
+  load(lo, 0);   // (on its way while the queries are read)
 
-  v16f o[NB][kBlocks];
-  float m_run[NB], mc[NB], sum[NB];
+  // this lane's row, and the keys [seen_lo, seen_hi] that it sees
+  const uint32_t m = t.row + wave * 32 + (lane & 31);
+  const bool live = m < rows;
+  const uint32_t mm = min(m, rows - 1), token_in = mm / a.nq;
+  const uint32_t token_of = t.s.first_query + token_in, head_of = head * a.nq + (mm - token_in * a.nq);
+  const int32_t pos = offset + (int32_t)token_in;
+  const int32_t seen_hi = a.causal ? min(pos, (int32_t)t.s.keys - 1) : (int32_t)t.s.keys - 1, seen_lo = window_start(pos, a.window);
+  w4 q[kSteps];
+  float slope = 0.f;
+  {
+    const uint16_t* const p = (const uint16_t*)a.q.data + token_of * a.q.token_stride + head_of * a.q.head_stride;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) q[s] = *(const w4*)(p + s * 16 + half * 8);
+    if (a.negate) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) q[s] ^= 0x80008000u;
+    }
+    // (used here, so that the compiler waits for them here and not in the loop over the keys, for every tile on its way)
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(q[s]));
+    if (MOD && a.slopes) {
+      slope = a.slopes[head_of] * 1.44269504088896341f;
+      asm volatile("" : "+v"(slope));
+    }
+  }
+  // the wave's rows
+  const uint32_t wave_row = t.row + wave * 32, wave_last = min(wave_row + 32, rows) - 1;
+  const bool wave_live = wave_row < rows;
+  const int32_t whi0 = a.causal ? offset + (int32_t)(wave_row / a.nq) : 0x7FFFFFFF;
+  const int32_t wlo1 = window_start(offset + (int32_t)(wave_last / a.nq), a.window);
+
+  v16f o[kBlocks];
+  float m_run, mc, sum;
 
   // Where a lane finds its operands in a tile. Keys: row lane % 32, chunk 2 s + half. Values: of the 16 lanes that a transposing
   // read serves, lanes 4 j .. 4 j + 3 name 16 neighbouring coordinates of key j.
@@ -219,104 +328,95 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void prompt_attention(PromptA
   const uint32_t vrow = half * 4 + ((lane >> 2) & 3), vchunk = ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1), vbyte = (lane & 1) * 8;
 
   auto tile = [&](int32_t k0, int buf, auto careful, uint32_t kind) {
-    v16f s[NB][2];
-    const lds_u8* const kt = (const lds_u8*)lds[buf][0];
-    const lds_u8* const vt = (const lds_u8*)lds[buf][1];
+    v16f s[2];
+    const lds_u8* const kt = (const lds_u8*)shared.tile[buf][0];
+    const lds_u8* const vt = (const lds_u8*)shared.tile[buf][1];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-#pragma unroll
-      for (int n = 0; n < NB; ++n) s[n][b] = v16f{};
+      s[b] = v16f{};
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
         const w4 k = *(const lds_w4*)(kt + (b * 32 + krow) * (D * 2) + key_place(krow, i * 2 + half) * 16);
-#pragma unroll
-        for (int n = 0; n < NB; ++n) s[n][b] = mfma(k, q[n][i], s[n][b]);
+        s[b] = mfma(k, q[i], s[b]);
       }
     }
     if constexpr (MOD) {
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const float slope = a.slopes ? a.slopes[head_of[n]] * 1.44269504088896341f : 0.f;
-        const int32_t away = (int32_t)((uint32_t)k0 + half * 4 - (uint32_t)offset - (token_of[n] - t.first_query));
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            float z = s[n][b][r] * a.pre;
-            if (a.cap > 0.f) {
-              // tanh(x) = sign(x) (1 - 2 / (e^2|x| + 1))
-              const float e = __builtin_amdgcn_exp2f(__builtin_fabsf(z) * a.cap_r);
-              z = __builtin_copysignf(__builtin_fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(e + 1.f), a.cap), z);
-            }
-            s[n][b][r] = __builtin_fmaf(slope, (float)(away + b * 32 + (r & 3) + 8 * (r >> 2)), z);
-          }
-      }
-    }
-    const bool masked = k0 + kKeys - 1 > whi0 || k0 < wlo1 || k0 + kKeys > (int32_t)t.keys;
-    if (masked) {
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const int32_t up = seen_hi[n] - k0 - (int32_t)half * 4, down = seen_lo[n] - k0 - (int32_t)half * 4;
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int32_t j = b * 32 + (r & 3) + 8 * (r >> 2);
-            if (j > up || j < down) s[n][b][r] = kNoScore;
-          }
-      }
-    }
-    // weights exp2(c (s - m)), with a maximum m that is followed only where scores outgrow it by kGrow
-    w4 p[NB][4];
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      if constexpr (careful) {
+        for (int r = 0; r < 16; ++r) {
+          // tanh(x) = 1 - 2 / (e^2x + 1)
+          if (a.cap > 0.f)
+            s[b][r] = __builtin_fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[b][r] * a.cap_r) + 1.f), a.cap);
+          else
+            s[b][r] *= a.pre;
+        }
+      if (a.slopes) {
+        const int32_t away = (int32_t)((uint32_t)k0 + half * 4 - (uint32_t)offset - token_in);
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (kind) s[n][b][r] = s[n][b][r] > kNoScore ? 1.f : 0.f;
+            s[b][r] = __builtin_fmaf(slope, (float)(away + b * 32 + (r & 3) + 8 * (r >> 2)), s[b][r]);
       }
-      if (!careful || !kind) {
-        // (the compiler does not see that the maxima below read what matrix instructions write: 16 wait states, 11 are needed)
-        asm("s_nop 7\n\ts_nop 7" : "+v"(s[n][0]), "+v"(s[n][1]));
-        float top = fmax3_hw(s[n][0][0], s[n][1][0], s[n][0][1]);
-        float top2 = fmax3_hw(s[n][1][1], s[n][0][2], s[n][1][2]);
-#pragma unroll
-        for (int r = 3; r < 15; r += 2) {
-          top = fmax3_hw(top, s[n][0][r], s[n][1][r]);
-          top2 = fmax3_hw(top2, s[n][0][r + 1], s[n][1][r + 1]);
-        }
-        top = fmax3_hw(top, s[n][0][15], s[n][1][15]);
-        top = max32(fmax_hw(top, top2), fmax_hw(top, top2));
-        const uint64_t grown = __ballot(__builtin_fmaf(top, a.c, -m_run[n] * a.c) > kGrow);
-        float keep = 1.f;
-        if (grown) {
-          const float next = fmax_hw(m_run[n], top);
-          const float nc = next == kNoScore ? 0.f : next * a.c;
-          keep = __builtin_amdgcn_exp2f(__builtin_fmaf(m_run[n], a.c, -nc));
-          sum[n] *= keep;
-          m_run[n] = next;
-          mc[n] = nc;
-        }
-#pragma unroll
-        for (int d = 0; d < kBlocks; ++d) scale_where(grown, keep, o[n][d]);
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][b][r], a.c, -mc[n]));
-            s[n][b][r] = w;
-            sum[n] += w;
-          }
-      }
+    }
+    const bool masked = k0 + kKeys - 1 > whi0 || k0 < wlo1 || k0 + kKeys > (int32_t)t.s.keys;
+    if (masked) {
+      const int32_t up = seen_hi - k0 - (int32_t)half * 4, down = seen_lo - k0 - (int32_t)half * 4;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) p[n][b * 2 + i][j] = pack2(s[n][b][i * 8 + j * 2], s[n][b][i * 8 + j * 2 + 1]);
+        for (int r = 0; r < 16; ++r) {
+          const int32_t j = b * 32 + (r & 3) + 8 * (r >> 2);
+          if (j > up || j < down) s[b][r] = kNoScore;
+        }
     }
+    // weights exp2(c (s - m)), with a maximum m that is followed only where scores outgrow it by kGrow
+    if (careful && kind) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[b][r] = s[b][r] > kNoScore ? 1.f : 0.f;
+    } else {
+      // (the compiler does not see that the maxima below read what matrix instructions write: 16 wait states, 11 are needed)
+      asm("s_nop 7\n\ts_nop 7" : "+v"(s[0]), "+v"(s[1]));
+      float top = fmax3_hw(s[0][0], s[1][0], s[0][1]);
+      float top2 = fmax3_hw(s[1][1], s[0][2], s[1][2]);
+#pragma unroll
+      for (int r = 3; r < 15; r += 2) {
+        top = fmax3_hw(top, s[0][r], s[1][r]);
+        top2 = fmax3_hw(top2, s[0][r + 1], s[1][r + 1]);
+      }
+      top = fmax_hw(fmax3_hw(top, s[0][15], s[1][15]), top2);
+      top = max32(top, top);
+      const uint64_t grown = __ballot(__builtin_fmaf(top, a.c, -m_run * a.c) > kGrow);
+      float keep = 1.f;
+      if (grown) {
+        const float next = fmax_hw(m_run, top);
+        const float nc = next == kNoScore ? 0.f : next * a.c;
+        keep = __builtin_amdgcn_exp2f(__builtin_fmaf(m_run, a.c, -nc));
+        sum *= keep;
+        m_run = next;
+        mc = nc;
+      }
+#pragma unroll
+      for (int d = 0; d < kBlocks; ++d) scale_where(grown, keep, o[d]);
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], a.c, -mc));
+          s[b][r] = w;
+          sum += w;
+        }
+    }
+    w4 p[4];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[b * 2 + i][j] = pack2(s[b][i * 8 + j * 2], s[b][i * 8 + j * 2 + 1]);
     // the weights lie as a product's second operand wants them, if its 16 keys are taken in the order 4 h .. 4 h + 3, 8 + 4 h ..
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -347,176 +447,211 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void prompt_attention(PromptA
             v[j] = out;
           }
         }
-#pragma unroll
-        for (int n = 0; n < NB; ++n) o[n][d] = mfma(v, p[n][i], o[n][d]);
+        o[d] = mfma(v, p[i], o[d]);
       }
   };
+  // (the first tile is on its way when a pass begins)
   auto pass = [&](auto careful, uint32_t kind) {
+    m_run = kNoScore;
+    mc = sum = 0.f;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      m_run[n] = kNoScore;
-      mc[n] = sum[n] = 0.f;
-#pragma unroll
-      for (int d = 0; d < kBlocks; ++d) o[n][d] = v16f{};
-    }
-    if (lo >= hi) return;
-    load(lo, 0);
+    for (int d = 0; d < kBlocks; ++d) o[d] = v16f{};
     int buf = 0;
     if (!wave_live) {   // a wave without rows loads its share for the others
       for (int32_t k0 = lo; k0 < hi; k0 += kKeys, buf ^= 1) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (k0 + kKeys < hi) load(k0 + kKeys, buf ^ 1);
+        load(k0 + kKeys, buf ^ 1);
       }
-      __syncthreads();
-      return;
-    }
-    for (int32_t k0 = lo; k0 < hi; k0 += kKeys, buf ^= 1) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      if (k0 + kKeys < hi) load(k0 + kKeys, buf ^ 1);
-      tile(k0, buf, careful, kind);
+    } else {
+      for (int32_t k0 = lo; k0 < hi; k0 += kKeys, buf ^= 1) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        load(k0 + kKeys, buf ^ 1);
+        tile(k0, buf, careful, kind);
+      }
     }
     __syncthreads();
   };
 
   struct Plain { constexpr operator bool() const { return false; } };
   struct Careful { constexpr operator bool() const { return true; } };
-  if (threadIdx.x == 0) odd = 0;
   pass(Plain{}, 0);
   // A value that is not finite reaches every row of a product, also those whose mask hides it (0 * inf). Results that are not finite
   // are therefore computed again: where NaN and infinities are among a row's own values, then the finite values' sum.
   float check = 0.f;
 #pragma unroll
-  for (int n = 0; n < NB; ++n)
+  for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
-    for (int d = 0; d < kBlocks; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) check = __builtin_fmaf(o[n][d][r], 0.f, check);
-  if (lo >= hi) __syncthreads();
-  if (check != 0.f) odd = 1;
+    for (int r = 0; r < 16; ++r) check = __builtin_fmaf(o[d][r], 0.f, check);
+  if (check != 0.f) shared.odd = 1;
   __syncthreads();
-  if (odd) {
-    uint64_t is[3][NB];
+  if (shared.odd) {
+    uint64_t is[3];
     for (uint32_t kind = 1; kind <= 3; ++kind) {
+      load(lo, 0);
       pass(Careful{}, kind);
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        uint64_t bits = 0;
-#pragma unroll
-        for (int d = 0; d < kBlocks; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) bits |= (uint64_t)(o[n][d][r] > 0.f) << (d * 16 + r);
-        if (kind == 1) is[0][n] = bits;
-        if (kind == 2) is[1][n] = bits;
-        if (kind == 3) is[2][n] = bits;
-      }
-    }
-    pass(Careful{}, 0);
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
+      uint64_t bits = 0;
 #pragma unroll
       for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = d * 16 + r;
-          const bool up = is[1][n] >> j & 1, down = is[2][n] >> j & 1;
-          if ((is[0][n] >> j & 1) || (up && down)) o[n][d][r] = __builtin_nanf("");
-          else if (up || down) o[n][d][r] += up ? __builtin_inff() : -__builtin_inff();
-        }
-  }
-
-  if (!wave_live) return;
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    const float total = fold32(sum[n], sum[n]);
-    if (a.splits > 1) {
-      // (maximum, sum, values) of the part, values by output coordinate
-      const uint64_t heads = (uint64_t)a.kv_heads * a.nq, at = (uint64_t)token_of[n] * heads + head_of[n], all = (uint64_t)a.rows * heads;
-      float* const ms = a.ws + (part * all + at) * 2;
-      float* const ov = a.ws + (uint64_t)a.splits * all * 2 + (part * all + at) * D;
-      if (live[n]) {
-        if (half == 0) {
-          ms[0] = total == 0.f ? kNoScore : mc[n];
-          ms[1] = total;
-        }
-#pragma unroll
-        for (int d = 0; d < kBlocks; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; r += 4) *(v4f*)(ov + d * 32 + r * 2 + half * 4) = v4f{o[n][d][r], o[n][d][r + 1], o[n][d][r + 2], o[n][d][r + 3]};
-      }
-      continue;
+        for (int r = 0; r < 16; ++r) bits |= (uint64_t)(o[d][r] > 0.f) << (d * 16 + r);
+      if (kind == 1) is[0] = bits;
+      if (kind == 2) is[1] = bits;
+      if (kind == 3) is[2] = bits;
     }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    if (a.lse && live[n] && half == 0)
-      a.lse[(uint64_t)token_of[n] * a.kv_heads * a.nq + head_of[n]] = total == 0.f ? kNoScore : (mc[n] + __builtin_amdgcn_logf(total)) * kLn2;
-    uint16_t* const out = (uint16_t*)a.out.data + token_of[n] * a.out.token_stride + head_of[n] * a.out.head_stride;
+    load(lo, 0);
+    pass(Careful{}, 0);
 #pragma unroll
     for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; r += 8) {
-        // of 16 coordinates a lane has 0 - 3 and 8 - 11, its partner at distance 32 the others; each stores eight neighbours
-        uint32_t x[2], y[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          x[j] = pack2(o[n][d][r + j * 2] * inv, o[n][d][r + j * 2 + 1] * inv);
-          y[j] = pack2(o[n][d][r + 4 + j * 2] * inv, o[n][d][r + 4 + j * 2 + 1] * inv);
-          const auto z = __builtin_amdgcn_permlane32_swap(x[j], y[j], false, false);
-          x[j] = z[0];
-          y[j] = z[1];
-        }
-        if (live[n]) *(w4*)(out + d * 32 + r * 2 + half * 8) = w4{x[0], x[1], y[0], y[1]};
+      for (int r = 0; r < 16; ++r) {
+        const int j = d * 16 + r;
+        const bool up = is[1] >> j & 1, down = is[2] >> j & 1;
+        if ((is[0] >> j & 1) || (up && down)) o[d][r] = __builtin_nanf("");
+        else if (up || down) o[d][r] += up ? __builtin_inff() : -__builtin_inff();
       }
+  }
+
+  const float total = fold32(sum, sum);
+  if (!wave_live) return;
+  if (part) {
+    if (live) {
+      const uint32_t r = wave * 32 + (lane & 31);
+      if (half == 0) {
+        part[r * 2] = total == 0.f ? kNoScore : mc;
+        part[r * 2 + 1] = total;
+      }
+      float* const ov = part + kRows * 2 + r * D;
+#pragma unroll
+      for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) *(v4f*)(ov + d * 32 + j * 2 + half * 4) = v4f{o[d][j], o[d][j + 1], o[d][j + 2], o[d][j + 3]};
+    }
+    return;
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  if (a.lse && live && half == 0)
+    a.lse[(uint64_t)token_of * a.kv_heads * a.nq + head_of] = total == 0.f ? kNoScore : (mc + __builtin_amdgcn_logf(total)) * kLn2;
+  uint16_t* const out = (uint16_t*)a.out.data + token_of * a.out.token_stride + head_of * a.out.head_stride;
+#pragma unroll
+  for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 8) {
+      // of 16 coordinates a lane has 0 - 3 and 8 - 11, its partner at distance 32 the others; each stores eight neighbours
+      uint32_t x[2], y[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        x[j] = pack2(o[d][r + j * 2] * inv, o[d][r + j * 2 + 1] * inv);
+        y[j] = pack2(o[d][r + 4 + j * 2] * inv, o[d][r + 4 + j * 2 + 1] * inv);
+        const auto z = __builtin_amdgcn_permlane32_swap(x[j], y[j], false, false);
+        x[j] = z[0];
+        y[j] = z[1];
+      }
+      if (live) *(w4*)(out + d * 32 + r * 2 + half * 8) = w4{x[0], x[1], y[0], y[1]};
+    }
+}
+
+template <bool MOD, bool LINE>
+__global__ __launch_bounds__(256, 2) void prompt_attention(PromptArgs a) {
+  __shared__ Shared shared;
+  const uint32_t head = blockIdx.x % a.kv_heads, number = blockIdx.x / a.kv_heads;
+  if constexpr (!LINE) {
+    const Tile t = find_tile(a, number);
+    if (t.any) attend<MOD>(a, shared, head, t, keys_of(a, t.s, t.row), nullptr);
+  } else {
+    const Line line = *line_of(a);
+    const LineTile* const tiles = line_tiles(a);
+    if (number >= line.runs) return;
+    const uint64_t begin = line.run ? number * line.run : tiles[number].before;
+    const uint64_t end = line.run ? min(begin + line.run, line.total) : tiles[number + 1].before;
+    uint32_t i = line.run ? line_find(tiles, line.tiles, begin) : number;
+    for (uint64_t at = begin; at < end; ++i) {
+      const LineTile l = tiles[i];
+      const uint64_t next = tiles[i + 1].before, stop = min(next, end);
+      Tile t{};
+      t.s = sequence(a, of_wave(l.sequence));
+      t.row = of_wave(l.row);
+      Range r = keys_of(a, t.s, t.row);
+      const bool whole = at == l.before && stop == next;
+      if (!whole) {   // (a tile that is cut has more than one tile of keys)
+        const int32_t lo = r.lo;
+        r.lo = lo + (int32_t)of_wave((uint32_t)(at - l.before)) * kKeys;
+        r.hi = min(r.hi, lo + (int32_t)of_wave((uint32_t)(stop - l.before)) * kKeys);
+      }
+      attend<MOD>(a, shared, head, t, r, whole ? nullptr : line_part(a, head, number, at == l.before));
+      __syncthreads();
+      at = stop;
+    }
   }
 }
 
-// The parts of split keys, joined: one wave for each row of (token, head), parts in their order.
+// The parts of the query tile that run number `from` begins and others go on with, joined: a wave for each of kJoinRows rows.
+constexpr uint32_t kJoinRows = 16;
 __global__ __launch_bounds__(256) void prompt_join(PromptArgs a) {
-  const uint64_t heads = (uint64_t)a.kv_heads * a.nq, all = (uint64_t)a.rows * heads;
-  const uint64_t at = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (at >= all) return;
-  const uint32_t lane = threadIdx.x & 63, token = (uint32_t)(at / heads), head = (uint32_t)(at % heads);
-  // a token of no sequence has no result
-  bool inside = false;
-  for (uint32_t b = lane; b < a.sequences; b += 64)
-    inside |= (int32_t)token >= a.row_starts[b] && (int32_t)token < a.row_starts[b + 1];
-  if (!__ballot(inside)) return;
-  // a lane for each part (64 at most): its maximum and its sum
-  const bool part = lane < a.splits;
-  const float mine = part ? a.ws[(lane * all + at) * 2] : kNoScore, mine_sum = part ? a.ws[(lane * all + at) * 2 + 1] : 0.f;
-  const bool nan = __ballot(mine != mine) != 0;
-  float m = wave_max(mine);
-  if (m == kNoScore) m = 0.f;
-  const float weight = nan ? __builtin_nanf("") : __builtin_amdgcn_exp2f(mine - m);
-  const float sum = wave_sum(weight == 0.f ? 0.f : weight * mine_sum);
-  float o[D / 64] = {};
-  const float* const ov = a.ws + (uint64_t)a.splits * all * 2;
-  // (parts without a visible key have not written values that count)
-  for (uint64_t todo = __ballot(part && weight != 0.f); todo;) {
-    float w[8], x[8][D / 64];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {   // eight parts on their way at once
-      w[i] = 0.f;
-      if (!todo) continue;
-      const int p = __ffsll((unsigned long long)todo) - 1;
-      todo &= todo - 1;
-      w[i] = lane_value(weight, p);
-#pragma unroll
-      for (int d = 0; d < D / 64; ++d) x[i][d] = ov[(p * all + at) * D + lane * (D / 64) + d];
+  const uint32_t lane = threadIdx.x & 63, wave = of_wave(threadIdx.x >> 6);
+  const uint32_t head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, block = rest % (kRows / kJoinRows);
+  const uint32_t from = rest / (kRows / kJoinRows);
+  const Line line = *line_of(a);
+  if (!line.run || from + 1 >= line.runs) return;
+  const LineTile* const tiles = line_tiles(a);
+  const uint64_t cut = (from + 1) * line.run;
+  const uint32_t i = line_find(tiles, line.tiles, cut);
+  const LineTile l = tiles[i];
+  // a tile that begins at the cut is whole there; of one that goes on from an earlier run, that run's turn joins the parts
+  if (l.before == cut || l.before < from * line.run) return;
+  const uint32_t to = (uint32_t)((tiles[i + 1].before - 1) / line.run), parts = to - from + 1;
+  const Sequence s = sequence(a, of_wave(l.sequence));
+  const uint32_t row0 = of_wave(l.row), rows = s.queries * a.nq;
+  auto part_of = [&](uint32_t p) { return line_part(a, head, from + p, p == 0); };
+  for (uint32_t r = block * kJoinRows + wave; r < (block + 1) * kJoinRows && row0 + r < rows; r += 4) {
+    float m = kNoScore;
+    bool nan = false;
+    for (uint32_t p = lane; p < (parts + 63) / 64 * 64; p += 64) {
+      const float x = p < parts ? part_of(p)[r * 2] : kNoScore;
+      nan |= x != x;
+      m = fmax_hw(m, x);
     }
+    m = wave_max(m);
+    if (__ballot(nan)) m = __builtin_nanf("");
+    if (m == kNoScore) m = 0.f;
+    float sum = 0.f, o[D / 64] = {};
+    for (uint32_t base = 0; base < parts; base += 64) {   // a lane for each of 64 parts: its weight
+      const float mine = base + lane < parts ? part_of(base + lane)[r * 2] : kNoScore;
+      const float weight = __builtin_amdgcn_exp2f(mine - m);
+      sum += mine == kNoScore ? 0.f : weighed(weight, part_of(base + lane)[r * 2 + 1]);
+      for (uint64_t todo = __ballot(!(mine == kNoScore)); todo;) {   // parts with a visible key
+        float w[8], x[8][D / 64];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+        for (int k = 0; k < 8; ++k) {   // eight parts on their way at once
+          w[k] = 0.f;
 #pragma unroll
-      for (int d = 0; d < D / 64; ++d)
-        if (w[i] != 0.f) o[d] = __builtin_fmaf(w[i], x[i][d], o[d]);
+          for (int d = 0; d < D / 64; ++d) x[k][d] = 0.f;
+          if (!todo) continue;
+          const int p = __ffsll((unsigned long long)todo) - 1;
+          todo &= todo - 1;
+          w[k] = lane_value(weight, p);
+          const float* const ov = part_of(base + p) + kRows * 2 + r * D + lane * (D / 64);
+#pragma unroll
+          for (int d = 0; d < D / 64; ++d) x[k][d] = ov[d];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+          for (int d = 0; d < D / 64; ++d) o[d] += weighed(w[k], x[k][d]);
+      }
+    }
+    sum = wave_sum(sum);
+    const uint32_t token = (row0 + r) / a.nq, h = head * a.nq + (row0 + r) % a.nq;
+    const uint64_t at = s.first_query + token;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (a.lse && lane == 0) a.lse[at * a.kv_heads * a.nq + h] = sum == 0.f ? kNoScore : (m + __builtin_amdgcn_logf(sum)) * kLn2;
+    uint16_t* const out = (uint16_t*)a.out.data + at * a.out.token_stride + h * a.out.head_stride + lane * (D / 64);
+    if constexpr (D == 128)
+      *(uint32_t*)out = pack2(o[0] * inv, o[1] * inv);
+    else
+      *out = (uint16_t)pack2(o[0] * inv, 0.f);
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  if (a.lse && lane == 0) a.lse[at] = sum == 0.f ? kNoScore : (m + __builtin_amdgcn_logf(sum)) * kLn2;
-  uint16_t* const out = (uint16_t*)a.out.data + token * a.out.token_stride + head * a.out.head_stride + lane * (D / 64);
-  if constexpr (D == 128)
-    *(uint32_t*)out = pack2(o[0] * inv, o[1] * inv);
-  else
-    *out = (uint16_t)pack2(o[0] * inv, 0.f);
 }
 
 }  // namespace
@@ -524,15 +659,26 @@ __global__ __launch_bounds__(256) void prompt_join(PromptArgs a) {
 #define PITCH_CAT_(a, b, c, d) a##b##c##d
 #define PITCH_CAT(a, b, c, d) PITCH_CAT_(a, b, c, d)
 hipError_t PITCH_CAT(launch_prompt_d, PITCH_DIM, _io, PITCH_IO)(const PromptArgs& a, hipStream_t s) {
-  const uint64_t groups = (uint64_t)a.tiles * a.kv_heads * a.splits;
-  if (a.slopes || a.cap > 0.f)
-    prompt_attention<true><<<dim3((uint32_t)groups), dim3(256), 0, s>>>(a);
-  else
-    prompt_attention<false><<<dim3((uint32_t)groups), dim3(256), 0, s>>>(a);
+  const bool mod = a.slopes || a.cap > 0.f;
+  if (!a.runs) {
+    const dim3 grid(a.tiles * a.kv_heads);
+    if (mod)
+      prompt_attention<true, false><<<grid, dim3(256), 0, s>>>(a);
+    else
+      prompt_attention<false, false><<<grid, dim3(256), 0, s>>>(a);
+    return hipGetLastError();
+  }
+  prompt_line<<<dim3(1), dim3(1024), 0, s>>>(a);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.splits == 1) return e;
-  const uint64_t rows = (uint64_t)a.rows * a.kv_heads * a.nq;
-  prompt_join<<<dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, s>>>(a);
+  if (e != hipSuccess) return e;
+  const dim3 grid((a.tiles > a.runs ? a.tiles : a.runs) * a.kv_heads);
+  if (mod)
+    prompt_attention<true, true><<<grid, dim3(256), 0, s>>>(a);
+  else
+    prompt_attention<false, true><<<grid, dim3(256), 0, s>>>(a);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  prompt_join<<<dim3((a.runs - 1) * (kRows / kJoinRows) * a.kv_heads), dim3(256), 0, s>>>(a);
   return hipGetLastError();
 }
 

@@ -79,6 +79,25 @@ def test_long_sequences(q, dtype, lengths):
     _check(q, lengths, 4, 2, 64, dtype, seed=4, window=400)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("more", [dict(), dict(causal=False), dict(window=2100), dict(softcap=8.0)])
+def test_tiles_that_are_cut(q, dtype, more):
+    """Few query tiles of very different lengths: workgroups share them, beginning and ending within a tile."""
+    _check(q, [(500, 4500), (130, 2500), (0, 100), (1, 5000), (33, 40), (20, 3), (64, 700)], 8, 2, 128, dtype, seed=30, **more)
+    _check(q, [(7, 9000)], 3, 1, 64, dtype, seed=31, **more)
+    _check(q, [(900, 2300), (300, 2900)], 2, 1, 64, dtype, seed=32, **more)
+
+
+def test_many_sequences_over_long_keys(q):
+    """A thousand sequences and more, most of a token, some of them long."""
+    for n in (700, 1024, 1025):
+        rng = np.random.default_rng(n)
+        lengths = [(int(a), int(a + b)) for a, b in zip(rng.integers(0, 3, n), rng.integers(0, 9, n))]
+        lengths[n // 2] = (40, 3000)
+        lengths[-1] = (1, 2500)
+        _check(q, lengths, 2, 1, 64, torch.bfloat16, seed=33)
+
+
 def test_more_sequences_than_a_wave_has_lanes(q):
     rng = np.random.default_rng(5)
     lengths = [(int(n), int(n + p)) for n, p in zip(rng.integers(0, 9, 333), rng.integers(0, 30, 333))]
@@ -135,7 +154,7 @@ def test_what_is_hidden_has_no_effect(q, dtype, dim):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("lengths", [[(70, 70), (200, 200)], [(3, 2000)]])   # (the second splits its keys)
+@pytest.mark.parametrize("lengths", [[(70, 70), (200, 200)], [(3, 3000)]])   # (the second's keys are cut into parts)
 def test_values_that_are_not_finite(q, dtype, lengths):
     """Each coordinate of each row gets NaN, an infinity or its sum, by what its visible values hold."""
     qq, k, v, rs, ks = _inputs(lengths, 4, 2, 64, dtype, 9)
@@ -184,8 +203,8 @@ def test_a_call_is_the_same_whatever_else_it_holds(q):
 
 
 def test_graph_and_streams(q):
-    """A captured call is replayed over changing contents and starts; split calls on several streams have workspaces of their own."""
-    qq, k, v, rs, ks = _inputs([(3, 1200), (2, 700)], 8, 2, 128, torch.bfloat16, 13)
+    """A captured call is replayed over changing contents and starts; calls on several streams have workspaces of their own."""
+    qq, k, v, rs, ks = _inputs([(3, 2400), (2, 700)], 8, 2, 128, torch.bfloat16, 13)
     drs, dks = _dev(rs), _dev(ks)
     out, lse = torch.full_like(qq, 7.0), torch.full(qq.shape[:2], 7.0, device="cuda")
     call = P.PromptAttention(q, qq, k, v, drs, out, keyStarts=dks, lse=lse)
@@ -205,7 +224,7 @@ def test_graph_and_streams(q):
         torch.cuda.synchronize()
         compare(out, lse, reference(qq, k, v, starts(new), starts(keys)))
     streams = [torch.cuda.Stream() for _ in range(3)]
-    sets = [_inputs([(2, 1500)], 8, 2, 128, torch.float16, 20 + i) for i in range(3)]
+    sets = [_inputs([(2, 2500)], 8, 2, 128, torch.float16, 20 + i) for i in range(3)]
     outs = [torch.zeros_like(s[0]) for s in sets]
     calls = [P.PromptAttention(q, *s[:3], _dev(s[3]), o, keyStarts=_dev(s[4])) for s, o in zip(sets, outs)]
     torch.cuda.synchronize()
