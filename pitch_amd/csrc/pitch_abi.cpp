@@ -1773,7 +1773,8 @@ int pitch_enqueue_prompt_attention(const pitch_prompt_attention_t* call, void* s
   a.causal = call->causal;
   a.window = call->window;
   a.tiles = plan.tiles;
-  a.runs = plan.runs;
+  a.places = plan.places;
+  a.most_items = plan.most_items;
   a.parts_at = plan.parts_at;
   // scores in log2 units; hidden scores are minus infinity, which a factor of zero would make NaN
   constexpr double kLog2E = 1.4426950408889634, kMost = std::numeric_limits<float>::max();

@@ -14,7 +14,7 @@ struct PromptArgs {
   const int32_t* key_starts;  // [sequences + 1]: keys of each sequence
   const float* slopes;        // [query heads] or null
   float* lse;                 // [rows][query heads] or null
-  float* ws;                  // with runs: the line of tiles (kPromptLineHead floats and 4 per tile and one more), parts from parts_at on
+  float* ws;                  // with places: 5 words per sequence and 2 more, parts of results from parts_at on
   uint32_t rows, keys;        // tokens that the queries' and the keys' buffers hold
   uint32_t sequences, kv_heads, nq;
   uint32_t causal, window;    // window 0: all
@@ -23,29 +23,34 @@ struct PromptArgs {
   float pre;                  // with a cap or slopes: what a product is multiplied by first
   float cap, cap_r;           // with a positive cap, products x give cap * tanh(x'), e^(2 x') = 2^(x * cap_r), in log2 units
   uint32_t tiles;             // an upper bound of the query tiles of a KV head
-  uint32_t runs;              // workgroups of a KV head that the line of tiles is cut for; 0: every workgroup takes a query tile
+  uint32_t places;            // workgroups of a KV head that run at once, where keys may be cut into parts; 0: they are not
+  uint32_t most_items;        // parts of a KV head's tiles that the workspace has room for, where any are cut
   uint64_t parts_at;
 };
 
-// Rows of (token, query head of a KV head) in a query tile; the most sequences of a call whose line of tiles is laid out, and the
-// keys from which that is done; tiles of keys that a cut costs a run; floats before the line's tiles.
-constexpr uint32_t kPromptRows = 128, kPromptLineSequences = 1024, kPromptLineKeys = 2048, kPromptCut = 12, kPromptLineHead = 8;
+#ifndef PCUT
+#define PCUT 7
+#endif
+// Rows of (token, query head of a KV head) in a query tile; the most sequences of a call whose keys may be cut into parts, and the
+// keys from which that is looked at; what writing and joining a part of 128 rows costs, in tiles of 64 keys.
+constexpr uint32_t kPromptRows = 128, kPromptCutSequences = 1024, kPromptCutKeys = 2048, kPromptCut = PCUT;
 struct PromptPlan {
-  uint32_t tiles, runs;
+  uint32_t tiles, places, most_items;
   uint64_t parts_at, ws_floats;
 };
-// What the host decides: with query tiles enough for four turns of every workgroup place (two on a compute unit), each takes one; else,
-// where tiles may be long, the line of tiles is laid out, and its lengths decide on the device.
+// What the host decides: with query tiles enough for four turns of every workgroup place (two on a compute unit), each workgroup takes
+// one; else, where tiles may be long, their lengths decide on the device whether keys are cut.
 inline PromptPlan prompt_plan(uint32_t rows, uint32_t keys, uint32_t window, uint32_t sequences, uint32_t kv_heads, uint32_t nq,
                               uint32_t dim, uint32_t cus) {
   PromptPlan p{};
   p.tiles = (uint32_t)((uint64_t)rows * nq / kPromptRows) + (sequences < rows ? sequences : rows);
   const uint32_t places = 2 * cus, seen = window && window < keys ? window : keys;
-  if (sequences > kPromptLineSequences || (uint64_t)p.tiles * kv_heads >= 4ull * places || seen < kPromptLineKeys || places / kv_heads < 2)
+  if (sequences > kPromptCutSequences || (uint64_t)p.tiles * kv_heads >= 4ull * places || seen < kPromptCutKeys || kv_heads > places)
     return p;
-  p.runs = places / kv_heads;
-  p.parts_at = kPromptLineHead + (p.tiles + 1ull) * 4;
-  p.ws_floats = p.parts_at + (uint64_t)p.runs * kv_heads * 2 * kPromptRows * (dim + 2);
+  p.places = places / kv_heads;
+  p.most_items = 4 * p.places;
+  p.parts_at = (sequences * 5 + 2 + 3) / 4 * 4;
+  p.ws_floats = p.parts_at + (uint64_t)p.most_items * kv_heads * kPromptRows * (dim + 2);
   return p;
 }
 

@@ -75,6 +75,18 @@ __device__ __forceinline__ void scale_where(uint64_t go, float f, v16f& x) {
   for (int r = 0; r < 16; ++r) x[r] = y[r];
 }
 
+// The sum over this lane and those below it.
+__device__ __forceinline__ uint32_t lanes_up_to(uint32_t x) {
+  x += __builtin_amdgcn_update_dpp(0u, x, 0x111, 0xF, 0xF, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0u, x, 0x112, 0xF, 0xF, false);  // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0u, x, 0x114, 0xF, 0xF, false);  // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0u, x, 0x118, 0xF, 0xF, false);  // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0u, x, 0x142, 0xA, 0xF, false);  // row_bcast:15, to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0u, x, 0x143, 0xC, 0xF, false);  // row_bcast:31, to rows 2 and 3
+  return x;
+}
+__device__ __forceinline__ uint32_t of_lane(uint32_t x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+
 // A sequence's queries and keys, within the buffers.
 struct Sequence {
   uint32_t first_query, queries, first_key, keys, tiles;
@@ -103,18 +115,11 @@ __device__ __forceinline__ Tile find_tile(const PromptArgs& a, uint32_t at) {
   Tile t{};
   for (uint32_t base = 0; base < a.sequences; base += 64) {
     const Sequence s = sequence(a, base + lane);
-    uint32_t sum = s.tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t up = __shfl_up(sum, d);
-      if (lane >= (uint32_t)d) sum += up;
-    }
-    const uint32_t total = of_wave(__shfl(sum, 63));
+    const uint32_t sum = lanes_up_to(s.tiles), total = of_lane(sum, 63);
     if (at < total) {
       const int who = __ffsll((unsigned long long)__ballot(sum > at)) - 1;
-      t.s = Sequence{of_wave(__shfl(s.first_query, who)), of_wave(__shfl(s.queries, who)), of_wave(__shfl(s.first_key, who)),
-                     of_wave(__shfl(s.keys, who)), 0};
-      t.row = (of_wave(__shfl(sum, who)) - 1 - at) * kRows;
+      t.s = Sequence{of_lane(s.first_query, who), of_lane(s.queries, who), of_lane(s.first_key, who), of_lane(s.keys, who), 0};
+      t.row = (of_lane(sum, who) - 1 - at) * kRows;
       t.any = true;
       return t;
     }
@@ -138,104 +143,113 @@ __device__ __forceinline__ Range keys_of(const PromptArgs& a, const Sequence& s,
   return Range{window_start(pos0, a.window), a.causal ? min(pos1 + 1, (int32_t)s.keys) : (int32_t)s.keys};
 }
 
-// ------------------------------------------------------------------------------------------------ the line of tiles
-// Where a KV head has few query tiles, or tiles of very different lengths, all of a KV head's tiles of keys form one line, which is cut into equal
-// runs, one per workgroup. A run that holds a query tile whole writes its output; of a tile that is cut, every run leaves its part
-// (maxima, sums, values) in the workspace, and prompt_join puts them together, in their order. A run has two such parts at most: of the
-// tile in which it begins and of the one in which it ends.
-struct LineTile {
-  uint64_t before;       // tiles of keys before this query tile's
-  uint32_t sequence, row;
+// ------------------------------------------------------------------------------------------------ keys in parts
+// Where query tiles are few, or of very different lengths, the keys of a sequence are cut into parts, the same for all of its tiles, and
+// a workgroup takes one part of one tile: it leaves maxima, sums and values in the workspace, and prompt_join puts a tile's parts
+// together, in their order. Parts of a sequence are numbered part by part and within one tile by tile, so that workgroups that run at the
+// same time read the same keys (a line of tiles cut into equal runs, each at other keys, found a fifth of its reads in L2 and took XXX).
+struct Cut {   // the workspace's first part: for each sequence, those with the longest parts first
+  uint32_t* items;     // [sequences + 1] parts of tiles before its own
+  uint32_t* tiles;     // [sequences + 1] tiles before its own
+  uint32_t* parts;     // [sequences]
+  uint32_t* each;      // [sequences] tiles of keys of a part
+  uint32_t* sequence;  // [sequences] its number
+  __device__ explicit Cut(const PromptArgs& a)
+      : items((uint32_t*)a.ws), tiles(items + a.sequences + 1), parts(tiles + a.sequences + 1), each(parts + a.sequences),
+        sequence(each + a.sequences) {}
 };
-struct Line {
-  uint64_t total, run;   // tiles of keys, of a run (0: a workgroup takes a whole query tile)
-  uint32_t tiles, runs;
-};
-__device__ __forceinline__ Line* line_of(const PromptArgs& a) { return (Line*)a.ws; }
-__device__ __forceinline__ LineTile* line_tiles(const PromptArgs& a) { return (LineTile*)(a.ws + kPromptLineHead); }
 constexpr uint32_t kPartFloats = kPromptRows * (PITCH_DIM + 2);   // [rows][2] maxima and sums, [rows][dim] values
-__device__ __forceinline__ float* line_part(const PromptArgs& a, uint32_t head, uint32_t run, uint32_t last) {
-  return a.ws + a.parts_at + ((uint64_t)(run * a.kv_heads + head) * 2 + last) * kPartFloats;
+__device__ __forceinline__ float* part_of(const PromptArgs& a, uint32_t head, uint32_t item) {
+  return a.ws + a.parts_at + ((uint64_t)item * a.kv_heads + head) * kPartFloats;
 }
 
-// The line's tiles, and whether it is cut: a cut costs about as much as kPromptCut tiles of keys in every run (its part written and
-// read, the join), which an uneven split over the workgroups has to outweigh.
-__global__ __launch_bounds__(1024) void prompt_line(PromptArgs a) {
-  __shared__ uint32_t first[kPromptLineSequences + 1], sums[16];
-  __shared__ uint64_t wide[16];
-  __shared__ uint32_t longest;
-  const uint32_t me = threadIdx.x, lane = me & 63, wave = me >> 6;
-  static_assert(kPromptLineSequences == 1024, "a thread for each sequence");
-  uint32_t x = sequence(a, me).tiles;
-  const uint32_t own = x;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t up = __shfl_up(x, d);
-    if (lane >= (uint32_t)d) x += up;
-  }
-  if (lane == 63) sums[wave] = x;
+// Chooses the longest part, of 64 candidates (the longest sequence in 1 .. 64 parts), by an estimate of the time, in sixteenths
+// of a tile of keys: all tiles of keys, 2 for each part's beginning and end and kPromptCut for a part of 128 rows that is written and
+// joined, over the workgroup places, and half of the longest part for the end, when places run empty; or, where there is a place for
+// each part, the longest.
+__global__ __launch_bounds__(1024) void prompt_cut(PromptArgs a) {
+  __shared__ uint32_t sums[2][16], longest, lengths[1024], counts[2][1024];
+  __shared__ unsigned long long cost[64], items[64];
+  const uint32_t me = threadIdx.x, lane = me & 63, wave = of_wave(me >> 6);
+  static_assert(kPromptCutSequences == 1024, "a thread for each sequence");
+  const Sequence s = sequence(a, me);
+  const uint32_t seen = a.window ? min(s.keys, (uint32_t)min((uint64_t)a.window + kRows, (uint64_t)0x7FFFFFFFu)) : s.keys;
+  const uint32_t units = s.tiles ? max((seen + kKeys - 1) / kKeys, 1u) : 0;
+  const uint32_t join = kPromptCut * 16 * min(s.queries * a.nq, (uint32_t)kRows) / kRows;
   if (me == 0) longest = 0;
+  if (me < 64) cost[me] = items[me] = 0;
   __syncthreads();
-  for (uint32_t w = 0; w < wave; ++w) x += sums[w];
-  first[me] = x - own;
-  if (me == 1023) first[1024] = x;
+  if (units) atomicMax(&longest, units);
   __syncthreads();
-  const uint32_t tiles = min(first[1024], a.tiles);
-  uint64_t before = 0;
-  for (uint32_t base = 0; base < tiles; base += 1024) {
-    const uint32_t i = base + me;
-    uint32_t units = 0, b = 0, row = 0;
-    if (i < tiles) {
-      uint32_t lo = 0, hi = a.sequences;   // the last sequence whose tiles begin at i or before it
-      while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        (first[mid] <= i ? lo : hi) = mid;
-      }
-      b = lo;
-      row = (i - first[b]) * kRows;
-      const Range r = keys_of(a, sequence(a, b), row);
-      units = r.lo < r.hi ? (uint32_t)(r.hi - r.lo + kKeys - 1) / kKeys : 1;   // (a tile without keys writes its zeros)
-      atomicMax(&longest, units);
-    }
-    uint64_t sum = units;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint64_t up = __shfl_up(sum, d);
-      if (lane >= (uint32_t)d) sum += up;
-    }
-    __syncthreads();
-    if (lane == 63) wide[wave] = sum;
-    __syncthreads();
-    uint64_t at = before + sum - units;
-    for (uint32_t w = 0; w < 16; ++w) {
-      at += w < wave ? wide[w] : 0;
-      before += wide[w];
-    }
-    if (i < tiles) line_tiles(a)[i] = LineTile{at, b, row};
+  const uint32_t run = max((longest + lane) / (lane + 1), 1u);   // the lane's candidate
+  uint64_t my_cost = 0, my_items = 0;
+  const uint32_t here = min(max((int32_t)(a.sequences - wave * 64), 0), 64);
+  for (uint32_t k = 0; k < here; ++k) {
+    const uint32_t u = __builtin_amdgcn_readlane(units, k), n = __builtin_amdgcn_readlane(s.tiles, k), j = __builtin_amdgcn_readlane(join, k);
+    if (n == 0) continue;
+    const uint32_t parts = (u + run - 1) / run;
+    my_items += (uint64_t)n * parts;
+    my_cost += (uint64_t)n * (16ull * u + parts * (32ull + (parts > 1 ? j : 0)));
+  }
+  if (here) {
+    atomicAdd(&cost[lane], (unsigned long long)my_cost);
+    atomicAdd(&items[lane], (unsigned long long)my_items);
   }
   __syncthreads();
-  if (me == 0) {
-    line_tiles(a)[tiles] = LineTile{before, 0, 0};
-    const uint64_t runs = a.runs, run = max((before + runs - 1) / runs, (uint64_t)4);
-    const uint64_t rounds = (tiles + a.runs - 1) / a.runs, whole = max((uint64_t)longest, tiles ? rounds * before / tiles : 0);
-    Line line{before, run, tiles, tiles};
-    if (run + kPromptCut < whole)
-      line.runs = (uint32_t)((before + run - 1) / run);
-    else
-      line.run = 0;
-    *line_of(a) = line;
+  // the cheapest candidate that the workspace has room for, the same in every wave; uncut is always possible
+  float best = items[lane] <= a.places ? 16.f * (float)run + 32.f + kPromptCut * 16.f : (float)cost[lane] / (float)a.places + 8.f * (float)run;
+  if (lane > 0 && items[lane] > a.most_items) best = __builtin_inff();
+  uint32_t choice = run;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    const float other = __shfl_xor(best, d);
+    const uint32_t its = __shfl_xor(choice, d);
+    if (other < best || (other == best && its > choice)) best = other, choice = its;
+  }
+  const uint32_t parts = s.tiles ? (units + choice - 1) / choice : 0, each = parts ? (units + parts - 1) / parts : 0;
+  // the sequences by the length of their parts: the shortest come last, when places run empty
+  lengths[me] = each;
+  __syncthreads();
+  uint32_t place = 0;
+  for (uint32_t i = 0; i < a.sequences; ++i) place += lengths[i] > each || (lengths[i] == each && i < me);
+  const Cut cut(a);
+  if (me < a.sequences) {
+    counts[0][place] = s.tiles * parts;
+    counts[1][place] = s.tiles;
+    cut.parts[place] = parts;
+    cut.each[place] = each;
+    cut.sequence[place] = me;
+  }
+  __syncthreads();
+  uint32_t mine[2], before[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    mine[i] = me < a.sequences ? counts[i][me] : 0;
+    const uint32_t x = lanes_up_to(mine[i]);
+    if (lane == 63) sums[i][wave] = x;
+    before[i] = x - mine[i];
+  }
+  __syncthreads();
+  for (uint32_t w = 0; w < wave; ++w) before[0] += sums[0][w], before[1] += sums[1][w];
+  if (me < a.sequences) {
+    cut.items[me] = before[0];
+    cut.tiles[me] = before[1];
+  }
+  if (me == a.sequences - 1) {
+    cut.items[a.sequences] = before[0] + mine[0];
+    cut.tiles[a.sequences] = before[1] + mine[1];
   }
 }
 
-// The query tile of the line's position `at`, below the line's total, found by the wave: 64 places at a time, then 64 tiles.
-__device__ __forceinline__ uint32_t line_find(const LineTile* tiles, uint32_t count, uint64_t at) {
+// The last sequence with at most `at` items (or tiles) before its own, found by the wave: every 64th sequence, then 64 of them.
+__device__ __forceinline__ uint32_t find_sequence(const uint32_t* before, uint32_t sequences, uint32_t at) {
   const uint32_t lane = threadIdx.x & 63;
   uint32_t from = 0;
-  for (uint32_t step = 4096; step; step /= 64) {
+  for (uint32_t step = 64; step; step /= 64) {
     const uint32_t i = from + lane * step;
-    from += (__popcll(__ballot(i < count && tiles[i].before <= at)) - 1) * step;
+    from += (max(__popcll(__ballot(i < sequences && before[i] <= at)), 1) - 1) * step;
   }
-  return from;
+  return of_wave(from);
 }
 
 // Chunks of 16 bytes of a tile's row lie at places that depend on the row: 16 lanes that read the same chunk of 16 rows (keys), or
@@ -471,7 +485,6 @@ __device__ __forceinline__ void attend(const PromptArgs& a, Shared& shared, uint
         tile(k0, buf, careful, kind);
       }
     }
-    __syncthreads();
   };
 
   struct Plain { constexpr operator bool() const { return false; } };
@@ -479,16 +492,17 @@ __device__ __forceinline__ void attend(const PromptArgs& a, Shared& shared, uint
   pass(Plain{}, 0);
   // A value that is not finite reaches every row of a product, also those whose mask hides it (0 * inf). Results that are not finite
   // are therefore computed again: where NaN and infinities are among a row's own values, then the finite values' sum.
-  float check = 0.f;
+  float check[4] = {};
 #pragma unroll
   for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) check = __builtin_fmaf(o[d][r], 0.f, check);
-  if (check != 0.f) shared.odd = 1;
+    for (int r = 0; r < 16; ++r) check[r & 3] = __builtin_fmaf(o[d][r], 0.f, check[r & 3]);
+  if ((check[0] + check[1]) + (check[2] + check[3]) != 0.f) shared.odd = 1;
   __syncthreads();
   if (shared.odd) {
     uint64_t is[3];
     for (uint32_t kind = 1; kind <= 3; ++kind) {
+      __syncthreads();   // (the pass before has read its tiles)
       load(lo, 0);
       pass(Careful{}, kind);
       uint64_t bits = 0;
@@ -500,6 +514,7 @@ __device__ __forceinline__ void attend(const PromptArgs& a, Shared& shared, uint
       if (kind == 2) is[1] = bits;
       if (kind == 3) is[2] = bits;
     }
+    __syncthreads();
     load(lo, 0);
     pass(Careful{}, 0);
 #pragma unroll
@@ -552,105 +567,94 @@ __device__ __forceinline__ void attend(const PromptArgs& a, Shared& shared, uint
     }
 }
 
-template <bool MOD, bool LINE>
+template <bool MOD, bool CUT>
 __global__ __launch_bounds__(256, 2) void prompt_attention(PromptArgs a) {
   __shared__ Shared shared;
   const uint32_t head = blockIdx.x % a.kv_heads, number = blockIdx.x / a.kv_heads;
-  if constexpr (!LINE) {
+  if constexpr (!CUT) {
     const Tile t = find_tile(a, number);
     if (t.any) attend<MOD>(a, shared, head, t, keys_of(a, t.s, t.row), nullptr);
   } else {
-    const Line line = *line_of(a);
-    const LineTile* const tiles = line_tiles(a);
-    if (number >= line.runs) return;
-    const uint64_t begin = line.run ? number * line.run : tiles[number].before;
-    const uint64_t end = line.run ? min(begin + line.run, line.total) : tiles[number + 1].before;
-    uint32_t i = line.run ? line_find(tiles, line.tiles, begin) : number;
-    for (uint64_t at = begin; at < end; ++i) {
-      const LineTile l = tiles[i];
-      const uint64_t next = tiles[i + 1].before, stop = min(next, end);
-      Tile t{};
-      t.s = sequence(a, of_wave(l.sequence));
-      t.row = of_wave(l.row);
-      Range r = keys_of(a, t.s, t.row);
-      const bool whole = at == l.before && stop == next;
-      if (!whole) {   // (a tile that is cut has more than one tile of keys)
-        const int32_t lo = r.lo;
-        r.lo = lo + (int32_t)of_wave((uint32_t)(at - l.before)) * kKeys;
-        r.hi = min(r.hi, lo + (int32_t)of_wave((uint32_t)(stop - l.before)) * kKeys);
-      }
-      attend<MOD>(a, shared, head, t, r, whole ? nullptr : line_part(a, head, number, at == l.before));
-      __syncthreads();
-      at = stop;
+    const Cut cut(a);
+    if (number >= cut.items[a.sequences]) return;
+    const uint32_t b = find_sequence(cut.items, a.sequences, number), parts = cut.parts[b], rest = number - cut.items[b];
+    Tile t{};
+    t.s = sequence(a, of_wave(cut.sequence[b]));
+    if (t.s.tiles == 0) return;
+    const uint32_t part = rest / t.s.tiles;
+    if (part >= parts) return;   // (starts that decrease)
+    t.row = (t.s.tiles - 1 - (rest - part * t.s.tiles)) * kRows;
+    Range r = keys_of(a, t.s, t.row);
+    if (parts > 1 && r.lo < r.hi) {   // (unsigned: a part may begin behind the last key)
+      const uint32_t each = cut.each[b] * kKeys, from = (uint32_t)r.lo + part * each;
+      r.lo = (int32_t)min(from, (uint32_t)r.hi);
+      r.hi = (int32_t)min((uint64_t)from + each, (uint64_t)(uint32_t)r.hi);
     }
+    attend<MOD>(a, shared, head, t, r, parts > 1 ? part_of(a, head, number) : nullptr);
   }
 }
 
-// The parts of the query tile that run number `from` begins and others go on with, joined: a wave for each of kJoinRows rows.
-constexpr uint32_t kJoinRows = 16;
+// The parts of a query tile, joined, kJoinRows rows by a workgroup, two by a wave.
+constexpr uint32_t kJoinRows = 8;
 __global__ __launch_bounds__(256) void prompt_join(PromptArgs a) {
+  constexpr int kOwn = 2, kDepth = 8, kPer = D / 64;   // rows of a wave, parts on their way at once, coordinates of a lane
+  typedef float values __attribute__((ext_vector_type(kPer)));
   const uint32_t lane = threadIdx.x & 63, wave = of_wave(threadIdx.x >> 6);
   const uint32_t head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, block = rest % (kRows / kJoinRows);
-  const uint32_t from = rest / (kRows / kJoinRows);
-  const Line line = *line_of(a);
-  if (!line.run || from + 1 >= line.runs) return;
-  const LineTile* const tiles = line_tiles(a);
-  const uint64_t cut = (from + 1) * line.run;
-  const uint32_t i = line_find(tiles, line.tiles, cut);
-  const LineTile l = tiles[i];
-  // a tile that begins at the cut is whole there; of one that goes on from an earlier run, that run's turn joins the parts
-  if (l.before == cut || l.before < from * line.run) return;
-  const uint32_t to = (uint32_t)((tiles[i + 1].before - 1) / line.run), parts = to - from + 1;
-  const Sequence s = sequence(a, of_wave(l.sequence));
-  const uint32_t row0 = of_wave(l.row), rows = s.queries * a.nq;
-  auto part_of = [&](uint32_t p) { return line_part(a, head, from + p, p == 0); };
-  for (uint32_t r = block * kJoinRows + wave; r < (block + 1) * kJoinRows && row0 + r < rows; r += 4) {
-    float m = kNoScore;
-    bool nan = false;
-    for (uint32_t p = lane; p < (parts + 63) / 64 * 64; p += 64) {
-      const float x = p < parts ? part_of(p)[r * 2] : kNoScore;
-      nan |= x != x;
-      m = fmax_hw(m, x);
-    }
-    m = wave_max(m);
-    if (__ballot(nan)) m = __builtin_nanf("");
-    if (m == kNoScore) m = 0.f;
-    float sum = 0.f, o[D / 64] = {};
-    for (uint32_t base = 0; base < parts; base += 64) {   // a lane for each of 64 parts: its weight
-      const float mine = base + lane < parts ? part_of(base + lane)[r * 2] : kNoScore;
-      const float weight = __builtin_amdgcn_exp2f(mine - m);
-      sum += mine == kNoScore ? 0.f : weighed(weight, part_of(base + lane)[r * 2 + 1]);
-      for (uint64_t todo = __ballot(!(mine == kNoScore)); todo;) {   // parts with a visible key
-        float w[8], x[8][D / 64];
+  const uint32_t number = rest / (kRows / kJoinRows);
+  const Cut cut(a);
+  if (number >= cut.tiles[a.sequences]) return;
+  const uint32_t b = find_sequence(cut.tiles, a.sequences, number), parts = cut.parts[b];
+  if (parts < 2) return;   // its results are in the output
+  const Sequence s = sequence(a, of_wave(cut.sequence[b]));
+  const uint32_t tile = number - cut.tiles[b], first = cut.items[b] + (s.tiles - 1 - tile);
+  if (tile >= s.tiles || first + (parts - 1) * s.tiles >= cut.items[b + 1]) return;   // (starts that decrease)
+  const uint32_t row0 = block * kJoinRows + wave * kOwn, left = s.queries * a.nq - tile * kRows;
+  if (row0 >= left) return;
+  const uint32_t own = min(left - row0, (uint32_t)kOwn);
+  auto part = [&](uint32_t p) { return part_of(a, head, first + p * s.tiles); };
+  // a lane for each part (there are 64 at most): the rows' maxima, sums and weights
+  float weight[kOwn], sum[kOwn], m[kOwn];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {   // eight parts on their way at once
-          w[k] = 0.f;
+  for (int k = 0; k < kOwn; ++k) {
+    const uint32_t r = row0 + min((uint32_t)k, own - 1);
+    const float mine = lane < parts ? part(lane)[r * 2] : kNoScore, mine_sum = lane < parts ? part(lane)[r * 2 + 1] : 0.f;
+    m[k] = wave_max(mine);
+    if (__ballot(mine != mine)) m[k] = __builtin_nanf("");
+    if (m[k] == kNoScore) m[k] = 0.f;
+    weight[k] = __builtin_amdgcn_exp2f(mine - m[k]);
+    sum[k] = wave_sum(mine == kNoScore ? 0.f : weighed(weight[k], mine_sum));
+  }
+  values o[kOwn] = {};
+  for (uint32_t p = 0; p < parts; p += kDepth) {
+    values x[kDepth][kOwn];
 #pragma unroll
-          for (int d = 0; d < D / 64; ++d) x[k][d] = 0.f;
-          if (!todo) continue;
-          const int p = __ffsll((unsigned long long)todo) - 1;
-          todo &= todo - 1;
-          w[k] = lane_value(weight, p);
-          const float* const ov = part_of(base + p) + kRows * 2 + r * D + lane * (D / 64);
+    for (int i = 0; i < kDepth; ++i)
 #pragma unroll
-          for (int d = 0; d < D / 64; ++d) x[k][d] = ov[d];
-        }
+      for (int k = 0; k < kOwn; ++k)
+        x[i][k] = *(const values*)(part(min(p + i, parts - 1)) + kRows * 2 + (row0 + min((uint32_t)k, own - 1)) * D + lane * kPer);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+    for (int i = 0; i < kDepth; ++i)
 #pragma unroll
-          for (int d = 0; d < D / 64; ++d) o[d] += weighed(w[k], x[k][d]);
+      for (int k = 0; k < kOwn; ++k) {
+        const float w = lane_value(weight[k], (int)min(p + i, parts - 1));
+#pragma unroll
+        for (int d = 0; d < kPer; ++d) o[k][d] += p + i < parts ? weighed(w, x[i][k][d]) : 0.f;   // (a part that sees no key holds zeros)
       }
-    }
-    sum = wave_sum(sum);
-    const uint32_t token = (row0 + r) / a.nq, h = head * a.nq + (row0 + r) % a.nq;
+  }
+#pragma unroll
+  for (int k = 0; k < kOwn; ++k) {
+    if ((uint32_t)k >= own) break;
+    const uint32_t row = tile * kRows + row0 + k, token = row / a.nq, h = head * a.nq + (row - token * a.nq);
     const uint64_t at = s.first_query + token;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (a.lse && lane == 0) a.lse[at * a.kv_heads * a.nq + h] = sum == 0.f ? kNoScore : (m + __builtin_amdgcn_logf(sum)) * kLn2;
-    uint16_t* const out = (uint16_t*)a.out.data + at * a.out.token_stride + h * a.out.head_stride + lane * (D / 64);
+    const float inv = sum[k] == 0.f ? 0.f : 1.f / sum[k];
+    if (a.lse && lane == 0)
+      a.lse[at * a.kv_heads * a.nq + h] = sum[k] == 0.f ? kNoScore : (m[k] + __builtin_amdgcn_logf(sum[k])) * kLn2;
+    uint16_t* const out = (uint16_t*)a.out.data + at * a.out.token_stride + h * a.out.head_stride + lane * kPer;
     if constexpr (D == 128)
-      *(uint32_t*)out = pack2(o[0] * inv, o[1] * inv);
+      *(uint32_t*)out = pack2(o[k][0] * inv, o[k][1] * inv);
     else
-      *out = (uint16_t)pack2(o[0] * inv, 0.f);
+      *out = (uint16_t)pack2(o[k][0] * inv, 0.f);
   }
 }
 
@@ -660,7 +664,7 @@ __global__ __launch_bounds__(256) void prompt_join(PromptArgs a) {
 #define PITCH_CAT(a, b, c, d) PITCH_CAT_(a, b, c, d)
 hipError_t PITCH_CAT(launch_prompt_d, PITCH_DIM, _io, PITCH_IO)(const PromptArgs& a, hipStream_t s) {
   const bool mod = a.slopes || a.cap > 0.f;
-  if (!a.runs) {
+  if (!a.places) {
     const dim3 grid(a.tiles * a.kv_heads);
     if (mod)
       prompt_attention<true, false><<<grid, dim3(256), 0, s>>>(a);
@@ -668,17 +672,17 @@ hipError_t PITCH_CAT(launch_prompt_d, PITCH_DIM, _io, PITCH_IO)(const PromptArgs
       prompt_attention<false, false><<<grid, dim3(256), 0, s>>>(a);
     return hipGetLastError();
   }
-  prompt_line<<<dim3(1), dim3(1024), 0, s>>>(a);
+  prompt_cut<<<dim3(1), dim3(1024), 0, s>>>(a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const dim3 grid((a.tiles > a.runs ? a.tiles : a.runs) * a.kv_heads);
+  const dim3 grid((a.tiles > a.most_items ? a.tiles : a.most_items) * a.kv_heads);
   if (mod)
     prompt_attention<true, true><<<grid, dim3(256), 0, s>>>(a);
   else
     prompt_attention<false, true><<<grid, dim3(256), 0, s>>>(a);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  prompt_join<<<dim3((a.runs - 1) * (kRows / kJoinRows) * a.kv_heads), dim3(256), 0, s>>>(a);
+  prompt_join<<<dim3(a.tiles * (kRows / kJoinRows) * a.kv_heads), dim3(256), 0, s>>>(a);
   return hipGetLastError();
 }
 
