@@ -28,25 +28,25 @@ struct PromptArgs {
   uint64_t parts_at;
 };
 
-#ifndef PCUT
-#define PCUT 7
-#endif
 // Rows of (token, query head of a KV head) in a query tile; the most sequences of a call whose keys may be cut into parts, and the
 // keys from which that is looked at; what writing and joining a part of 128 rows costs, in tiles of 64 keys.
-constexpr uint32_t kPromptRows = 128, kPromptCutSequences = 1024, kPromptCutKeys = 2048, kPromptCut = PCUT;
+constexpr uint32_t kPromptRows = 128, kPromptCutSequences = 1024, kPromptCutKeys = 2048, kPromptCut = 7;
 struct PromptPlan {
   uint32_t tiles, places, most_items;
   uint64_t parts_at, ws_floats;
 };
-// What the host decides: with query tiles enough for four turns of every workgroup place (two on a compute unit), each workgroup takes
-// one; else, where tiles may be long, their lengths decide on the device whether keys are cut.
+// What the host decides. Workgroups take whole query tiles where these are enough for four turns of every workgroup place (two on a
+// compute unit), or fill half of the places and belong to whole prompts, whose tiles grow in number as they grow in length. Else, where tiles may be
+// long, the lengths decide on the device whether keys are cut: two launches more, about 10 us (eight sequences of five drafted tokens
+// behind up to 32,000: 123 us; 500 and more if a workgroup has the longest by itself).
 inline PromptPlan prompt_plan(uint32_t rows, uint32_t keys, uint32_t window, uint32_t sequences, uint32_t kv_heads, uint32_t nq,
                               uint32_t dim, uint32_t cus) {
   PromptPlan p{};
   p.tiles = (uint32_t)((uint64_t)rows * nq / kPromptRows) + (sequences < rows ? sequences : rows);
   const uint32_t places = 2 * cus, seen = window && window < keys ? window : keys;
-  if (sequences > kPromptCutSequences || (uint64_t)p.tiles * kv_heads >= 4ull * places || seen < kPromptCutKeys || kv_heads > places)
-    return p;
+  const uint64_t tiles = (uint64_t)p.tiles * kv_heads;
+  if (tiles >= 4ull * places || (tiles >= places / 2 && keys < 2ull * rows)) return p;
+  if (sequences > kPromptCutSequences || seen < kPromptCutKeys || kv_heads > places) return p;
   p.places = places / kv_heads;
   p.most_items = 4 * p.places;
   p.parts_at = (sequences * 5 + 2 + 3) / 4 * 4;

@@ -1,4 +1,34 @@
 // Attention over whole prompts, for one dimension (PITCH_DIM = 64 or 128) and one 16-bit type (PITCH_IO = 1: float16, 2: bfloat16).
+//
+//   out_i = sum_j softmax(z_i)_j v_j,  z_ij = cap(scale q_i . k_j) + slope (j - p_i),  p_i = nk - nq + i,  p_i - window < j <= p_i
+//
+// Work split. The query heads of a KV head share its keys, so a row is a pair of token and head, and 128 neighbouring rows of a sequence
+// are a query tile, a workgroup's work: four waves of 32 rows, two workgroups on a compute unit. It goes over the keys 64 at a time
+// with the running maximum and sum of a softmax (Milakov and Gimelshein 2018; Rabe and Staats 2021). Workgroups that follow each other
+// have different KV heads, so that an XCD, every eighth workgroup, finds the keys of few heads in its L2; a sequence's last tiles,
+// which see most keys, come first. Grid and workspace follow from sizes that the host knows, the lengths stay on the device.
+//
+// Products. v_mfma_f32_32x32x16 gives 32 x 32 scores as K Q^T, keys down and queries across: a lane holds 16 scores of one query, its
+// partner at distance 32 the other 16, and maxima, sums and rescaling stay within the lane but for one exchange a tile. The weights
+// are then the second operand of V^T P^T as they lie, if the 16 keys of a product are taken in the order 4 h .. 4 h + 3, 8 + 4 h ..
+// 8 + 4 h + 3 in the lanes' halves h; V^T is read in that order by the transposing LDS reads (ds_read_b64_tr_b16, four keys by 16
+// coordinates). Weights are rounded to the values' type, once; scores, maxima, sums and accumulators are float32. With bfloat16 the
+// rounding of the weights is as large as the output's own, and averages like it: errors of outputs are 1.3 to 1.4 times those of
+// the exact result's rounding (0.0021 to 0.0016 of the norm; float16 0.00029 to 0.00021).
+//
+// Data. Tiles go from memory to LDS without registers (buffer_load ... lds), one ahead; chunks of 16 bytes lie swizzled, by the address that each lane asks
+// for, so that no read finds a bank conflict (the counter says none). Rows behind the sequence come back as zeros (the buffers'
+// bounds), and a mask is applied only in tiles that need one. The maximum in use lags by up to 2^8 behind a row's true one, so that
+// the accumulators are rarely rescaled; weights up to 256 are as exact as those below 1.
+//
+// What bounds it. 16,381 tokens of 8 KV and 32 query heads of 128, bfloat16, causal: 2.02 ms, 1,090 TFLOP/s, where a large library
+// product reaches 1,400. Matrix instructions are on their way in 55 % of the cycles; the rest is mostly the softmax, 32 exponentials and about 120
+// other vector instructions for each 32 matrix instructions. The card lowers its clock under this load (1.9 GHz): a step that took 12 % of the
+// cycles out took 8 % of the time. Fourteen ragged prompts of up to 3,000 tokens 409 us (880 TFLOP/s): a workgroup's beginning and end
+// cost about two tiles of keys. Heads of 64 with soft caps are bound by the softmax's instructions (three of the
+// quarter-rate kind a score). Slower were: 64 rows a wave (half the LDS reads, but one wave a SIMD), eight waves that share a tile's keys by twos
+// (2,250 us; the waves keep step), two tiles an iteration (2,110 us, spills), and skipping of tiles that all rows of a wave are blind
+// to (no change). Queries that are waited for inside the loop cost 14 % (the counter of loads also counts the tiles on their way).
 #include "pitch_attn_shared.h"
 #include "pitch_prompt.h"
 
@@ -13,8 +43,8 @@ namespace pitch {
 namespace {
 
 constexpr int D = PITCH_DIM;
-constexpr int kWaves = 4;            // of a group, 32 rows each
-constexpr int kRows = kWaves * 32;  // rows of a tile of queries
+constexpr int kWaves = 4;            // of a workgroup, 32 rows each
+constexpr int kRows = kWaves * 32;   // rows of a query tile
 constexpr int kKeys = 64;            // keys of a tile
 constexpr int kSteps = D / 16;       // steps of the contraction over the coordinates
 constexpr int kBlocks = D / 32;      // blocks of 32 output coordinates
@@ -52,7 +82,8 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
 __device__ __forceinline__ uint32_t of_wave(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // x *= f where `go` is not zero. The branch is inside the statement: with one around it, the compiler keeps two copies of the
-// accumulators and moves them, 64 registers there and back for every tile (2,190 us of a prompt of 16,381 tokens, 8 KV and 32 query heads; XXX without).
+// accumulators and moves them, 64 registers there and back for every tile (2,190 us for 16,381 tokens; 2,016 without, and with maxima of
+// three).
 // Waits: 16 states behind the matrix instructions that wrote x, two before those that read it.
 __device__ __forceinline__ void scale_where(uint64_t go, float f, v16f& x) {
   float y[16];
@@ -147,7 +178,8 @@ __device__ __forceinline__ Range keys_of(const PromptArgs& a, const Sequence& s,
 // Where query tiles are few, or of very different lengths, the keys of a sequence are cut into parts, the same for all of its tiles, and
 // a workgroup takes one part of one tile: it leaves maxima, sums and values in the workspace, and prompt_join puts a tile's parts
 // together, in their order. Parts of a sequence are numbered part by part and within one tile by tile, so that workgroups that run at the
-// same time read the same keys (a line of tiles cut into equal runs, each at other keys, found a fifth of its reads in L2 and took XXX).
+// same time read the same keys (all tiles as one line, cut into equal runs at keys of their own, found a fifth of their reads in L2: eight
+// chunks of up to 500 tokens behind up to 8,000, 245 us without the join, 217 so).
 struct Cut {   // the workspace's first part: for each sequence, those with the longest parts first
   uint32_t* items;     // [sequences + 1] parts of tiles before its own
   uint32_t* tiles;     // [sequences + 1] tiles before its own
@@ -570,6 +602,9 @@ __device__ __forceinline__ void attend(const PromptArgs& a, Shared& shared, uint
 template <bool MOD, bool CUT>
 __global__ __launch_bounds__(256, 2) void prompt_attention(PromptArgs a) {
   __shared__ Shared shared;
+  // Of the waves that share a SIMD (one of each workgroup on the compute unit) those in odd places go first, so that one's softmax
+  // falls together with the other's matrix instructions: 16 sequences in a window 35.3 us without, 31.6 with; chunks 246, 237.
+  if (__builtin_amdgcn_s_getreg((3 << 11) | 4) & 1) __builtin_amdgcn_s_setprio(1);   // (the wave's place: four bits of HW_ID)
   const uint32_t head = blockIdx.x % a.kv_heads, number = blockIdx.x / a.kv_heads;
   if constexpr (!CUT) {
     const Tile t = find_tile(a, number);
@@ -603,7 +638,7 @@ __global__ __launch_bounds__(256) void prompt_join(PromptArgs a) {
   const uint32_t head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, block = rest % (kRows / kJoinRows);
   const uint32_t number = rest / (kRows / kJoinRows);
   const Cut cut(a);
-  if (number >= cut.tiles[a.sequences]) return;
+  if (number >= cut.tiles[a.sequences] || cut.items[a.sequences] == cut.tiles[a.sequences]) return;
   const uint32_t b = find_sequence(cut.tiles, a.sequences, number), parts = cut.parts[b];
   if (parts < 2) return;   // its results are in the output
   const Sequence s = sequence(a, of_wave(cut.sequence[b]));
