@@ -1784,8 +1784,9 @@ int pitch_enqueue_prompt_attention(const pitch_prompt_attention_t* call, void* s
     a.pre = (float)to_log2;
     a.c = 1.f;
     a.cap = (float)std::min(cap, kMost);
-    const double cap_r = call->softcap > 0.f ? 2.0 * kLog2E * call->scale / call->softcap : 0.0;   // e^(2 scale x / softcap) as a power of two
-    a.cap_r = (float)std::max(-kMost, std::min(kMost, cap_r));
+    const double k = call->softcap > 0.f ? (double)call->scale / call->softcap : 0.0;
+    a.cap_k = (float)std::max(-kMost, std::min(kMost, k));
+    a.cap_r = (float)std::max(-kMost, std::min(kMost, 2.0 * kLog2E * k));
   } else {
     a.negate = call->scale < 0.f;
     a.c = (float)std::max(std::abs(to_log2), 1e-37);

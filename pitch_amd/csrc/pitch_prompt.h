@@ -21,7 +21,7 @@ struct PromptArgs {
   uint32_t negate;            // 1: a negative scale, whose sign the queries take
   float c;                    // |scale| log2(e): scores to log2 units (1 with a cap or slopes, which give such units)
   float pre;                  // with a cap or slopes: what a product is multiplied by first
-  float cap, cap_r;           // with a positive cap, products x give cap * tanh(x'), e^(2 x') = 2^(x * cap_r), in log2 units
+  float cap, cap_k, cap_r;    // with a positive cap, products s give cap * tanh(x), x = s * cap_k, e^2x = 2^(s * cap_r), in log2 units
   uint32_t tiles;             // an upper bound of the query tiles of a KV head
   uint32_t places;            // workgroups of a KV head that run at once, where keys may be cut into parts; 0: they are not
   uint32_t most_items;        // parts of a KV head's tiles that the workspace has room for, where any are cut

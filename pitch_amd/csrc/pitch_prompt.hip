@@ -53,6 +53,7 @@ constexpr int kLaneRows = 1024 / (D * 2);            // rows of a tile that a wa
 constexpr int kLoads = kKeys / (kLaneRows * kWaves); // loads of a wave for a tile of keys or values
 constexpr float kGrow = 8.f;         // log2 units that a row's scores may exceed the maximum in use by
 constexpr float kNoScore = -__builtin_inff();
+constexpr float kTanhSplit = 0.55f;
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -81,6 +82,20 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
 }
 __device__ __forceinline__ uint32_t of_wave(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 
+__device__ __forceinline__ float fmax3_abs(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// pre s tanh(x) / x, x = k s, for |x| below kTanhSplit: an even polynomial fitted at Chebyshev's points.
+__device__ __forceinline__ float capped(float s, float k, float pre) {
+  const float x = s * k, t = x * x, z = s * pre;
+  float f = __builtin_fmaf(t, -0x1.b191fep-8f, 0x1.5d3024p-6f);
+  f = __builtin_fmaf(t, f, -0x1.b9a19ap-5f);
+  f = __builtin_fmaf(t, f, 0x1.110ff0p-3f);
+  f = __builtin_fmaf(t, f, -0x1.555554p-2f);
+  return __builtin_fmaf(z * t, f, z);
+}
 // x *= f where `go` is not zero. The branch is inside the statement: with one around it, the compiler keeps two copies of the
 // accumulators and moves them, 64 registers there and back for every tile (2,190 us for 16,381 tokens; 2,016 without, and with maxima of
 // three).
@@ -386,17 +401,36 @@ __device__ __forceinline__ void attend(const PromptArgs& a, Shared& shared, uint
         s[b] = mfma(k, q[i], s[b]);
       }
     }
+    // (the compiler does not see that the statements below read what matrix instructions write: 16 wait states, 11 are needed)
+    asm("s_nop 7\n\ts_nop 7" : "+v"(s[0]), "+v"(s[1]));
     if constexpr (MOD) {
+      if (a.cap > 0.f) {
+        // cap tanh(x) = (cap x) (tanh(x) / x): a polynomial in x^2 below 0.55 (6e-9 off; the usual case, and exact to float32 for caps
+        // of any size), above that 1 - 2 / (e^2x + 1), which would lose digits to the 1 for small x
+        float big = 0.f;
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+        for (int r = 0; r < 16; ++r) big = fmax3_abs(big, s[0][r], s[1][r]);
+        const float k = a.cap_k, pre = a.pre;
+        if (__ballot(big * __builtin_fabsf(k) >= kTanhSplit)) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          // tanh(x) = 1 - 2 / (e^2x + 1)
-          if (a.cap > 0.f)
-            s[b][r] = __builtin_fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[b][r] * a.cap_r) + 1.f), a.cap);
-          else
-            s[b][r] *= a.pre;
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float e = __builtin_amdgcn_exp2f(s[b][r] * a.cap_r), y = __builtin_fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(e + 1.f), a.cap);
+              s[b][r] = __builtin_fabsf(s[b][r] * k) < kTanhSplit ? capped(s[b][r], k, pre) : y;
+            }
+        } else {
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[b][r] = capped(s[b][r], k, pre);
         }
+      } else {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[b][r] *= a.pre;
+      }
       if (a.slopes) {
         const int32_t away = (int32_t)((uint32_t)k0 + half * 4 - (uint32_t)offset - token_in);
 #pragma unroll
@@ -424,8 +458,6 @@ __device__ __forceinline__ void attend(const PromptArgs& a, Shared& shared, uint
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[b][r] = s[b][r] > kNoScore ? 1.f : 0.f;
     } else {
-      // (the compiler does not see that the maxima below read what matrix instructions write: 16 wait states, 11 are needed)
-      asm("s_nop 7\n\ts_nop 7" : "+v"(s[0]), "+v"(s[1]));
       float top = fmax3_hw(s[0][0], s[1][0], s[0][1]);
       float top2 = fmax3_hw(s[1][1], s[0][2], s[1][2]);
 #pragma unroll
@@ -600,7 +632,7 @@ __device__ __forceinline__ void attend(const PromptArgs& a, Shared& shared, uint
 }
 
 template <bool MOD, bool CUT>
-__global__ __launch_bounds__(256, 2) void prompt_attention(PromptArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prompt_attention(PromptArgs a) {
   __shared__ Shared shared;
   // Of the waves that share a SIMD (one of each workgroup on the compute unit) those in odd places go first, so that one's softmax
   // falls together with the other's matrix instructions: 16 sequences in a window 35.3 us without, 31.6 with; chunks 246, 237.

@@ -48,9 +48,12 @@ def reference(q, k, v, row_starts, key_starts, causal=True, scale=None, softcap=
             weighed = torch.where(w[:, :, None] > 0, w[:, :, None] * values[None], 0.0) if not torch.isfinite(values).all() else None
             out[r0:r1, h] = weighed.sum(1) if weighed is not None else w @ values
             lse[r0:r1, h] = (top + torch.log(total))[:, 0]
-            # a score's error: dim + 4 roundings of float32 of its terms, and for a cap the tanh's (two exponentials, a quotient)
+            # a score's error: dim + 4 roundings of float32 of its terms, and for a cap the tanh's (an exponential, a quotient and a
+            # difference of half their size at least, or a polynomial: at most 16 roundings of the score)
             off = ((dim + 4) * eps * size).amax(-1, keepdim=True) if nk else torch.zeros((nq, 1), dtype=torch.float64)
-            off = off + 16 * eps * (1 + softcap)
+            if nk and softcap:
+                off = off + 16 * eps * torch.where(seen, z, 0.0).abs().amax(-1, keepdim=True)
+            off = off + 16 * eps
             # the weights' rounding, their own error, the sums' (one rounding a term at most); float16 weights below 2^-14 have
             # steps of 2^-24, against a sum of 1 at least
             a = w @ values.abs().nan_to_num(0, 0, 0)

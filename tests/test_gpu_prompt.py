@@ -62,6 +62,14 @@ def test_masks_and_scores(q, dim, more):
         _check(q, MIXED, 6, 2, dim, dtype, seed=1, **more)
 
 
+@pytest.mark.parametrize("softcap", [1e-30, 1e-3, 0.1, 1.0, 100.0, 1e4, 1e20, 3e38])
+def test_soft_caps_of_any_size(q, softcap):
+    """A cap far above the scores leaves them as they are, one far below makes them signs."""
+    for dtype in TYPES:
+        _check(q, [(1, 1), (40, 90), (3, 3)], 4, 2, 64, dtype, seed=34, softcap=softcap)
+        _check(q, [(70, 70)], 2, 1, 128, dtype, seed=35, softcap=softcap, scale=-0.4)
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("window,softcap", [(0, 0.0), (50, 0.0), (0, 20.0)])
 def test_slopes(q, dim, window, softcap):
