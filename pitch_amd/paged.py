@@ -277,15 +277,21 @@ class WorkspaceCall:
             self._admit(stream, handle)
         return handle
 
+    def _stream(self, stream, handle: int):
+        """The torch stream of a call's stream."""
+        torch = _torch()
+        if stream is None:
+            return torch.cuda.current_stream(self._device)
+        if isinstance(stream, torch.cuda.Stream):
+            return stream
+        return torch.cuda.ExternalStream(handle, device=self._device) if handle else torch.cuda.default_stream(self._device)
+
     def _admit(self, stream, handle: int) -> None:
         """Lets another stream use a workspace allocated here: behind the work that the allocation's stream holds (the memory may
         have been freed by it just before), and known to torch's allocator, which else hands it out again on its own stream
         as soon as this object is gone."""
         torch = _torch()
-        if stream is None:
-            stream = torch.cuda.current_stream(self._device)
-        elif not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(handle, device=self._device) if handle else torch.cuda.default_stream(self._device)
+        stream = self._stream(stream, handle)
         self._workspace.record_stream(stream)
         with torch.cuda.stream(stream):
             capturing = torch.cuda.is_current_stream_capturing()

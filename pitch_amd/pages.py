@@ -27,14 +27,14 @@ class PagedTables(WorkspaceCall):
     def __init__(self, caches, sequences: int | None = None, width: int | None = None, blockTables=None, lengths=None, references=None,
                  missing=None):
         torch = _torch()
-        self.caches = [caches] if isinstance(caches, PagedCache) else list(caches)
+        self.caches = [caches] if isinstance(caches, PagedCache) else list(caches) if isinstance(caches, (list, tuple)) else []
         if not self.caches or not all(isinstance(c, PagedCache) for c in self.caches):
             raise InvalidInput("caches must be PagedCache objects, at least one")
         first = self.caches[0]
         self.pitch, self.pages, self.pageSize = first.pitch, first.pages, first.pageSize
         if any((c.pages, c.pageSize) != (self.pages, self.pageSize) for c in self.caches):
             raise InvalidInput("all caches need as many pages of the same size")
-        device = self.pitch.device
+        device, given = self.pitch.device, blockTables is not None
         if blockTables is None:
             if sequences is None or width is None:
                 raise InvalidInput("sequences and width are needed where blockTables is not given")
@@ -44,8 +44,15 @@ class PagedTables(WorkspaceCall):
         c = _lib.PitchPagedTablesC()
         c.block_tables, c.block_tables_bytes = _tables(blockTables)
         self.sequences, self.width = blockTables.shape
-        given = lambda t, n: torch.zeros(n, dtype=torch.int32, device=device) if t is None else t  # noqa: E731
-        lengths, references, missing = given(lengths, self.sequences), given(references, self.pages), given(missing, 1)
+        made = [] if given else [blockTables]   # what is allocated here, as the workspace is
+
+        def zeros(n):
+            made.append(torch.zeros(n, dtype=torch.int32, device=device))
+            return made[-1]
+
+        lengths = zeros(self.sequences) if lengths is None else lengths
+        references = zeros(self.pages) if references is None else references
+        missing = zeros(1) if missing is None else missing
         c.lengths, c.lengths_bytes = _flat(lengths, "lengths", torch.int32, self.sequences)
         c.references, c.references_bytes = _flat(references, "references", torch.int32, self.pages)
         c.missing, c.missing_bytes = _flat(missing, "missing", torch.int32, 1)
@@ -54,6 +61,7 @@ class PagedTables(WorkspaceCall):
         needed = ctypes.c_uint64(0)
         _raise_for(self.pitch._lib.pitch_paged_tables_workspace_size(ctypes.byref(c), ctypes.byref(needed)))
         self._hold_workspace(c, None, int(needed.value), device)
+        self._made = made
         self._cstruct, self._device = c, device
         self._layers = (_lib.PitchPagedCacheC * len(self.caches))(*[cache._cstruct for cache in self.caches])
 
@@ -72,6 +80,11 @@ class PagedTables(WorkspaceCall):
     def enqueueCompact(self, mapping=None, used=None, stream=None) -> None:
         """One PagedCompact call."""
         PagedCompact(self, mapping=mapping, used=used).enqueue(stream)
+
+    def _admit(self, stream, handle: int) -> None:
+        super()._admit(stream, handle)
+        for t in self._made:
+            t.record_stream(self._stream(stream, handle))
 
 
 class _TablesCall:
@@ -101,8 +114,8 @@ class PagedReserve(_TablesCall):
         torch = _torch()
         c = _lib.PitchPagedReserveC()
         c.new_tokens, c.new_tokens_bytes = _flat(newTokens, "newTokens", torch.int32, tables.sequences)
+        c.capacity = _device_tensor(slots, "slots", (torch.int64,)).numel()
         c.slots, c.slots_bytes = _flat(slots, "slots", torch.int64, None)
-        c.capacity = slots.numel()
         c.positions, c.positions_bytes = _flat(positions, "positions", torch.int64, c.capacity)
         self._held, self._call, self._ref = (newTokens, slots, positions), c, ctypes.byref(c)
 
