@@ -53,7 +53,9 @@ struct PagesLayer {
   uint32_t head_major;
 };
 constexpr uint32_t kPagesLayers = 48;  // of a launch: its arguments hold them
-constexpr uint32_t kPagesSlice = 1u << 16;  // bytes of a layer's page that a workgroup copies at a time
+// Bytes of a layer's page that a workgroup copies at a time. One index over all pieces of a page instead, divided for each: 642 us where
+// slices of buffers take 408 to 470 (1.1 GB).
+constexpr uint32_t kPagesSlice = 1u << 16;
 struct PagesCopyArgs {
   const uint32_t* count;   // pages to copy
   const uint32_t* source;  // page numbers

@@ -4,6 +4,12 @@
 // Free pages are ranked, not listed: a pool's references are counted in segments by one launch, and the next gives page number k
 // among the free ones to the k-th place that needs a page. Every order is that of the numbers, never that of arrival: the same state
 // gives the same pages. Counts of references change by atomic additions, whose order does not matter.
+//
+// What bounds it. Bookkeeping is a chain of dependent reads of a few KB: a launch takes 3 to 8 us on the device, and a call of one or
+// two of them the 8 to 10 us of the host. 64 sequences of about 3,000 tokens that reserve up to 2,000 each in pages of 16, of 40,000,
+// and give some back: 13.7 us (plan 3.4, places 7.8, trim 3.0). 64 beams of 1,000 tokens, 32 layers: 26 us, 14 of them the copies of
+// their last pages. A pool of 2,000 pages of 32 layers, 1.1 GB of which move: 410 to 475 us on different cards, the copies at the rate
+// of a large copy (4.7 to 5.5 TB/s), and 10 us for the bookkeeping.
 #include "pitch_pages.h"
 
 namespace pitch {
@@ -12,7 +18,9 @@ namespace {
 constexpr uint32_t kThreads = 256, kOneThreads = 1024, kMostWaves = kOneThreads / 64;
 constexpr uint32_t kMostSequences = 2048;
 // The largest calls whose bookkeeping one workgroup does, in one launch: it costs the host about 2 us less for each launch saved, but
-// a workgroup's wave turns to one row, or to 64 pages, after the other.
+// a workgroup's wave turns to one row, or to 64 pages, after the other. Kernels' times, one workgroup against several launches: reserve of
+// 4,096 pages 5.0 us against 5.9 and a launch more; a fork of 64 rows 17.0 against 10.3 (so the limit on rows), of 8 rows a call of 9.8
+// against 15.8; a compaction of 2,000 pages 9.5 against 13.8.
 constexpr uint32_t kReserveOnePages = 4096, kReserveOneRows = 256, kReserveOneTokens = 4096;
 constexpr uint32_t kForkOnePages = 4096, kForkOneRows = 16;
 constexpr uint32_t kCompactOnePages = 4096, kCompactOneRows = 64;
@@ -204,9 +212,9 @@ __device__ __forceinline__ void reserve_pages(const PagesReserveArgs& a, const R
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   // the pages' tokens, 64 at a time whatever the page's size
-  const uint64_t all = (uint64_t)__popcll(mask) * page;
-  for (uint64_t i = lane; i < all; i += 64) {
-    const uint32_t k = (uint32_t)(i / page), at = (uint32_t)(i - (uint64_t)k * page);
+  const uint32_t all = __popcll(mask) * page;   // (at most 64 pages of 65,536)
+  for (uint32_t i = lane; i < all; i += 64) {
+    const uint32_t k = i / page, at = i - k * page;
     const Handed h = handed[k];
     if (at >= h.tokens) continue;
     a.slots[h.from + at] = (int64_t)((uint64_t)h.page * page + at);
@@ -657,7 +665,8 @@ hipError_t launch_pages_copy(const PagesCopyArgs& call, uint32_t cus, hipStream_
   PagesCopyArgs a = call;
   const uint64_t slices = (uint64_t)a.most * a.layers * a.slices, most = 8ull * cus;
   if (slices == 0) return hipSuccess;
-  // Where there are few slices, a workgroup takes one buffer of a slice: the four do not wait for each other.
+  // Where there are few slices, a workgroup takes one buffer of a slice: the four do not wait for each other (two pages of 12 layers
+  // 4.0 us instead of 5.4). Where there are many, a unit of all four costs fewer divisions and looks at its pages' numbers once.
   a.parts = slices < 2ull * cus ? 4 : 1;
   const uint64_t units = slices * a.parts;
   pages_copy<<<dim3((uint32_t)(units < most ? units : most)), dim3(kThreads), 0, s>>>(a);
