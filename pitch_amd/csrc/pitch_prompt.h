@@ -36,9 +36,9 @@ struct PromptPlan {
   uint64_t parts_at, ws_floats;
 };
 // What the host decides. Workgroups take whole query tiles where these are enough for four turns of every workgroup place (two on a
-// compute unit), or fill half of the places and belong to whole prompts, whose tiles grow in number as they grow in length. Else, where tiles may be
-// long, the lengths decide on the device whether keys are cut: two launches more, about 10 us (eight sequences of five drafted tokens
-// behind up to 32,000: 123 us; 500 and more if a workgroup has the longest by itself).
+// compute unit), or fill half of the places and belong to whole prompts, whose tiles grow in number as they grow in length. Else, where
+// tiles may be long, the lengths decide on the device whether keys are cut: two launches more, about 10 us (eight sequences of five
+// drafted tokens behind up to 32,000: 123 us; 500 and more if a workgroup has the longest by itself).
 inline PromptPlan prompt_plan(uint32_t rows, uint32_t keys, uint32_t window, uint32_t sequences, uint32_t kv_heads, uint32_t nq,
                               uint32_t dim, uint32_t cus) {
   PromptPlan p{};

@@ -16,19 +16,21 @@
 // rounding of the weights is as large as the output's own, and averages like it: errors of outputs are 1.3 to 1.4 times those of
 // the exact result's rounding (0.0021 to 0.0016 of the norm; float16 0.00029 to 0.00021).
 //
-// Data. Tiles go from memory to LDS without registers (buffer_load ... lds), one ahead; chunks of 16 bytes lie swizzled, by the address that each lane asks
-// for, so that no read finds a bank conflict (the counter says none). Rows behind the sequence come back as zeros (the buffers'
-// bounds), and a mask is applied only in tiles that need one. The maximum in use lags by up to 2^8 behind a row's true one, so that
-// the accumulators are rarely rescaled; weights up to 256 are as exact as those below 1.
+// Data. Tiles go from memory to LDS without registers (buffer_load ... lds), one ahead; chunks of 16 bytes lie swizzled, by the address
+// that each lane asks for, so that no read finds a bank conflict (the counter says none). Rows behind the sequence come back as zeros
+// (the buffers' bounds), and a mask is applied only in tiles that need one. The maximum in use lags by up to 2^8 behind a row's true
+// one, so that the accumulators are rarely rescaled; weights up to 256 are as exact as those below 1.
 //
-// What bounds it. 16,381 tokens of 8 KV and 32 query heads of 128, bfloat16, causal: 2.02 ms, 1,090 TFLOP/s, where a large library
-// product reaches 1,400. Matrix instructions are on their way in 55 % of the cycles; the rest is mostly the softmax, 32 exponentials and about 120
-// other vector instructions for each 32 matrix instructions. The card lowers its clock under this load (1.9 GHz): a step that took 12 % of the
-// cycles out took 8 % of the time. Fourteen ragged prompts of up to 3,000 tokens 409 us (880 TFLOP/s): a workgroup's beginning and end
-// cost about two tiles of keys. Heads of 64 with soft caps are bound by the softmax's instructions (three of the
-// quarter-rate kind a score). Slower were: 64 rows a wave (half the LDS reads, but one wave a SIMD), eight waves that share a tile's keys by twos
-// (2,250 us; the waves keep step), two tiles an iteration (2,110 us, spills), and skipping of tiles that all rows of a wave are blind
-// to (no change). Queries that are waited for inside the loop cost 14 % (the counter of loads also counts the tiles on their way).
+// What bounds it. 16,381 tokens of 8 KV and 32 query heads of 128, bfloat16, causal: 2.02 to 2.12 ms on different cards, up to 1,090
+// TFLOP/s, where a large library product reaches 1,400. Matrix instructions are on their way in 57 % of the cycles; the rest is mostly
+// the softmax, 32 exponentials and about 120 other vector instructions for each 32 matrix instructions. The card lowers its clock under
+// this load (1.9 GHz): a step that took 12 % of the cycles out took 8 % of the time. Fourteen ragged prompts of up to 3,000 tokens
+// 409 us (880 TFLOP/s): a workgroup's beginning and end cost about two tiles of keys. Heads of 64 with soft caps in a window, 30 us,
+// are bound by vector instructions (three in four cycles): the cap's polynomial, eight a score, and the softmax. Slower were: 64 rows a
+// wave (half the LDS reads, but one wave a SIMD); eight waves that share a tile of keys for 256 rows (2,050 us instead of 2,100, but
+// 47 instead of 30 in the window and 137 instead of 124 for drafts) or by twos (2,250 us; the waves keep step); two tiles an iteration
+// (2,110 us, spills); and skipping of tiles that all rows of a wave are blind to (no change). Queries that are waited for inside
+// the loop cost 14 % (the counter of loads also counts the tiles on their way).
 #include "pitch_attn_shared.h"
 #include "pitch_prompt.h"
 
@@ -194,7 +196,7 @@ __device__ __forceinline__ Range keys_of(const PromptArgs& a, const Sequence& s,
 // a workgroup takes one part of one tile: it leaves maxima, sums and values in the workspace, and prompt_join puts a tile's parts
 // together, in their order. Parts of a sequence are numbered part by part and within one tile by tile, so that workgroups that run at the
 // same time read the same keys (all tiles as one line, cut into equal runs at keys of their own, found a fifth of their reads in L2: eight
-// chunks of up to 500 tokens behind up to 8,000, 245 us without the join, 217 so).
+// chunks of up to 500 tokens behind up to 8,000, 245 us without the join, 217 so; with all 240).
 struct Cut {   // the workspace's first part: for each sequence, those with the longest parts first
   uint32_t* items;     // [sequences + 1] parts of tiles before its own
   uint32_t* tiles;     // [sequences + 1] tiles before its own
@@ -232,7 +234,7 @@ __global__ __launch_bounds__(1024) void prompt_cut(PromptArgs a) {
   uint64_t my_cost = 0, my_items = 0;
   const uint32_t here = min(max((int32_t)(a.sequences - wave * 64), 0), 64);
   for (uint32_t k = 0; k < here; ++k) {
-    const uint32_t u = __builtin_amdgcn_readlane(units, k), n = __builtin_amdgcn_readlane(s.tiles, k), j = __builtin_amdgcn_readlane(join, k);
+    const uint32_t u = of_lane(units, k), n = of_lane(s.tiles, k), j = of_lane(join, k);
     if (n == 0) continue;
     const uint32_t parts = (u + run - 1) / run;
     my_items += (uint64_t)n * parts;
@@ -244,7 +246,8 @@ __global__ __launch_bounds__(1024) void prompt_cut(PromptArgs a) {
   }
   __syncthreads();
   // the cheapest candidate that the workspace has room for, the same in every wave; uncut is always possible
-  float best = items[lane] <= a.places ? 16.f * (float)run + 32.f + kPromptCut * 16.f : (float)cost[lane] / (float)a.places + 8.f * (float)run;
+  float best = items[lane] <= a.places ? 16.f * (float)run + 32.f + kPromptCut * 16.f
+                                       : (float)cost[lane] / (float)a.places + 8.f * (float)run;
   if (lane > 0 && items[lane] > a.most_items) best = __builtin_inff();
   uint32_t choice = run;
 #pragma unroll
@@ -416,7 +419,8 @@ __device__ __forceinline__ void attend(const PromptArgs& a, Shared& shared, uint
           for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-              const float e = __builtin_amdgcn_exp2f(s[b][r] * a.cap_r), y = __builtin_fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(e + 1.f), a.cap);
+              const float e = __builtin_amdgcn_exp2f(s[b][r] * a.cap_r);
+              const float y = __builtin_fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(e + 1.f), a.cap);
               s[b][r] = __builtin_fabsf(s[b][r] * k) < kTanhSplit ? capped(s[b][r], k, pre) : y;
             }
         } else {
@@ -661,14 +665,15 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prompt_attention(PromptA
   }
 }
 
-// The parts of a query tile, joined, kJoinRows rows by a workgroup, two by a wave.
-constexpr uint32_t kJoinRows = 8;
-__global__ __launch_bounds__(256) void prompt_join(PromptArgs a) {
-  constexpr int kOwn = 2, kDepth = 8, kPer = D / 64;   // rows of a wave, parts on their way at once, coordinates of a lane
-  typedef float values __attribute__((ext_vector_type(kPer)));
+// The parts of a query tile, joined: a lane has four coordinates of a row, a wave as many rows as it has lanes for, so many times one
+// after the other. A workgroup's beginning is a chain of five reads, which four turns share where there are workgroups enough (chunks:
+// 26 us, with one turn 28 to 33; a join of few rows 7.4 either way, but then a workgroup should not take more than it must).
+constexpr uint32_t kRowLanes = D / 4, kWaveRows = 64 / kRowLanes, kJoinRows = 4 * kWaveRows;
+__global__ __launch_bounds__(256) void prompt_join(PromptArgs a, uint32_t turns) {
+  constexpr uint32_t kDepth = 8;   // parts on their way at once
   const uint32_t lane = threadIdx.x & 63, wave = of_wave(threadIdx.x >> 6);
-  const uint32_t head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, block = rest % (kRows / kJoinRows);
-  const uint32_t number = rest / (kRows / kJoinRows);
+  const uint32_t blocks = kRows / kJoinRows / turns;   // of a query tile
+  const uint32_t head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, block = rest % blocks, number = rest / blocks;
   const Cut cut(a);
   if (number >= cut.tiles[a.sequences] || cut.items[a.sequences] == cut.tiles[a.sequences]) return;
   const uint32_t b = find_sequence(cut.tiles, a.sequences, number), parts = cut.parts[b];
@@ -676,52 +681,67 @@ __global__ __launch_bounds__(256) void prompt_join(PromptArgs a) {
   const Sequence s = sequence(a, of_wave(cut.sequence[b]));
   const uint32_t tile = number - cut.tiles[b], first = cut.items[b] + (s.tiles - 1 - tile);
   if (tile >= s.tiles || first + (parts - 1) * s.tiles >= cut.items[b + 1]) return;   // (starts that decrease)
-  const uint32_t row0 = block * kJoinRows + wave * kOwn, left = s.queries * a.nq - tile * kRows;
-  if (row0 >= left) return;
-  const uint32_t own = min(left - row0, (uint32_t)kOwn);
-  auto part = [&](uint32_t p) { return part_of(a, head, first + p * s.tiles); };
-  // a lane for each part (there are 64 at most): the rows' maxima, sums and weights
-  float weight[kOwn], sum[kOwn], m[kOwn];
+  const uint32_t left = s.queries * a.nq - tile * kRows;
+  for (uint32_t turn = 0; turn < turns; ++turn) {
+    const uint32_t row0 = (block * turns + turn) * kJoinRows + wave * kWaveRows;
+    if (row0 >= left) return;
+    const uint32_t own = min(left - row0, kWaveRows), mine = lane / kRowLanes;   // the wave's rows, the lane's among them
+    const uint32_t at = kRows * 2 + (row0 + min(mine, own - 1)) * D + lane % kRowLanes * 4;
+    auto part = [&](uint32_t p) { return part_of(a, head, first + p * s.tiles); };
+    v4f x[kDepth];
+    auto read = [&](uint32_t p) {
 #pragma unroll
-  for (int k = 0; k < kOwn; ++k) {
-    const uint32_t r = row0 + min((uint32_t)k, own - 1);
-    const float mine = lane < parts ? part(lane)[r * 2] : kNoScore, mine_sum = lane < parts ? part(lane)[r * 2 + 1] : 0.f;
-    m[k] = wave_max(mine);
-    if (__ballot(mine != mine)) m[k] = __builtin_nanf("");
-    if (m[k] == kNoScore) m[k] = 0.f;
-    weight[k] = __builtin_amdgcn_exp2f(mine - m[k]);
-    sum[k] = wave_sum(mine == kNoScore ? 0.f : weighed(weight[k], mine_sum));
-  }
-  values o[kOwn] = {};
-  for (uint32_t p = 0; p < parts; p += kDepth) {
-    values x[kDepth][kOwn];
+      for (uint32_t i = 0; i < kDepth; ++i) x[i] = *(const v4f*)(part(min(p + i, parts - 1)) + at);
+    };
+    read(0);
+    // a lane for each part (there are 64 at most): the rows' maxima, sums and weights
+    float weight[kWaveRows], sum = 0.f, m = 0.f;
 #pragma unroll
-    for (int i = 0; i < kDepth; ++i)
+    for (uint32_t k = 0; k < kWaveRows; ++k) {
+      const uint32_t r = row0 + min(k, own - 1);
+      const float top = lane < parts ? part(lane)[r * 2] : kNoScore, total = lane < parts ? part(lane)[r * 2 + 1] : 0.f;
+      float most = wave_max(top);
+      if (__ballot(top != top)) most = __builtin_nanf("");
+      if (most == kNoScore) most = 0.f;
+      weight[k] = __builtin_amdgcn_exp2f(top - most);
+      const float all = wave_sum(top == kNoScore ? 0.f : weighed(weight[k], total));
+      if (mine == k) sum = all, m = most;
+    }
+    // this row's weight of a part; behind the last part 0
+    auto weight_of = [&](uint32_t p) {
+      float w = lane_value(weight[0], (int)p);
 #pragma unroll
-      for (int k = 0; k < kOwn; ++k)
-        x[i][k] = *(const values*)(part(min(p + i, parts - 1)) + kRows * 2 + (row0 + min((uint32_t)k, own - 1)) * D + lane * kPer);
+      for (uint32_t k = 1; k < kWaveRows; ++k) w = mine == k ? lane_value(weight[k], (int)p) : w;
+      return w;
+    };
+    v4f o = {};
+    for (uint32_t p = 0;;) {
 #pragma unroll
-    for (int i = 0; i < kDepth; ++i)
+      for (uint32_t i = 0; i < kDepth; ++i) {
+        const float w = weight_of(p + i);
 #pragma unroll
-      for (int k = 0; k < kOwn; ++k) {
-        const float w = lane_value(weight[k], (int)min(p + i, parts - 1));
-#pragma unroll
-        for (int d = 0; d < kPer; ++d) o[k][d] += p + i < parts ? weighed(w, x[i][k][d]) : 0.f;   // (a part that sees no key holds zeros)
+        for (int d = 0; d < 4; ++d) o[d] = __builtin_fmaf(w, x[i][d], o[d]);   // (a part that sees no key holds zeros)
       }
-  }
+      if ((p += kDepth) >= parts) break;
+      read(p);
+    }
+    if (__ballot(((o[0] + o[1]) + (o[2] + o[3])) * 0.f != 0.f)) {   // something is not finite: a weight of zero leaves it so
+      o = v4f{};
+      for (uint32_t p = 0; p < parts; ++p) {
+        const float w = weight_of(p);
+        const v4f y = *(const v4f*)(part(p) + at);
 #pragma unroll
-  for (int k = 0; k < kOwn; ++k) {
-    if ((uint32_t)k >= own) break;
-    const uint32_t row = tile * kRows + row0 + k, token = row / a.nq, h = head * a.nq + (row - token * a.nq);
-    const uint64_t at = s.first_query + token;
-    const float inv = sum[k] == 0.f ? 0.f : 1.f / sum[k];
-    if (a.lse && lane == 0)
-      a.lse[at * a.kv_heads * a.nq + h] = sum[k] == 0.f ? kNoScore : (m[k] + __builtin_amdgcn_logf(sum[k])) * kLn2;
-    uint16_t* const out = (uint16_t*)a.out.data + at * a.out.token_stride + h * a.out.head_stride + lane * kPer;
-    if constexpr (D == 128)
-      *(uint32_t*)out = pack2(o[k][0] * inv, o[k][1] * inv);
-    else
-      *out = (uint16_t)pack2(o[k][0] * inv, 0.f);
+        for (int d = 0; d < 4; ++d) o[d] += weighed(w, y[d]);
+      }
+    }
+    if (mine >= own) continue;
+    const uint32_t row = tile * kRows + row0 + mine, token = row / a.nq, h = head * a.nq + (row - token * a.nq);
+    const uint64_t to = s.first_query + token;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (a.lse && lane % kRowLanes == 0)
+      a.lse[to * a.kv_heads * a.nq + h] = sum == 0.f ? kNoScore : (m + __builtin_amdgcn_logf(sum)) * kLn2;
+    uint16_t* const out = (uint16_t*)a.out.data + to * a.out.token_stride + h * a.out.head_stride + lane % kRowLanes * 4;
+    *(w2*)out = w2{pack2(o[0] * inv, o[1] * inv), pack2(o[2] * inv, o[3] * inv)};
   }
 }
 
@@ -749,7 +769,8 @@ hipError_t PITCH_CAT(launch_prompt_d, PITCH_DIM, _io, PITCH_IO)(const PromptArgs
     prompt_attention<false, true><<<grid, dim3(256), 0, s>>>(a);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  prompt_join<<<dim3(a.tiles * (kRows / kJoinRows) * a.kv_heads), dim3(256), 0, s>>>(a);
+  const uint32_t blocks = a.tiles * a.kv_heads * (kRows / kJoinRows), turns = blocks > 8 * a.places * a.kv_heads ? 4 : 1;
+  prompt_join<<<dim3(blocks / turns), dim3(256), 0, s>>>(a, turns);
   return hipGetLastError();
 }
 
