@@ -484,8 +484,9 @@ int pitch_enqueue_paged_attention(const pitch_paged_cache_t* cache, const pitch_
  * summed in float32; the softmax's weights are rounded to the vectors' type. A query that sees no key (more queries than keys) gives
  * zeros and an lse of minus infinity; scores of minus infinity take no part; what is hidden from a query has no effect on it, also
  * where it is not finite; a visible value that is not finite gives what its sum is, a score that is NaN or plus infinity gives NaN to
- * its query. Rows of no sequence are left as they were. row_starts and key_starts do not decrease; they lie in device memory, are cut
- * to the buffers' rows and taken on trust no further. Kernels only: captured into graphs like the others. */
+ * its query. (Sums of weighted values are held in float32 before they are divided by the weights': bfloat16 values beyond 2^89
+ * may overflow there.) Rows of no sequence are left as they were. row_starts and key_starts do not decrease; they lie in device
+ * memory, are cut to the buffers' rows and taken on trust no further. Kernels only: captured into graphs like the others. */
 typedef struct pitch_prompt_attention {
   uint32_t io_type;   /* PITCH_IO_F16 or PITCH_IO_BF16 */
   uint32_t dim;       /* 64 or 128 */
@@ -547,10 +548,10 @@ typedef struct pitch_paged_tables {
 int pitch_paged_tables_workspace_size(const pitch_paged_tables_t* tables, uint64_t* bytes);
 
 /* Takes new_tokens[b] (int32; 0 or less: none) further tokens into every sequence b: pages are handed out where the held ones do not
- * suffice, and lengths grow. The call's tokens are packed in the order of the sequences, as a batch of prompts or a decode step has them: token
- * t's slot (page * page_size + slot, for pitch_enqueue_paged_append) goes to slots[t] and its position in its sequence to positions[t]
- * (or null). A token without a page or a place in its row has -1 in both, one whose entry of the table is no page has slot -1;
- * so do the entries behind the last token. Tokens beyond `capacity` are not taken. */
+ * suffice, and lengths grow. The call's tokens are packed in the order of the sequences, as a batch of prompts or a decode step has
+ * them: token t's slot (page * page_size + slot, for pitch_enqueue_paged_append) goes to slots[t] and its position in its sequence to
+ * positions[t] (or null). A token without a page or a place in its row has -1 in both, one whose entry of the table is no page has
+ * slot -1; the entries behind the last token have -1 in both. Tokens beyond `capacity` are not taken. */
 typedef struct pitch_paged_reserve {
   const void* new_tokens; /* int32 [sequences] */
   uint64_t new_tokens_bytes;
@@ -563,12 +564,14 @@ typedef struct pitch_paged_reserve {
 int pitch_enqueue_paged_reserve(const pitch_paged_tables_t* tables, const pitch_paged_reserve_t* call, void* stream);
 
 /* Cuts every sequence b to at most keep[b] tokens (int32; 0 or less: the whole sequence is given back): the pages behind lose a
- * reference. The tokens that remain are untouched: drafted tokens that were rejected, sequences that have ended. */
+ * reference. The tokens that remain are untouched: drafted tokens that were rejected, sequences that have ended. A row that is cut into
+ * a page that another row holds as well shares it from then on partly filled, and its next tokens would be written over the other's:
+ * such a row is first forked into an empty one, which gets that page as a copy, and given back behind that. */
 int pitch_enqueue_paged_trim(const pitch_paged_tables_t* tables, const void* keep, uint64_t keep_bytes, void* stream);
 
 /* Makes every row b a copy of row parents[b] (int32) as it was before the call: b itself leaves the row alone, a number outside the
- * rows empties it. Whole pages are shared and counted. A last page that is partly filled goes to one row (the parent's own if that stays, else its first
- * child); the others get a page of their own, into which its tokens are copied in all n_caches caches. Pages that lose their last
+ * rows empties it. Whole pages are shared and counted. A last page that is partly filled goes to one row (the parent's own if that
+ * stays, else its first child); the others get a page of their own, into which its tokens are copied in all n_caches caches. Pages that lose their last
  * reference are handed out again in the same call. */
 int pitch_enqueue_paged_fork(const pitch_paged_tables_t* tables, const pitch_paged_cache_t* caches, uint32_t n_caches,
                              const void* parents, uint64_t parents_bytes, void* stream);

@@ -7,7 +7,9 @@ reference/pitch_reference.py (``turbo_encode``, ``polar_decode``, ``channel_enco
 that run on device tensors. ``PITCH.enqueueEncodeBatch`` / ``EncodeBatch`` encode many caches' segments (a
 token's append to every layer) in one call, and ``PITCH.enqueueDecodeBatch`` / ``DecodeBatch`` decode them. ``attention_decode`` / ``PITCH.enqueueAttentionDecode`` compute decode-step
 attention directly over the compressed caches. ``PagedCache`` keeps many sequences' keys and values as codes in the pages of
-one pool, written by ``PagedAppend``, read back by ``PagedDecode`` and attended over by ``PagedAttention``.
+one pool, written by ``PagedAppend``, read back by ``PagedDecode`` and attended over by ``PagedAttention``; ``PagedTables`` hands the
+pages out and takes them back on the device (``PagedReserve``, ``PagedTrim``, ``PagedFork``, ``PagedCompact``). ``PromptAttention`` /
+``PITCH.enqueuePromptAttention`` compute attention over whole prompts, or chunks of them behind a cached prefix.
 """
 from .api import (  # noqa: F401
     CHANNEL_DEFAULT_GROUP, DECODERS, DEFAULT_SEED, ENCODERS, FP16_MAX, PITCH, SUPPORTED_BITS, SUPPORTED_DIMS,

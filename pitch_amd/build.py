@@ -7,7 +7,8 @@ dimension and element type of the uncompressed vectors (-DPITCH_DIM=2..1024, -DP
 float32/float16/bfloat16), csrc/pitch_channel.hip once per element type, csrc/pitch_attention.hip once per
 attention dimension (64, 128), csrc/pitch_attn_codes.hip once per attention dimension and kind of caches, csrc/pitch_paged.hip once per
 attention dimension and element type, csrc/pitch_paged_attn.hip once per attention dimension and width of the key codes,
-csrc/pitch_prompt.hip once per attention dimension and 16-bit type, csrc/pitch_pages.hip and csrc/pitch_abi.cpp, and link the shared library next to this file. Object files go to <repo>/_build/.
+csrc/pitch_prompt.hip once per attention dimension and 16-bit type, csrc/pitch_pages.hip and csrc/pitch_abi.cpp, and link the shared
+library next to this file. Object files go to <repo>/_build/.
 Also builds libpitch_calib.so from csrc/pitch_calib.hip: the measurement kernels bench.py times beside the
 codec (not part of the codec's C ABI).
 """

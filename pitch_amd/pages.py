@@ -104,10 +104,10 @@ class _TablesCall:
 
 class PagedReserve(_TablesCall):
     """Takes newTokens[b] (int32 [sequences]; 0 or less: none) further tokens into every sequence b: hands out pages where those that
-    it holds do not suffice, and adds to lengths. The tokens are packed in the order of the sequences; token t's slot (page * pageSize + slot,
-    for ``PagedAppend``) goes to slots[t] and its position in its sequence to positions[t] (int64, both as many as a step has room for).
-    A token without a page, or without a place in its row of the table, has -1 in both, and so have the entries behind the last token:
-    ``PagedAppend`` leaves them out. Tokens for which slots has no room are not taken."""
+    it holds do not suffice, and adds to lengths. The tokens are packed in the order of the sequences; token t's slot (page * pageSize +
+    slot, for ``PagedAppend``) goes to slots[t] and its position in its sequence to positions[t] (int64, both as many as a step has
+    room for). A token without a page, or without a place in its row of the table, has -1 in both, and so have the entries behind the last
+    token: ``PagedAppend`` leaves them out. Tokens for which slots has no room are not taken."""
 
     def __init__(self, tables: PagedTables, newTokens, slots, positions=None):
         super().__init__(tables)
@@ -125,7 +125,9 @@ class PagedReserve(_TablesCall):
 
 class PagedTrim(_TablesCall):
     """Cuts every sequence b to at most keep[b] tokens (int32 [sequences]; 0 or less: the whole sequence is given back). The pages
-    behind lose a reference; what remains is untouched."""
+    behind lose a reference; what remains is untouched. A row that is cut into a page that another row holds as well shares it from then
+    on partly filled, and its next tokens would be written over the other's: fork such a row into an empty one, which gets that page as
+    a copy, and give it back behind that."""
 
     def __init__(self, tables: PagedTables, keep):
         super().__init__(tables)
@@ -137,8 +139,8 @@ class PagedTrim(_TablesCall):
 
 class PagedFork(_TablesCall):
     """Makes every row b a copy of row parents[b] (int32 [sequences]) as it was before the call; b itself leaves the row alone, a number
-    outside the rows (-1) empties it. Whole pages are shared; a partly filled last page goes to one row (the parent's own if that stays, else its
-    first child), and the others get a page of their own with its tokens, in every cache of the tables."""
+    outside the rows (-1) empties it. Whole pages are shared; a partly filled last page goes to one row (the parent's own if that stays,
+    else its first child), and the others get a page of their own with its tokens, in every cache of the tables."""
 
     def __init__(self, tables: PagedTables, parents):
         super().__init__(tables)

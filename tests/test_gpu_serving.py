@@ -108,6 +108,24 @@ def test_a_program(q):
     assert not bool(p.tables.references.any())
 
 
+def test_a_row_that_is_cut_into_a_shared_page(q):
+    """What the documentation says of such a row: forked into an empty one it gets a page of its own, and the others keep their tokens."""
+    p = Program(q, 4, 12, 60)
+    p.tokens([50, 0, 0, 7])
+    p.fork([0, 0, 0, 3])                          # rows 0, 1 and 2 share three pages of 16
+    p.tokens([3, 1, 1, 0])
+    p.trim([60, 21, 40, 60])                      # rows 1 and 2 end inside of the second and the third
+    p.trim([60, 60, 60, 0])
+    p.fork([0, 1, 2, 1])
+    p.trim([60, 0, 60, 60])
+    p.fork([0, 2, 2, 3])
+    p.trim([60, 60, 0, 60])
+    p.check_pages()
+    for _ in range(2):
+        p.tokens([2, 13, 20, 9])                  # (the older tokens of all rows are compared here)
+        p.check_pages()
+
+
 def test_a_captured_decode_step(q):
     """Reserve, append and attend of one step in a graph, replayed over changing tables."""
     p = Program(q, 4, 12, 60)
