@@ -24,7 +24,7 @@
 // What bounds it. 16,381 tokens of 8 KV and 32 query heads of 128, bfloat16, causal: 2.02 to 2.12 ms on different cards, up to 1,090
 // TFLOP/s, where a large library product reaches 1,400. Matrix instructions are on their way in 57 % of the cycles; the rest is mostly
 // the softmax, 32 exponentials and about 120 other vector instructions for each 32 matrix instructions. The card lowers its clock under
-// this load (1.9 GHz): a step that took 12 % of the cycles out took 8 % of the time. Fourteen ragged prompts of up to 3,000 tokens
+// this load (1.9 GHz): a step that took 12 % of the cycles out took 8 % of the time. Twelve ragged prompts of up to 3,000 tokens
 // 409 us (880 TFLOP/s): a workgroup's beginning and end cost about two tiles of keys. Heads of 64 with soft caps in a window, 30 us,
 // are bound by vector instructions (three in four cycles): the cap's polynomial, eight a score, and the softmax. Slower were: 64 rows a
 // wave (half the LDS reads, but one wave a SIMD); eight waves that share a tile of keys for 256 rows (2,050 us instead of 2,100, but
