@@ -1773,6 +1773,7 @@ int pitch_enqueue_prompt_attention(const pitch_prompt_attention_t* call, void* s
   a.causal = call->causal;
   a.window = call->window;
   a.tiles = plan.tiles;
+  a.by_height = plan.by_height;
   a.places = plan.places;
   a.most_items = plan.most_items;
   a.parts_at = plan.parts_at;

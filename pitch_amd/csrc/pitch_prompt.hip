@@ -5,8 +5,8 @@
 // Work split. The query heads of a KV head share its keys, so a row is a pair of token and head, and 128 neighbouring rows of a sequence
 // are a query tile, a workgroup's work: four waves of 32 rows, two workgroups on a compute unit. It goes over the keys 64 at a time
 // with the running maximum and sum of a softmax (Milakov and Gimelshein 2018; Rabe and Staats 2021). Workgroups that follow each other
-// have different KV heads, so that an XCD, every eighth workgroup, finds the keys of few heads in its L2; a sequence's last tiles,
-// which see most keys, come first. Grid and workspace follow from sizes that the host knows, the lengths stay on the device.
+// have different KV heads, so that an XCD, every eighth workgroup, finds the keys of few heads in its L2; tiles that see most keys
+// come first, of each sequence or of all. Grid and workspace follow from sizes that the host knows, the lengths stay on the device.
 //
 // Products. v_mfma_f32_32x32x16 gives 32 x 32 scores as K Q^T, keys down and queries across: a lane holds 16 scores of one query, its
 // partner at distance 32 the other 16, and maxima, sums and rescaling stay within the lane but for one exchange a tile. The weights
@@ -25,7 +25,7 @@
 // TFLOP/s, where a large library product reaches 1,400. Matrix instructions are on their way in 57 % of the cycles; the rest is mostly
 // the softmax, 32 exponentials and about 120 other vector instructions for each 32 matrix instructions. The card lowers its clock under
 // this load (1.9 GHz): a step that took 12 % of the cycles out took 8 % of the time. Twelve ragged prompts of up to 3,000 tokens
-// 409 us (880 TFLOP/s): a workgroup's beginning and end cost about two tiles of keys. Heads of 64 with soft caps in a window, 30 us,
+// 409 us (880 TFLOP/s): a workgroup's beginning and end cost about two tiles of keys. Heads of 64 with soft caps in a window, 28 us,
 // are bound by vector instructions (three in four cycles): the cap's polynomial, eight a score, and the softmax. Slower were: 64 rows a
 // wave (half the LDS reads, but one wave a SIMD); eight waves that share a tile of keys for 256 rows (2,050 us instead of 2,100, but
 // 47 instead of 30 in the window and 137 instead of 124 for drafts) or by twos (2,250 us; the waves keep step); two tiles an iteration
@@ -134,6 +134,16 @@ __device__ __forceinline__ uint32_t lanes_up_to(uint32_t x) {
   return x;
 }
 __device__ __forceinline__ uint32_t of_lane(uint32_t x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+// The largest of all lanes.
+__device__ __forceinline__ uint32_t most(uint32_t x) {
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x111, 0xF, 0xF, false));  // row_shr:1
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x112, 0xF, 0xF, false));  // row_shr:2
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x114, 0xF, 0xF, false));  // row_shr:4
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x118, 0xF, 0xF, false));  // row_shr:8
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x142, 0xA, 0xF, false));  // row_bcast:15, to rows 1 and 3
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x143, 0xC, 0xF, false));  // row_bcast:31, to rows 2 and 3
+  return of_lane(x, 63);
+}
 
 // A sequence's queries and keys, within the buffers.
 struct Sequence {
@@ -157,21 +167,43 @@ struct Tile {
   uint32_t row;
   bool any;
 };
-// Tile number `at` of all sequences, found by all of the waves alike; a sequence's last tile, whose rows see most, comes first.
+// Tile number `at` of all sequences, found by all of the waves alike. A sequence's last tile, whose rows see most, comes first; with
+// by_height the highest of 64 sequences do, a tile's height being its number in its sequence and those that the keys before the queries
+// would fill, and tiles of a height lie in the order of the sequences.
 __device__ __forceinline__ Tile find_tile(const PromptArgs& a, uint32_t at) {
   const uint32_t lane = threadIdx.x & 63;
   Tile t{};
   for (uint32_t base = 0; base < a.sequences; base += 64) {
     const Sequence s = sequence(a, base + lane);
     const uint32_t sum = lanes_up_to(s.tiles), total = of_lane(sum, 63);
-    if (at < total) {
-      const int who = __ffsll((unsigned long long)__ballot(sum > at)) - 1;
-      t.s = Sequence{of_lane(s.first_query, who), of_lane(s.queries, who), of_lane(s.first_key, who), of_lane(s.keys, who), 0};
-      t.row = (of_lane(sum, who) - 1 - at) * kRows;
-      t.any = true;
-      return t;
+    if (at >= total) {
+      at -= total;
+      continue;
     }
-    at -= total;
+    int who;
+    if (!a.by_height) {
+      who = __ffsll((unsigned long long)__ballot(sum > at)) - 1;
+      t.row = (of_lane(sum, who) - 1 - at) * kRows;
+    } else {
+      const uint32_t before = (uint32_t)max((int32_t)(s.keys - s.queries), 0);
+      const uint32_t bottom = (uint32_t)min((uint64_t)before * a.nq / kRows, (uint64_t)1 << 30), top = bottom + s.tiles;
+      uint32_t lo = 0, hi = most(top), more = 0;   // the tile's height is in (lo, hi]; as many tiles lie above hi
+      while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2, above = s.tiles - min(s.tiles, max(mid, bottom) - bottom);
+        const uint32_t n = of_lane(lanes_up_to(above), 63);
+        if (n > at)
+          lo = mid;
+        else
+          hi = mid, more = n;
+      }
+      const uint64_t here = __ballot(hi > bottom && hi <= top);
+      const uint32_t rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(here >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)here, 0u));
+      who = __ffsll((unsigned long long)__ballot((here >> lane & 1) && rank == at - more)) - 1;
+      t.row = (hi - of_lane(bottom, who) - 1) * kRows;
+    }
+    t.s = Sequence{of_lane(s.first_query, who), of_lane(s.queries, who), of_lane(s.first_key, who), of_lane(s.keys, who), 0};
+    t.any = true;
+    return t;
   }
   return t;
 }

@@ -106,6 +106,22 @@ def test_many_sequences_over_long_keys(q):
         _check(q, lengths, 2, 1, 64, torch.bfloat16, seed=33)
 
 
+@pytest.mark.parametrize("dim,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+def test_parts_of_many_rows(q, dim, dtype):
+    """A long sequence among short ones: its tiles are cut, and joined by workgroups that take rows one after the other."""
+    _check(q, [(500, 560), (600, 5000), (1, 1), (500, 520), (590, 600)], 32, 8, dim, dtype, seed=34)
+
+
+@pytest.mark.parametrize("heads", [(4, 2), (8, 8)])
+def test_orders_of_tiles(q, heads):
+    """Uneven sequences, with and without keys before their queries, some empty: few tiles and many (which come in another order)."""
+    rng = np.random.default_rng(35)
+    lengths = [(int(n), int(n + p * (p % 3 == 0))) for n, p in zip(rng.integers(0, 300, 290), rng.integers(0, 400, 290))]
+    lengths[7] = lengths[100] = (0, 0)
+    _check(q, lengths, *heads, 64, torch.bfloat16, seed=35)
+    _check(q, lengths[:50], *heads, 64, torch.float16, seed=36)
+
+
 def test_more_sequences_than_a_wave_has_lanes(q):
     rng = np.random.default_rng(5)
     lengths = [(int(n), int(n + p)) for n, p in zip(rng.integers(0, 9, 333), rng.integers(0, 30, 333))]
@@ -172,6 +188,20 @@ def test_values_that_are_not_finite(q, dtype, lengths):
     v[at, 1, 9], v[ks[1] - 2, 0, 0] = math.nan, math.inf
     out, lse = _run(q, qq, k, v, rs, ks)
     compare(out, lse, reference(qq, k, v, rs, ks))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_values_that_are_not_finite_in_other_parts(q, dim):
+    """What one part holds reaches the joined row, also where that part's weight has become zero (e^-106
+    and less against the others' scores)."""
+    qq, k, v, rs, ks = _inputs([(3, 3000), (5, 2500)], 4, 2, dim, torch.bfloat16, 37)
+    qq[:, :, 0] = 4.0
+    k[:, :, 0] = torch.where(torch.arange(len(k), device="cuda") % 2600 < 200, -300.0, 0.0)[:, None]
+    v[20, 0, 3], v[30, 0, 3], v[40, 0, 4], v[50, 1, 5], v[3100, 1, 6] = math.inf, -math.inf, math.inf, math.nan, -math.inf
+    v[2900, 1, 7], v[5300, 0, 8], v[5310, 1, 9] = math.inf, math.nan, math.inf
+    out, lse = _run(q, qq, k, v, rs, ks)
+    compare(out, lse, reference(qq, k, v, rs, ks))
+    assert bool(torch.isnan(out[:3, :2, 3]).all()) and bool((out[:3, :2, 4] == math.inf).all())
 
 
 def test_scores_of_minus_infinity_take_no_part(q):
