@@ -24,13 +24,16 @@
 // What bounds it. 16,381 tokens of 8 KV and 32 query heads of 128, bfloat16, causal: 2.02 to 2.12 ms on different cards, up to 1,090
 // TFLOP/s, where a large library product reaches 1,400. Matrix instructions are on their way in 57 % of the cycles; the rest is mostly
 // the softmax, 32 exponentials and about 120 other vector instructions for each 32 matrix instructions. The card lowers its clock under
-// this load (1.9 GHz): a step that took 12 % of the cycles out took 8 % of the time. Twelve ragged prompts of up to 3,000 tokens
-// 409 us (880 TFLOP/s): a workgroup's beginning and end cost about two tiles of keys. Heads of 64 with soft caps in a window, 28 us,
-// are bound by vector instructions (three in four cycles): the cap's polynomial, eight a score, and the softmax. Slower were: 64 rows a
-// wave (half the LDS reads, but one wave a SIMD); eight waves that share a tile of keys for 256 rows (2,050 us instead of 2,100, but
-// 47 instead of 30 in the window and 137 instead of 124 for drafts) or by twos (2,250 us; the waves keep step); two tiles an iteration
-// (2,110 us, spills); and skipping of tiles that all rows of a wave are blind to (no change). Queries that are waited for inside
-// the loop cost 14 % (the counter of loads also counts the tiles on their way).
+// this load (1.9 GHz): a step that took 12 % of the cycles out took 8 % of the time. Twelve ragged prompts of up to 3,000 tokens 400 to
+// 420 us (880 TFLOP/s): of a workgroup's 17 tiles of keys, 1.8 us each beside another's, 5 us are its beginning (0.8 until it knows its
+// tile, 2.2 until queries and keys are there, 0.6 of the slowest wave) and its end (1.3), and 30 us pass while places run empty. Heads
+// of 64 with soft caps in a window, 28 us, are bound by vector instructions (three in four cycles): the cap's polynomial, eight a score,
+// and the softmax. Slower were: 64 rows a wave (half the LDS reads, but one wave a SIMD); eight waves that share a tile of keys for 256
+// rows (2,050 us instead of 2,100, but 47 instead of 30 in the window and 137 instead of 124 for drafts) or by twos (2,250 us; the waves
+// keep step); two tiles an iteration (2,110 us, spills); the next tile's scores among this one's weights (2,360 us: two tiles of scores
+// leave too few registers, and what is spilled is waited for together with the tiles on their way); and skipping of tiles that all rows
+// of a wave are blind to (no change). Queries that are waited for inside the loop cost 14 % (the counter of loads also counts the tiles
+// on their way).
 #include "pitch_attn_shared.h"
 #include "pitch_prompt.h"
 
