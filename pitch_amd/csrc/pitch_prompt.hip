@@ -30,10 +30,10 @@
 // of 64 with soft caps in a window, 28 us, are bound by vector instructions (three in four cycles): the cap's polynomial, eight a score,
 // and the softmax. Slower were: 64 rows a wave (half the LDS reads, but one wave a SIMD); eight waves that share a tile of keys for 256
 // rows (2,050 us instead of 2,100, but 47 instead of 30 in the window and 137 instead of 124 for drafts) or by twos (2,250 us; the waves
-// keep step); two tiles an iteration (2,110 us, spills); the next tile's scores among this one's weights (2,360 us: two tiles of scores
-// leave too few registers, and what is spilled is waited for together with the tiles on their way); and skipping of tiles that all rows
-// of a wave are blind to (no change). Queries that are waited for inside the loop cost 14 % (the counter of loads also counts the tiles
-// on their way).
+// keep step); two tiles an iteration (2,110 us, spills); the next tile's scores among this one's weights (2,115 us beside 2,020, the
+// second pass over what is not finite apart: two tiles of scores leave too few registers, and 30 are moved for each tile); and skipping
+// of tiles that all rows of a wave are blind to, and the longest sequence first (no change). Queries that are waited for inside the loop
+// cost 14 % (the counter of loads also counts the tiles on their way).
 #include "pitch_attn_shared.h"
 #include "pitch_prompt.h"
 

@@ -53,6 +53,12 @@ def test_packed_sequences(q, dtype, dim, kv, group):
     _check(q, MIXED, kv * group, kv, dim, dtype)
 
 
+@pytest.mark.parametrize("kv,group,lengths", [(1, 200, [(3, 70), (130, 140)]), (600, 1, [(2, 2100), (3, 3)]), (1, 64, [(2, 2500)])])
+def test_many_heads(q, kv, group, lengths):
+    """A token that fills more than a query tile, and more KV heads than the device has places for workgroups."""
+    _check(q, lengths, kv * group, kv, 64, torch.float16, seed=38)
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("more", [
     dict(causal=False), dict(window=1), dict(window=7), dict(window=64), dict(window=100), dict(window=2 ** 31 - 1), dict(softcap=5.0),
