@@ -54,7 +54,8 @@ struct PagesLayer {
 };
 constexpr uint32_t kPagesLayers = 48;  // of a launch: its arguments hold them
 // Bytes of a layer's page that a workgroup copies at a time. One index over all pieces of a page instead, divided for each: 642 us where
-// slices of buffers take 408 to 470 (1.1 GB).
+// slices of buffers take 408 to 470 (1.1 GB). Four pieces read before one is written, or four times as many workgroups: no change to 2
+// %.
 constexpr uint32_t kPagesSlice = 1u << 16;
 struct PagesCopyArgs {
   const uint32_t* count;   // pages to copy
