@@ -1788,6 +1788,17 @@ int pitch_enqueue_prompt_attention(const pitch_prompt_attention_t* call, void* s
     const double k = call->softcap > 0.f ? (double)call->scale / call->softcap : 0.0;
     a.cap_k = (float)std::max(-kMost, std::min(kMost, k));
     a.cap_r = (float)std::max(-kMost, std::min(kMost, 2.0 * kLog2E * k));
+    // tanh(x) / x - 1 in x^2 for |x| < 0.3, fitted for the smallest of the largest errors; not where factors leave float32's range
+    constexpr double kTanh[3] = {-0.33333063, 0.13314908, -0.0503723};
+    double factor = to_log2;
+    bool fits = k != 0;
+    for (int i = 0; i < 3; ++i) {
+      factor *= k * k;
+      const double p = kTanh[i] * factor;
+      fits = fits && std::abs(p) >= 1e-37 && std::abs(p) <= 1e37;
+      a.cap_p[i] = (float)p;
+    }
+    a.cap_small = fits ? (float)(0.3 / std::abs(k)) : 0.f;
   } else {
     a.negate = call->scale < 0.f;
     a.c = (float)std::max(std::abs(to_log2), 1e-37);

@@ -22,6 +22,7 @@ struct PromptArgs {
   float c;                    // |scale| log2(e): scores to log2 units (1 with a cap or slopes, which give such units)
   float pre;                  // with a cap or slopes: what a product is multiplied by first
   float cap, cap_k, cap_r;    // with a positive cap, products s give cap * tanh(x), x = s * cap_k, e^2x = 2^(s * cap_r), in log2 units
+  float cap_small, cap_p[3];  // for |s| below cap_small (0: never) that is s (pre + cap_p[0] t + cap_p[1] t^2 + cap_p[2] t^3), t = s^2
   uint32_t tiles;             // an upper bound of the query tiles of a KV head
   uint32_t by_height;         // 1: the tiles of all sequences in the order of the keys that they see, not sequence by sequence
   uint32_t places;            // workgroups of a KV head that run at once, where keys may be cut into parts; 0: they are not

@@ -27,13 +27,14 @@
 // this load (1.9 GHz): a step that took 12 % of the cycles out took 8 % of the time. Twelve ragged prompts of up to 3,000 tokens 400 to
 // 420 us (880 TFLOP/s): of a workgroup's 17 tiles of keys, 1.8 us each beside another's, 5 us are its beginning (0.8 until it knows its
 // tile, 2.2 until queries and keys are there, 0.6 of the slowest wave) and its end (1.3), and 30 us pass while places run empty. Heads
-// of 64 with soft caps in a window, 28 us, are bound by vector instructions (three in four cycles): the cap's polynomial, eight a score,
-// and the softmax. Slower were: 64 rows a wave (half the LDS reads, but one wave a SIMD); eight waves that share a tile of keys for 256
-// rows (2,050 us instead of 2,100, but 47 instead of 30 in the window and 137 instead of 124 for drafts) or by twos (2,250 us; the waves
-// keep step); two tiles an iteration (2,110 us, spills); the next tile's scores among this one's weights (2,115 us beside 2,020, the
-// second pass over what is not finite apart: two tiles of scores leave too few registers, and 30 are moved for each tile); and skipping
-// of tiles that all rows of a wave are blind to, and the longest sequence first (no change). Queries that are waited for inside the loop
-// cost 14 % (the counter of loads also counts the tiles on their way).
+// of 64 with soft caps in a window, 25.5 us, are bound by vector instructions (three in four cycles): the cap's polynomial, five a score
+// (27.8 with nine; 11,486 tokens of four heads of 128 351 us, with nine 405), and the softmax. Slower were: 64 rows a wave (half the LDS
+// reads, but one wave a SIMD); eight waves that share a tile of keys for 256 rows (2,050 us instead of 2,100, but 47 instead of 30 in
+// the window and 137 instead of 124 for drafts) or by twos (2,250 us; the waves keep step); two tiles an iteration (2,110 us, spills);
+// the next tile's scores among this one's weights (2,115 us beside 2,020, the second pass over what is not finite apart: two tiles of
+// scores leave too few registers, and 30 are moved for each tile); and skipping of tiles that all rows of a wave are blind to, and the
+// longest sequence first (no change). Queries that are waited for inside the loop cost 14 % (the counter of loads also counts the tiles
+// on their way).
 #include "pitch_attn_shared.h"
 #include "pitch_prompt.h"
 
@@ -443,13 +444,22 @@ __device__ __forceinline__ void attend(const PromptArgs& a, Shared& shared, uint
     asm("s_nop 7\n\ts_nop 7" : "+v"(s[0]), "+v"(s[1]));
     if constexpr (MOD) {
       if (a.cap > 0.f) {
-        // cap tanh(x) = (cap x) (tanh(x) / x): a polynomial in x^2 below 0.55 (6e-9 off; the usual case, and exact to float32 for caps
-        // of any size), above that 1 - 2 / (e^2x + 1), which would lose digits to the 1 for small x
+        // cap tanh(x) = (cap x) (tanh(x) / x), x = k s. The quotient is a polynomial in s^2 below 0.3 (1.2e-8 off, five instructions
+        // with its factors made by the host), in x^2 below 0.55 (6e-9 off, for caps of any size); above that cap (1 - 2 / (e^2x + 1)),
+        // which would lose digits to the 1 for small x.
         float big = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) big = fmax3_abs(big, s[0][r], s[1][r]);
         const float k = a.cap_k, pre = a.pre;
-        if (__ballot(big * __builtin_fabsf(k) >= kTanhSplit)) {
+        if (!__ballot(big >= a.cap_small)) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float t = s[b][r] * s[b][r];
+              s[b][r] *= __builtin_fmaf(t, __builtin_fmaf(t, __builtin_fmaf(t, a.cap_p[2], a.cap_p[1]), a.cap_p[0]), pre);
+            }
+        } else if (__ballot(big * __builtin_fabsf(k) >= kTanhSplit)) {
 #pragma unroll
           for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -471,12 +481,11 @@ __device__ __forceinline__ void attend(const PromptArgs& a, Shared& shared, uint
           for (int r = 0; r < 16; ++r) s[b][r] *= a.pre;
       }
       if (a.slopes) {
-        const int32_t away = (int32_t)((uint32_t)k0 + half * 4 - (uint32_t)offset - token_in);
+        const float away = slope * (float)(int32_t)((uint32_t)k0 + half * 4 - (uint32_t)offset - token_in);
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            s[b][r] = __builtin_fmaf(slope, (float)(away + b * 32 + (r & 3) + 8 * (r >> 2)), s[b][r]);
+          for (int r = 0; r < 16; ++r) s[b][r] += __builtin_fmaf(slope, (float)(b * 32 + (r & 3) + 8 * (r >> 2)), away);
       }
     }
     const bool masked = k0 + kKeys - 1 > whi0 || k0 < wlo1 || k0 + kKeys > (int32_t)t.s.keys;
