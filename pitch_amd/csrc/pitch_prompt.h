@@ -32,7 +32,7 @@ struct PromptArgs {
 
 // Rows of (token, query head of a KV head) in a query tile; the most sequences of a call whose keys may be cut into parts, and the
 // keys from which that is looked at; what writing and joining a part of 128 rows costs, in tiles of 64 keys.
-constexpr uint32_t kPromptRows = 128, kPromptCutSequences = 1024, kPromptCutKeys = 2048, kPromptCut = 7;
+constexpr uint32_t kPromptRows = 128, kPromptCutSequences = 1024, kPromptCutKeys = 1024, kPromptCut = 7;
 struct PromptPlan {
   uint32_t tiles, by_height, places, most_items;
   uint64_t parts_at, ws_floats;
@@ -40,7 +40,8 @@ struct PromptPlan {
 // What the host decides. Workgroups take whole query tiles where these are enough for four turns of every workgroup place (two on a
 // compute unit), or fill half of the places and belong to whole prompts, whose tiles grow in number as they grow in length. Else, where
 // tiles may be long, the lengths decide on the device whether keys are cut: two launches more, about 10 us (eight sequences of five
-// drafted tokens behind up to 32,000: 123 us; 500 and more if a workgroup has the longest by itself).
+// drafted tokens behind up to 32,000: 123 us; 500 and more if a workgroup has the longest by itself). From 1,024 keys on: 20 queries over
+// 1,500 keys of 8 heads of 128 take 18 us cut and 34 uncut, over 700 keys about 17 either way.
 //
 // Whole tiles of several sequences come in the order of their keys where a place has fewer than four: the longest do not come last (16
 // sequences of 12 heads in a window, one or two tiles a place: 27.8 us, sequence by sequence 30.3). With more, the search for a tile, 0.9

@@ -251,7 +251,7 @@ __device__ __forceinline__ float* part_of(const PromptArgs& a, uint32_t head, ui
 // Chooses the longest part, of 64 candidates (the longest sequence in 1 .. 64 parts), by an estimate of the time, in sixteenths
 // of a tile of keys: all tiles of keys, 2 for each part's beginning and end and kPromptCut for a part of 128 rows that is written and
 // joined, over the workgroup places, and half of the longest part for the end, when places run empty; or, where there is a place for
-// each part, the longest.
+// each part, the longest and, if any are cut, a part's join (five sequences of 100 queries over 600 keys: 26.7 us uncut, 35.5 cut).
 __global__ __launch_bounds__(1024) void prompt_cut(PromptArgs a) {
   __shared__ uint32_t sums[2][16], longest, lengths[1024], counts[2][1024];
   __shared__ unsigned long long cost[64], items[64];
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(1024) void prompt_cut(PromptArgs a) {
   }
   __syncthreads();
   // the cheapest candidate that the workspace has room for, the same in every wave; uncut is always possible
-  float best = items[lane] <= a.places ? 16.f * (float)run + 32.f + kPromptCut * 16.f
+  float best = items[lane] <= a.places ? 16.f * (float)run + 32.f + (lane ? kPromptCut * 16.f : 0.f)
                                        : (float)cost[lane] / (float)a.places + 8.f * (float)run;
   if (lane > 0 && items[lane] > a.most_items) best = __builtin_inff();
   uint32_t choice = run;
