@@ -27,7 +27,7 @@
 // this load (1.9 GHz): a step that took 12 % of the cycles out took 8 % of the time. Twelve ragged prompts of up to 3,000 tokens 400 to
 // 420 us (880 TFLOP/s): of a workgroup's 17 tiles of keys, 1.8 us each beside another's, 5 us are its beginning (0.8 until it knows its
 // tile, 2.2 until queries and keys are there, 0.6 of the slowest wave) and its end (1.3), and 30 us pass while places run empty. Heads
-// of 64 with soft caps in a window, 25.5 us, are bound by vector instructions (three in four cycles): the cap's polynomial, five a score
+// of 64 with soft caps in a window, 25.5 us, are bound by vector instructions (two in three cycles): the cap's polynomial, five a score
 // (27.8 with nine; 11,486 tokens of four heads of 128 351 us, with nine 405), and the softmax. Slower were: 64 rows a wave (half the LDS
 // reads, but one wave a SIMD); eight waves that share a tile of keys for 256 rows (2,050 us instead of 2,100, but 47 instead of 30 in
 // the window and 137 instead of 124 for drafts) or by twos (2,250 us; the waves keep step); two tiles an iteration (2,110 us, spills);
