@@ -527,7 +527,7 @@ int pitch_enqueue_prompt_attention(const pitch_prompt_attention_t* call, void* s
  * 0 .. table_width * page_size; entries outside the pool are no pages; entries behind a row's length are left as they are. Where free
  * pages are handed out, the lowest number goes first, in the order of the sequences and their tokens; where they run out, a row ends
  * with its last token that has a page, and *missing is the number of pages that were lacking (0 where none were).
- * Calls that share tables, pools or a workspace run one after the other. */
+ * Calls that share tables, pools or a workspace run one after the other: the caller orders those on different streams. */
 typedef struct pitch_paged_tables {
   void* block_tables; /* int32 [sequences][table_width] */
   uint64_t block_tables_bytes;

@@ -8,6 +8,7 @@ call's checked arguments between calls; ``PagedTables.enqueueReserve`` and the l
 from __future__ import annotations
 
 import ctypes
+import threading
 
 from . import _lib
 from .api import InvalidInput, _raise_for, _torch
@@ -21,8 +22,10 @@ class PagedTables(WorkspaceCall):
     last reserve or fork lacked) are allocated empty, for ``sequences`` rows (at most 2,048) of ``width`` pages, or given. A
     program that keeps a page for itself, a prefix's say, adds 1 to its references. Free pages are handed out lowest
     number first, in the order of the sequences and their tokens. Where they run out, a row ends with its last token that has a
-    page. Calls on the same tables run one after the other; on another stream than the one that the workspace was allocated on a call
-    waits for that stream's work."""
+    page. Calls on the same tables run one after the other, in the order in which they are made: on another stream than the last one's, or
+    the first on another than the one that the tables were made on, a call waits for that stream's work. (A captured call waits for
+    nothing outside of its graph, and nothing waits for it: the program orders captured calls of several streams, and replays. So it does
+    appends to the pools and attention over them.)"""
 
     def __init__(self, caches, sequences: int | None = None, width: int | None = None, blockTables=None, lengths=None, references=None,
                  missing=None):
@@ -63,6 +66,8 @@ class PagedTables(WorkspaceCall):
         self._hold_workspace(c, None, int(needed.value), device)
         self._made = made
         self._cstruct, self._device = c, device
+        # the stream of the last call, or an event behind it, and the stream's handle where a call on it needs no wait
+        self._last, self._last_handle, self._turn = self._own, self._own.cuda_stream, threading.Lock()
         self._layers = (_lib.PitchPagedCacheC * len(self.caches))(*[cache._cstruct for cache in self.caches])
 
     def enqueueReserve(self, newTokens, slots, positions=None, stream=None) -> None:
@@ -86,6 +91,33 @@ class PagedTables(WorkspaceCall):
         for t in self._made:
             t.record_stream(self._stream(stream, handle))
 
+    def _capturing(self, stream) -> bool:
+        torch = _torch()
+        with torch.cuda.stream(stream):
+            return torch.cuda.is_current_stream_capturing()
+
+    def _issue(self, launch, stream) -> int:
+        """Makes a call behind the last one on these tables."""
+        with self._turn:   # (two threads' calls: the second looks for the first when that has been made)
+            handle = self._handle(stream)
+            if handle == self._last_handle:
+                return launch(handle)
+            now = self._stream(stream, handle)
+            if self._capturing(now):
+                return launch(handle)
+            if isinstance(self._last, _torch().cuda.Event):
+                now.wait_event(self._last)
+            elif not self._capturing(self._last):   # (a capture that has begun since then began behind all of the device's work)
+                now.wait_event(self._last.record_event())
+            rc = launch(handle)
+            # A stream that is not torch's own, known by a number that is its handle, may be gone before the next call, or another one with
+            # the same handle in its place: its event is recorded now. Torch's own streams stay, and cost their calls nothing.
+            if handle and now.stream_id == handle:
+                self._last, self._last_handle = now.record_event(), None
+            else:
+                self._last, self._last_handle = now, handle
+            return rc
+
 
 class _TablesCall:
     """A call on tables, whose workspace is the tables'."""
@@ -97,7 +129,7 @@ class _TablesCall:
         self._pool, self._lib = ctypes.byref(tables._cstruct), tables.pitch._lib
 
     def enqueue(self, stream=None) -> None:
-        rc = self._launch(self.tables._handle(stream))
+        rc = self.tables._issue(self._launch, stream)
         if rc:
             _raise_for(rc)
 
