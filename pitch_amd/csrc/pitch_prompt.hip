@@ -377,7 +377,7 @@ __device__ __forceinline__ void attend(const PromptArgs& a, Shared& shared, uint
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                   :: "s"(of_wave(to + (i * kWaves + wave) * 1024)), "v"(at + i * kWaves * kLaneRows * stride), "s"(r) : "memory");
+                   :: "s"(of_wave(to + (i * kWaves + wave) * 1024)), "v"(at + i * kWaves * kLaneRows * stride), "s"(r) : "memory", "m0");
   };
   auto load = [&](int32_t k0, int buf) {
     if (k0 >= hi) return;
@@ -440,7 +440,7 @@ __device__ __forceinline__ void attend(const PromptArgs& a, Shared& shared, uint
         s[b] = mfma(k, q[i], s[b]);
       }
     }
-    // (the compiler does not see that the statements below read what matrix instructions write: 16 wait states, 11 are needed)
+    // (the compiler does not see that the statements below read what matrix instructions write: 16 wait states, 12 are needed)
     asm("s_nop 7\n\ts_nop 7" : "+v"(s[0]), "+v"(s[1]));
     if constexpr (MOD) {
       if (a.cap > 0.f) {
