@@ -564,9 +564,13 @@ typedef struct pitch_paged_reserve {
 int pitch_enqueue_paged_reserve(const pitch_paged_tables_t* tables, const pitch_paged_reserve_t* call, void* stream);
 
 /* Cuts every sequence b to at most keep[b] tokens (int32; 0 or less: the whole sequence is given back): the pages behind lose a
- * reference. The tokens that remain are untouched: drafted tokens that were rejected, sequences that have ended. A row that is cut into
- * a page that another row holds as well shares it from then on partly filled, and its next tokens would be written over the other's:
- * such a row is first forked into an empty one, which gets that page as a copy, and given back behind that. */
+ * reference. The tokens that remain are untouched: drafted tokens that were rejected, sequences that have ended. A row that is cut below
+ * the length that it had in the last fork, as parent or as child, may end within a page that another row holds as well; it shares that
+ * page from then on partly filled, and reserve, which does not look at who else holds a page, would have its next tokens written over the other's. Such
+ * a row is first forked into an empty one, which gets that page as a copy, and given back behind that. A program that cannot know
+ * which rows these are (a captured step) keeps n empty rows behind its n, and forks with the parents 0 .. n - 1, 0 .. n - 1, then n .. 2 n - 1
+ * and n times -1: every row's partly filled last page is then its own, for a free page and a copy a row. (*missing above 0 behind the
+ * first of these forks: rows have lost their last tokens.) */
 int pitch_enqueue_paged_trim(const pitch_paged_tables_t* tables, const void* keep, uint64_t keep_bytes, void* stream);
 
 /* Makes every row b a copy of row parents[b] (int32) as it was before the call: b itself leaves the row alone, a number outside the

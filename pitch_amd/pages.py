@@ -157,9 +157,15 @@ class PagedReserve(_TablesCall):
 
 class PagedTrim(_TablesCall):
     """Cuts every sequence b to at most keep[b] tokens (int32 [sequences]; 0 or less: the whole sequence is given back). The pages
-    behind lose a reference; what remains is untouched. A row that is cut into a page that another row holds as well shares it from then
-    on partly filled, and its next tokens would be written over the other's: fork such a row into an empty one, which gets that page as
-    a copy, and give it back behind that."""
+    behind lose a reference; what remains is untouched.
+
+    A row that is cut below the length that it had in the last fork, as parent or as child, may end within a page that another row holds as well. It shares
+    that page from then on partly filled, and PagedReserve, which looks at lengths and not at who else holds a page, would have its next
+    tokens written over the other's. (Rows that are cut by no more than they have grown since, drafted tokens, are not concerned.) Such a row
+    is forked into an empty one, which gets that page as a copy, and given back behind that. A program that cannot know which rows these
+    are, a captured step, gives its n rows n empty ones and forks with the parents 0 .. n - 1, 0 .. n - 1, then n .. 2 n - 1 and n
+    times -1: behind that every row is what it was, and its partly filled last page its own. It takes a free page and a copy of that page's
+    tokens for each row that ends within a page; with ``missing`` above 0 behind the first of the two, rows have lost their last tokens."""
 
     def __init__(self, tables: PagedTables, keep):
         super().__init__(tables)
