@@ -513,8 +513,9 @@ typedef struct pitch_prompt_attention {
   void* workspace; /* pitch_prompt_attention_workspace_size bytes (null for none); not used by another call until this one has completed */
   uint64_t workspace_bytes;
 } pitch_prompt_attention_t;
-/* Bytes of device workspace pitch_enqueue_prompt_attention needs on the current device (0 for many or short sequences) for these
- * dim, sequences, heads, rows, key_rows and window. */
+/* Bytes of device workspace pitch_enqueue_prompt_attention needs on the current device (0 for many tiles or few keys; else up to 136 MB
+ * with vectors of 128 and 69 MB with vectors of 64 on 256 compute units) for these dim, sequences, heads, rows, key_rows and window.
+ * Calls that run one after the other, a step's layers, may share one. */
 int pitch_prompt_attention_workspace_size(const pitch_prompt_attention_t* call, uint64_t* bytes);
 int pitch_enqueue_prompt_attention(const pitch_prompt_attention_t* call, void* stream);
 

@@ -43,6 +43,12 @@ struct PromptPlan {
 // drafted tokens behind up to 32,000: 123 us; 500 and more if a workgroup has the longest by itself). From 1,024 keys on: 20 queries over
 // 1,500 keys of 8 heads of 128 take 18 us cut and 34 uncut, over 700 keys about 17 either way.
 //
+// The host knows the keys of all sequences together, not the longest, and errs both ways. A call of short sequences with 1,024 keys and
+// more in all is looked at for nothing: seven of 29 queries over 385 keys 21.7 us and 15.0 if it were not, five of 100 over 600
+// 26.7 and 19.8 (8 KV and 32 query heads of 128). One long sequence among many tiles is not cut: a chunk of 8,192 tokens and 31
+// drafts behind up to 2,000 take 567 us, with one more draft behind 32,000 1,098. The places are those of heads of 128, two workgroups on
+// a compute unit; three of heads of 64 run there.
+//
 // Whole tiles of several sequences come in the order of their keys where a place has fewer than four: the longest do not come last (16
 // sequences of 12 heads in a window, one or two tiles a place: 27.8 us, sequence by sequence 30.3). With more, the search for a tile, 0.9
 // us each, costs what the shorter end gains (ten tiles a place: 415 us, sequence by sequence 410).

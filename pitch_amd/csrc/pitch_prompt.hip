@@ -13,19 +13,19 @@
 // are then the second operand of V^T P^T as they lie, if the 16 keys of a product are taken in the order 4 h .. 4 h + 3, 8 + 4 h ..
 // 8 + 4 h + 3 in the lanes' halves h; V^T is read in that order by the transposing LDS reads (ds_read_b64_tr_b16, four keys by 16
 // coordinates). Weights are rounded to the values' type, once; scores, maxima, sums and accumulators are float32. With bfloat16 the
-// rounding of the weights is as large as the output's own, and averages like it: errors of outputs are 1.3 to 1.4 times those of
-// the exact result's rounding (0.0021 to 0.0016 of the norm; float16 0.00029 to 0.00021).
+// rounding of the weights is as large as the output's own, and averages like it: errors of outputs are 1.04 to 1.41 times those
+// of the exact result's rounding (0.0021 to 0.0016 of the norm in a batch of prompts; float16 0.00029 to 0.00021 in chunks).
 //
 // Data. Tiles go from memory to LDS without registers (buffer_load ... lds), one ahead; chunks of 16 bytes lie swizzled, by the address
 // that each lane asks for, so that no read finds a bank conflict (the counter says none). Rows behind the sequence come back as zeros
 // (the buffers' bounds), and a mask is applied only in tiles that need one. The maximum in use lags by up to 2^8 behind a row's true
 // one, so that the accumulators are rarely rescaled; weights up to 256 are as exact as those below 1.
 //
-// What bounds it. 16,381 tokens of 8 KV and 32 query heads of 128, bfloat16, causal: 2.02 to 2.12 ms on different cards, up to 1,090
+// What bounds it. 16,381 tokens of 8 KV and 32 query heads of 128, bfloat16, causal: 2.02 to 2.18 ms on different cards, up to 1,090
 // TFLOP/s, where a large library product reaches 1,400. Matrix instructions are on their way in 57 % of the cycles; the rest is mostly
 // the softmax, 32 exponentials and about 120 other vector instructions for each 32 matrix instructions. The card lowers its clock under
 // this load (1.9 GHz): a step that took 12 % of the cycles out took 8 % of the time. Twelve ragged prompts of up to 3,000 tokens 400 to
-// 420 us (880 TFLOP/s): of a workgroup's 17 tiles of keys, 1.8 us each beside another's, 5 us are its beginning (0.8 until it knows its
+// 440 us (820 to 900 TFLOP/s): of a workgroup's 17 tiles of keys, 1.8 us each beside another's, 5 us are its beginning (0.8 until it knows its
 // tile, 2.2 until queries and keys are there, 0.6 of the slowest wave) and its end (1.3), and 30 us pass while places run empty. Heads
 // of 64 with soft caps in a window, 25.5 us, are bound by vector instructions (two in three cycles): the cap's polynomial, five a score
 // (27.8 with nine; 11,486 tokens of four heads of 128 351 us, with nine 405), and the softmax. Slower were: 64 rows a wave (half the LDS
@@ -251,7 +251,8 @@ __device__ __forceinline__ float* part_of(const PromptArgs& a, uint32_t head, ui
 // Chooses the longest part, of 64 candidates (the longest sequence in 1 .. 64 parts), by an estimate of the time, in sixteenths
 // of a tile of keys: all tiles of keys, 2 for each part's beginning and end and kPromptCut for a part of 128 rows that is written and
 // joined, over the workgroup places, and half of the longest part for the end, when places run empty; or, where there is a place for
-// each part, the longest and, if any are cut, a part's join (five sequences of 100 queries over 600 keys: 26.7 us uncut, 35.5 cut).
+// each part, the longest and, if any are cut, a part's join (five sequences of 100 queries over 600 keys: 35.5 us cut, 26.7 with no cut
+// found; 19.8 are the attention alone, in a call whose plan does not look).
 __global__ __launch_bounds__(1024) void prompt_cut(PromptArgs a) {
   __shared__ uint32_t sums[2][16], longest, lengths[1024], counts[2][1024];
   __shared__ unsigned long long cost[64], items[64];
@@ -536,6 +537,8 @@ __device__ __forceinline__ void attend(const PromptArgs& a, Shared& shared, uint
           sum += w;
         }
     }
+    // the weights, rounded to the values' type: all that is held in fewer bits than float32 here (in two parts of that type they would
+    // cost the second product, half of the matrix work, twice); `sum` is that of the weights before it
     w4 p[4];
 #pragma unroll
     for (int b = 0; b < 2; ++b)
