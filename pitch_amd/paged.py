@@ -306,8 +306,9 @@ class PagedAttention(WorkspaceCall):
     int32 [sequences] with the new token counted. The scores are softcap * tanh(scale q.k / softcap) (softcap 0: scale q.k; scale defaults to 1 / sqrt(dim))
     plus slopes[h] * (t - (length - 1)) (float32 [heads]) over the last ``window`` tokens (0: all). lse, float32
     [sequences][heads], receives the natural-log sum of exp. A sequence of length 0 gives zeros (and minus infinity). Without
-    a workspace one is allocated and held, and a call on another stream waits for the work of the stream that it was allocated on;
-    a graph needs the object as long as it is replayed. Two calls that may run at the same time must not share a workspace."""
+    a workspace one is allocated and held; the first call on another stream waits for the work that the stream of its allocation has by
+    then, later ones for nothing. A graph needs the object as long as it is replayed. Two calls that may run at the same time must not
+    share a workspace: the program orders one object's calls on several streams."""
 
     def __init__(self, cache: PagedCache, q, blockTables, lengths, output, scale: float | None = None, softcap: float = 0.0,
                  window: int = 0, slopes=None, lse=None, workspace=None):
