@@ -23,9 +23,9 @@ class PromptAttention(WorkspaceCall):
     [rows][heads], receives the natural-log sum of exp. A query that sees no key gives zeros (and minus infinity); rows of no sequence
     are left as they were; the output may be q itself. Like ``PagedAttention``, the object keeps the checked arguments and, without a
     workspace of the caller's, one that is allocated here (few queries over long keys need one): two calls that may run at the same time
-    must not share it (the program orders one object's calls on several streams), and a graph needs the object as long as it is replayed. ``workspaceBytes`` is 0, or on 256 compute units
-    up to 136 MB for heads of 128 and 69 MB for heads of 64, few queries or many: the layers of a step, whose calls follow each other on one
-    stream, are best given one ``workspace`` (uint8) of that size."""
+    must not share it (the program orders one object's calls on several streams), and a graph needs the object as long as it is
+    replayed. ``workspaceBytes`` is 0, or on 256 compute units up to 136 MB for heads of 128 and 69 MB for heads of 64, few queries or many:
+    the layers of a step, whose calls follow each other on one stream, are best given one ``workspace`` (uint8) of that size."""
 
     def __init__(self, pitch: PITCH, q, k, v, rowStarts, output, keyStarts=None, causal: bool = True, scale: float | None = None,
                  softcap: float = 0.0, window: int = 0, slopes=None, lse=None, workspace=None):
